@@ -1,0 +1,123 @@
+// C ABI of the attention over a 4-bit paged cache (include/hstu_cache.h): checks, the cut into runs, launches.
+#include "hstu_cache.h"
+#include "hstu_cache_host.h"
+#include "hstu_paged_attention_kernel.h"
+
+namespace {
+
+struct Plan {
+    int mt, rw;        // 16-row tiles of a wave, waves that share out the rows
+    int row_blocks, splits;
+    int64_t workspace;
+};
+
+int check(const HstuPagedCache* c, const HstuPagedAttentionArgs* a, hstu::PagedAttentionParams& p) {
+    const int rc = hstu_cache_fill(c, p.cache);
+    if (rc) return rc;
+    if (!a) return HSTU_ERR_NULL_POINTER;
+    if (a->delta_size < 0 || a->max_seq_len <= 0 || a->q_heads <= 0 || a->q_heads % c->heads != 0) return HSTU_ERR_BAD_SHAPE;
+    if (a->max_attn_len < 0 || a->contextual_seq_len < 0 || a->kv_splits < 0) return HSTU_ERR_BAD_SHAPE;
+    if (c->dqk == 256 || c->dv == 256) {
+        if (c->dqk != c->dv) return HSTU_ERR_BAD_HEAD_DIM;
+    }
+    if ((int64_t)a->delta_size * a->q_heads > (1 << 30) || (int64_t)c->batch * a->delta_size > (1ll << 31)) return HSTU_ERR_UNSUPPORTED;
+    return 0;
+}
+
+Plan plan_of(const HstuPagedCache* c, const HstuPagedAttentionArgs* a) {
+    Plan p{1, 1, 1, 1, 0};
+    const int64_t rows = (int64_t)a->delta_size * (a->q_heads / c->heads);
+    if (rows > 16) p.mt = c->dv == 256 ? 1 : 2;
+    if (rows > 16 * p.mt) p.rw = 4;
+    const int block = 16 * p.mt * p.rw;
+    p.row_blocks = (int)((rows + block - 1) / block);
+    int64_t longest = a->max_seq_len;
+    if (a->max_attn_len > 0 && (int64_t)a->max_attn_len + a->delta_size + a->contextual_seq_len < longest)
+        longest = (int64_t)a->max_attn_len + a->delta_size + a->contextual_seq_len;
+    const int64_t chunks = (longest + 31) / 32, wgs = (int64_t)p.row_blocks * c->heads * c->batch;
+    const int64_t most = (chunks + 15) / 16;
+    int64_t splits = a->kv_splits > 0 ? a->kv_splits : wgs > 0 ? (2048 + wgs - 1) / wgs : 1;
+    if (splits > most) splits = most;
+    if (splits > 64) splits = 64;
+    if (splits < 1) splits = 1;
+    p.splits = (int)splits;
+    if (splits > 1) p.workspace = splits * c->batch * a->delta_size * a->q_heads * (int64_t)c->dv * 4;
+    return p;
+}
+
+template <class TT, int DK, int DV>
+int launch_sized(const hstu::PagedAttentionParams& p, const Plan& plan, hipStream_t stream) {
+    const unsigned blocks = (unsigned)((p.items + 7) / 8 * 8 * (int64_t)plan.row_blocks);
+    auto go = [&](auto mt, auto rw) {
+        hipLaunchKernelGGL((hstu::hstu_paged_attention_kernel<TT, DK, DV, decltype(mt)::value, decltype(rw)::value>), dim3(blocks), dim3(256), 0, stream, p);
+    };
+    typedef std::integral_constant<int, 1> One;
+    typedef std::integral_constant<int, DV == 256 ? 1 : 2> Most;
+    typedef std::integral_constant<int, 4> Four;
+    if (plan.rw == 4) go(Most{}, Four{});
+    else if (plan.mt == 1) go(One{}, One{});
+    else if constexpr (DV != 256) go(Most{}, One{});
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && p.splits > 1) {
+        const int64_t total8 = p.partial_stride / 8;
+        hipLaunchKernelGGL((hstu::hstu_paged_join_kernel<TT>), dim3((unsigned)((total8 + 255) / 256)), dim3(256), 0, stream, p, 16 * plan.mt * plan.rw, total8);
+        e = hipGetLastError();
+    }
+    if (e == hipSuccess) return 0;
+    hstu_cache_set_last_error("paged attention kernel launch", (int)e);
+    return HSTU_ERR_LAUNCH;
+}
+
+template <class TT>
+int launch(const hstu::PagedAttentionParams& p, const Plan& plan, hipStream_t stream) {
+    auto with_dv = [&](auto dk) {
+        constexpr int DK = decltype(dk)::value;
+        if (p.cache.dv == 32) return launch_sized<TT, DK, 32>(p, plan, stream);
+        if (p.cache.dv == 64) return launch_sized<TT, DK, 64>(p, plan, stream);
+        return launch_sized<TT, DK, 128>(p, plan, stream);
+    };
+    if (p.cache.dqk == 32) return with_dv(std::integral_constant<int, 32>{});
+    if (p.cache.dqk == 64) return with_dv(std::integral_constant<int, 64>{});
+    if (p.cache.dqk == 128) return with_dv(std::integral_constant<int, 128>{});
+    return launch_sized<TT, 256, 256>(p, plan, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t hstu_cache_attention_workspace_bytes(const HstuPagedCache* c, const HstuPagedAttentionArgs* a) {
+    hstu::PagedAttentionParams p{};
+    if (check(c, a, p) != 0 || c->batch == 0 || a->delta_size == 0) return 0;
+    return (size_t)plan_of(c, a).workspace;
+}
+
+int hstu_cache_attention(const HstuPagedCache* c, const HstuPagedAttentionArgs* a, void* stream) {
+    hstu::PagedAttentionParams p{};
+    const int rc = check(c, a, p);
+    if (rc) return rc;
+    if (c->batch == 0 || a->delta_size == 0) return 0;
+    if (c->pages == 0) return HSTU_ERR_BAD_SHAPE;
+    if (!a->q || !a->out || !a->seq_lengths || !c->page_table) return HSTU_ERR_NULL_POINTER;
+    if (!hstu_cache_aligned(a->q) || !hstu_cache_aligned(a->out)) return HSTU_ERR_MISALIGNED;
+    if (a->q_row_stride < 0 || a->q_head_stride < 0 || a->q_row_stride % 8 != 0 || a->q_head_stride % 8 != 0) return HSTU_ERR_MISALIGNED;
+    const Plan plan = plan_of(c, a);
+    if (plan.workspace > 0) {
+        if (!a->workspace) return HSTU_ERR_NULL_POINTER;
+        if (!hstu_cache_aligned(a->workspace)) return HSTU_ERR_MISALIGNED;
+        if (a->workspace_bytes < plan.workspace) return HSTU_ERR_BAD_SHAPE;
+    }
+    const int64_t items = (int64_t)c->batch * c->heads * plan.splits;
+    if (items * plan.row_blocks > (1ll << 30)) return HSTU_ERR_UNSUPPORTED;
+    if (!hstu_cache_device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
+    p.q = (const char*)a->q, p.q_rs = a->q_row_stride, p.q_hs = a->q_head_stride, p.out = (char*)a->out;
+    p.lengths = a->seq_lengths, p.lengths_i64 = a->seq_lengths_i64, p.targets = a->num_targets, p.targets_i64 = a->num_targets_i64;
+    p.group = a->q_heads / c->heads, p.delta = a->delta_size, p.w = a->max_attn_len, p.c = a->contextual_seq_len;
+    const float log2e = 1.4426950408889634f;
+    p.c1 = -a->alpha * log2e, p.oscale = -1.f / (a->max_seq_len * log2e);
+    p.row_blocks = plan.row_blocks, p.splits = plan.splits, p.items = (int)items;
+    p.partial = (float*)a->workspace, p.partial_stride = (int64_t)c->batch * a->delta_size * a->q_heads * c->dv;
+    return c->dtype == HSTU_BF16 ? launch<hstu::PagedBf16>(p, plan, (hipStream_t)stream) : launch<hstu::PagedF16>(p, plan, (hipStream_t)stream);
+}
+
+}  // extern "C"

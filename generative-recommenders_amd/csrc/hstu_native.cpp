@@ -1,5 +1,5 @@
 // Native front of the operators: a Python module (`hstu_native`) that takes torch tensors, checks them, allocates the
-// result and the scratch memory and calls the C ABI (hstu_hip.h, hstu_linear.h) -- the work that ops/*.py does through
+// result and the scratch memory and calls the C ABI (hstu_hip.h, hstu_linear.h, hstu_cache.h) -- the work that ops/*.py does through
 // ctypes for every argument it has to look at, in a few microseconds instead of ten to thirty.
 //
 // The operators that are differentiable record a backward node of their own here (torch::autograd::Function): nothing but inputs
@@ -19,6 +19,7 @@
 #include <optional>
 #include <tuple>
 
+#include "hstu_cache.h"
 #include "hstu_hip.h"
 #include "hstu_linear.h"
 
@@ -690,6 +691,264 @@ OptTensor compute_output(const Tensor& attn, const Tensor& u, const Tensor& x, c
     }
 }
 
+// ---- rotated positions, the 4-bit paged cache ---------------------------------------------------------------------------
+// `checked`: the Python operator has made the checks of HSTU_HIP_CHECK_CONTRACT.
+
+void check_cache(int rc) {
+    if (rc == 0) return;
+    const std::string what = c10::str("hstu_cache: ", hstu_hip_status_string(rc), " (", hstu_cache_last_error(), ") [status ", rc, "]");
+    TORCH_CHECK_VALUE(rc != HSTU_ERR_NULL_POINTER && rc != HSTU_ERR_BAD_SHAPE, what);
+    TORCH_CHECK_NOT_IMPLEMENTED(rc != HSTU_ERR_UNSUPPORTED, what);
+    TORCH_CHECK(false, what);
+}
+
+// [rows, heads, dim] for the kernels: as kernel_layout, on the device asked for; the stride of a dimension of one is never used.
+bool head_rows(const Tensor& t, const at::Device& device) {
+    if (t.dim() != 3 || !t.is_cuda() || t.device() != device || t.numel() == 0 || t.stride(2) != 1) return false;
+    const int64_t per16 = 16 / t.element_size();
+    return (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0 && (t.size(0) == 1 || (t.stride(0) % per16 == 0 && t.stride(0) >= 0)) &&
+           (t.size(1) == 1 || (t.stride(1) % per16 == 0 && t.stride(1) >= 0));
+}
+int64_t row_pitch(const Tensor& t) { return t.size(0) == 1 ? 0 : t.stride(0); }
+int64_t head_pitch(const Tensor& t) { return t.size(1) == 1 ? 0 : t.stride(1); }
+// any values and layout to what head_rows takes
+Tensor to_head_rows(const Tensor& t) { return head_rows(t, t.device()) ? t : t.clone(at::MemoryFormat::Contiguous); }
+
+bool index_vector(const Tensor& t, int64_t size, const at::Device& device) {
+    return index_tensor(t) && t.dim() == 1 && t.numel() == size && t.device() == device;
+}
+bool is_i64(const Tensor& t) { return t.scalar_type() == at::kLong; }
+
+// The weight of a norm for heads like those of x, and the table of a rotation.
+bool norm_weight_of(const OptTensor& w, const Tensor& x) { return !w || (w->dim() == 1 && w->size(0) == x.size(2) && w->device() == x.device() && parameter(*w, x)); }
+bool rotary_table(const OptTensor& t, const Tensor& x) {
+    return !t || (t->dim() == 2 && t->scalar_type() == at::kFloat && t->device() == x.device() && t->is_contiguous() && aligned16(*t) && t->size(1) > 0 &&
+                  !(t->requires_grad() && at::GradMode::is_enabled()));
+}
+
+// One of q and k on the way through norm and rotation.
+struct NormRopeCall {
+    int64_t rows, dim;
+    double eps;
+    bool interleaved;
+};
+
+void fill_norm_rope(HstuNormRopeArgs& a, const NormRopeCall& c, at::ScalarType type, const OptTensor& positions, const OptTensor& table) {
+    a.eps = (float)c.eps, a.interleaved = c.interleaved, a.rows = c.rows, a.dim = (int32_t)c.dim, a.dtype = attention_dtype(type);
+    if (table) {
+        a.table = (const float*)table->const_data_ptr(), a.table_rows = table->size(0), a.rotary = (int32_t)table->size(1);
+        a.positions = positions->const_data_ptr(), a.positions_i64 = is_i64(*positions);
+    }
+}
+void fill_q(HstuNormRopeArgs& a, const Tensor& x, const OptTensor& w) {
+    a.q = x.const_data_ptr(), a.q_row_stride = row_pitch(x), a.q_head_stride = head_pitch(x), a.q_heads = (int32_t)x.size(1);
+    a.q_weight = w ? w->const_data_ptr() : nullptr;
+}
+void fill_k(HstuNormRopeArgs& a, const Tensor& x, const OptTensor& w) {
+    a.k = x.const_data_ptr(), a.k_row_stride = row_pitch(x), a.k_head_stride = head_pitch(x), a.k_heads = (int32_t)x.size(1);
+    a.k_weight = w ? w->const_data_ptr() : nullptr;
+}
+
+typedef std::tuple<Tensor, OptTensor> QAndK;
+
+QAndK norm_rope_result(const Tensor& q, const OptTensor& k, const OptTensor& positions, const OptTensor& table, const OptTensor& qw, const OptTensor& kw,
+                       const NormRopeCall& c) {
+    HstuNormRopeArgs a{};
+    fill_norm_rope(a, c, q.scalar_type(), positions, table);
+    Tensor q_out = at::empty(q.sizes(), q.options());
+    OptTensor k_out;
+    fill_q(a, q, qw);
+    a.q_out = q_out.data_ptr();
+    if (k) {
+        k_out = at::empty(k->sizes(), k->options());
+        fill_k(a, *k, kw);
+        a.k_out = k_out->data_ptr();
+    }
+    const c10::DeviceGuard on_device(q.device());
+    check_cache(hstu_cache_norm_rope(&a, stream_of(q)));
+    return {q_out, k_out};
+}
+
+// Of q and k only what a norm needs is saved: without weights, positions and table alone.
+struct NormRopeFunction : torch::autograd::Function<NormRopeFunction> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k, const OptTensor& qw, const OptTensor& kw,
+                                 const OptTensor& positions, const OptTensor& table, const NormRopeCall& c) {
+        auto [q_out, k_out] = norm_rope_result(q, k, positions, table, qw, kw, c);
+        auto saved = [](const OptTensor& t, bool wanted = true) { return wanted && t ? *t : Tensor(); };
+        ctx->save_for_backward({qw ? q : Tensor(), saved(k, kw.has_value()), saved(qw), saved(kw), saved(positions, table.has_value()), saved(table)});
+        ctx->saved_data["call"] = std::vector<int64_t>{c.rows, c.dim, c.interleaved, q.size(1), k ? k->size(1) : 0, (int64_t)q.scalar_type()};
+        ctx->saved_data["eps"] = c.eps;
+        ctx->set_materialize_grads(false);
+        if (k) return {q_out, *k_out};
+        return {q_out};
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const BackwardScope scope;
+        const auto saved = ctx->get_saved_variables();
+        const auto i = ctx->saved_data["call"].toIntVector();
+        const NormRopeCall c{i[0], i[1], ctx->saved_data["eps"].toDouble(), i[2] != 0};
+        const auto type = (at::ScalarType)i[5];
+        const OptTensor positions = saved[4].defined() ? OptTensor(saved[4].contiguous()) : OptTensor(),
+                        table = saved[5].defined() ? OptTensor(saved_dense(saved[5])) : OptTensor();
+        // inputs as autograd counts them: those that there are
+        const bool has_k = i[4] > 0;
+        size_t at_input = 1 + has_k;
+        variable_list got(7);
+        HstuNormRopeArgs a{};
+        HstuNormRopeGrads g{};
+        fill_norm_rope(a, c, type, positions, table);
+        Tensor alive[2][3];  // incoming gradient, x and weight as the kernels read them
+        bool any = false;
+        for (int side = 0; side < 2; ++side) {
+            const bool weighted = saved[2 + side].defined();
+            const bool weight_wanted = weighted && ctx->needs_input_grad(at_input);
+            at_input += weighted;
+            if (side >= (int)grads.size() || !grads[side].defined()) continue;
+            any = true;
+            auto& [dy, x, w] = alive[side];
+            dy = to_head_rows(grads[side].to(type));
+            x = weighted ? to_head_rows(saved[side]) : dy;  // (not read without a weight)
+            if (weighted) w = saved_dense(saved[2 + side]);
+            Tensor dx = at::empty({c.rows, i[3 + side], c.dim}, dy.options()), dw = weight_wanted ? at::empty_like(w) : Tensor();
+            if (side == 0) {
+                fill_q(a, x, weighted ? OptTensor(w) : OptTensor());
+                g.dq_out = dy.const_data_ptr(), g.dq_out_row_stride = row_pitch(dy), g.dq_out_head_stride = head_pitch(dy), g.dq = dx.data_ptr();
+                if (weight_wanted) g.dq_weight = dw.data_ptr();
+            } else {
+                fill_k(a, x, weighted ? OptTensor(w) : OptTensor());
+                g.dk_out = dy.const_data_ptr(), g.dk_out_row_stride = row_pitch(dy), g.dk_out_head_stride = head_pitch(dy), g.dk = dx.data_ptr();
+                if (weight_wanted) g.dk_weight = dw.data_ptr();
+            }
+            got[side] = dx, got[2 + side] = dw;
+        }
+        if (!any) return got;
+        const Tensor& like = alive[0][0].defined() ? alive[0][0] : alive[1][0];
+        const c10::DeviceGuard on_device(like.device());
+        Tensor scratch;
+        if (g.dq_weight || g.dk_weight) {
+            g.workspace_bytes = (int64_t)hstu_cache_norm_rope_bwd_workspace_bytes(&a);
+            scratch = at::empty({g.workspace_bytes}, like.options().dtype(at::kByte));
+            g.workspace = scratch.data_ptr();
+        }
+        check_cache(hstu_cache_norm_rope_bwd(&a, &g, stream_of(like)));
+        return got;
+    }
+};
+
+std::optional<QAndK> qk_norm_rope(const Tensor& q, const OptTensor& k, const OptTensor& positions, const OptTensor& table, const OptTensor& qw,
+                                  const OptTensor& kw, double eps, bool interleaved, bool checked) {
+    const auto type = q.scalar_type();
+    if ((type != at::kBFloat16 && type != at::kHalf && type != at::kFloat) || !q.is_cuda() || !head_rows(q, q.device())) return {};
+    if (k && (!head_rows(*k, q.device()) || k->scalar_type() != type || k->size(0) != q.size(0) || k->size(2) != q.size(2))) return {};
+    if (!rotary_table(table, q) || !norm_weight_of(qw, q) || !norm_weight_of(kw, q) || (kw && !k) || (!table && !qw && !kw)) return {};
+    if (table && (!positions || !index_vector(*positions, q.size(0), q.device()) || table->size(1) > q.size(2))) return {};
+    if (!checked && contract_checks() && table) return {};
+    const NormRopeCall c{q.size(0), q.size(2), eps, interleaved};
+    bool grad = wants_grad({&q});
+    for (const OptTensor* t : {&k, &qw, &kw}) grad = grad || (*t && wants_grad({&**t}));
+    RECORD_USER_SCOPE("qk_norm_rope");
+    if (!grad) return norm_rope_result(q, k, positions, table, qw, kw, c);
+    const variable_list o = NormRopeFunction::apply(q, k, qw, kw, positions, table, c);
+    return QAndK(o[0], k ? OptTensor(o[1]) : OptTensor());
+}
+
+typedef std::tuple<Tensor, Tensor, Tensor, Tensor> CacheTensors;  // codes and scales of K, of V
+
+// False: not as the kernels take it.
+bool fill_cache(HstuPagedCache& c, const CacheTensors& t, const Tensor& table) {
+    const auto& [kc, ks, vc, vs] = t;
+    if (!kc.is_cuda() || !table.is_cuda() || table.device() != kc.device()) return false;
+    for (const Tensor* x : {&kc, &ks, &vc, &vs})
+        if (x->dim() != 4 || x->device() != kc.device() || !x->is_contiguous() || !aligned16(*x) || x->numel() == 0 || x->requires_grad()) return false;
+    const auto type = ks.scalar_type();
+    if (kc.scalar_type() != at::kByte || vc.scalar_type() != at::kByte || vs.scalar_type() != type || (type != at::kBFloat16 && type != at::kHalf)) return false;
+    for (const Tensor* x : {&ks, &vc, &vs})
+        for (int d = 0; d < 3; ++d)
+            if (x->size(d) != kc.size(d)) return false;
+    if (ks.size(3) != 2 || vs.size(3) != 2) return false;
+    if (table.dim() != 2 || table.numel() == 0 || (table.scalar_type() != at::kInt && table.scalar_type() != at::kLong)) return false;
+    if ((table.size(1) > 1 && table.stride(1) != 1) || (table.size(0) > 1 && table.stride(0) < 0)) return false;
+    c.k_codes = kc.data_ptr(), c.k_scales = ks.data_ptr(), c.v_codes = vc.data_ptr(), c.v_scales = vs.data_ptr();
+    c.pages = kc.size(0), c.heads = (int32_t)kc.size(1), c.page_size = (int32_t)kc.size(2);
+    c.dqk = (int32_t)(2 * kc.size(3)), c.dv = (int32_t)(2 * vc.size(3)), c.dtype = attention_dtype(type);
+    c.page_table = table.const_data_ptr(), c.table_row_stride = table.size(0) > 1 ? table.stride(0) : 0;
+    c.table_columns = (int32_t)table.size(1), c.page_table_i64 = is_i64(table), c.batch = (int32_t)table.size(0);
+    return true;
+}
+
+// Where rows of a call belong: one per sequence with `start`, or by offsets.
+bool placing(const Tensor& start, const OptTensor& offsets, int64_t rows, int64_t batch, const at::Device& device) {
+    if (!index_vector(start, batch, device)) return false;
+    return offsets ? index_vector(*offsets, batch + 1, device) : rows % batch == 0;
+}
+
+bool append_paged_kv(const CacheTensors& cache, const Tensor& k, const Tensor& v, const Tensor& pages, const Tensor& start, const OptTensor& offsets,
+                     const OptTensor& table, const OptTensor& positions, const OptTensor& kw, double eps, bool interleaved,
+                     bool checked) {
+    HstuPagedCache c{};
+    if ((!checked && contract_checks()) || !fill_cache(c, cache, pages)) return false;
+    const Tensor& scales = std::get<1>(cache);
+    if (!head_rows(k, scales.device()) || !head_rows(v, scales.device()) || k.scalar_type() != scales.scalar_type() || v.scalar_type() != k.scalar_type()) return false;
+    if (k.size(1) != c.heads || v.size(1) != c.heads || k.size(2) != c.dqk || v.size(2) != c.dv || v.size(0) != k.size(0)) return false;
+    if (!placing(start, offsets, k.size(0), c.batch, k.device()) || !rotary_table(table, k) || !norm_weight_of(kw, k)) return false;
+    if (table && table->size(1) > k.size(2)) return false;
+    if (positions && !index_vector(*positions, k.size(0), k.device())) return false;
+    if (wants_grad({&k, &v}) || (kw && wants_grad({&*kw}))) return false;
+    HstuAppendArgs a{};
+    a.k = k.const_data_ptr(), a.v = v.const_data_ptr(), a.rows = k.size(0);
+    a.k_row_stride = row_pitch(k), a.k_head_stride = head_pitch(k), a.v_row_stride = row_pitch(v), a.v_head_stride = head_pitch(v);
+    a.start = start.const_data_ptr(), a.start_i64 = is_i64(start);
+    if (offsets) a.seq_offsets = offsets->const_data_ptr(), a.seq_offsets_i64 = is_i64(*offsets);
+    a.k_weight = kw ? kw->const_data_ptr() : nullptr, a.eps = (float)eps, a.interleaved = interleaved;
+    if (table) a.table = (const float*)table->const_data_ptr(), a.table_rows = table->size(0), a.rotary = (int32_t)table->size(1);
+    if (positions) a.positions = positions->const_data_ptr(), a.positions_i64 = is_i64(*positions);
+    RECORD_USER_SCOPE("append_paged_kv");
+    const c10::DeviceGuard on_device(k.device());
+    check_cache(hstu_cache_append(&c, &a, stream_of(k)));
+    return true;
+}
+
+std::optional<std::tuple<Tensor, Tensor>> read_paged_kv(const CacheTensors& cache, int64_t rows, const Tensor& pages, const Tensor& start,
+                                                        const OptTensor& offsets, bool checked) {
+    HstuPagedCache c{};
+    if (rows <= 0 || (!checked && contract_checks()) || !fill_cache(c, cache, pages)) return {};
+    const Tensor& scales = std::get<1>(cache);
+    if (!placing(start, offsets, rows, c.batch, scales.device())) return {};
+    RECORD_USER_SCOPE("read_paged_kv");
+    Tensor k = at::empty({rows, c.heads, c.dqk}, scales.options()), v = at::empty({rows, c.heads, c.dv}, scales.options());
+    const c10::DeviceGuard on_device(scales.device());
+    check_cache(hstu_cache_read(&c, rows, start.const_data_ptr(), is_i64(start), offsets ? offsets->const_data_ptr() : nullptr, offsets && is_i64(*offsets),
+                                k.data_ptr(), v.data_ptr(), stream_of(scales)));
+    return std::make_tuple(k, v);
+}
+
+OptTensor delta_hstu_mha_paged(int64_t max_seq_len, double alpha, const Tensor& q, const CacheTensors& cache, const Tensor& pages, const Tensor& lengths,
+                               const OptTensor& targets, int64_t w, int64_t ctx, int64_t kv_splits, bool checked) {
+    HstuPagedCache c{};
+    if (max_seq_len <= 0 || max_seq_len > INT32_MAX || (!checked && contract_checks()) || !fill_cache(c, cache, pages)) return {};
+    const Tensor& scales = std::get<1>(cache);
+    if (!head_rows(q, scales.device()) || q.scalar_type() != scales.scalar_type() || q.size(2) != c.dqk || q.size(1) % c.heads != 0) return {};
+    if (q.size(0) % c.batch != 0 || !index_vector(lengths, c.batch, q.device()) || (targets && !index_vector(*targets, c.batch, q.device()))) return {};
+    if (w < 0 || w > INT32_MAX || ctx < 0 || ctx > INT32_MAX || kv_splits < 0 || kv_splits > INT32_MAX || wants_grad({&q})) return {};
+    HstuPagedAttentionArgs a{};
+    a.q = q.const_data_ptr(), a.q_row_stride = row_pitch(q), a.q_head_stride = head_pitch(q);
+    a.seq_lengths = lengths.const_data_ptr(), a.seq_lengths_i64 = is_i64(lengths);
+    if (targets) a.num_targets = targets->const_data_ptr(), a.num_targets_i64 = is_i64(*targets);
+    a.q_heads = (int32_t)q.size(1), a.delta_size = (int32_t)(q.size(0) / c.batch), a.max_seq_len = (int32_t)max_seq_len, a.alpha = (float)alpha;
+    a.max_attn_len = (int32_t)w, a.contextual_seq_len = (int32_t)ctx, a.kv_splits = (int32_t)kv_splits;
+    RECORD_USER_SCOPE("delta_hstu_mha_paged");
+    Tensor out = at::empty({q.size(0), q.size(1), c.dv}, q.options()), scratch;
+    a.out = out.data_ptr();
+    const c10::DeviceGuard on_device(q.device());
+    const size_t need = hstu_cache_attention_workspace_bytes(&c, &a);
+    if (need > 0) {
+        scratch = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
+        a.workspace = scratch.data_ptr(), a.workspace_bytes = (int64_t)need;
+    }
+    check_cache(hstu_cache_attention(&c, &a, stream_of(q)));
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -703,4 +962,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("compute_uqvk", &compute_uqvk, nogil);
     m.def("preprocess_and_attention", &preprocess_and_attention, nogil);
     m.def("compute_output", &compute_output, nogil);
+    m.def("qk_norm_rope", &qk_norm_rope, nogil);
+    m.def("append_paged_kv", &append_paged_kv, nogil);
+    m.def("read_paged_kv", &read_paged_kv, nogil);
+    m.def("delta_hstu_mha_paged", &delta_hstu_mha_paged, nogil);
 }

@@ -1,0 +1,438 @@
+// HSTU attention of the newest positions against a K/V cache held in 4 bits, in pages.
+//
+// All matrix work is on v_mfma_f32_16x16x32, transposed as in hstu_common.h so that the scores never leave their lanes:
+//
+//   S^T[pos, row] = K[pos, :] . Q[row, :]^T     A = K, B = Q (registers, loaded once)
+//   O^T[d, row]  += V^T[d, pos] . P^T[pos, row] A = V^T, B = P^T (registers)
+//
+// Both A operands come straight from the packed rows, with no LDS between: which of its 32 depths a lane's eight slots stand for
+// is free as long as A and B agree.  K: lane (m, g) holds the words NK g .. of position m, a word being the eight depths of one
+// product, in the order in which unpacking yields them (pairs four columns apart: one AND-OR makes two columns).  V: lane (m, g)
+// holds the same NV = dv / 16 columns of eight positions (the eight that its scores have), so one permute joins the halves of two
+// positions' words and the AND-ORs then yield (position, position + 1) pairs of each column: about one instruction per value.
+//
+// A code c enters a product as the float OFF + c, OFF the power of two whose mantissa step is where the code's bits lie (exact).
+// What OFF adds is taken out again in fp32: from S by starting the accumulator at -sum(q OFF), from O through psum, the sum of the
+// rounded P as one more product sees it (a row of ones).  With step s and lowest value l of a row
+//     <q, k> = s (acc) + l sum(q),     O = sum_pos (P s) (c - 7.5) + sum_pos P (l + 7.5 s),
+// the first sum on the matrix cores with P s rounded to bf16, the second in fp32: around the middle code the rounding of P s weighs
+// a third of what it would around the lowest value.  For fp16 results P s is kept in two bf16 words (16 bits, and bf16's range).
+#pragma once
+#include "hstu_paged_rows.h"
+
+namespace hstu {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 pa_bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 pa_f16x8;
+typedef __attribute__((ext_vector_type(4))) float pa_f32x4;
+
+struct PagedAttentionParams {
+    PagedCache cache;
+    const char* q;
+    int64_t q_rs, q_hs;
+    char* out;
+    const void *lengths, *targets;
+    int lengths_i64, targets_i64;
+    int group, delta, w, c;  // heads of q to one of the cache; max_attn_len, contextual_seq_len
+    float c1, oscale;        // t = c1 <q, k> with c1 = -alpha log2(e);  out = oscale * sum t / (1 + 2^t) v
+    int row_blocks, splits, items;
+    float* partial;          // [splits][batch * delta][q heads][dv], used where splits > 1
+    int64_t partial_stride;
+};
+
+// What the rows of one block see, in chunks of 32 positions: those of [a0, a0 + na), then those of [b0, b0 + nb).
+struct PagedSpan {
+    int n, u;  // length and its part that is no target
+    int a0, na, b0, nb;
+    bool bad;  // the sequence has no room in the page table
+};
+
+// Rows i0 .. i1 - 1 of the newest `delta` positions of sequence b.
+__device__ __forceinline__ PagedSpan paged_span(const PagedAttentionParams& p, int b, int i0, int i1) {
+    PagedSpan s;
+    const int64_t n64 = index_at(p.lengths, p.lengths_i64, b), room = (int64_t)p.cache.table_columns << p.cache.page_shift;
+    s.bad = n64 > room || n64 > (1 << 30);
+    s.n = s.bad || n64 < 0 ? 0 : (int)n64;
+    int64_t t = p.targets ? index_at(p.targets, p.targets_i64, b) : 0;
+    t = t < 0 ? 0 : t > s.n ? s.n : t;
+    s.u = s.n - (int)t;
+    const int first = max(s.n - p.delta + i0, 0), end = s.n - p.delta + i1;  // positions of the rows
+    s.a0 = s.na = s.b0 = s.nb = 0;
+    if (end <= first) return s;
+    const bool contextual = first < p.c;
+    const int a_end = contextual ? max(s.u, min(end, s.u)) : min(end, s.u);
+    const int id = min(p.c ? first - p.c + 1 : first, p.c ? s.u - p.c + 1 : s.u);  // of the first row: the others' are not less
+    const int from = p.w > 0 && !contextual && id > p.w ? max(0, id - p.w + (p.c ? p.c - 1 : 0)) : 0;
+    if (a_end > from) s.a0 = from >> 5, s.na = ((a_end + 31) >> 5) - s.a0;
+    if (end > s.u) {  // targets: the positions that only they themselves see
+        const int self = max(s.u, first), done = s.a0 + s.na;
+        s.b0 = max(self >> 5, s.na ? done : 0);
+        s.nb = max(((end + 31) >> 5) - s.b0, 0);
+    }
+    return s;
+}
+
+// What one row sees: positions [lo, hi), [0, chi) and itself.
+struct RowSpan {
+    int lo, hi, chi, self;
+    __device__ __forceinline__ bool sees(int pos) const { return (pos >= lo && pos < hi) || pos < chi || pos == self; }
+};
+
+__device__ __forceinline__ RowSpan row_span(const PagedAttentionParams& p, const PagedSpan& s, int pos) {
+    RowSpan r;
+    if (pos < 0) {
+        r.lo = r.hi = r.chi = 0, r.self = -1;
+    } else if (p.c == 0) {
+        const int id = min(pos, s.u);
+        r.hi = id, r.chi = 0, r.self = pos;
+        r.lo = p.w > 0 ? max(0, id - p.w) : 0;
+    } else if (pos < p.c) {
+        r.lo = 0, r.hi = s.u, r.chi = 0, r.self = pos;
+    } else {
+        const int id = min(pos - p.c + 1, s.u - p.c + 1);
+        r.hi = id + p.c - 1, r.self = pos;
+        r.chi = id > 0 && (p.w <= 0 || id <= p.w) ? p.c : 0;
+        r.lo = p.w > 0 ? max(p.c, id - p.w + p.c - 1) : p.c;
+        if (r.chi && r.lo <= p.c) r.lo = 0;
+    }
+    return r;
+}
+
+// Codes as the floats OFF + code, two to a word: column k and column k + 4 of a word of eight, k = 0 .. 3.
+struct CodesBf16 {  // 128 + code where the code lies at bit 0, 16 + code from bit 3
+    static __device__ __forceinline__ void four(unsigned w, unsigned (&o)[4]) {
+        o[0] = (w & 0x000F000Fu) | 0x43004300u;
+        o[1] = ((w >> 1) & 0x00780078u) | 0x41804180u;
+        o[2] = ((w >> 5) & 0x00780078u) | 0x41804180u;
+        o[3] = ((w >> 9) & 0x00780078u) | 0x41804180u;
+    }
+    static __device__ __forceinline__ constexpr float off(int k) { return k == 0 ? 128.f : 16.f; }
+};
+struct CodesF16 {  // 64 + code, the code at bit 4
+    static __device__ __forceinline__ void four(unsigned w, unsigned (&o)[4]) {
+        o[0] = ((w << 4) & 0x00F000F0u) | 0x54005400u;
+        o[1] = (w & 0x00F000F0u) | 0x54005400u;
+        o[2] = ((w >> 4) & 0x00F000F0u) | 0x54005400u;
+        o[3] = ((w >> 8) & 0x00F000F0u) | 0x54005400u;
+    }
+    static __device__ __forceinline__ constexpr float off(int) { return 64.f; }
+};
+
+struct PagedBf16 {
+    typedef __bf16 elem;
+    typedef CodesBf16 codes;
+    static constexpr int P_WORDS = 1;
+    static __device__ __forceinline__ pa_f32x4 mma(u32x4_t a, u32x4_t b, pa_f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_bf16x8, a), __builtin_bit_cast(pa_bf16x8, b), c, 0, 0, 0);
+    }
+};
+struct PagedF16 {
+    typedef _Float16 elem;
+    typedef CodesF16 codes;
+    static constexpr int P_WORDS = 2;
+    static __device__ __forceinline__ pa_f32x4 mma(u32x4_t a, u32x4_t b, pa_f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pa_f16x8, a), __builtin_bit_cast(pa_f16x8, b), c, 0, 0, 0);
+    }
+};
+
+// The packed rows of 32 positions as one wave holds them, and their steps and lowest values: lane (m, g) has K of positions m and
+// 16 + m, V of positions 4 g + i and 16 + 4 g + i, and the pairs of the latter positions.
+template <int NK, int NV>
+struct PagedChunk {
+    static constexpr int VW = NV == 16 ? 2 : 1;
+    unsigned k[2][NK], v[8][VW];
+    u32x4_t ks[2], vs[2];
+};
+
+template <int DK, int DV>
+struct PagedReader {
+    static constexpr int NK = DK / 32, NV = DV / 16;
+    const PagedCache& c;
+    int64_t table_row;
+    int head, n, lane;
+    bool bad;
+
+    // Row of head `head` where 16 positions from `pos` on lie (pos a multiple of 16).  Positions that do not exist get the first page.
+    __device__ __forceinline__ int64_t row_of(int pos) {
+        int64_t page = 0;
+        if (pos < n) {
+            page = index_at(c.page_table, c.page_table_i64, table_row + (pos >> c.page_shift));
+            if (page < 0 || page >= c.pages) bad = true, page = 0;
+        }
+        return ((page * c.heads + head) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
+    }
+
+    __device__ __forceinline__ void load(PagedChunk<NK, NV>& x, int chunk) {
+        const int m = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+            const int64_t row = row_of(chunk * 32 + tt * 16);
+            const char* k = c.k_codes + row * (DK / 2) + m * (DK / 2) + g * (4 * NK);
+            if constexpr (NK == 1) {
+                x.k[tt][0] = *(const unsigned*)k;
+            } else if constexpr (NK == 2) {
+                typedef __attribute__((ext_vector_type(2))) unsigned u2;
+                const u2 a = *(const u2*)k;
+                x.k[tt][0] = a.x, x.k[tt][1] = a.y;
+            } else {
+#pragma unroll
+                for (int j = 0; j < NK; j += 4) {
+                    const u32x4_t a = *(const u32x4_t*)(k + 4 * j);
+                    x.k[tt][j] = a.x, x.k[tt][j + 1] = a.y, x.k[tt][j + 2] = a.z, x.k[tt][j + 3] = a.w;
+                }
+            }
+            const char* v = c.v_codes + row * (DV / 2) + 4 * g * (DV / 2) + m * (NV / 2);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const char* vi = v + i * (DV / 2);
+                if constexpr (NV == 2) x.v[4 * tt + i][0] = *(const unsigned char*)vi;
+                else if constexpr (NV == 4) x.v[4 * tt + i][0] = *(const unsigned short*)vi;
+                else {
+#pragma unroll
+                    for (int j = 0; j < NV / 8; ++j) x.v[4 * tt + i][j] = *(const unsigned*)(vi + 4 * j);
+                }
+            }
+            x.ks[tt] = *(const u32x4_t*)(c.k_scales + (row + 4 * g) * 4);
+            x.vs[tt] = *(const u32x4_t*)(c.v_scales + (row + 4 * g) * 4);
+        }
+    }
+};
+
+// grid: one workgroup of four waves per (block of 16 MT RW rows, head of the cache, run, sequence), numbered so that the row blocks
+// of one run, which read the same pages, are on one XCD.  RW waves share out the rows, the others the chunks of the run; the sums of
+// the latter meet in LDS.
+template <class TT, int DK, int DV, int MT, int RW>
+__global__ __launch_bounds__(256) void hstu_paged_attention_kernel(const PagedAttentionParams p) {
+    typedef typename TT::elem T;
+    constexpr int NK = DK / 32, NV = DV / 16, KW = 4 / RW;
+    __shared__ float meet[KW > 1 ? 4 * NV * 4 * 64 : 1];
+    const int xcd = blockIdx.x & 7, q8 = blockIdx.x >> 3;
+    const int rb = q8 % p.row_blocks, item = (q8 / p.row_blocks) * 8 + xcd;
+    if (item >= p.items) return;
+    const int hk = item % p.cache.heads, split = (item / p.cache.heads) % p.splits, b = item / (p.cache.heads * p.splits);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const int rw = wave / KW, kw = wave % KW;
+    constexpr int ROWS = 16 * MT * RW;
+    const int rows = p.delta * p.group, r_end = min((rb + 1) * ROWS, rows);
+    const PagedSpan span = paged_span(p, b, rb * ROWS / p.group, (r_end - 1) / p.group + 1);
+    const int chunks = span.na + span.nb, per = (chunks + p.splits - 1) / p.splits;
+    const int chunk_end = min((split + 1) * per, chunks);
+    if (p.splits > 1 && split * per >= chunks) return;  // (the joining kernel knows)
+
+    u32x4_t qf[MT][NK];
+    float qs[MT], qo[MT];
+    RowSpan see[MT];
+    int64_t out_at[MT];
+    int lo_max = 0, hi_min = 1 << 30;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int r = rb * ROWS + (rw * MT + mt) * 16 + m;
+        const int i = r / p.group, head = hk * p.group + (r - i * p.group);
+        qs[mt] = qo[mt] = 0.f;
+        see[mt].lo = see[mt].hi = see[mt].chi = 0, see[mt].self = -1;
+        out_at[mt] = -1;
+        const int64_t row = (int64_t)b * p.delta + i;
+        if (r < rows) {
+            see[mt] = row_span(p, span, span.n - p.delta + i);
+            out_at[mt] = (row * (p.cache.heads * p.group) + head) * DV;
+            lo_max = max(lo_max, see[mt].lo), hi_min = min(hi_min, see[mt].hi);
+        }
+#pragma unroll
+        for (int j = 0; j < NK; ++j) {
+            u32x4_t x = {0, 0, 0, 0};
+            if (r < rows) x = *(const u32x4_t*)(p.q + (row * p.q_rs + head * p.q_hs + 8 * (NK * g + j)) * 2);
+            // columns k and k + 4 side by side, as the codes come
+            qf[mt][j] = u32x4_t{__builtin_amdgcn_perm(x.z, x.x, 0x05040100u), __builtin_amdgcn_perm(x.z, x.x, 0x07060302u),
+                                __builtin_amdgcn_perm(x.w, x.y, 0x05040100u), __builtin_amdgcn_perm(x.w, x.y, 0x07060302u)};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                typedef __attribute__((ext_vector_type(2))) T T2;
+                const T2 two = __builtin_bit_cast(T2, (unsigned)qf[mt][j][k]);
+                const float sum = (float)two[0] + (float)two[1];
+                qs[mt] += sum, qo[mt] += sum * TT::codes::off(k);
+            }
+        }
+        qs[mt] += __shfl_xor(qs[mt], 16, 64), qo[mt] += __shfl_xor(qo[mt], 16, 64);
+        qs[mt] += __shfl_xor(qs[mt], 32, 64), qo[mt] += __shfl_xor(qo[mt], 32, 64);
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) lo_max = max(lo_max, __shfl_xor(lo_max, d, 64)), hi_min = min(hi_min, __shfl_xor(hi_min, d, 64));
+    lo_max = __builtin_amdgcn_readfirstlane(lo_max), hi_min = __builtin_amdgcn_readfirstlane(hi_min);
+
+    pa_f32x4 acc[MT][NV], psum[MT];
+    float plo[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        psum[mt] = pa_f32x4{0, 0, 0, 0}, plo[mt] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) acc[mt][j] = pa_f32x4{0, 0, 0, 0};
+    }
+    PagedReader<DK, DV> reader{p.cache, b * p.cache.table_row_stride, hk, span.n, lane, span.bad};
+
+    auto chunk_at = [&](int i) { return i < span.na ? span.a0 + i : span.b0 + (i - span.na); };
+    auto work = [&](const PagedChunk<NK, NV>& x, int chunk) __attribute__((always_inline)) {
+        const int pos0 = chunk * 32 + 4 * g;
+        const bool whole = chunk * 32 >= lo_max && chunk * 32 + 32 <= hi_min;
+        float ka[8], kb[8], va[8], vm[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            typedef __attribute__((ext_vector_type(2))) T T2;
+            const T2 k2 = __builtin_bit_cast(T2, (unsigned)x.ks[e >> 2][e & 3]), v2 = __builtin_bit_cast(T2, (unsigned)x.vs[e >> 2][e & 3]);
+            ka[e] = p.c1 * (float)k2[0], kb[e] = p.c1 * (float)k2[1];
+            va[e] = (float)v2[0], vm[e] = (float)v2[1] + 7.5f * (float)v2[0];
+        }
+        u32x4_t kf[2][NK], vf[NV];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int j = 0; j < NK; ++j) {
+                unsigned o[4];
+                TT::codes::four(x.k[tt][j], o);
+                kf[tt][j] = u32x4_t{o[0], o[1], o[2], o[3]};
+            }
+#pragma unroll
+        for (int pair = 0; pair < 4; ++pair)
+#pragma unroll
+            for (int h = 0; h < (NV + 3) / 4; ++h) {
+                unsigned two, o[4];
+                if constexpr (NV <= 4) two = x.v[2 * pair][0] | (x.v[2 * pair + 1][0] << 16);
+                else two = __builtin_amdgcn_perm(x.v[2 * pair + 1][h >> 1], x.v[2 * pair][h >> 1], h & 1 ? 0x07060302u : 0x05040100u);
+                CodesBf16::four(two, o);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (4 * h + k < NV) vf[4 * h + k][pair] = o[k];
+            }
+        const u32x4_t ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            pa_f32x4 s[2];
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) {
+                s[tt] = pa_f32x4{-qo[mt], -qo[mt], -qo[mt], -qo[mt]};
+#pragma unroll
+                for (int j = 0; j < NK; ++j) s[tt] = TT::mma(kf[tt][j], qf[mt][j], s[tt]);
+            }
+            float ps[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float t = ka[e] * s[e >> 2][e & 3] + kb[e] * qs[mt];
+                const float pr = t * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(t));
+                ps[e] = pr * va[e];
+                float lower = pr * vm[e];
+                if (!whole) {
+                    const bool seen = see[mt].sees(pos0 + (e >> 2) * 16 + (e & 3));
+                    ps[e] = seen ? ps[e] : 0.f, lower = seen ? lower : 0.f;
+                }
+                plo[mt] += lower;
+            }
+            pa_bf16x8 high;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) high[e] = (__bf16)ps[e];
+            const u32x4_t ph = __builtin_bit_cast(u32x4_t, high);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) acc[mt][j] = PagedBf16::mma(vf[j], ph, acc[mt][j]);
+            psum[mt] = PagedBf16::mma(ones, ph, psum[mt]);
+            if constexpr (TT::P_WORDS == 2) {
+                pa_bf16x8 rest;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) rest[e] = (__bf16)(ps[e] - (float)high[e]);
+                const u32x4_t pl = __builtin_bit_cast(u32x4_t, rest);
+#pragma unroll
+                for (int j = 0; j < NV; ++j) acc[mt][j] = PagedBf16::mma(vf[j], pl, acc[mt][j]);
+                psum[mt] = PagedBf16::mma(ones, pl, psum[mt]);
+            }
+        }
+    };
+
+    // two chunks in flight: the next one's loads are issued before the work on this one
+    PagedChunk<NK, NV> x0, x1;
+    int i = split * per + kw;
+    if (i < chunk_end) reader.load(x0, chunk_at(i));
+    while (i < chunk_end) {
+        if (i + KW < chunk_end) reader.load(x1, chunk_at(i + KW));
+        work(x0, chunk_at(i));
+        i += KW;
+        if (i >= chunk_end) break;
+        if (i + KW < chunk_end) reader.load(x0, chunk_at(i + KW));
+        work(x1, chunk_at(i));
+        i += KW;
+    }
+
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        float lower = plo[mt];
+        lower += __shfl_xor(lower, 16, 64);
+        lower += __shfl_xor(lower, 32, 64);
+        if (reader.bad) lower = __builtin_nanf("");
+        float o[4][NV];  // [i][j]: column NV (4 g + i) + j
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4)
+#pragma unroll
+            for (int j = 0; j < NV; ++j) o[i4][j] = acc[mt][j][i4] - (CodesBf16::off(j & 3) + 7.5f) * psum[mt][i4] + lower;
+        auto put = [&](int i4, const float (&x)[NV]) __attribute__((always_inline)) {
+            if (out_at[mt] < 0) return;
+            const int64_t at = out_at[mt] + NV * (4 * g + i4);
+            if (p.splits > 1) {
+#pragma unroll
+                for (int j = 0; j < NV; ++j) p.partial[split * p.partial_stride + at + j] = x[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < NV; ++j) ((T*)p.out)[at + j] = (T)(x[j] * p.oscale);
+            }
+        };
+        if constexpr (KW == 1) {
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) put(i4, o[i4]);
+        } else {
+            __syncthreads();
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4)
+#pragma unroll
+                for (int j = 0; j < NV; ++j) meet[((wave * 4 + i4) * NV + j) * 64 + lane] = o[i4][j];
+            __syncthreads();
+            // wave kw of the KW that share these rows adds up i4 = kw, kw + KW, ...
+#pragma unroll
+            for (int step = 0; step < 4 / KW; ++step) {
+                const int i4 = kw + step * KW;
+                float x[NV];
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    x[j] = 0.f;
+#pragma unroll
+                    for (int w = 0; w < KW; ++w) x[j] += meet[(((rw * KW + w) * 4 + i4) * NV + j) * 64 + lane];
+                }
+                put(i4, x);
+            }
+        }
+    }
+}
+
+// out = oscale * the sum of the runs there are, eight columns to a thread.
+template <class TT>
+__global__ __launch_bounds__(256) void hstu_paged_join_kernel(const PagedAttentionParams p, int block_rows, int64_t total8) {
+    typedef typename TT::elem T;
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (at >= total8) return;
+    const int heads = p.cache.heads * p.group, words = p.cache.dv >> 3;
+    const int64_t row_head = at / words, row = row_head / heads;
+    const int b = (int)(row / p.delta), r = (int)(row - (int64_t)b * p.delta) * p.group + (int)(row_head - row * heads) % p.group;
+    const int rb = r / block_rows, r_end = min((rb + 1) * block_rows, p.delta * p.group);
+    const PagedSpan span = paged_span(p, b, rb * block_rows / p.group, (r_end - 1) / p.group + 1);
+    const int chunks = span.na + span.nb, per = (chunks + p.splits - 1) / p.splits, runs = per ? (chunks + per - 1) / per : 0;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = span.bad ? __builtin_nanf("") : 0.f;
+    for (int s = 0; s < runs; ++s) {
+        const pa_f32x4* from = (const pa_f32x4*)(p.partial + s * p.partial_stride + at * 8);
+        const pa_f32x4 a = from[0], c = from[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] += a[i], x[4 + i] += c[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= p.oscale;
+    Cols<T> out;
+    out.put(x);
+    out.store((T*)p.out + at * 8);
+}
+
+}  // namespace hstu
