@@ -38,10 +38,6 @@ struct Cols {
 #pragma unroll
         for (int i = 0; i < WORDS / 4; ++i) q[i] = u32x4_t{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
     }
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) w[i] = 0;
-    }
     __device__ __forceinline__ void get(float (&x)[8]) const {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -78,93 +74,140 @@ struct Cols {
     }
 };
 
-template <int LPV>
-__device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-    for (int d = LPV / 2; d >= 1; d >>= 1) v += __shfl_xor(v, d, 64);
-    return v;
+// v of another lane of 16, by the data path of the instruction that uses it (no LDS).
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
 }
 
-// How a lane's eight columns turn: cosines and sines of its columns for one row, and where its partners are.
+// op over LPV lanes, the result in each: neighbours, pairs, then halves of 8 and of 16 mirrored (their lanes agree by then).
+template <int LPV, class F>
+__device__ __forceinline__ float group_reduce(float v, F&& op) {
+    if constexpr (LPV >= 2) v = op(v, dpp<0xB1>(v));
+    if constexpr (LPV >= 4) v = op(v, dpp<0x4E>(v));
+    if constexpr (LPV >= 8) v = op(v, dpp<0x141>(v));
+    if constexpr (LPV >= 16) v = op(v, dpp<0x140>(v));
+    if constexpr (LPV >= 32) v = op(v, __shfl_xor(v, 16, 64));
+    if constexpr (LPV >= 64) v = op(v, __shfl_xor(v, 32, 64));
+    return v;
+}
+template <int LPV>
+__device__ __forceinline__ float group_sum(float v) {
+    return group_reduce<LPV>(v, [](float a, float b) { return a + b; });
+}
+
 struct Turn {
     const float* table;
     int64_t table_rows;
     int rotary, interleaved;
 };
 
+// How a lane's eight columns turn: y = n c + partner s for each, s with its sign.  Where nothing turns c = 1, s = 0.
 struct LaneTurn {
-    float c[8], s[8];  // interleaved: of the four pairs, in c[0..3], s[0..3]
-    int byte_lane;     // half-split: 4 * the partner's lane
-    bool turns;        // whether these columns turn
-    float sign;        // half-split: y = n c + sign * partner s
+    float c[8], s[8];
+    int byte_lane;      // half-split: 4 * the partner's lane
+    unsigned keep;      // all ones where the partner counts (an infinity times s = 0 is no zero)
+    bool turns, first;  // whether these columns turn; half-split: whether they are in front of their partners
 
     // Everything that does not depend on the row.
-    __device__ __forceinline__ void lane(const Turn& t, int col0) {
-        const int half = t.rotary >> 1, me = threadIdx.x & 63;
-        turns = col0 < t.rotary;
-        byte_lane = 4 * me;
-        sign = -1.f;
-        if (!t.interleaved && turns) {
-            const bool first = col0 < half;
-            byte_lane = 4 * (me + (first ? half >> 3 : -(half >> 3)));
-            sign = first ? -1.f : 1.f;
-        }
-    }
-    // Cosines and sines of position `pos`; false (and zeros) where it is not in the table.
-    __device__ __forceinline__ bool row(const Turn& t, int64_t pos, int col0) {
-        const bool there = pos >= 0 && pos < t.table_rows;
+    // `l`: number of the lane in its group (its columns may be another lane's, see the kernels).
+    __device__ __forceinline__ void lane(const Turn& t, int col0, int l) {
+        const int half = t.rotary >> 1, group = (threadIdx.x & 63) - l;
+        turns = col0 < t.rotary, first = col0 < half;
+        byte_lane = 4 * (group + ((turns && !t.interleaved ? (first ? col0 + half : col0 - half) : col0) >> 3));
+        keep = turns ? ~0u : 0u;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = s[i] = 0.f;
-        if (!turns || !there) return there;
+        for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
+    }
+    // Cosines and sines of position `pos`; false where it is not in the table.
+    __device__ __forceinline__ bool row(const Turn& t, int64_t pos, int col0) {
+        if (pos < 0 || pos >= t.table_rows) return false;
+        if (!turns) return true;
         const int half = t.rotary >> 1;
-        const float* cp = t.table + pos * t.rotary + (t.interleaved ? col0 >> 1 : (col0 < half ? col0 : col0 - half));
+        const float* cp = t.table + pos * t.rotary + (t.interleaved ? col0 >> 1 : (first ? col0 : col0 - half));
         typedef __attribute__((ext_vector_type(4))) float f4;
         const f4 c0 = *(const f4*)cp, s0 = *(const f4*)(cp + half);
+        if (t.interleaved) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = c0[i], s[i] = s0[i];
-        if (!t.interleaved) {
+            for (int i = 0; i < 4; ++i) c[2 * i] = c[2 * i + 1] = c0[i], s[2 * i] = -s0[i], s[2 * i + 1] = s0[i];
+        } else {
             const f4 c1 = *(const f4*)(cp + 4), s1 = *(const f4*)(cp + half + 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[4 + i] = c1[i], s[4 + i] = s1[i];
+            for (int i = 0; i < 4; ++i) {
+                c[i] = c0[i], c[4 + i] = c1[i];
+                s[i] = first ? -s0[i] : s0[i], s[4 + i] = first ? -s1[i] : s1[i];
+            }
         }
         return true;
     }
 };
 
-// y = R n for a lane's columns; `p`: the partners' columns (half-split only).  BACK: R^T.
-template <bool BACK>
-__device__ __forceinline__ void turn(const LaneTurn& t, int interleaved, const float (&n)[8], const float (&p)[8], float (&y)[8]) {
-    if (!t.turns) {
+// The partners of a lane's columns.
+template <class T>
+__device__ __forceinline__ void partners(const LaneTurn& t, int interleaved, const Cols<T>& in, const float (&x)[8], float (&p)[8]) {
+    if (interleaved) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = n[i];
-    } else if (interleaved) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float s = BACK ? -t.s[i] : t.s[i];
-            y[2 * i] = n[2 * i] * t.c[i] - n[2 * i + 1] * s;
-            y[2 * i + 1] = n[2 * i + 1] * t.c[i] + n[2 * i] * s;
-        }
+        for (int i = 0; i < 8; ++i) p[i] = __uint_as_float(__float_as_uint(x[i ^ 1]) & t.keep);
     } else {
-        const float sign = BACK ? -t.sign : t.sign;
+        Cols<T> o = in.from_lane(t.byte_lane);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = n[i] * t.c[i] + sign * (p[i] * t.s[i]);
+        for (int i = 0; i < Cols<T>::WORDS; ++i) o.w[i] &= t.keep;
+        o.get(p);
     }
 }
 
-// The weights of a lane's columns and of their partners; ones without a norm.
+// The weights of a lane's columns, ones without a norm.
 template <class T>
-__device__ __forceinline__ void lane_weights(const T* weight, int col0, bool there, const LaneTurn& t, float (&w)[8], float (&wp)[8]) {
+__device__ __forceinline__ void lane_weights(const T* weight, int col0, float (&w)[8]) {
     if (weight) {
         Cols<T> c;
-        c.zero();
-        if (there) c.load(weight + col0);
+        c.load(weight + col0);
         c.get(w);
-        c.from_lane(t.byte_lane).get(wp);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = wp[i] = 1.f;
+        for (int i = 0; i < 8; ++i) w[i] = 1.f;
     }
 }
+
+// Norm and turn as one: y = r (x cw + partner sw), the weights gone into cosines and sines (a partner's weight into its sine), which
+// the heads of a row share.
+struct NormTurn {
+    float cw[8], sw[8];
+    template <class T>
+    __device__ __forceinline__ void fill(const LaneTurn& t, int interleaved, const T* weight, int col0) {
+        if (weight) {
+            float w[8], wp[8];
+            lane_weights(weight, col0, w);
+            Cols<T> raw;
+            raw.put(w);
+            partners(t, interleaved, raw, w, wp);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) cw[i] = t.c[i] * w[i], sw[i] = t.s[i] * wp[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) cw[i] = t.c[i], sw[i] = t.s[i];
+        }
+    }
+    // A vector as loaded to what is rounded and stored; `known`: whether its position is.
+    // `there`: whether the lane's columns are the vector's (one that has none holds another's).
+    template <class T, int LPV>
+    __device__ __forceinline__ void apply(const LaneTurn& t, int interleaved, const Cols<T>& in, bool there, bool norm, float inv_dim, float eps, bool known,
+                                          float (&y)[8]) const {
+        float x[8], p[8];
+        in.get(x);
+        partners(t, interleaved, in, x, p);
+        float r = 1.f;
+        if (norm) {
+            float sq = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sq += x[i] * x[i];
+            r = rsqrtf(group_sum<LPV>(there ? sq : 0.f) * inv_dim + eps);
+        }
+        if (!known) r = __builtin_nanf("");
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = r * (x[i] * cw[i] + p[i] * sw[i]);
+    }
+};
 
 // One side (q or k) of the step.
 struct NormRopeSide {
@@ -195,16 +238,18 @@ struct NormRopeParams {
 template <class T, int LPV>
 __global__ __launch_bounds__(256) void hstu_norm_rope_kernel(const NormRopeParams p) {
     constexpr int GROUPS = 256 / LPV, AHEAD = 4;
-    const int l = threadIdx.x % LPV, col0 = 8 * l;
-    const int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LPV;
-    const bool there = col0 < p.dim && row < p.rows;
+    // Lanes without columns, and groups without a row, go along with the last of them that there are and store nothing: loads need no
+    // condition then.
+    const int l = threadIdx.x % LPV;
+    const bool cols = 8 * l < p.dim;
+    const int col0 = cols ? 8 * l : p.dim - 8;
+    int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LPV;
+    const bool there = cols && row < p.rows;
+    if (row >= p.rows) row = p.rows - 1;
     LaneTurn t;
-    t.lane(p.turn, col0);
+    t.lane(p.turn, col0, l);
     bool known = true;
-    if (p.turn.rotary) {
-        const int64_t pos = row < p.rows ? index_at(p.positions, p.positions_i64, row) : 0;
-        known = t.row(p.turn, pos, col0);
-    }
+    if (p.turn.rotary) known = t.row(p.turn, index_at(p.positions, p.positions_i64, row), col0);
     const int first = blockIdx.y * p.heads_per_group, last = min(first + p.heads_per_group, p.side[0].heads + p.side[1].heads);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
@@ -212,35 +257,22 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_kernel(const NormRopeParam
         const int base = which ? p.side[0].heads : 0;
         const int h0 = max(first - base, 0), h1 = min(last - base, s.heads);
         if (h0 >= h1) continue;
-        float w[8], wp[8];
-        lane_weights((const T*)s.weight, col0, col0 < p.dim, t, w, wp);
+        NormTurn nt;
+        nt.fill(t, p.turn.interleaved, (const T*)s.weight, col0);
+        const T* x = (const T*)s.x + row * s.rs + col0;
+        T* out = (T*)s.y + row * s.heads * p.dim + col0;
         for (int h = h0; h < h1; h += AHEAD) {
             Cols<T> in[AHEAD];
 #pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                in[a].zero();
-                if (there && h + a < h1) in[a].load((const T*)s.x + row * s.rs + (int64_t)(h + a) * s.hs + col0);
-            }
+            for (int a = 0; a < AHEAD; ++a) in[a].load(x + (int64_t)min(h + a, h1 - 1) * s.hs);
 #pragma unroll
             for (int a = 0; a < AHEAD; ++a) {
                 if (h + a >= h1) break;  // (the same for the whole workgroup)
-                float x[8], q[8], y[8];
-                in[a].get(x);
-                in[a].from_lane(t.byte_lane).get(q);
-                float r = 1.f;
-                if (s.weight) {
-                    float sq = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) sq += x[i] * x[i];
-                    r = rsqrtf(group_sum<LPV>(sq) * p.inv_dim + p.eps);
-                }
-                if (!known) r = __builtin_nanf("");
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i], q[i] = q[i] * r * wp[i];
-                turn<false>(t, p.turn.interleaved, x, q, y);
-                Cols<T> out;
-                out.put(y);
-                if (there) out.store((T*)s.y + (row * s.heads + h + a) * p.dim + col0);
+                float y[8];
+                nt.apply<T, LPV>(t, p.turn.interleaved, in[a], cols, s.weight != nullptr, p.inv_dim, p.eps, known, y);
+                Cols<T> o;
+                o.put(y);
+                if (there) o.store(out + (h + a) * p.dim);
             }
         }
     }
@@ -252,24 +284,23 @@ template <class T, int LPV>
 __global__ __launch_bounds__(256) void hstu_norm_rope_bwd_kernel(const NormRopeParams p) {
     constexpr int GROUPS = 256 / LPV, AHEAD = 2;
     __shared__ float meet[256 * 8];
-    const int l = threadIdx.x % LPV, col0 = 8 * l;
-    const int64_t row0 = (int64_t)blockIdx.x * GROUPS;
+    const int l = threadIdx.x % LPV;
+    const bool cols = 8 * l < p.dim;  // (as in the forward)
+    const int col0 = cols ? 8 * l : p.dim - 8;
     LaneTurn t;
-    t.lane(p.turn, col0);
+    t.lane(p.turn, col0, l);
     const int first = blockIdx.y * p.heads_per_group, last = min(first + p.heads_per_group, p.side[0].heads + p.side[1].heads);
     float sum[2][8];
 #pragma unroll
     for (int which = 0; which < 2; ++which)
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum[which][i] = 0.f;
-    for (int64_t base_row = row0; base_row < p.rows; base_row += (int64_t)gridDim.x * GROUPS) {
-        const int64_t row = base_row + threadIdx.x / LPV;
-        const bool there = col0 < p.dim && row < p.rows;
+    for (int64_t base_row = (int64_t)blockIdx.x * GROUPS; base_row < p.rows; base_row += (int64_t)gridDim.x * GROUPS) {
+        int64_t row = base_row + threadIdx.x / LPV;
+        const bool there = cols && row < p.rows;
+        if (row >= p.rows) row = p.rows - 1;
         bool known = true;
-        if (p.turn.rotary) {
-            const int64_t pos = row < p.rows ? index_at(p.positions, p.positions_i64, row) : 0;
-            known = t.row(p.turn, pos, col0);
-        }
+        if (p.turn.rotary) known = t.row(p.turn, index_at(p.positions, p.positions_i64, row), col0);
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             const NormRopeSide& s = p.side[which];
@@ -277,54 +308,52 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_bwd_kernel(const NormRopeP
             const int h0 = max(first - base, 0), h1 = min(last - base, s.heads);
             if (h0 >= h1) continue;
             float w[8];
-            {
-                Cols<T> c;
-                c.zero();
-                if (s.weight && col0 < p.dim) c.load((const T*)s.weight + col0);
-                c.get(w);
-            }
+            lane_weights((const T*)s.weight, col0, w);
+            const T* x_of = (const T*)s.x + row * s.rs + col0;
+            const T* dy_of = (const T*)s.dy + row * s.dy_rs + col0;
+            T* dx_of = (T*)s.dx + row * s.heads * p.dim + col0;
             for (int h = h0; h < h1; h += AHEAD) {
                 Cols<T> in[AHEAD], dy[AHEAD];
 #pragma unroll
                 for (int a = 0; a < AHEAD; ++a) {
-                    in[a].zero(), dy[a].zero();
-                    if (there && h + a < h1) {
-                        dy[a].load((const T*)s.dy + row * s.dy_rs + (int64_t)(h + a) * s.dy_hs + col0);
-                        if (s.weight) in[a].load((const T*)s.x + row * s.rs + (int64_t)(h + a) * s.hs + col0);
-                    }
+                    const int64_t at = min(h + a, h1 - 1);
+                    dy[a].load(dy_of + at * s.dy_hs);
+                    if (s.weight) in[a].load(x_of + at * s.hs);
                 }
 #pragma unroll
                 for (int a = 0; a < AHEAD; ++a) {
                     if (h + a >= h1) break;
                     float x[8], d[8], q[8], g[8];
                     dy[a].get(d);
-                    dy[a].from_lane(t.byte_lane).get(q);
-                    turn<true>(t, p.turn.interleaved, d, q, g);
+                    partners(t, p.turn.interleaved, dy[a], d, q);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) g[i] = d[i] * t.c[i] - q[i] * t.s[i];  // R^T: the partner's sine is the other's with its sign changed
                     if (!known) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) g[i] = there ? __builtin_nanf("") : 0.f;
+                        for (int i = 0; i < 8; ++i) g[i] = __builtin_nanf("");
                     }
                     if (s.weight) {
                         in[a].get(x);
                         float sq = 0.f;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) sq += x[i] * x[i];
-                        const float r = rsqrtf(group_sum<LPV>(sq) * p.inv_dim + p.eps);
+                        const float r = rsqrtf(group_sum<LPV>(cols ? sq : 0.f) * p.inv_dim + p.eps);
                         float dot = 0.f;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             x[i] *= r;
-                            sum[which][i] += g[i] * x[i];
+                            const float term = g[i] * x[i];
+                            sum[which][i] += there ? term : 0.f;
+                            dot += term * w[i];
                             g[i] *= w[i];
-                            dot += g[i] * x[i];
                         }
-                        const float m = group_sum<LPV>(dot) * p.inv_dim;
+                        const float m = group_sum<LPV>(cols ? dot : 0.f) * p.inv_dim;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) g[i] = r * (g[i] - x[i] * m);
                     }
                     Cols<T> out;
                     out.put(g);
-                    if (there) out.store((T*)s.dx + (row * s.heads + h + a) * p.dim + col0);
+                    if (there) out.store(dx_of + (h + a) * p.dim);
                 }
             }
         }
@@ -335,7 +364,7 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_bwd_kernel(const NormRopeP
         if (!p.side[which].dw) continue;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) meet[(threadIdx.x / LPV) * (LPV * 8) + col0 + i] = sum[which][i];
+        for (int i = 0; i < 8; ++i) meet[(threadIdx.x / LPV) * (LPV * 8) + 8 * l + i] = sum[which][i];
         __syncthreads();
         for (int col = threadIdx.x; col < p.dim; col += 256) {
             float v = 0.f;
@@ -345,24 +374,42 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_bwd_kernel(const NormRopeP
     }
 }
 
-// dw[col] = sum over workgroups of partial[workgroup][which][col]: 16 columns to a workgroup, 16 lanes to a column.
+// dw[col] = sum over workgroups of partial[workgroup][which][col]: 16 columns to a workgroup, as four lanes of four, and 64 parts of
+// the workgroups' sums, four of them in flight.  (With 16 parts of single columns, one load in flight, 2048 sums took 53 us.)
 template <class T>
 __global__ __launch_bounds__(256) void hstu_norm_rope_dw_kernel(const float* partial, int64_t workgroups, int dim, T* dq_weight, T* dk_weight) {
-    __shared__ float meet[16][17];
-    const int c = threadIdx.x & 15, part = threadIdx.x >> 4, which = blockIdx.y;
-    const int col = blockIdx.x * 16 + c;
+    typedef __attribute__((ext_vector_type(4))) float f4;
+    __shared__ float meet[64][17];
+    const int c = threadIdx.x & 3, part = threadIdx.x >> 2, which = blockIdx.y;
+    const int col = blockIdx.x * 16 + 4 * c;
     T* out = which ? dk_weight : dq_weight;
     if (!out) return;
-    float v = 0.f;
-    if (col < dim)
-        for (int64_t w = part; w < workgroups; w += 16) v += partial[(w * 2 + which) * dim + col];
-    meet[part][c] = v;
-    __syncthreads();
-    if (part == 0 && col < dim) {
-        float total = 0.f;
+    f4 v = {0, 0, 0, 0};
+    if (col < dim) {  // (a multiple of 8)
+        const float* from = partial + which * dim + col;
+        int64_t w = part;
+        for (; w + 192 < workgroups; w += 256) {
+            f4 x[4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) total += meet[i][c];
-        out[col] = (T)total;
+            for (int i = 0; i < 4; ++i) x[i] = *(const f4*)(from + (w + 64 * i) * 2 * dim);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v += x[i];
+        }
+        for (; w < workgroups; w += 64) v += *(const f4*)(from + w * 2 * dim);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) meet[part][4 * c + i] = v[i];
+    __syncthreads();
+    const int one = threadIdx.x & 15, lane16 = threadIdx.x >> 4;
+    float total = meet[lane16][one] + meet[lane16 + 16][one] + meet[lane16 + 32][one] + meet[lane16 + 48][one];
+    __syncthreads();
+    meet[lane16][one] = total;
+    __syncthreads();
+    if (threadIdx.x < 16 && blockIdx.x * 16 + threadIdx.x < dim) {
+        total = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) total += meet[i][threadIdx.x];
+        out[blockIdx.x * 16 + threadIdx.x] = (T)total;
     }
 }
 

@@ -1,7 +1,7 @@
 // Rows into and out of a K/V cache that holds them in 4 bits, in pages: bound by HBM bandwidth.
 //
 // The lanes are laid out as in hstu_norm_rope.h, eight columns to a lane, so that a lane's codes are one word of the row.  The
-// extremes of a row are log2(LPV) lane exchanges.  Codes are found by a division that is rounded as IEEE says, so that a tie between
+// extremes of a row are log2(LPV) lane exchanges.  Codes are found by a quotient that is rounded as IEEE says, so that a tie between
 // two codes (K and V have 8 or 11 bits, a step too: ties do occur) falls the same way on any machine.
 #pragma once
 #include "hstu_norm_rope.h"
@@ -85,105 +85,121 @@ __device__ __forceinline__ int64_t cache_row(const PagedCache& c, int b, int64_t
     return ((page * c.heads) << c.page_shift) + (place & ((1 << c.page_shift) - 1));
 }
 
-// Eight columns (of LPV lanes' row; lanes behind the row's end have `there` false) to a word of codes, and step and lowest value.
+// Smallest and largest of eight columns, NaN where one is; and over LPV lanes (numbers only).  The instructions themselves: the
+// compiler puts another in front of each operand of its min and max, to quiet NaNs.
+__device__ __forceinline__ void extremes(const float (&x)[8], float& lo, float& hi) {
+    asm("v_minimum3_f32 %0, %2, %3, %4\n\tv_maximum3_f32 %1, %2, %3, %4\n\t"
+        "v_minimum3_f32 %0, %0, %5, %6\n\tv_maximum3_f32 %1, %1, %5, %6\n\t"
+        "v_minimum3_f32 %0, %0, %7, %8\n\tv_maximum3_f32 %1, %1, %7, %8\n\t"
+        "v_minimum3_f32 %0, %0, %9, %9\n\tv_maximum3_f32 %1, %1, %9, %9"
+        : "=&v"(lo), "=&v"(hi)
+        : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]), "v"(x[7]));
+}
+#define HSTU_EXTREMES_DPP(how)                                                                                                              \
+    asm("s_nop 1\n\tv_min_f32_dpp %0, %0, %0 " how " row_mask:0xf bank_mask:0xf\n\tv_max_f32_dpp %1, %1, %1 " how " row_mask:0xf bank_mask:0xf" \
+        : "+v"(lo), "+v"(hi))
+template <int LPV>
+__device__ __forceinline__ void group_extremes(float& lo, float& hi) {
+    static_assert(LPV >= 4 && LPV <= 32, "lanes of a cache's row");
+    HSTU_EXTREMES_DPP("quad_perm:[1,0,3,2]");
+    HSTU_EXTREMES_DPP("quad_perm:[2,3,0,1]");
+    if constexpr (LPV >= 8) HSTU_EXTREMES_DPP("row_half_mirror");
+    if constexpr (LPV >= 16) HSTU_EXTREMES_DPP("row_mirror");
+    if constexpr (LPV >= 32) lo = fminf(lo, __shfl_xor(lo, 16, 64)), hi = fmaxf(hi, __shfl_xor(hi, 16, 64));
+}
+#undef HSTU_EXTREMES_DPP
+
+// Eight columns of LPV lanes' row to a word of codes, and step and lowest value.  (Lanes behind the row's end hold other columns of it.)
+// The quotient x / step is rounded as IEEE says by Markstein's correction: q = a y with y the reciprocal of b to a unit in the last
+// place, then q + (a - q b) y, whose remainder is exact; three operations a column where the compiler's division takes some fourteen.
+// It is exact where the quotient is a float, which a tie between two codes is.
 template <class T, int LPV>
-__device__ __forceinline__ unsigned to_four_bits(const float (&x)[8], bool there, unsigned& scale) {
-    float lo = __builtin_inff(), hi = -__builtin_inff();
-    bool odd = false;
-    if (there) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            lo = fminf(lo, x[i]), hi = fmaxf(hi, x[i]);
-            odd |= !(x[i] - x[i] == 0.f);
-        }
-    }
-#pragma unroll
-    for (int d = LPV / 2; d >= 1; d >>= 1) lo = fminf(lo, __shfl_xor(lo, d, 64)), hi = fmaxf(hi, __shfl_xor(hi, d, 64));
+__device__ __forceinline__ unsigned to_four_bits(const float (&x)[8], unsigned& scale) {
+    float lo, hi;
+    extremes(x, lo, hi);
     const int me = threadIdx.x & 63;
     const uint64_t group = ((1ull << LPV) - 1) << (me - me % LPV);
+    const bool nan = (__ballot(lo != lo) & group) != 0;
+    group_extremes<LPV>(lo, hi);
     // (half of everything, which is exact, so that the range of a row of large values is a float)
-    const float lo2 = 0.5f * lo;
-    T step_t = (T)((0.5f * hi - lo2) / 7.5f), lo_t = (T)lo;
+    const float range = 0.5f * hi - 0.5f * lo, fifteenth = range * (1.f / 7.5f);
+    T step_t = (T)__builtin_fmaf(__builtin_fmaf(-fifteenth, 7.5f, range), 1.f / 7.5f, fifteenth), lo_t = (T)lo;
     const float step = (float)step_t;
-    if ((__ballot(odd) & group) != 0 || !(step - step == 0.f)) step_t = lo_t = (T)__builtin_nanf("");
+    if (nan || !(step - step == 0.f)) step_t = lo_t = (T)__builtin_nanf("");
     typedef __attribute__((ext_vector_type(2))) T T2;
     T2 both;
     both[0] = step_t, both[1] = lo_t;
     scale = __builtin_bit_cast(unsigned, both);
-    unsigned codes = 0;
-    if (step > 0.f) {
-        const float step2 = 0.5f * step;
+    if (!(step > 0.f)) return 0;
+    // step and columns by a power of two that takes the step to 1/2 .. 1, or some way there from below 2^-100
+    const float by = __builtin_amdgcn_ldexpf(1.f, -max(__builtin_amdgcn_frexp_expf(step), -100) - 1), from = -lo * by, b = step * by;
+    const float y0 = __builtin_amdgcn_rcpf(b), y = __builtin_fmaf(__builtin_fmaf(-b, y0, 1.f), y0, y0);
+    float code[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float c = fminf(fmaxf(rintf(__builtin_fmaf(x[i], 0.5f, -lo2) / step2), 0.f), 15.f);
-            codes |= (unsigned)c << (4 * i);
-        }
+    for (int i = 0; i < 8; ++i) {
+        const float a = __builtin_fmaf(x[i], by, from), q = a * y;
+        code[i] = __builtin_amdgcn_fmed3f(__builtin_rintf(__builtin_fmaf(__builtin_fmaf(-q, b, a), y, q)), 0.f, 15.f);
     }
-    return codes;
+    // four codes are one number below 2^16, exact in a float
+    const float low = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(code[3], 16.f, code[2]), 16.f, code[1]), 16.f, code[0]);
+    const float high = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(code[7], 16.f, code[6]), 16.f, code[5]), 16.f, code[4]);
+    return (unsigned)low | ((unsigned)high << 16);
 }
 
 // grid (rows / groups of a workgroup, vectors / vectors_per_group): a row's vectors count through its heads of K, then of V.
 template <class T, int LPV>
 __global__ __launch_bounds__(256) void hstu_paged_append_kernel(const AppendParams p) {
     constexpr int GROUPS = 256 / LPV, AHEAD = 4;
-    const int l = threadIdx.x % LPV, col0 = 8 * l;
-    const int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LPV;
+    const int l = threadIdx.x % LPV;
     const PagedCache& c = p.cache;
-    int64_t place = 0;
+    int64_t row = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LPV, place = 0;
     const int b = find_sequence<LPV>(p.place, c.batch, row, place);
     const int64_t to = cache_row(c, b, place);
     const bool stored = to >= 0;
+    if (row >= p.place.rows) row = p.place.rows - 1;  // (loads need no condition; nothing is stored)
     const int first = blockIdx.y * p.vectors_per_group, last = min(first + p.vectors_per_group, 2 * c.heads);
-    LaneTurn t;
-    t.lane(p.turn, col0);
-    bool known = true;
-    if (p.turn.rotary && first < c.heads && stored) known = t.row(p.turn, p.positions ? index_at(p.positions, p.positions_i64, row) : place, col0);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         const int base = which ? c.heads : 0, h0 = max(first - base, 0), h1 = min(last - base, c.heads);
         if (h0 >= h1) continue;
         const int dim = which ? c.dv : c.dqk;
-        const bool there = stored && col0 < dim;
+        const bool cols = 8 * l < dim;
+        const int col0 = cols ? 8 * l : dim - 8;
         const T* x_of = (const T*)(which ? p.v : p.k) + row * (which ? p.v_rs : p.k_rs) + col0;
         const int64_t hs = which ? p.v_hs : p.k_hs;
         unsigned* codes_of = (unsigned*)(which ? c.v_codes : c.k_codes);
         unsigned* scales_of = (unsigned*)(which ? c.v_scales : c.k_scales);
-        float w[8], wp[8];
-        if (!which) lane_weights((const T*)p.k_weight, col0, col0 < dim, t, w, wp);
+        const bool changed = !which && (p.k_weight || p.turn.rotary);
+        LaneTurn t;
+        NormTurn nt;
+        bool known = true;
+        if (changed) {
+            t.lane(p.turn, col0, l);
+            if (p.turn.rotary && stored) known = t.row(p.turn, p.positions ? index_at(p.positions, p.positions_i64, row) : place, col0);
+            nt.fill(t, p.turn.interleaved, (const T*)p.k_weight, col0);
+        }
         for (int h = h0; h < h1; h += AHEAD) {
             Cols<T> in[AHEAD];
 #pragma unroll
-            for (int a = 0; a < AHEAD; ++a) {
-                in[a].zero();
-                if (there && h + a < h1) in[a].load(x_of + (h + a) * hs);
-            }
+            for (int a = 0; a < AHEAD; ++a) in[a].load(x_of + min(h + a, h1 - 1) * hs);
 #pragma unroll
             for (int a = 0; a < AHEAD; ++a) {
                 if (h + a >= h1) break;  // (the same for the whole workgroup)
                 float x[8];
-                in[a].get(x);
-                if (!which && (p.k_weight || p.turn.rotary)) {
-                    float q[8], y[8], r = 1.f;
-                    in[a].from_lane(t.byte_lane).get(q);
-                    if (p.k_weight) {
-                        float sq = 0.f;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) sq += x[i] * x[i];
-                        r = rsqrtf(group_sum<LPV>(sq) * p.inv_dim + p.eps);
-                    }
-                    if (!known) r = __builtin_nanf("");
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i], q[i] = q[i] * r * wp[i];
-                    turn<false>(t, p.turn.interleaved, x, q, y);
+                if (changed) {
+                    float y[8];
+                    nt.apply<T, LPV>(t, p.turn.interleaved, in[a], cols, p.k_weight != nullptr, p.inv_dim, p.eps, known, y);
                     Cols<T> rounded;
                     rounded.put(y);
                     rounded.get(x);
+                } else {
+                    in[a].get(x);
                 }
                 unsigned scale;
-                const unsigned codes = to_four_bits<T, LPV>(x, col0 < dim, scale);
+                const unsigned codes = to_four_bits<T, LPV>(x, scale);
                 const int64_t at = to + ((int64_t)(h + a) << c.page_shift);
-                if (there) codes_of[at * (dim >> 3) + l] = codes;
-                if (there && l == 0) scales_of[at] = scale;
+                if (stored && cols) codes_of[at * (dim >> 3) + l] = codes;
+                if (stored && l == 0) scales_of[at] = scale;
             }
         }
     }

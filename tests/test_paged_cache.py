@@ -254,6 +254,20 @@ def test_norm_rope_positions_outside_of_the_table_and_partial_gradients(pkg, dev
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_norm_rope_leaves_an_infinity_where_it_is(pkg, dev, interleaved):
+    """Columns that do not turn are what they were, infinities too; those that turn with one are not numbers or infinite."""
+    print(f"[case] norm and rotation: an infinity {interleaved}", flush=True)
+    q, _, pos, table, *_ = _norm_rope_inputs((6, 2, 1, 64, 32, interleaved, False, BF16))
+    q[2, 1, 40], q[3, 0, 4] = float("inf"), float("-inf")
+    got = pkg.qk_norm_rope(q.to(dev), None, pos.to(dev), table.to(dev), interleaved=interleaved)[0].cpu()
+    assert torch.equal(got[..., 32:], q[..., 32:])
+    pair = [4, 5 if interleaved else 20]
+    rest = [i for i in range(32) if i not in pair]
+    assert not torch.isfinite(got[3, 0, pair]).any() and torch.isfinite(got[3, 0, rest]).all() and torch.isfinite(got[2, 1, :32]).all()
+
+
+@pytest.mark.gpu
 def test_norm_rope_refusals(pkg, dev):
     q, k, pos, table, qw, kw, _ = _norm_rope_inputs((12, 2, 1, 32, 32, False, True, BF16))
     q, k, pos, table, qw, kw = _to(dev, q, k, pos, table, qw, kw)
@@ -365,6 +379,7 @@ def test_rows_without_a_place(pkg, dev, monkeypatch):
     k, v = _rand(1, (45, heads, dim), BF16), _rand(2, (45, heads, dim), BF16)
     k[3, 0, 5], k[4, 1, 0], k[5, 0] = float("nan"), float("inf"), 3.0
     v[6, 1, :2], v[7, 0, :2] = torch.tensor([-3e38, 3e38]), torch.tensor([1e-38, 1e-40])
+    v[8], v[9], k[10], k[11] = v[8] * 1e-38, v[9] * 1e-30, k[10] * 1e30, 1 + k[11] / 300  # steps below the normal numbers, far ones, few of them
     cache = O.fill_cache(3, 5, heads, page, dim, dim, BF16)
     on = [c.to(dev) for c in cache]
     args = _to(dev, table, start)
