@@ -6,8 +6,9 @@
 namespace {
 
 struct Plan {
-    int mt, rw;        // 16-row tiles of a wave, waves that share out the rows
-    int row_blocks, splits;
+    int step;          // rows of the kernel for few (1, 2, 4 or 8), or 0
+    int mt, rw;        // else: 16-row tiles of a wave, waves that share out the rows
+    int block, row_blocks, splits, run, share;
     int64_t workspace;
 };
 
@@ -25,25 +26,38 @@ int check(const HstuPagedCache* c, const HstuPagedAttentionArgs* a, hstu::PagedA
 }
 
 Plan plan_of(const HstuPagedCache* c, const HstuPagedAttentionArgs* a) {
-    Plan p{1, 1, 1, 1, 0};
+    Plan p{0, 1, 1, 16, 1, 1, 1, 4, 0};
     const int64_t rows = (int64_t)a->delta_size * (a->q_heads / c->heads);
-    if (rows > 16) p.mt = c->dv == 256 ? 1 : 2;
-    if (rows > 16 * p.mt) p.rw = 4;
-    const int block = 16 * p.mt * p.rw;
-    p.row_blocks = (int)((rows + block - 1) / block);
+    if (rows <= 8) {
+        p.step = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
+        p.block = p.step;
+    } else {
+        if (rows > 16) p.mt = c->dv == 256 ? 1 : 2;
+        if (rows > 16 * p.mt) p.rw = 4;
+        p.block = 16 * p.mt * p.rw;
+    }
+    p.row_blocks = (int)((rows + p.block - 1) / p.block);
     int64_t longest = a->max_seq_len;
     if (a->max_attn_len > 0 && (int64_t)a->max_attn_len + a->delta_size + a->contextual_seq_len < longest)
         longest = (int64_t)a->max_attn_len + a->delta_size + a->contextual_seq_len;
-    const int64_t chunks = (longest + 31) / 32, wgs = (int64_t)p.row_blocks * c->heads * c->batch;
-    const int64_t most = (chunks + 15) / 16;
-    int64_t splits = a->kv_splits > 0 ? a->kv_splits : wgs > 0 ? (2048 + wgs - 1) / wgs : 1;
-    if (splits > most) splits = most;
-    if (splits > 64) splits = 64;
-    if (splits < 1) splits = 1;
-    p.splits = (int)splits;
-    if (splits > 1) p.workspace = splits * c->batch * a->delta_size * a->q_heads * (int64_t)c->dv * 4;
+    const int64_t chunks = (longest + 31) / 32 + 1, wgs = (int64_t)p.row_blocks * c->heads * c->batch;
+    // Runs of a step: as many workgroups as the card holds at once (two of a CU), for each begins with some microseconds of loads that wait
+    // for each other (64 sequences of 1024 .. 4096 positions and four heads, 256 workgroups for whole sequences: runs of 129 chunks, all of one, 28 us,
+    // of 80 26, of 16 35), but none so long that the last of them run alone (128 sequences of up to 16384 and eight heads: runs of 513 290 us, of 384 262,
+    // of 64 286).  Sequences of a few chunks, more of them than fit, are a wave's each (1600 of up to 10 chunks: 12.5 us, 16 by workgroups).
+    const int64_t fill = (chunks * wgs + 511) / 512;
+    int64_t run = a->kv_splits > 0 ? (chunks + a->kv_splits - 1) / a->kv_splits : (fill + 15) / 16 * 16;
+    if (!a->kv_splits && run > 384) run = 384;
+    if (run < 16) run = 16;
+    if (p.step && chunks <= 17 && wgs > 1024) p.share = 1, run = chunks;
+    if (run > chunks) run = chunks;
+    p.run = (int)run;
+    p.splits = (int)((chunks + run - 1) / run);
+    if (p.splits > 1) p.workspace = p.splits * c->batch * a->delta_size * a->q_heads * (int64_t)c->dv * 4;
     return p;
 }
+
+typedef std::integral_constant<int, 1> One;
 
 template <class TT, int DK, int DV>
 int launch_sized(const hstu::PagedAttentionParams& p, const Plan& plan, hipStream_t stream) {
@@ -51,16 +65,27 @@ int launch_sized(const hstu::PagedAttentionParams& p, const Plan& plan, hipStrea
     auto go = [&](auto mt, auto rw) {
         hipLaunchKernelGGL((hstu::hstu_paged_attention_kernel<TT, DK, DV, decltype(mt)::value, decltype(rw)::value>), dim3(blocks), dim3(256), 0, stream, p);
     };
-    typedef std::integral_constant<int, 1> One;
     typedef std::integral_constant<int, DV == 256 ? 1 : 2> Most;
     typedef std::integral_constant<int, 4> Four;
-    if (plan.rw == 4) go(Most{}, Four{});
+    auto step = [&](auto rp) {
+        hipLaunchKernelGGL((hstu::hstu_paged_step_kernel<TT, DK, DV, decltype(rp)::value>), dim3((unsigned)((p.items * p.share + 3) / 4)), dim3(256), 0, stream, p);
+    };
+    if (plan.step == 1) step(One{});
+    else if (plan.step == 2) step(std::integral_constant<int, 2>{});
+    else if (plan.step == 4) step(Four{});
+    else if (plan.step == 8) step(std::integral_constant<int, 8>{});
+    else if (plan.rw == 4) go(Most{}, Four{});
     else if (plan.mt == 1) go(One{}, One{});
     else if constexpr (DV != 256) go(Most{}, One{});
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && p.splits > 1) {
         const int64_t total8 = p.partial_stride / 8;
-        hipLaunchKernelGGL((hstu::hstu_paged_join_kernel<TT>), dim3((unsigned)((total8 + 255) / 256)), dim3(256), 0, stream, p, 16 * plan.mt * plan.rw, total8);
+        auto join = [&](auto parts) {
+            constexpr int P = decltype(parts)::value;
+            hipLaunchKernelGGL((hstu::hstu_paged_join_kernel<TT, P>), dim3((unsigned)((total8 * P + 255) / 256)), dim3(256), 0, stream, p, plan.block, total8);
+        };
+        if (p.splits > 4) join(std::integral_constant<int, 8>{});
+        else join(One{});
         e = hipGetLastError();
     }
     if (e == hipSuccess) return 0;
@@ -98,6 +123,7 @@ int hstu_cache_attention(const HstuPagedCache* c, const HstuPagedAttentionArgs* 
     if (rc) return rc;
     if (c->batch == 0 || a->delta_size == 0) return 0;
     if (c->pages == 0) return HSTU_ERR_BAD_SHAPE;
+    if (c->pages > 2147483647) return HSTU_ERR_UNSUPPORTED;
     if (!a->q || !a->out || !a->seq_lengths || !c->page_table) return HSTU_ERR_NULL_POINTER;
     if (!hstu_cache_aligned(a->q) || !hstu_cache_aligned(a->out)) return HSTU_ERR_MISALIGNED;
     if (a->q_row_stride < 0 || a->q_head_stride < 0 || a->q_row_stride % 8 != 0 || a->q_head_stride % 8 != 0) return HSTU_ERR_MISALIGNED;
@@ -115,7 +141,7 @@ int hstu_cache_attention(const HstuPagedCache* c, const HstuPagedAttentionArgs* 
     p.group = a->q_heads / c->heads, p.delta = a->delta_size, p.w = a->max_attn_len, p.c = a->contextual_seq_len;
     const float log2e = 1.4426950408889634f;
     p.c1 = -a->alpha * log2e, p.oscale = -1.f / (a->max_seq_len * log2e);
-    p.row_blocks = plan.row_blocks, p.splits = plan.splits, p.items = (int)items;
+    p.row_blocks = plan.row_blocks, p.splits = plan.splits, p.run = plan.run, p.share = plan.share, p.items = (int)items;
     p.partial = (float*)a->workspace, p.partial_stride = (int64_t)c->batch * a->delta_size * a->q_heads * c->dv;
     return c->dtype == HSTU_BF16 ? launch<hstu::PagedBf16>(p, plan, (hipStream_t)stream) : launch<hstu::PagedF16>(p, plan, (hipStream_t)stream);
 }

@@ -35,7 +35,8 @@ struct PagedAttentionParams {
     int lengths_i64, targets_i64;
     int group, delta, w, c;  // heads of q to one of the cache; max_attn_len, contextual_seq_len
     float c1, oscale;        // t = c1 <q, k> with c1 = -alpha log2(e);  out = oscale * sum t / (1 + 2^t) v
-    int row_blocks, splits, items;
+    int share;  // step kernel: waves to a run, 4 (a workgroup) or 1
+    int row_blocks, splits, run, items;  // run: chunks of one of the splits, at least
     float* partial;          // [splits][batch * delta][q heads][dv], used where splits > 1
     int64_t partial_stride;
 };
@@ -72,6 +73,9 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttentionParams& p, i
     return s;
 }
 
+// Chunks of a run: `run`, or more where a sequence is longer than it should be.
+__device__ __forceinline__ int chunks_per_run(const PagedAttentionParams& p, int chunks) { return max(p.run, (chunks + p.splits - 1) / p.splits); }
+
 // What one row sees: positions [lo, hi), [0, chi) and itself.
 struct RowSpan {
     int lo, hi, chi, self;
@@ -98,22 +102,54 @@ __device__ __forceinline__ RowSpan row_span(const PagedAttentionParams& p, const
     return r;
 }
 
-// Codes as the floats OFF + code, two to a word: column k and column k + 4 of a word of eight, k = 0 .. 3.
+// Codes as the floats OFF + code, two to a word: column k and column k + 4 of a word of eight, k = 0 .. 3.  AND and OR are one
+// instruction, which takes one scalar and no literal: mask and offset are kept in a scalar and a vector register, and their values from the
+// compiler, which would make two instructions with literals of it.  (The instruction itself in an asm block is no way: a product that
+// reads its result needs wait states that the compiler does not count there.)
+__device__ __forceinline__ unsigned kept_scalar(unsigned x) {
+    asm("" : "+s"(x));
+    return x;
+}
+__device__ __forceinline__ unsigned kept_vector(unsigned x) {
+    asm("" : "+v"(x));
+    return x;
+}
+// Rows that are the same for all lanes, read at a lane's 32-bit offset: by buffer loads, which add the two themselves (with global loads the
+// compiler spends two registers and two instructions on each address).  The rows end `bytes` behind the pointer.
+typedef __attribute__((ext_vector_type(2))) unsigned u32x2_t;
+struct UniformRows {
+    __amdgpu_buffer_rsrc_t r;
+    __device__ __forceinline__ UniformRows(const char* rows, unsigned bytes)
+        : r(__builtin_amdgcn_make_buffer_rsrc((void*)rows, 0, (int)bytes, 0x00027000)) {}
+    template <class V>
+    __device__ __forceinline__ V at(unsigned offset) const {
+        if constexpr (sizeof(V) == 16) return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(r, (int)offset, 0, 0));
+        else if constexpr (sizeof(V) == 8) return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b64(r, (int)offset, 0, 0));
+        else if constexpr (sizeof(V) == 4) return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b32(r, (int)offset, 0, 0));
+        else if constexpr (sizeof(V) == 2) return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b16(r, (int)offset, 0, 0));
+        else return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b8(r, (int)offset, 0, 0));
+    }
+};
 struct CodesBf16 {  // 128 + code where the code lies at bit 0, 16 + code from bit 3
-    static __device__ __forceinline__ void four(unsigned w, unsigned (&o)[4]) {
-        o[0] = (w & 0x000F000Fu) | 0x43004300u;
-        o[1] = ((w >> 1) & 0x00780078u) | 0x41804180u;
-        o[2] = ((w >> 5) & 0x00780078u) | 0x41804180u;
-        o[3] = ((w >> 9) & 0x00780078u) | 0x41804180u;
+    unsigned mask0, bits0, mask, bits;
+    __device__ __forceinline__ CodesBf16()
+        : mask0(kept_scalar(0x000F000Fu)), bits0(kept_vector(0x43004300u)), mask(kept_scalar(0x00780078u)), bits(kept_vector(0x41804180u)) {}
+    __device__ __forceinline__ void four(unsigned w, unsigned (&o)[4]) const {
+        o[0] = (w & mask0) | bits0;
+        o[1] = ((w >> 1) & mask) | bits;
+        o[2] = ((w >> 5) & mask) | bits;
+        o[3] = ((w >> 9) & mask) | bits;
     }
     static __device__ __forceinline__ constexpr float off(int k) { return k == 0 ? 128.f : 16.f; }
 };
 struct CodesF16 {  // 64 + code, the code at bit 4
-    static __device__ __forceinline__ void four(unsigned w, unsigned (&o)[4]) {
-        o[0] = ((w << 4) & 0x00F000F0u) | 0x54005400u;
-        o[1] = (w & 0x00F000F0u) | 0x54005400u;
-        o[2] = ((w >> 4) & 0x00F000F0u) | 0x54005400u;
-        o[3] = ((w >> 8) & 0x00F000F0u) | 0x54005400u;
+    unsigned mask, bits;
+    __device__ __forceinline__ CodesF16() : mask(kept_scalar(0x00F000F0u)), bits(kept_vector(0x54005400u)) {}
+    __device__ __forceinline__ void four(unsigned w, unsigned (&o)[4]) const {
+        o[0] = ((w << 4) & mask) | bits;
+        o[1] = (w & mask) | bits;
+        o[2] = ((w >> 4) & mask) | bits;
+        o[3] = ((w >> 8) & mask) | bits;
     }
     static __device__ __forceinline__ constexpr float off(int) { return 64.f; }
 };
@@ -215,7 +251,7 @@ __global__ __launch_bounds__(256) void hstu_paged_attention_kernel(const PagedAt
     constexpr int ROWS = 16 * MT * RW;
     const int rows = p.delta * p.group, r_end = min((rb + 1) * ROWS, rows);
     const PagedSpan span = paged_span(p, b, rb * ROWS / p.group, (r_end - 1) / p.group + 1);
-    const int chunks = span.na + span.nb, per = (chunks + p.splits - 1) / p.splits;
+    const int chunks = span.na + span.nb, per = chunks_per_run(p, chunks);
     const int chunk_end = min((split + 1) * per, chunks);
     if (p.splits > 1 && split * per >= chunks) return;  // (the joining kernel knows)
 
@@ -267,6 +303,8 @@ __global__ __launch_bounds__(256) void hstu_paged_attention_kernel(const PagedAt
 #pragma unroll
         for (int j = 0; j < NV; ++j) acc[mt][j] = pa_f32x4{0, 0, 0, 0};
     }
+    const typename TT::codes k_codes;
+    const CodesBf16 v_codes;
     PagedReader<DK, DV> reader{p.cache, b * p.cache.table_row_stride, hk, span.n, lane, span.bad};
 
     auto chunk_at = [&](int i) { return i < span.na ? span.a0 + i : span.b0 + (i - span.na); };
@@ -287,7 +325,7 @@ __global__ __launch_bounds__(256) void hstu_paged_attention_kernel(const PagedAt
 #pragma unroll
             for (int j = 0; j < NK; ++j) {
                 unsigned o[4];
-                TT::codes::four(x.k[tt][j], o);
+                k_codes.four(x.k[tt][j], o);
                 kf[tt][j] = u32x4_t{o[0], o[1], o[2], o[3]};
             }
 #pragma unroll
@@ -297,7 +335,7 @@ __global__ __launch_bounds__(256) void hstu_paged_attention_kernel(const PagedAt
                 unsigned two, o[4];
                 if constexpr (NV <= 4) two = x.v[2 * pair][0] | (x.v[2 * pair + 1][0] << 16);
                 else two = __builtin_amdgcn_perm(x.v[2 * pair + 1][h >> 1], x.v[2 * pair][h >> 1], h & 1 ? 0x07060302u : 0x05040100u);
-                CodesBf16::four(two, o);
+                v_codes.four(two, o);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     if (4 * h + k < NV) vf[4 * h + k][pair] = o[k];
@@ -407,32 +445,336 @@ __global__ __launch_bounds__(256) void hstu_paged_attention_kernel(const PagedAt
     }
 }
 
-// out = oscale * the sum of the runs there are, eight columns to a thread.
-template <class TT>
+// The same for few rows (at most 8 of one head of the cache), where a product of 16 columns would waste most of them: F = 16 / RP chunks
+// side by side.  Column n of a score tile stands for row n % RP and chunk n / RP of F: a chunk's product fills all columns, and each lane keeps
+// it where the chunk is its own.  silu and what surrounds it then run once for F chunks, on full lanes, and so do the loads of the pairs
+// (step, lowest value).  For the second product each chunk's columns alone have P, the others zero: its sums land in columns of their own,
+// which are added up over the chunks at the end.
+// Waves of a SIMD: three in 168 registers each took 281 us for attention_step's 1.45 GB where two in 172 took 290; heads of 256 need
+// the registers of one.
+template <int DK, int DV>
+constexpr int STEP_WAVES = DK == 256 ? 1 : DK + DV >= 256 ? 2 : DK + DV >= 128 ? 3 : 4;
+
+template <class TT, int DK, int DV, int RP>
+__global__ __launch_bounds__(256, (STEP_WAVES<DK, DV>)) void hstu_paged_step_kernel(const PagedAttentionParams p) {
+    typedef typename TT::elem T;
+    typedef __attribute__((ext_vector_type(2))) T T2;
+    constexpr int NK = DK / 32, NV = DV / 16, F = 16 / RP, VW = NV == 16 ? 2 : 1, U = 2;
+    __shared__ float meet[4 * RP * DV];
+    const PagedCache& c = p.cache;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int part = p.share == 4 ? wave : 0, item = p.share == 4 ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave;
+    const bool idle = item >= p.items;
+    const int known = idle ? 0 : item;
+    const int hk = known % c.heads, b = (known / c.heads) % c.batch, split = known / (c.heads * c.batch);  // whole runs first, what is left of sequences last
+    const int own = n / RP, r = n % RP, rows = p.delta * p.group;
+    const PagedSpan span = paged_span(p, b, 0, p.delta);
+    const int chunks = span.na + span.nb, per = chunks_per_run(p, chunks);
+    const bool silent = idle || (p.splits > 1 && split * per >= chunks);  // no run: the joining kernel knows
+    if (silent && p.share == 4) return;
+    const int run_end = min((split + 1) * per, chunks), each = (max(run_end - split * per, 0) + p.share - 1) / p.share;
+    const int begin = silent ? 0 : min(split * per + part * each, run_end), end = silent ? 0 : min(begin + each, run_end);
+    auto chunk_at = [&](int i) { return i < span.na ? span.a0 + i : span.b0 + (i - span.na); };
+
+    RowSpan see{0, 0, 0, -1};
+    int lo_max = 0, hi_min = 1 << 30;
+    const int row_i = r / p.group, head = hk * p.group + (r - row_i * p.group);
+    if (r < rows) {
+        see = row_span(p, span, span.n - p.delta + row_i);
+        lo_max = see.lo, hi_min = see.hi;
+    }
+    u32x4_t qf[NK];
+    float qs = 0.f, qo = 0.f;
+#pragma unroll
+    for (int j = 0; j < NK; ++j) {
+        qf[j] = u32x4_t{0, 0, 0, 0};
+        if (r < rows) qf[j] = *(const u32x4_t*)(p.q + (((int64_t)b * p.delta + row_i) * p.q_rs + head * p.q_hs + 8 * (NK * g + j)) * 2);
+    }
+    auto prepare_q = [&]() __attribute__((always_inline)) {  // columns k and k + 4 side by side, as the codes come; their sums
+#pragma unroll
+        for (int j = 0; j < NK; ++j) {
+            const u32x4_t x = qf[j];
+            qf[j] = u32x4_t{__builtin_amdgcn_perm(x.z, x.x, 0x05040100u), __builtin_amdgcn_perm(x.z, x.x, 0x07060302u),
+                            __builtin_amdgcn_perm(x.w, x.y, 0x05040100u), __builtin_amdgcn_perm(x.w, x.y, 0x07060302u)};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const T2 two = __builtin_bit_cast(T2, (unsigned)qf[j][k]);
+                const float sum = (float)two[0] + (float)two[1];
+                qs += sum, qo += sum * TT::codes::off(k);
+            }
+        }
+        qs += __shfl_xor(qs, 16, 64), qo += __shfl_xor(qo, 16, 64);
+        qs += __shfl_xor(qs, 32, 64), qo += __shfl_xor(qo, 32, 64);
+#pragma unroll
+        for (int d = 1; d < RP; d <<= 1) lo_max = max(lo_max, __shfl_xor(lo_max, d, 64)), hi_min = min(hi_min, __shfl_xor(hi_min, d, 64));
+        lo_max = __builtin_amdgcn_readfirstlane(lo_max), hi_min = __builtin_amdgcn_readfirstlane(hi_min);
+    };
+
+    const typename TT::codes k_codes;
+    const CodesBf16 v_codes;
+    pa_f32x4 acc[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) acc[j] = pa_f32x4{0, 0, 0, 0};
+    float psum = 0.f, plo = 0.f;
+    bool bad = span.bad;
+    const int in_page = (1 << c.page_shift) - 1;
+    const unsigned k_lane = n * (DK / 2) + g * (4 * NK), v_lane = 4 * g * (DV / 2) + n * (NV / 2);
+
+    // Pages of the tiles of 16 of the F chunks from s0 on, one to a lane; what does not exist has the first page.
+    auto pages_of = [&](int s0) __attribute__((always_inline)) {
+        int page = 0;
+        const int pos = chunk_at(min(s0 + ((lane >> 1) & (F - 1)), end - 1)) * 32 + (lane & 1) * 16;
+        if (pos < span.n) {
+            const int64_t at = index_at(c.page_table, c.page_table_i64, b * c.table_row_stride + (pos >> c.page_shift));
+            if (at < 0 || at >= c.pages) bad = true;
+            else page = (int)at;
+        }
+        return page;
+    };
+    auto row_of = [&](int page, int s0, int ci, int tt) __attribute__((always_inline)) {  // of the cache, in rows: uniform
+        const int64_t pg = __builtin_amdgcn_readlane(page, 2 * ci + tt);
+        return ((pg * c.heads + hk) << c.page_shift) + ((chunk_at(s0 + ci) * 32 + tt * 16) & in_page);
+    };
+    auto load_k = [&](unsigned (&x)[U][2][NK], int page, int s0, int c0) __attribute__((always_inline)) {
+        const int nc = min(F, end - s0);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) {
+                const UniformRows k(c.k_codes + row_of(page, s0, min(c0 + u, nc - 1), tt) * (DK / 2), 16 * (DK / 2));
+                if constexpr (NK == 1) {
+                    x[u][tt][0] = k.at<unsigned>(k_lane);
+                } else if constexpr (NK == 2) {
+                    const u32x2_t a = k.at<u32x2_t>(k_lane);
+                    x[u][tt][0] = a.x, x[u][tt][1] = a.y;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < NK; j += 4) {
+                        const u32x4_t a = k.at<u32x4_t>(k_lane + 4 * j);
+                        x[u][tt][j] = a.x, x[u][tt][j + 1] = a.y, x[u][tt][j + 2] = a.z, x[u][tt][j + 3] = a.w;
+                    }
+                }
+            }
+    };
+    auto load_v = [&](unsigned (&x)[U][8][VW], int page, int s0, int c0) __attribute__((always_inline)) {
+        const int nc = min(F, end - s0);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) {
+                const UniformRows v(c.v_codes + row_of(page, s0, min(c0 + u, nc - 1), tt) * (DV / 2), 16 * (DV / 2));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const unsigned at = v_lane + i * (DV / 2);
+                    if constexpr (NV == 2) x[u][4 * tt + i][0] = v.at<unsigned char>(at);
+                    else if constexpr (NV == 4) x[u][4 * tt + i][0] = v.at<unsigned short>(at);
+                    else {
+#pragma unroll
+                        for (int j = 0; j < VW; ++j) x[u][4 * tt + i][j] = v.at<unsigned>(at + 4 * j);
+                    }
+                }
+            }
+    };
+    // This lane's pairs: of its own chunk's positions 4 g .. and 16 + 4 g ..
+    u32x4_t ks[2], vs[2];
+    auto load_pairs = [&](int page, int s0) __attribute__((always_inline)) {
+        const int ci = min(own, min(F, end - s0) - 1), pos = chunk_at(s0 + ci) * 32 + 4 * g;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+            const int64_t pg = __shfl(page, 2 * ci + tt, 64);
+            const int64_t at = ((pg * c.heads + hk) << c.page_shift) + ((pos + 16 * tt) & in_page);
+            ks[tt] = *(const u32x4_t*)(c.k_scales + at * 4);
+            vs[tt] = *(const u32x4_t*)(c.v_scales + at * 4);
+        }
+    };
+
+    // Loads run ahead of the work on what they bring: K and V two chunks, the first V before the scores, the next F chunks' pages before
+    // the scores and their first K and pairs before the sums.  (With each F chunks begun from nothing a run of 257 chunks took a sixth
+    // longer than one of 256.)
+    unsigned k_now[U][2][NK], k_next[U][2][NK], v_now[U][8][VW], v_next[U][8][VW];
+    int page = 0, page_next = 0;
+    if (begin < end) {
+        page = pages_of(begin);
+        load_k(k_now, page, begin, 0);
+        load_pairs(page, begin);
+        prepare_q();
+    }
+    for (int s0 = begin; s0 < end; s0 += F) {
+        const int nc = min(F, end - s0);
+        const bool more = s0 + F < end;
+        if (more) page_next = pages_of(s0 + F);
+        load_v(v_now, page, s0, 0);
+        pa_f32x4 s[2] = {pa_f32x4{0, 0, 0, 0}, pa_f32x4{0, 0, 0, 0}};
+        auto scores = [&](const unsigned (&x)[U][2][NK], int c0) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool mine = own == c0 + u;
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt) {
+                    pa_f32x4 t = {-qo, -qo, -qo, -qo};
+#pragma unroll
+                    for (int j = 0; j < NK; ++j) {
+                        unsigned o[4];
+                        k_codes.four(x[u][tt][j], o);
+                        t = TT::mma(u32x4_t{o[0], o[1], o[2], o[3]}, qf[j], t);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[tt][i] = mine ? t[i] : s[tt][i];
+                }
+            }
+        };
+        // (chunks behind the last are the last again: their scores are masked, P of theirs is zero)
+        for (int c0 = 0; c0 < nc; c0 += U) {
+            load_k(k_next, page, s0, c0 + U);
+            scores(k_now, c0);
+            __builtin_memcpy(k_now, k_next, sizeof(k_now));
+        }
+        u32x4_t ph, pl;
+        {
+            const bool whole = nc == F && s0 + F <= span.na && chunk_at(s0) * 32 >= lo_max && chunk_at(s0 + F - 1) * 32 + 32 <= hi_min;
+            const int own_pos = chunk_at(min(s0 + own, end - 1)) * 32 + 4 * g;
+            float ps[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const T2 k2 = __builtin_bit_cast(T2, (unsigned)ks[e >> 2][e & 3]), v2 = __builtin_bit_cast(T2, (unsigned)vs[e >> 2][e & 3]);
+                const float t = p.c1 * ((float)k2[0] * s[e >> 2][e & 3] + (float)k2[1] * qs);
+                const float pr = t * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(t));
+                ps[e] = pr * (float)v2[0];
+                float lower = pr * ((float)v2[1] + 7.5f * (float)v2[0]);
+                if (!whole) {
+                    const bool seen = own < nc && see.sees(own_pos + (e >> 2) * 16 + (e & 3));
+                    ps[e] = seen ? ps[e] : 0.f, lower = seen ? lower : 0.f;
+                }
+                plo += lower;
+            }
+            pa_bf16x8 high;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) high[e] = (__bf16)ps[e], psum += (float)high[e];
+            ph = __builtin_bit_cast(u32x4_t, high);
+            if constexpr (TT::P_WORDS == 2) {
+                pa_bf16x8 rest;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) rest[e] = (__bf16)(ps[e] - (float)high[e]), psum += (float)rest[e];
+                pl = __builtin_bit_cast(u32x4_t, rest);
+            }
+        }
+        auto sums = [&](const unsigned (&x)[U][8][VW], int c0) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool mine = own == c0 + u;
+                u32x4_t bh, bl;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    bh[i] = mine ? ph[i] : 0u;
+                    if constexpr (TT::P_WORDS == 2) bl[i] = mine ? pl[i] : 0u;
+                }
+#pragma unroll
+                for (int h = 0; h < (NV + 3) / 4; ++h) {
+                    u32x4_t vf[4];
+#pragma unroll
+                    for (int pair = 0; pair < 4; ++pair) {
+                        unsigned two, o[4];
+                        if constexpr (NV <= 4) two = x[u][2 * pair][0] | (x[u][2 * pair + 1][0] << 16);
+                        else two = __builtin_amdgcn_perm(x[u][2 * pair + 1][h >> 1], x[u][2 * pair][h >> 1], h & 1 ? 0x07060302u : 0x05040100u);
+                        v_codes.four(two, o);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) vf[k][pair] = o[k];
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if (4 * h + k >= NV) break;
+                        acc[4 * h + k] = PagedBf16::mma(vf[k], bh, acc[4 * h + k]);
+                        if constexpr (TT::P_WORDS == 2) acc[4 * h + k] = PagedBf16::mma(vf[k], bl, acc[4 * h + k]);
+                    }
+                }
+            }
+        };
+        if (more) {
+            load_k(k_now, page_next, s0 + F, 0);
+            load_pairs(page_next, s0 + F);
+        }
+        for (int c0 = 0; c0 < nc; c0 += U) {
+            load_v(v_next, page, s0, c0 + U);
+            sums(v_now, c0);
+            __builtin_memcpy(v_now, v_next, sizeof(v_now));
+        }
+        page = page_next;
+    }
+
+    // columns of one row, over the chunks; psum and plo over the positions' lanes too
+    auto columns = [&](float v) __attribute__((always_inline)) {
+        if constexpr (RP <= 8) v += dpp<0x128>(v);  // rotations within 16 lanes
+        if constexpr (RP <= 4) v += dpp<0x124>(v);
+        if constexpr (RP <= 2) v += dpp<0x122>(v);
+        if constexpr (RP <= 1) v += dpp<0x121>(v);
+        return v;
+    };
+    psum += __shfl_xor(psum, 16, 64), plo += __shfl_xor(plo, 16, 64);
+    psum += __shfl_xor(psum, 32, 64), plo += __shfl_xor(plo, 32, 64);
+    psum = columns(psum), plo = columns(plo);
+    if (__any(bad)) plo = __builtin_nanf("");
+#pragma unroll
+    for (int i4 = 0; i4 < 4; ++i4)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const float o = columns(acc[j][i4]) - (CodesBf16::off(j & 3) + 7.5f) * psum + plo;
+            if (n < RP) meet[(wave * RP + n) * DV + NV * (4 * g + i4) + j] = o;
+        }
+    __syncthreads();
+    // the sums of the waves that share a run, or each wave's own
+    const int64_t row0 = (int64_t)b * p.delta;
+    for (int at = p.share == 4 ? threadIdx.x : lane; at < RP * DV && !silent; at += 64 * p.share) {
+        const int rr = at / DV, d = at % DV;
+        if (rr >= rows) break;
+        const float x = p.share == 4 ? meet[at] + meet[RP * DV + at] + meet[2 * RP * DV + at] + meet[3 * RP * DV + at] : meet[wave * RP * DV + at];
+        const int64_t to = ((row0 + rr / p.group) * (c.heads * p.group) + hk * p.group + rr % p.group) * DV + d;
+        if (p.splits > 1) p.partial[split * p.partial_stride + to] = x;
+        else ((T*)p.out)[to] = (T)(x * p.oscale);
+    }
+}
+
+// out = oscale * the sum of the runs there are: eight columns to PARTS threads, which share out the runs and add up in a fixed order.
+template <class TT, int PARTS>
 __global__ __launch_bounds__(256) void hstu_paged_join_kernel(const PagedAttentionParams p, int block_rows, int64_t total8) {
     typedef typename TT::elem T;
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (at >= total8) return;
+    const int64_t thread = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int part = (int)(thread % PARTS);
+    const bool there = thread / PARTS < total8;
+    const int64_t at = there ? thread / PARTS : total8 - 1;
     const int heads = p.cache.heads * p.group, words = p.cache.dv >> 3;
     const int64_t row_head = at / words, row = row_head / heads;
     const int b = (int)(row / p.delta), r = (int)(row - (int64_t)b * p.delta) * p.group + (int)(row_head - row * heads) % p.group;
     const int rb = r / block_rows, r_end = min((rb + 1) * block_rows, p.delta * p.group);
     const PagedSpan span = paged_span(p, b, rb * block_rows / p.group, (r_end - 1) / p.group + 1);
-    const int chunks = span.na + span.nb, per = (chunks + p.splits - 1) / p.splits, runs = per ? (chunks + per - 1) / per : 0;
-    float x[8];
+    const int chunks = span.na + span.nb, per = chunks_per_run(p, chunks), runs = (chunks + per - 1) / per;
+    pa_f32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+    const float* from = p.partial + at * 8;
+    int s = part;
+    for (; s + 3 * PARTS < runs; s += 4 * PARTS) {  // four loads in flight
+        pa_f32x4 a[4], c[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = span.bad ? __builtin_nanf("") : 0.f;
-    for (int s = 0; s < runs; ++s) {
-        const pa_f32x4* from = (const pa_f32x4*)(p.partial + s * p.partial_stride + at * 8);
-        const pa_f32x4 a = from[0], c = from[1];
+        for (int i = 0; i < 4; ++i) {
+            const pa_f32x4* f = (const pa_f32x4*)(from + (s + i * PARTS) * p.partial_stride);
+            a[i] = f[0], c[i] = f[1];
+        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] += a[i], x[4 + i] += c[i];
+        for (int i = 0; i < 4; ++i) x += a[i], y += c[i];
     }
+    for (; s < runs; s += PARTS) {
+        const pa_f32x4* f = (const pa_f32x4*)(from + s * p.partial_stride);
+        x += f[0], y += f[1];
+    }
+    float o[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= p.oscale;
+    for (int i = 0; i < 4; ++i) o[i] = x[i], o[4 + i] = y[i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        o[i] = group_sum<PARTS>(o[i]) * p.oscale;
+        if (span.bad) o[i] = __builtin_nanf("");
+    }
     Cols<T> out;
-    out.put(x);
-    out.store((T*)p.out + at * 8);
+    out.put(o);
+    if (there && part == 0) out.store((T*)p.out + at * 8);
 }
 
 }  // namespace hstu
