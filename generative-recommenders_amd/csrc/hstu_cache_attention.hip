@@ -33,7 +33,10 @@ Plan plan_of(const HstuPagedCache* c, const HstuPagedAttentionArgs* a) {
         p.block = p.step;
     } else {
         if (rows > 16) p.mt = c->dv == 256 ? 1 : 2;
-        if (rows > 16 * p.mt) p.rw = 4;
+        if (rows > 16 * p.mt) {
+            p.rw = 4;
+            if (rows <= 64) p.mt = 1;
+        }
         p.block = 16 * p.mt * p.rw;
     }
     p.row_blocks = (int)((rows + p.block - 1) / p.block);
@@ -45,9 +48,14 @@ Plan plan_of(const HstuPagedCache* c, const HstuPagedAttentionArgs* a) {
     // for each other (64 sequences of 1024 .. 4096 positions and four heads, 256 workgroups for whole sequences: runs of 129 chunks, all of one, 28 us,
     // of 80 26, of 16 35), but none so long that the last of them run alone (128 sequences of up to 16384 and eight heads: runs of 513 290 us, of 384 262,
     // of 64 286).  Sequences of a few chunks, more of them than fit, are a wave's each (1600 of up to 10 chunks: 12.5 us, 16 by workgroups).
-    const int64_t fill = (chunks * wgs + 511) / 512;
+    // Blocks of many rows: one workgroup of a CU, so whole sequences where there are 256 of them, for a run more is a partial sum of every row to write
+    // and read (32 sequences of 1280 .. 4352 positions, 256 rows, four heads: 106 us, of two runs 124); below that as many as there are CUs, none
+    // longer than 96 chunks (8 sequences of up to 8192, 512 rows, four heads: runs of 129 111 us, of 86 82).
+    const bool blocks = !p.step && p.rw == 4;
+    const int64_t slots = blocks ? 256 : 512, fill = (chunks * wgs + slots - 1) / slots;
     int64_t run = a->kv_splits > 0 ? (chunks + a->kv_splits - 1) / a->kv_splits : (fill + 15) / 16 * 16;
-    if (!a->kv_splits && run > 384) run = 384;
+    if (!a->kv_splits && !blocks && run > 384) run = 384;
+    if (!a->kv_splits && blocks && wgs < 256 && run > 96) run = 96;
     if (run < 16) run = 16;
     if (p.step && chunks <= 17 && wgs > 1024) p.share = 1, run = chunks;
     if (run > chunks) run = chunks;
@@ -62,21 +70,27 @@ typedef std::integral_constant<int, 1> One;
 template <class TT, int DK, int DV>
 int launch_sized(const hstu::PagedAttentionParams& p, const Plan& plan, hipStream_t stream) {
     const unsigned blocks = (unsigned)((p.items + 7) / 8 * 8 * (int64_t)plan.row_blocks);
-    auto go = [&](auto mt, auto rw) {
-        hipLaunchKernelGGL((hstu::hstu_paged_attention_kernel<TT, DK, DV, decltype(mt)::value, decltype(rw)::value>), dim3(blocks), dim3(256), 0, stream, p);
+    auto go = [&](auto mt) {
+        hipLaunchKernelGGL((hstu::hstu_paged_attention_kernel<TT, DK, DV, decltype(mt)::value, 1>), dim3(blocks), dim3(256), 0, stream, p);
     };
-    typedef std::integral_constant<int, DV == 256 ? 1 : 2> Most;
+    auto block = [&](auto mt) {
+        hipLaunchKernelGGL((hstu::hstu_paged_block_kernel<TT, DK, DV, decltype(mt)::value>), dim3(blocks), dim3(512), 0, stream, p);
+    };
+    typedef std::integral_constant<int, 2> Two;
     typedef std::integral_constant<int, 4> Four;
     auto step = [&](auto rp) {
         hipLaunchKernelGGL((hstu::hstu_paged_step_kernel<TT, DK, DV, decltype(rp)::value>), dim3((unsigned)((p.items * p.share + 3) / 4)), dim3(256), 0, stream, p);
     };
     if (plan.step == 1) step(One{});
-    else if (plan.step == 2) step(std::integral_constant<int, 2>{});
+    else if (plan.step == 2) step(Two{});
     else if (plan.step == 4) step(Four{});
     else if (plan.step == 8) step(std::integral_constant<int, 8>{});
-    else if (plan.rw == 4) go(Most{}, Four{});
-    else if (plan.mt == 1) go(One{}, One{});
-    else if constexpr (DV != 256) go(Most{}, One{});
+    else if (plan.rw == 4 && plan.mt == 1) block(One{});
+    else if (plan.mt == 1) go(One{});
+    else if constexpr (DV != 256) {
+        if (plan.rw == 4) block(Two{});
+        else go(Two{});
+    }
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && p.splits > 1) {
         const int64_t total8 = p.partial_stride / 8;

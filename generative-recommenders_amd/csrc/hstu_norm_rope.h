@@ -5,8 +5,7 @@
 //
 // A vector (one row, one head) is taken by LPV = dim / 8 lanes (rounded up to a power of two), eight columns to a lane: one 16-byte
 // access each way in 16 bits, and the sums over a vector are log2(LPV) lane exchanges.  The partner of a column in the half-split
-// form lies rotary / 2 columns on, rotary / 16 lanes away: lanes exchange the columns as they were loaded (four words in 16 bits)
-// and norm their partner's themselves, with its weights.  A group of LPV lanes stays with one row for several heads, so that
+// form lies rotary / 2 columns on, rotary / 16 lanes away: lanes exchange them.  A group of LPV lanes stays with one row for several heads, so that
 // positions and table rows, which the heads of a row share, are read once.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -64,13 +63,6 @@ struct Cols {
                 w[i] = __builtin_bit_cast(unsigned, v);
             }
         }
-    }
-    // the same columns of lane `byte_lane / 4` of the wave
-    __device__ __forceinline__ Cols from_lane(int byte_lane) const {
-        Cols o;
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) o.w[i] = (unsigned)__builtin_amdgcn_ds_bpermute(byte_lane, (int)w[i]);
-        return o;
     }
 };
 
@@ -142,17 +134,13 @@ struct LaneTurn {
     }
 };
 
-// The partners of a lane's columns.
-template <class T>
-__device__ __forceinline__ void partners(const LaneTurn& t, int interleaved, const Cols<T>& in, const float (&x)[8], float (&p)[8]) {
-    if (interleaved) {
+// The partners of a lane's columns.  `all`: whether every column of a vector turns.
+__device__ __forceinline__ void partners(const LaneTurn& t, int interleaved, bool all, const float (&x)[8], float (&p)[8]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = __uint_as_float(__float_as_uint(x[i ^ 1]) & t.keep);
-    } else {
-        Cols<T> o = in.from_lane(t.byte_lane);
+    for (int i = 0; i < 8; ++i) p[i] = interleaved ? x[i ^ 1] : __uint_as_float((unsigned)__builtin_amdgcn_ds_bpermute(t.byte_lane, (int)__float_as_uint(x[i])));
+    if (!all) {
 #pragma unroll
-        for (int i = 0; i < Cols<T>::WORDS; ++i) o.w[i] &= t.keep;
-        o.get(p);
+        for (int i = 0; i < 8; ++i) p[i] = __uint_as_float(__float_as_uint(p[i]) & t.keep);
     }
 }
 
@@ -169,45 +157,51 @@ __device__ __forceinline__ void lane_weights(const T* weight, int col0, float (&
     }
 }
 
-// Norm and turn as one: y = r (x cw + partner sw), the weights gone into cosines and sines (a partner's weight into its sine), which
-// the heads of a row share.
-struct NormTurn {
-    float cw[8], sw[8];
-    template <class T>
-    __device__ __forceinline__ void fill(const LaneTurn& t, int interleaved, const T* weight, int col0) {
-        if (weight) {
-            float w[8], wp[8];
-            lane_weights(weight, col0, w);
-            Cols<T> raw;
-            raw.put(w);
-            partners(t, interleaved, raw, w, wp);
+// 1 / sqrt(mean of squares + eps) of a vector, rounded as exactly as torch's mean and rsqrt over the last dimension give it (measured: the same
+// bits): squares added pairwise, from sums of four on where a vector has 128 columns or more, and the instruction's root, good to a unit in
+// the last place, corrected once by its residual.
+template <int LPV>
+__device__ __forceinline__ float inverse_rms(const float (&x)[8], bool there, float inv_dim, float eps) {
+#pragma clang fp contract(off)
+    float q[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) cw[i] = t.c[i] * w[i], sw[i] = t.s[i] * wp[i];
-        } else {
+    for (int i = 0; i < 8; ++i) q[i] = x[i] * x[i];
+    const float sum = LPV >= 16 ? (q[0] + q[1] + q[2] + q[3]) + (q[4] + q[5] + q[6] + q[7]) : ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+    const float v = group_sum<LPV>(there ? sum : 0.f) * inv_dim + eps;
+    const float r = rsqrtf(v), h = v * r, low = __builtin_fmaf(v, r, -h);
+    const float fixed = __builtin_fmaf(0.5f * r, __builtin_fmaf(-low, r, __builtin_fmaf(-h, r, 1.f)), r);
+    return v > 0x1p-100f && v < 0x1p100f ? fixed : r;
+}
+
+// A vector as loaded to what is rounded and stored; `there`: whether the lane's columns are the vector's (one that has none holds another's),
+// `known`: whether its position is.  The operations are rounded one by one, as the definition has them: K is rounded to its type next and then
+// to codes, where a value that comes out a unit in the last place off now and then is a whole step off.  (Weights multiplied into cosines and
+// sines, and sums by fused operations, gave twenty such codes in 18 million; this costs no more.)
+template <class T, int LPV>
+__device__ __forceinline__ void norm_and_turn(const LaneTurn& t, const Turn& how, const Cols<T>& in, const float (&w)[8], bool there, bool norm, int dim,
+                                              float inv_dim, float eps, bool known, float (&y)[8]) {
+#pragma clang fp contract(off)
+    float n[8], p[8];
+    in.get(n);
+    if (norm) {
+        const float r = inverse_rms<LPV>(n, there, inv_dim, eps);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) cw[i] = t.c[i], sw[i] = t.s[i];
-        }
+        for (int i = 0; i < 8; ++i) n[i] = n[i] * r * w[i];
     }
-    // A vector as loaded to what is rounded and stored; `known`: whether its position is.
-    // `there`: whether the lane's columns are the vector's (one that has none holds another's).
-    template <class T, int LPV>
-    __device__ __forceinline__ void apply(const LaneTurn& t, int interleaved, const Cols<T>& in, bool there, bool norm, float inv_dim, float eps, bool known,
-                                          float (&y)[8]) const {
-        float x[8], p[8];
-        in.get(x);
-        partners(t, interleaved, in, x, p);
-        float r = 1.f;
-        if (norm) {
-            float sq = 0.f;
+    if (how.rotary) {
+        partners(t, how.interleaved, how.rotary == dim, n, p);
+        const float nan = known ? 0.f : __builtin_nanf("");
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sq += x[i] * x[i];
-            r = rsqrtf(group_sum<LPV>(there ? sq : 0.f) * inv_dim + eps);
+        for (int i = 0; i < 8; ++i) y[i] = n[i] * t.c[i] + p[i] * t.s[i];
+        if (!known) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = nan;
         }
-        if (!known) r = __builtin_nanf("");
+    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = r * (x[i] * cw[i] + p[i] * sw[i]);
+        for (int i = 0; i < 8; ++i) y[i] = n[i];
     }
-};
+}
 
 // One side (q or k) of the step.
 struct NormRopeSide {
@@ -257,8 +251,8 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_kernel(const NormRopeParam
         const int base = which ? p.side[0].heads : 0;
         const int h0 = max(first - base, 0), h1 = min(last - base, s.heads);
         if (h0 >= h1) continue;
-        NormTurn nt;
-        nt.fill(t, p.turn.interleaved, (const T*)s.weight, col0);
+        float w[8];
+        lane_weights((const T*)s.weight, col0, w);
         const T* x = (const T*)s.x + row * s.rs + col0;
         T* out = (T*)s.y + row * s.heads * p.dim + col0;
         for (int h = h0; h < h1; h += AHEAD) {
@@ -269,7 +263,7 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_kernel(const NormRopeParam
             for (int a = 0; a < AHEAD; ++a) {
                 if (h + a >= h1) break;  // (the same for the whole workgroup)
                 float y[8];
-                nt.apply<T, LPV>(t, p.turn.interleaved, in[a], cols, s.weight != nullptr, p.inv_dim, p.eps, known, y);
+                norm_and_turn<T, LPV>(t, p.turn, in[a], w, cols, s.weight != nullptr, p.dim, p.inv_dim, p.eps, known, y);
                 Cols<T> o;
                 o.put(y);
                 if (there) o.store(out + (h + a) * p.dim);
@@ -325,7 +319,7 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_bwd_kernel(const NormRopeP
                     if (h + a >= h1) break;
                     float x[8], d[8], q[8], g[8];
                     dy[a].get(d);
-                    partners(t, p.turn.interleaved, dy[a], d, q);
+                    partners(t, p.turn.interleaved, p.turn.rotary == p.dim, d, q);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) g[i] = d[i] * t.c[i] - q[i] * t.s[i];  // R^T: the partner's sine is the other's with its sign changed
                     if (!known) {
@@ -334,10 +328,7 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_bwd_kernel(const NormRopeP
                     }
                     if (s.weight) {
                         in[a].get(x);
-                        float sq = 0.f;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) sq += x[i] * x[i];
-                        const float r = rsqrtf(group_sum<LPV>(cols ? sq : 0.f) * p.inv_dim + p.eps);
+                        const float r = inverse_rms<LPV>(x, cols, p.inv_dim, p.eps);
                         float dot = 0.f;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {

@@ -79,7 +79,7 @@ __device__ __forceinline__ int chunks_per_run(const PagedAttentionParams& p, int
 // What one row sees: positions [lo, hi), [0, chi) and itself.
 struct RowSpan {
     int lo, hi, chi, self;
-    __device__ __forceinline__ bool sees(int pos) const { return (pos >= lo && pos < hi) || pos < chi || pos == self; }
+    __device__ __forceinline__ bool sees(int pos) const { return ((pos >= lo) & (pos < hi)) | (pos < chi) | (pos == self); }
 };
 
 __device__ __forceinline__ RowSpan row_span(const PagedAttentionParams& p, const PagedSpan& s, int pos) {
@@ -234,6 +234,26 @@ struct PagedReader {
     }
 };
 
+// NV columns each at 4 places NV apart: to the run's partial sums, or scaled to the result.
+template <class T, int NV>
+__device__ __forceinline__ void store_columns(const PagedAttentionParams& p, int split, int64_t at, const float (&o)[4][NV]) {
+    if (p.splits > 1) {
+        float* to = p.partial + split * p.partial_stride + at;
+#pragma unroll
+        for (int i = 0; i < 4 * NV; i += 4) *(pa_f32x4*)(to + i) = pa_f32x4{o[i / NV][i % NV], o[(i + 1) / NV][(i + 1) % NV], o[(i + 2) / NV][(i + 2) % NV], o[(i + 3) / NV][(i + 3) % NV]};
+    } else {
+        typedef __attribute__((ext_vector_type(8))) T T8;
+        T* to = (T*)p.out + at;
+#pragma unroll
+        for (int i = 0; i < 4 * NV; i += 8) {
+            T8 x;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = (T)(o[(i + k) / NV][(i + k) % NV] * p.oscale);
+            *(T8*)(to + i) = x;
+        }
+    }
+}
+
 // grid: one workgroup of four waves per (block of 16 MT RW rows, head of the cache, run, sequence), numbered so that the row blocks
 // of one run, which read the same pages, are on one XCD.  RW waves share out the rows, the others the chunks of the run; the sums of
 // the latter meet in LDS.
@@ -308,9 +328,8 @@ __global__ __launch_bounds__(256) void hstu_paged_attention_kernel(const PagedAt
     PagedReader<DK, DV> reader{p.cache, b * p.cache.table_row_stride, hk, span.n, lane, span.bad};
 
     auto chunk_at = [&](int i) { return i < span.na ? span.a0 + i : span.b0 + (i - span.na); };
-    auto work = [&](const PagedChunk<NK, NV>& x, int chunk) __attribute__((always_inline)) {
+    auto work_masked = [&](const PagedChunk<NK, NV>& x, int chunk, auto masked) __attribute__((always_inline)) {
         const int pos0 = chunk * 32 + 4 * g;
-        const bool whole = chunk * 32 >= lo_max && chunk * 32 + 32 <= hi_min;
         float ka[8], kb[8], va[8], vm[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -356,12 +375,12 @@ __global__ __launch_bounds__(256) void hstu_paged_attention_kernel(const PagedAt
                 const float t = ka[e] * s[e >> 2][e & 3] + kb[e] * qs[mt];
                 const float pr = t * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(t));
                 ps[e] = pr * va[e];
-                float lower = pr * vm[e];
-                if (!whole) {
+                float lower = __builtin_fmaf(pr, vm[e], plo[mt]);
+                if constexpr (decltype(masked)::value) {
                     const bool seen = see[mt].sees(pos0 + (e >> 2) * 16 + (e & 3));
-                    ps[e] = seen ? ps[e] : 0.f, lower = seen ? lower : 0.f;
+                    ps[e] = seen ? ps[e] : 0.f, lower = seen ? lower : plo[mt];
                 }
-                plo[mt] += lower;
+                plo[mt] = lower;
             }
             pa_bf16x8 high;
 #pragma unroll
@@ -380,6 +399,12 @@ __global__ __launch_bounds__(256) void hstu_paged_attention_kernel(const PagedAt
                 psum[mt] = PagedBf16::mma(ones, pl, psum[mt]);
             }
         }
+    };
+
+    // (code of their own for chunks that all rows see whole: a condition at each score would stand between them)
+    auto work = [&](const PagedChunk<NK, NV>& x, int chunk) __attribute__((always_inline)) {
+        if (chunk * 32 >= lo_max && chunk * 32 + 32 <= hi_min) work_masked(x, chunk, std::false_type{});
+        else work_masked(x, chunk, std::true_type{});
     };
 
     // two chunks in flight: the next one's loads are issued before the work on this one
@@ -442,6 +467,321 @@ __global__ __launch_bounds__(256) void hstu_paged_attention_kernel(const PagedAt
                 put(i4, x);
             }
         }
+    }
+}
+
+// The same for many rows: two teams of four waves; a team's waves take 16 MT rows each and share what unpacking yields.  A step is 32 CH positions
+// for each team; each wave unpacks its part of them -- a tile of 16 positions of K, a quarter of the columns of V -- into LDS, in the order in which the
+// products' operands lie in registers (a lane's 16 bytes side by side: reads and writes without bank conflicts), and the pairs as four
+// floats a position: c1 s, c1 l of K, s, l + 7.5 s of V.  Two buffers, one barrier a step; the packed rows of the next step are on their way
+// while this one is worked on.  The teams' sums meet at the end: two waves to a SIMD, without the joining kernel that as many
+// workgroups of one team would need.  Unpacking per wave, as above, cost as much as half of the rest and the registers of a second wave.
+template <class TT, int DK, int DV, int MT>
+__global__ __launch_bounds__(512, 2) void hstu_paged_block_kernel(const PagedAttentionParams p) {
+    typedef typename TT::elem T;
+    typedef __attribute__((ext_vector_type(2))) T T2;
+    constexpr int NK = DK / 32, NV = DV / 16, CH = DK == 256 ? 1 : 2, TILES = 2 * CH, HALVES = (NV + 3) / 4, KB = TILES * NK, VB = CH * NV;
+    constexpr int V_UNITS = CH * HALVES, ROWS = 64 * MT, STEP = 2 * CH;
+    static_assert(TILES <= 4 && V_UNITS <= 4, "one unit of K and one of V to a wave");
+    __shared__ u32x4_t frags_of[2][2][(KB + VB) * 64];  // [team][buffer]
+    __shared__ pa_f32x4 pairs_of[2][2][4][CH * 8];      // [team][buffer][which][position / 4]
+    const PagedCache& c = p.cache;
+    const int xcd = blockIdx.x & 7, q8 = blockIdx.x >> 3;
+    const int rb = q8 % p.row_blocks, item = (q8 / p.row_blocks) * 8 + xcd;
+    if (item >= p.items) return;
+    const int hk = item % c.heads, b = (item / c.heads) % c.batch, split = item / (c.heads * c.batch);
+    const int wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), team = wave8 >> 2, wave = wave8 & 3, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const int rows = p.delta * p.group, r_end = min((rb + 1) * ROWS, rows);
+    const PagedSpan span = paged_span(p, b, rb * ROWS / p.group, (r_end - 1) / p.group + 1);
+    const int chunks = span.na + span.nb, per = chunks_per_run(p, chunks), begin = split * per, end = min(begin + per, chunks);
+    if (p.splits > 1 && begin >= chunks) return;  // (the joining kernel knows)
+    auto chunk_at = [&](int i) { return i < span.na ? span.a0 + i : span.b0 + (i - span.na); };
+
+    // ---- unpacking ----
+    auto& frags = frags_of[team];
+    auto& pairs = pairs_of[team];
+    const typename TT::codes k_codes;
+    const CodesBf16 v_codes;
+    const int in_page = (1 << c.page_shift) - 1;
+    const unsigned k_lane = m * (DK / 2) + g * (4 * NK);
+    const int v_chunk = wave / HALVES, v_half = wave % HALVES;  // of the wave's unit of V
+    const unsigned v_lane = 4 * g * (DV / 2) + m * (NV / 2) + 2 * v_half;
+    bool bad = span.bad;
+    unsigned raw_k[NK], raw_v[8], raw_ks = 0, raw_vs = 0;
+    // Pages of the 64 tiles of 16 positions from chunk ci on, one to a lane; what does not exist has the first page.  Two sets: the next one
+    // has been loaded when its turn comes.  (A page looked up where it is needed is two loads that the wave waits for, three times a step.)
+    auto pages_of = [&](int ci) __attribute__((always_inline)) {
+        int page = 0;
+        const int pos = ci + (lane >> 1) < end ? chunk_at(ci + (lane >> 1)) * 32 + (lane & 1) * 16 : span.n;
+        if (pos < span.n) {
+            const int64_t at = index_at(c.page_table, c.page_table_i64, b * c.table_row_stride + (pos >> c.page_shift));
+            if (at < 0 || at >= c.pages) bad = true;
+            else page = (int)at;
+        }
+        return page;
+    };
+    int page_base = begin, page = 0, page_next = 0;
+    if (begin < end) page = pages_of(begin), page_next = pages_of(begin + 32);
+    // Row of the cache where the 16 positions of tile tt of chunk ci lie.
+    auto row_of = [&](int ci, int tt) __attribute__((always_inline)) {
+        ci = min(ci, end - 1);
+        const int64_t pg = __builtin_amdgcn_readlane(page, 2 * (ci - page_base) + tt);
+        return ((pg * c.heads + hk) << c.page_shift) + ((chunk_at(ci) * 32 + tt * 16) & in_page);
+    };
+    auto load = [&](int ci) __attribute__((always_inline)) {
+        if (ci >= page_base + 32) page_base += 32, page = page_next, page_next = pages_of(page_base + 32);
+        if (wave < TILES) {
+            const int64_t row = row_of(ci + (wave >> 1), wave & 1);
+            const UniformRows k(c.k_codes + row * (DK / 2), 16 * (DK / 2));
+            if constexpr (NK == 1) {
+                raw_k[0] = k.at<unsigned>(k_lane);
+            } else if constexpr (NK == 2) {
+                const u32x2_t a = k.at<u32x2_t>(k_lane);
+                raw_k[0] = a.x, raw_k[1] = a.y;
+            } else {
+#pragma unroll
+                for (int j = 0; j < NK; j += 4) {
+                    const u32x4_t a = k.at<u32x4_t>(k_lane + 4 * j);
+                    raw_k[j] = a.x, raw_k[j + 1] = a.y, raw_k[j + 2] = a.z, raw_k[j + 3] = a.w;
+                }
+            }
+            const UniformRows ks(c.k_scales + row * 4, 64), vs(c.v_scales + row * 4, 64);
+            raw_ks = ks.at<unsigned>(4 * m), raw_vs = vs.at<unsigned>(4 * m);
+        }
+        if (wave < V_UNITS) {
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) {
+                const UniformRows v(c.v_codes + row_of(ci + v_chunk, tt) * (DV / 2), 16 * (DV / 2));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (NV == 2) raw_v[4 * tt + i] = v.at<unsigned char>(v_lane + i * (DV / 2));
+                    else raw_v[4 * tt + i] = v.at<unsigned short>(v_lane + i * (DV / 2));
+                }
+            }
+        }
+    };
+    auto unpack = [&](int buffer) __attribute__((always_inline)) {
+        if (wave < TILES) {
+#pragma unroll
+            for (int j = 0; j < NK; ++j) {
+                unsigned o[4];
+                k_codes.four(raw_k[j], o);
+                frags[buffer][(wave * NK + j) * 64 + lane] = u32x4_t{o[0], o[1], o[2], o[3]};
+            }
+            const T2 k2 = __builtin_bit_cast(T2, raw_ks), v2 = __builtin_bit_cast(T2, raw_vs);
+            float* out = (float*)&pairs[buffer][0][0] + g * (CH * 32) + wave * 16 + m;  // lane (m, g) writes one of the position's four
+            const float ka = p.c1 * (float)k2[0], kb = p.c1 * (float)k2[1], va = (float)v2[0], vm = (float)v2[1] + 7.5f * (float)v2[0];
+            *out = g == 0 ? ka : g == 1 ? kb : g == 2 ? va : vm;
+        }
+        if (wave < V_UNITS) {
+            u32x4_t vf[4];
+#pragma unroll
+            for (int pair = 0; pair < 4; ++pair) {
+                unsigned o[4];
+                v_codes.four(raw_v[2 * pair] | (raw_v[2 * pair + 1] << 16), o);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) vf[k][pair] = o[k];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (4 * v_half + k < NV) frags[buffer][(KB + v_chunk * NV + 4 * v_half + k) * 64 + lane] = vf[k];
+        }
+    };
+
+    if (begin < end) load(begin + team * CH);
+    // ---- rows ----
+    u32x4_t qf[MT][NK];
+    float qs[MT], qo[MT];
+    RowSpan see[MT];
+    int64_t out_at[MT];
+    int any_lo = 1 << 30, any_hi = 0, any_chi = 0, self_lo = 1 << 30, self_hi = -1;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int r = rb * ROWS + (wave * MT + mt) * 16 + m;
+        const int i = r / p.group, head = hk * p.group + (r - i * p.group);
+        qs[mt] = qo[mt] = 0.f;
+        see[mt].lo = see[mt].hi = see[mt].chi = 0, see[mt].self = -1;
+        out_at[mt] = -1;
+        const int64_t row = (int64_t)b * p.delta + i;
+        if (r < rows) {
+            see[mt] = row_span(p, span, span.n - p.delta + i);
+            out_at[mt] = (row * (c.heads * p.group) + head) * DV;
+            any_lo = min(any_lo, see[mt].lo), any_hi = max(any_hi, see[mt].hi), any_chi = max(any_chi, see[mt].chi);
+            if (see[mt].self >= 0) self_lo = min(self_lo, see[mt].self), self_hi = max(self_hi, see[mt].self);
+        }
+#pragma unroll
+        for (int j = 0; j < NK; ++j) {
+            u32x4_t x = {0, 0, 0, 0};
+            if (r < rows) x = *(const u32x4_t*)(p.q + (row * p.q_rs + head * p.q_hs + 8 * (NK * g + j)) * 2);
+            // columns k and k + 4 side by side, as the codes come
+            qf[mt][j] = u32x4_t{__builtin_amdgcn_perm(x.z, x.x, 0x05040100u), __builtin_amdgcn_perm(x.z, x.x, 0x07060302u),
+                                __builtin_amdgcn_perm(x.w, x.y, 0x05040100u), __builtin_amdgcn_perm(x.w, x.y, 0x07060302u)};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const T2 two = __builtin_bit_cast(T2, (unsigned)qf[mt][j][k]);
+                const float sum = (float)two[0] + (float)two[1];
+                qs[mt] += sum, qo[mt] += sum * TT::codes::off(k);
+            }
+        }
+        qs[mt] += __shfl_xor(qs[mt], 16, 64), qo[mt] += __shfl_xor(qo[mt], 16, 64);
+        qs[mt] += __shfl_xor(qs[mt], 32, 64), qo[mt] += __shfl_xor(qo[mt], 32, 64);
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+        any_lo = min(any_lo, __shfl_xor(any_lo, d, 64)), any_hi = max(any_hi, __shfl_xor(any_hi, d, 64)), any_chi = max(any_chi, __shfl_xor(any_chi, d, 64));
+        self_lo = min(self_lo, __shfl_xor(self_lo, d, 64)), self_hi = max(self_hi, __shfl_xor(self_hi, d, 64));
+    }
+    any_lo = __builtin_amdgcn_readfirstlane(any_lo), any_hi = __builtin_amdgcn_readfirstlane(any_hi), any_chi = __builtin_amdgcn_readfirstlane(any_chi);
+    self_lo = __builtin_amdgcn_readfirstlane(self_lo), self_hi = __builtin_amdgcn_readfirstlane(self_hi);
+
+    pa_f32x4 acc[MT][NV], psum[MT], start[MT];
+    float plo[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        start[mt] = pa_f32x4{-qo[mt], -qo[mt], -qo[mt], -qo[mt]};  // four registers of their own, not four moves for each tile
+        asm("" : "+v"(start[mt]));
+        psum[mt] = pa_f32x4{0, 0, 0, 0}, plo[mt] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) acc[mt][j] = pa_f32x4{0, 0, 0, 0};
+    }
+    const u32x4_t ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+
+    auto work_masked = [&](int buffer, int cc, int chunk, auto masked) __attribute__((always_inline)) {
+        const int first = chunk * 32;
+        pa_f32x4 s[MT][2];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+#pragma unroll
+            for (int j = 0; j < NK; ++j) {
+                const u32x4_t kf = frags[buffer][((2 * cc + tt) * NK + j) * 64 + lane];
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) s[mt][tt] = TT::mma(kf, qf[mt][j], j == 0 ? start[mt] : s[mt][tt]);
+            }
+        }
+        // (V's operands are on their way while silu is worked on)
+        u32x4_t vf[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) vf[j] = frags[buffer][(KB + cc * NV + j) * 64 + lane];
+        u32x4_t ph[MT], pl[MT];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+            const int at = cc * 8 + tt * 4 + g;
+            const pa_f32x4 ka = pairs[buffer][0][at], kb = pairs[buffer][1][at], va = pairs[buffer][2][at], vm = pairs[buffer][3][at];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                float ps[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float t = ka[e] * s[mt][tt][e] + kb[e] * qs[mt];
+                    const float pr = t * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(t));
+                    ps[e] = pr * va[e];
+                    float lower = __builtin_fmaf(pr, vm[e], plo[mt]);
+                    if constexpr (decltype(masked)::value) {
+                        const bool seen = see[mt].sees(first + tt * 16 + 4 * g + e);
+                        ps[e] = seen ? ps[e] : 0.f, lower = seen ? lower : plo[mt];
+                    }
+                    plo[mt] = lower;
+                }
+                typedef __attribute__((ext_vector_type(4))) __bf16 b4;
+                b4 high;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) high[e] = (__bf16)ps[e];
+                const u32x2_t h2 = __builtin_bit_cast(u32x2_t, high);
+                ph[mt][2 * tt] = h2.x, ph[mt][2 * tt + 1] = h2.y;
+                if constexpr (TT::P_WORDS == 2) {
+                    b4 rest;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) rest[e] = (__bf16)(ps[e] - (float)high[e]);
+                    const u32x2_t l2 = __builtin_bit_cast(u32x2_t, rest);
+                    pl[mt][2 * tt] = l2.x, pl[mt][2 * tt + 1] = l2.y;
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                acc[mt][j] = PagedBf16::mma(vf[j], ph[mt], acc[mt][j]);
+                if constexpr (TT::P_WORDS == 2) acc[mt][j] = PagedBf16::mma(vf[j], pl[mt], acc[mt][j]);
+            }
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            psum[mt] = PagedBf16::mma(ones, ph[mt], psum[mt]);
+            if constexpr (TT::P_WORDS == 2) psum[mt] = PagedBf16::mma(ones, pl[mt], psum[mt]);
+        }
+    };
+
+    // Chunks [whole0, whole1) of the list are seen whole by every row of the block: lowest positions grow with the rows, and so do ends, but for
+    // those of contextual rows, which lie behind all others'.
+    const int pos0 = span.n - p.delta + rb * ROWS / p.group, pos1 = span.n - p.delta + (r_end - 1) / p.group;
+    int whole0 = 0, whole1 = 0;
+    if (pos0 >= 0) {
+        const int lo = row_span(p, span, pos1).lo, hi = pos1 >= p.c ? row_span(p, span, max(pos0, p.c)).hi : span.u;
+        whole0 = max(((lo + 31) >> 5) - span.a0, 0), whole1 = min((hi >> 5) - span.a0, span.na);
+    }
+    int buffer = 0;
+    auto step = [&](int i, auto masked) __attribute__((always_inline)) {
+        const bool more = i + STEP < end;
+        const int mine = i + team * CH;
+        if (more) load(mine + STEP);
+#pragma unroll
+        for (int cc = 0; cc < CH; ++cc) {
+            if constexpr (decltype(masked)::value) {
+                if (mine + cc < end) {
+                    const int chunk = chunk_at(mine + cc), first = chunk * 32;  // (not where this wave's rows see nothing of it)
+                    if ((first < any_hi && first + 32 > any_lo) || first < any_chi || (first <= self_hi && first + 32 > self_lo)) work_masked(buffer, cc, chunk, masked);
+                }
+            } else {
+                work_masked(buffer, cc, chunk_at(mine + cc), masked);
+            }
+        }
+        if (more) unpack(buffer ^ 1);
+        __syncthreads();
+        buffer ^= 1;
+    };
+    if (begin < end) unpack(0);
+    __syncthreads();
+    int i = begin;
+    for (; i < end && !(i >= whole0 && i + STEP <= whole1); i += STEP) step(i, std::true_type{});
+    for (; i + STEP <= min(end, whole1); i += STEP) step(i, std::false_type{});
+    for (; i < end; i += STEP) step(i, std::true_type{});
+
+    // one wave's bad page is everyone's
+    int* said = (int*)&pairs_of[0][0][0][0];
+    if (threadIdx.x == 0) *said = 0;
+    __syncthreads();
+    if (bad) *said = 1;
+    __syncthreads();
+    bad = *said != 0;
+    // the second team's sums through LDS, one tile of rows at a time
+    float* meet = (float*)&frags_of[0][0][0] + wave * (4 * NV * 64);
+    static_assert(sizeof(frags_of) >= 4 * 4 * NV * 64 * sizeof(float), "room for the sums of four waves");
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        float lower = plo[mt];
+        lower += __shfl_xor(lower, 16, 64);
+        lower += __shfl_xor(lower, 32, 64);
+        if (bad) lower = __builtin_nanf("");
+        float o[4][NV];
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4)
+#pragma unroll
+            for (int j = 0; j < NV; ++j) o[i4][j] = acc[mt][j][i4] - (CodesBf16::off(j & 3) + 7.5f) * psum[mt][i4] + lower;
+        if (mt > 0) __syncthreads();
+        if (team == 1) {
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4)
+#pragma unroll
+                for (int j = 0; j < NV; ++j) meet[(i4 * NV + j) * 64 + lane] = o[i4][j];
+        }
+        __syncthreads();
+        if (team == 1 || out_at[mt] < 0) continue;
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4)
+#pragma unroll
+            for (int j = 0; j < NV; ++j) o[i4][j] += meet[(i4 * NV + j) * 64 + lane];
+        store_columns<T, NV>(p, split, out_at[mt] + NV * 4 * g, o);
     }
 }
 
@@ -630,8 +970,7 @@ __global__ __launch_bounds__(256, (STEP_WAVES<DK, DV>)) void hstu_paged_step_ker
             __builtin_memcpy(k_now, k_next, sizeof(k_now));
         }
         u32x4_t ph, pl;
-        {
-            const bool whole = nc == F && s0 + F <= span.na && chunk_at(s0) * 32 >= lo_max && chunk_at(s0 + F - 1) * 32 + 32 <= hi_min;
+        auto silu = [&](auto masked) __attribute__((always_inline)) {
             const int own_pos = chunk_at(min(s0 + own, end - 1)) * 32 + 4 * g;
             float ps[8];
 #pragma unroll
@@ -641,7 +980,7 @@ __global__ __launch_bounds__(256, (STEP_WAVES<DK, DV>)) void hstu_paged_step_ker
                 const float pr = t * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(t));
                 ps[e] = pr * (float)v2[0];
                 float lower = pr * ((float)v2[1] + 7.5f * (float)v2[0]);
-                if (!whole) {
+                if constexpr (decltype(masked)::value) {
                     const bool seen = own < nc && see.sees(own_pos + (e >> 2) * 16 + (e & 3));
                     ps[e] = seen ? ps[e] : 0.f, lower = seen ? lower : 0.f;
                 }
@@ -657,7 +996,9 @@ __global__ __launch_bounds__(256, (STEP_WAVES<DK, DV>)) void hstu_paged_step_ker
                 for (int e = 0; e < 8; ++e) rest[e] = (__bf16)(ps[e] - (float)high[e]), psum += (float)rest[e];
                 pl = __builtin_bit_cast(u32x4_t, rest);
             }
-        }
+        };
+        if (nc == F && s0 + F <= span.na && chunk_at(s0) * 32 >= lo_max && chunk_at(s0 + F - 1) * 32 + 32 <= hi_min) silu(std::false_type{});
+        else silu(std::true_type{});
         auto sums = [&](const unsigned (&x)[U][8][VW], int c0) __attribute__((always_inline)) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {

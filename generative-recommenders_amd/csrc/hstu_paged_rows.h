@@ -171,12 +171,12 @@ __global__ __launch_bounds__(256) void hstu_paged_append_kernel(const AppendPara
         unsigned* scales_of = (unsigned*)(which ? c.v_scales : c.k_scales);
         const bool changed = !which && (p.k_weight || p.turn.rotary);
         LaneTurn t;
-        NormTurn nt;
+        float w[8];
         bool known = true;
         if (changed) {
             t.lane(p.turn, col0, l);
             if (p.turn.rotary && stored) known = t.row(p.turn, p.positions ? index_at(p.positions, p.positions_i64, row) : place, col0);
-            nt.fill(t, p.turn.interleaved, (const T*)p.k_weight, col0);
+            lane_weights((const T*)p.k_weight, col0, w);
         }
         for (int h = h0; h < h1; h += AHEAD) {
             Cols<T> in[AHEAD];
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(256) void hstu_paged_append_kernel(const AppendPara
                 float x[8];
                 if (changed) {
                     float y[8];
-                    nt.apply<T, LPV>(t, p.turn.interleaved, in[a], cols, p.k_weight != nullptr, p.inv_dim, p.eps, known, y);
+                    norm_and_turn<T, LPV>(t, p.turn, in[a], w, cols, p.k_weight != nullptr, dim, p.inv_dim, p.eps, known, y);
                     Cols<T> rounded;
                     rounded.put(y);
                     rounded.get(x);
