@@ -16,7 +16,7 @@ thread_local char g_last_error[256] = "";
 constexpr int64_t kMaxBlocks = 2147483647;
 
 int lanes_of(int dim) {
-    int lanes = 1;
+    int lanes = 4;
     while (lanes * 8 < dim) lanes *= 2;
     return lanes;
 }
@@ -80,14 +80,18 @@ int launch_status(const char* what) {
 template <class F>
 int with_lanes(int lanes, F&& f) {
     switch (lanes) {
-        case 1: return f(std::integral_constant<int, 1>{});
-        case 2: return f(std::integral_constant<int, 2>{});
         case 4: return f(std::integral_constant<int, 4>{});
         case 8: return f(std::integral_constant<int, 8>{});
         case 16: return f(std::integral_constant<int, 16>{});
         case 32: return f(std::integral_constant<int, 32>{});
         default: return f(std::integral_constant<int, 64>{});
     }
+}
+
+template <class F>
+int with_turn(int rotary, int interleaved, F&& f) {
+    if (!rotary) return f(std::integral_constant<int, hstu::TURN_NONE>{});
+    return interleaved ? f(std::integral_constant<int, hstu::TURN_PAIRS>{}) : f(std::integral_constant<int, hstu::TURN_HALVES>{});
 }
 
 template <class F>
@@ -166,9 +170,11 @@ int hstu_cache_norm_rope(const HstuNormRopeArgs* a, void* stream) {
     return with_type(a->dtype, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
         return with_lanes(lanes, [&](auto l) {
-            hipLaunchKernelGGL((hstu::hstu_norm_rope_kernel<T, decltype(l)::value>), dim3((unsigned)blocks, (unsigned)chunks), dim3(256), 0,
-                               (hipStream_t)stream, p);
-            return launch_status("norm and rotation kernel launch");
+            return with_turn(a->rotary, a->interleaved, [&](auto turn) {
+                hipLaunchKernelGGL((hstu::hstu_norm_rope_kernel<T, decltype(l)::value, decltype(turn)::value>), dim3((unsigned)blocks, (unsigned)chunks), dim3(256), 0,
+                                   (hipStream_t)stream, p);
+                return launch_status("norm and rotation kernel launch");
+            });
         });
     });
 }
@@ -215,8 +221,12 @@ int hstu_cache_norm_rope_bwd(const HstuNormRopeArgs* a, const HstuNormRopeGrads*
     return with_type(a->dtype, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
         return with_lanes(lanes_of(a->dim), [&](auto l) {
-            hipLaunchKernelGGL((hstu::hstu_norm_rope_bwd_kernel<T, decltype(l)::value>), dim3((unsigned)x, (unsigned)y), dim3(256), 0, (hipStream_t)stream, p);
-            if (const int status = launch_status("norm and rotation backward kernel launch")) return status;
+            const int status = with_turn(a->rotary, a->interleaved, [&](auto turn) {
+                hipLaunchKernelGGL((hstu::hstu_norm_rope_bwd_kernel<T, decltype(l)::value, decltype(turn)::value>), dim3((unsigned)x, (unsigned)y), dim3(256), 0,
+                                   (hipStream_t)stream, p);
+                return launch_status("norm and rotation backward kernel launch");
+            });
+            if (status) return status;
             if (!weights) return 0;
             hipLaunchKernelGGL((hstu::hstu_norm_rope_dw_kernel<T>), dim3((a->dim + 15) / 16, 2), dim3(256), 0, (hipStream_t)stream, p.partial, x * y, a->dim,
                                p.side[0].dw ? (T*)g->dq_weight : nullptr, p.side[1].dw ? (T*)g->dk_weight : nullptr);
@@ -251,8 +261,11 @@ int hstu_cache_append(const HstuPagedCache* cache, const HstuAppendArgs* a, void
     if (blocks > kMaxBlocks || chunks > 65535) return HSTU_ERR_UNSUPPORTED;
     auto launch = [&](auto* t, auto l) {
         typedef std::remove_pointer_t<decltype(t)> T;
-        hipLaunchKernelGGL((hstu::hstu_paged_append_kernel<T, decltype(l)::value>), dim3((unsigned)blocks, (unsigned)chunks), dim3(256), 0, (hipStream_t)stream, p);
-        return launch_status("cache append kernel launch");
+        return with_turn(a->rotary, a->interleaved, [&](auto turn) {
+            hipLaunchKernelGGL((hstu::hstu_paged_append_kernel<T, decltype(l)::value, decltype(turn)::value>), dim3((unsigned)blocks, (unsigned)chunks), dim3(256), 0,
+                               (hipStream_t)stream, p);
+            return launch_status("cache append kernel launch");
+        });
     };
     return hstu_cache_dispatch(cache->dtype, lanes, launch);
 }

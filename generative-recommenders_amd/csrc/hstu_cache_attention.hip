@@ -45,16 +45,17 @@ Plan plan_of(const HstuPagedCache* c, const HstuPagedAttentionArgs* a) {
         longest = (int64_t)a->max_attn_len + a->delta_size + a->contextual_seq_len;
     const int64_t chunks = (longest + 31) / 32 + 1, wgs = (int64_t)p.row_blocks * c->heads * c->batch;
     // Runs of a step: as many workgroups as the card holds at once (two of a CU), for each begins with some microseconds of loads that wait
-    // for each other (64 sequences of 1024 .. 4096 positions and four heads, 256 workgroups for whole sequences: runs of 129 chunks, all of one, 28 us,
-    // of 80 26, of 16 35), but none so long that the last of them run alone (128 sequences of up to 16384 and eight heads: runs of 513 290 us, of 384 262,
-    // of 64 286).  Sequences of a few chunks, more of them than fit, are a wave's each (1600 of up to 10 chunks: 12.5 us, 16 by workgroups).
+    // for each other (64 sequences of 1024 .. 4096 positions and four heads, 256 workgroups for whole sequences: runs of 130 chunks, all of one, 28 us,
+    // of 80 26, of 16 30), but none longer than 96 chunks, so that the last of them do not run alone (128 sequences of up to 16384 and eight heads:
+    // whole sequences 291 us, runs of 384 chunks 281, of 103 264, of 33 281).  Sequences of a few chunks, more of them than fit, are a wave's each (1600 of
+    // up to 10 chunks: 12 us, 16 by workgroups).
     // Blocks of many rows: one workgroup of a CU, so whole sequences where there are 256 of them, for a run more is a partial sum of every row to write
     // and read (32 sequences of 1280 .. 4352 positions, 256 rows, four heads: 106 us, of two runs 124); below that as many as there are CUs, none
     // longer than 96 chunks (8 sequences of up to 8192, 512 rows, four heads: runs of 129 111 us, of 86 82).
     const bool blocks = !p.step && p.rw == 4;
     const int64_t slots = blocks ? 256 : 512, fill = (chunks * wgs + slots - 1) / slots;
     int64_t run = a->kv_splits > 0 ? (chunks + a->kv_splits - 1) / a->kv_splits : (fill + 15) / 16 * 16;
-    if (!a->kv_splits && !blocks && run > 384) run = 384;
+    if (!a->kv_splits && !blocks && run > 96) run = 96;
     if (!a->kv_splits && blocks && wgs < 256 && run > 96) run = 96;
     if (run < 16) run = 16;
     if (p.step && chunks <= 17 && wgs > 1024) p.share = 1, run = chunks;

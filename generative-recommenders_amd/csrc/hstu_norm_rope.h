@@ -3,7 +3,7 @@
 //     n = x * rsqrt(mean(x^2) + eps) * w,   y = R n       with R the rotation of the row's position (pairs of columns)
 //     g = R^T dy,   dw = sum over rows and heads of g * x * r,   dx = r * (g w - x r * mean(g w x r)),   r = rsqrt(...)
 //
-// A vector (one row, one head) is taken by LPV = dim / 8 lanes (rounded up to a power of two), eight columns to a lane: one 16-byte
+// A vector (one row, one head) is taken by LPV = dim / 8 lanes (rounded up to a power of two, at least four), eight columns to a lane: one 16-byte
 // access each way in 16 bits, and the sums over a vector are log2(LPV) lane exchanges.  The partner of a column in the half-split
 // form lies rotary / 2 columns on, rotary / 16 lanes away: lanes exchange them.  A group of LPV lanes stays with one row for several heads, so that
 // positions and table rows, which the heads of a row share, are read once.
@@ -101,8 +101,7 @@ struct LaneTurn {
     unsigned keep;      // all ones where the partner counts (an infinity times s = 0 is no zero)
     bool turns, first;  // whether these columns turn; half-split: whether they are in front of their partners
 
-    // Everything that does not depend on the row.
-    // `l`: number of the lane in its group (its columns may be another lane's, see the kernels).
+    // Everything that does not depend on the row.  `l`: number of the lane in its group (its columns may be another lane's, see the kernels).
     __device__ __forceinline__ void lane(const Turn& t, int col0, int l) {
         const int half = t.rotary >> 1, group = (threadIdx.x & 63) - l;
         turns = col0 < t.rotary, first = col0 < half;
@@ -111,36 +110,44 @@ struct LaneTurn {
 #pragma unroll
         for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
     }
-    // Cosines and sines of position `pos`; false where it is not in the table.
-    __device__ __forceinline__ bool row(const Turn& t, int64_t pos, int col0) {
-        if (pos < 0 || pos >= t.table_rows) return false;
-        if (!turns) return true;
+    // Cosines and sines of position `pos`; NaN, for every column, where it is not in the table.
+    __device__ __forceinline__ void row(const Turn& t, int64_t pos, int col0) {
+        const bool there = pos >= 0 && pos < t.table_rows;
+        const float one = there ? 1.f : __builtin_nanf("");
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = one, s[i] = 0.f;
+        if (!turns || !there) return;
         const int half = t.rotary >> 1;
         const float* cp = t.table + pos * t.rotary + (t.interleaved ? col0 >> 1 : (first ? col0 : col0 - half));
         typedef __attribute__((ext_vector_type(4))) float f4;
-        const f4 c0 = *(const f4*)cp, s0 = *(const f4*)(cp + half);
         if (t.interleaved) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[2 * i] = c[2 * i + 1] = c0[i], s[2 * i] = -s0[i], s[2 * i + 1] = s0[i];
-        } else {
-            const f4 c1 = *(const f4*)(cp + 4), s1 = *(const f4*)(cp + half + 4);
+            for (int k = 0; k < 4; k += 4) {
+                const f4 ck = *(const f4*)(cp + k), sk = *(const f4*)(cp + half + k);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                c[i] = c0[i], c[4 + i] = c1[i];
-                s[i] = first ? -s0[i] : s0[i], s[4 + i] = first ? -s1[i] : s1[i];
+                for (int i = 0; i < 4; ++i) c[2 * (k + i)] = c[2 * (k + i) + 1] = ck[i], s[2 * (k + i)] = -sk[i], s[2 * (k + i) + 1] = sk[i];
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k += 4) {
+                const f4 ck = *(const f4*)(cp + k), sk = *(const f4*)(cp + half + k);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) c[k + i] = ck[i], s[k + i] = first ? -sk[i] : sk[i];
             }
         }
-        return true;
     }
 };
 
-// The partners of a lane's columns.  `all`: whether every column of a vector turns.
-__device__ __forceinline__ void partners(const LaneTurn& t, int interleaved, bool all, const float (&x)[8], float (&p)[8]) {
+// How vectors turn, as the kernels are built for it: not at all, halves or neighbouring pairs.
+enum { TURN_NONE = 0, TURN_HALVES = 1, TURN_PAIRS = 2 };
+
+// The partners of a lane's columns, zero where they do not count.
+template <int TURN>
+__device__ __forceinline__ void partners(const LaneTurn& t, const float (&x)[8], float (&p)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = interleaved ? x[i ^ 1] : __uint_as_float((unsigned)__builtin_amdgcn_ds_bpermute(t.byte_lane, (int)__float_as_uint(x[i])));
-    if (!all) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = __uint_as_float(__float_as_uint(p[i]) & t.keep);
+    for (int i = 0; i < 8; ++i) {
+        const unsigned w = TURN == TURN_PAIRS ? __float_as_uint(x[i ^ 1]) : (unsigned)__builtin_amdgcn_ds_bpermute(t.byte_lane, (int)__float_as_uint(x[i]));
+        p[i] = __uint_as_float(w & t.keep);
     }
 }
 
@@ -168,38 +175,30 @@ __device__ __forceinline__ float inverse_rms(const float (&x)[8], bool there, fl
     for (int i = 0; i < 8; ++i) q[i] = x[i] * x[i];
     const float sum = LPV >= 16 ? (q[0] + q[1] + q[2] + q[3]) + (q[4] + q[5] + q[6] + q[7]) : ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
     const float v = group_sum<LPV>(there ? sum : 0.f) * inv_dim + eps;
-    const float r = rsqrtf(v), h = v * r, low = __builtin_fmaf(v, r, -h);
+    const float r = __builtin_amdgcn_rsqf(v), h = v * r, low = __builtin_fmaf(v, r, -h);
     const float fixed = __builtin_fmaf(0.5f * r, __builtin_fmaf(-low, r, __builtin_fmaf(-h, r, 1.f)), r);
     return v > 0x1p-100f && v < 0x1p100f ? fixed : r;
 }
 
-// A vector as loaded to what is rounded and stored; `there`: whether the lane's columns are the vector's (one that has none holds another's),
-// `known`: whether its position is.  The operations are rounded one by one, as the definition has them: K is rounded to its type next and then
+// A vector as loaded to what is rounded and stored; `there`: whether the lane's columns are the vector's (one that has none holds another's).
+// The operations are rounded one by one, as the definition has them: K is rounded to its type next and then
 // to codes, where a value that comes out a unit in the last place off now and then is a whole step off.  (Weights multiplied into cosines and
 // sines, and sums by fused operations, gave twenty such codes in 18 million; this costs no more.)
-template <class T, int LPV>
-__device__ __forceinline__ void norm_and_turn(const LaneTurn& t, const Turn& how, const Cols<T>& in, const float (&w)[8], bool there, bool norm, int dim,
-                                              float inv_dim, float eps, bool known, float (&y)[8]) {
+template <class T, int LPV, int TURN>
+__device__ __forceinline__ void norm_and_turn(const LaneTurn& t, const Cols<T>& in, const float (&w)[8], bool there, bool norm, float inv_dim, float eps,
+                                              float (&y)[8]) {
 #pragma clang fp contract(off)
-    float n[8], p[8];
-    in.get(n);
+    in.get(y);
     if (norm) {
-        const float r = inverse_rms<LPV>(n, there, inv_dim, eps);
+        const float r = inverse_rms<LPV>(y, there, inv_dim, eps);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) n[i] = n[i] * r * w[i];
+        for (int i = 0; i < 8; ++i) y[i] = y[i] * r * w[i];
     }
-    if (how.rotary) {
-        partners(t, how.interleaved, how.rotary == dim, n, p);
-        const float nan = known ? 0.f : __builtin_nanf("");
+    if constexpr (TURN != TURN_NONE) {
+        float p[8];
+        partners<TURN>(t, y, p);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = n[i] * t.c[i] + p[i] * t.s[i];
-        if (!known) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = nan;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = n[i];
+        for (int i = 0; i < 8; ++i) y[i] = y[i] * t.c[i] + p[i] * t.s[i];
     }
 }
 
@@ -229,7 +228,7 @@ struct NormRopeParams {
 };
 
 // grid (rows / groups of a workgroup, heads / heads_per_group): heads count through q's, then k's.
-template <class T, int LPV>
+template <class T, int LPV, int TURN>
 __global__ __launch_bounds__(256) void hstu_norm_rope_kernel(const NormRopeParams p) {
     constexpr int GROUPS = 256 / LPV, AHEAD = 4;
     // Lanes without columns, and groups without a row, go along with the last of them that there are and store nothing: loads need no
@@ -242,8 +241,7 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_kernel(const NormRopeParam
     if (row >= p.rows) row = p.rows - 1;
     LaneTurn t;
     t.lane(p.turn, col0, l);
-    bool known = true;
-    if (p.turn.rotary) known = t.row(p.turn, index_at(p.positions, p.positions_i64, row), col0);
+    if constexpr (TURN != TURN_NONE) t.row(p.turn, index_at(p.positions, p.positions_i64, row), col0);
     const int first = blockIdx.y * p.heads_per_group, last = min(first + p.heads_per_group, p.side[0].heads + p.side[1].heads);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
@@ -263,7 +261,7 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_kernel(const NormRopeParam
             for (int a = 0; a < AHEAD; ++a) {
                 if (h + a >= h1) break;  // (the same for the whole workgroup)
                 float y[8];
-                norm_and_turn<T, LPV>(t, p.turn, in[a], w, cols, s.weight != nullptr, p.dim, p.inv_dim, p.eps, known, y);
+                norm_and_turn<T, LPV, TURN>(t, in[a], w, cols, s.weight != nullptr, p.inv_dim, p.eps, y);
                 Cols<T> o;
                 o.put(y);
                 if (there) o.store(out + (h + a) * p.dim);
@@ -274,7 +272,7 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_kernel(const NormRopeParam
 
 // The same grid, but a workgroup goes on to further rows, so that the sums for the weights stay in registers: each lane adds up its
 // columns, the groups of a workgroup meet in LDS, and the workgroups' sums are added by the kernel below.
-template <class T, int LPV>
+template <class T, int LPV, int TURN>
 __global__ __launch_bounds__(256) void hstu_norm_rope_bwd_kernel(const NormRopeParams p) {
     constexpr int GROUPS = 256 / LPV, AHEAD = 2;
     __shared__ float meet[256 * 8];
@@ -293,8 +291,7 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_bwd_kernel(const NormRopeP
         int64_t row = base_row + threadIdx.x / LPV;
         const bool there = cols && row < p.rows;
         if (row >= p.rows) row = p.rows - 1;
-        bool known = true;
-        if (p.turn.rotary) known = t.row(p.turn, index_at(p.positions, p.positions_i64, row), col0);
+        if constexpr (TURN != TURN_NONE) t.row(p.turn, index_at(p.positions, p.positions_i64, row), col0);
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             const NormRopeSide& s = p.side[which];
@@ -319,12 +316,13 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_bwd_kernel(const NormRopeP
                     if (h + a >= h1) break;
                     float x[8], d[8], q[8], g[8];
                     dy[a].get(d);
-                    partners(t, p.turn.interleaved, p.turn.rotary == p.dim, d, q);
+                    if constexpr (TURN != TURN_NONE) {
+                        partners<TURN>(t, d, q);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) g[i] = d[i] * t.c[i] - q[i] * t.s[i];  // R^T: the partner's sine is the other's with its sign changed
-                    if (!known) {
+                        for (int i = 0; i < 8; ++i) g[i] = d[i] * t.c[i] - q[i] * t.s[i];  // R^T: the partner's sine is the other's with its sign changed
+                    } else {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) g[i] = __builtin_nanf("");
+                        for (int i = 0; i < 8; ++i) g[i] = d[i];
                     }
                     if (s.weight) {
                         in[a].get(x);

@@ -88,12 +88,12 @@ __device__ __forceinline__ int64_t cache_row(const PagedCache& c, int b, int64_t
 // Smallest and largest of eight columns, NaN where one is; and over LPV lanes (numbers only).  The instructions themselves: the
 // compiler puts another in front of each operand of its min and max, to quiet NaNs.
 __device__ __forceinline__ void extremes(const float (&x)[8], float& lo, float& hi) {
-    asm("v_minimum3_f32 %0, %2, %3, %4\n\tv_maximum3_f32 %1, %2, %3, %4\n\t"
-        "v_minimum3_f32 %0, %0, %5, %6\n\tv_maximum3_f32 %1, %1, %5, %6\n\t"
-        "v_minimum3_f32 %0, %0, %7, %8\n\tv_maximum3_f32 %1, %1, %7, %8\n\t"
-        "v_minimum3_f32 %0, %0, %9, %9\n\tv_maximum3_f32 %1, %1, %9, %9"
-        : "=&v"(lo), "=&v"(hi)
-        : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]), "v"(x[7]));
+    lo = hi = x[0];
+#pragma unroll
+    for (int i = 1; i < 8; i += 2) {
+        const float a = x[i], b = x[i < 7 ? i + 1 : i];
+        asm("v_minimum3_f32 %0, %0, %2, %3\n\tv_maximum3_f32 %1, %1, %2, %3" : "+&v"(lo), "+&v"(hi) : "v"(a), "v"(b));
+    }
 }
 #define HSTU_EXTREMES_DPP(how)                                                                                                              \
     asm("s_nop 1\n\tv_min_f32_dpp %0, %0, %0 " how " row_mask:0xf bank_mask:0xf\n\tv_max_f32_dpp %1, %1, %1 " how " row_mask:0xf bank_mask:0xf" \
@@ -109,7 +109,7 @@ __device__ __forceinline__ void group_extremes(float& lo, float& hi) {
 }
 #undef HSTU_EXTREMES_DPP
 
-// Eight columns of LPV lanes' row to a word of codes, and step and lowest value.  (Lanes behind the row's end hold other columns of it.)
+// Eight columns of each of LPV lanes to a word of codes, and the row's step and lowest value.  (Lanes behind the row's end hold other columns of it.)
 // The quotient x / step is rounded as IEEE says by Markstein's correction: q = a y with y the reciprocal of b to a unit in the last
 // place, then q + (a - q b) y, whose remainder is exact; three operations a column where the compiler's division takes some fourteen.
 // It is exact where the quotient is a float, which a tie between two codes is.
@@ -130,7 +130,6 @@ __device__ __forceinline__ unsigned to_four_bits(const float (&x)[8], unsigned& 
     T2 both;
     both[0] = step_t, both[1] = lo_t;
     scale = __builtin_bit_cast(unsigned, both);
-    if (!(step > 0.f)) return 0;
     // step and columns by a power of two that takes the step to 1/2 .. 1, or some way there from below 2^-100
     const float by = __builtin_amdgcn_ldexpf(1.f, -max(__builtin_amdgcn_frexp_expf(step), -100) - 1), from = -lo * by, b = step * by;
     const float y0 = __builtin_amdgcn_rcpf(b), y = __builtin_fmaf(__builtin_fmaf(-b, y0, 1.f), y0, y0);
@@ -143,11 +142,13 @@ __device__ __forceinline__ unsigned to_four_bits(const float (&x)[8], unsigned& 
     // four codes are one number below 2^16, exact in a float
     const float low = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(code[3], 16.f, code[2]), 16.f, code[1]), 16.f, code[0]);
     const float high = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(code[7], 16.f, code[6]), 16.f, code[5]), 16.f, code[4]);
-    return (unsigned)low | ((unsigned)high << 16);
+    return step > 0.f ? (unsigned)low | ((unsigned)high << 16) : 0u;
 }
 
 // grid (rows / groups of a workgroup, vectors / vectors_per_group): a row's vectors count through its heads of K, then of V.
-template <class T, int LPV>
+// (16 columns to a lane, which do what a row takes once in half as many lanes, came to a third fewer instructions and to the same time: 98 us
+// for append_prefill, four waves of a SIMD in 107 registers where six have 78.  So did the first loads in front of the lookups.)
+template <class T, int LPV, int TURN>
 __global__ __launch_bounds__(256) void hstu_paged_append_kernel(const AppendParams p) {
     constexpr int GROUPS = 256 / LPV, AHEAD = 4;
     const int l = threadIdx.x % LPV;
@@ -166,16 +167,15 @@ __global__ __launch_bounds__(256) void hstu_paged_append_kernel(const AppendPara
         const bool cols = 8 * l < dim;
         const int col0 = cols ? 8 * l : dim - 8;
         const T* x_of = (const T*)(which ? p.v : p.k) + row * (which ? p.v_rs : p.k_rs) + col0;
-        const int64_t hs = which ? p.v_hs : p.k_hs;
-        unsigned* codes_of = (unsigned*)(which ? c.v_codes : c.k_codes);
-        unsigned* scales_of = (unsigned*)(which ? c.v_scales : c.k_scales);
-        const bool changed = !which && (p.k_weight || p.turn.rotary);
+        const int64_t hs = which ? p.v_hs : p.k_hs, next_codes = (int64_t)(dim >> 1) << c.page_shift, next_scales = 4ll << c.page_shift;  // bytes to the next head
+        char* codes_at = (which ? c.v_codes : c.k_codes) + to * (dim >> 1) + 4 * l;
+        char* scales_at = (which ? c.v_scales : c.k_scales) + to * 4;
+        const bool changed = !which && (TURN != TURN_NONE || p.k_weight);
         LaneTurn t;
         float w[8];
-        bool known = true;
         if (changed) {
             t.lane(p.turn, col0, l);
-            if (p.turn.rotary && stored) known = t.row(p.turn, p.positions ? index_at(p.positions, p.positions_i64, row) : place, col0);
+            if (TURN != TURN_NONE && stored) t.row(p.turn, p.positions ? index_at(p.positions, p.positions_i64, row) : place, col0);
             lane_weights((const T*)p.k_weight, col0, w);
         }
         for (int h = h0; h < h1; h += AHEAD) {
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(256) void hstu_paged_append_kernel(const AppendPara
                 float x[8];
                 if (changed) {
                     float y[8];
-                    norm_and_turn<T, LPV>(t, p.turn, in[a], w, cols, p.k_weight != nullptr, dim, p.inv_dim, p.eps, known, y);
+                    norm_and_turn<T, LPV, TURN>(t, in[a], w, cols, p.k_weight != nullptr, p.inv_dim, p.eps, y);
                     Cols<T> rounded;
                     rounded.put(y);
                     rounded.get(x);
@@ -197,9 +197,8 @@ __global__ __launch_bounds__(256) void hstu_paged_append_kernel(const AppendPara
                 }
                 unsigned scale;
                 const unsigned codes = to_four_bits<T, LPV>(x, scale);
-                const int64_t at = to + ((int64_t)(h + a) << c.page_shift);
-                if (stored && cols) codes_of[at * (dim >> 3) + l] = codes;
-                if (stored && l == 0) scales_of[at] = scale;
+                if (stored && cols) *(unsigned*)(codes_at + (h + a) * next_codes) = codes;
+                if (stored && l == 0) *(unsigned*)(scales_at + (h + a) * next_scales) = scale;
             }
         }
     }
