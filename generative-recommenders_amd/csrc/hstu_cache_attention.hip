@@ -35,7 +35,8 @@ Plan plan_of(const HstuPagedCache* c, const HstuPagedAttentionArgs* a) {
         if (rows > 16) p.mt = c->dv == 256 ? 1 : 2;
         if (rows > 16 * p.mt) {
             p.rw = 4;
-            if (rows <= 64) p.mt = 1;
+            // (blocks of 128 rows take 1.75 times as long as blocks of 64: 132 rows in three of 64 25 us, in two of 128 30)
+            if (4 * ((rows + 63) / 64) < 7 * ((rows + 127) / 128)) p.mt = 1;
         }
         p.block = 16 * p.mt * p.rw;
     }
@@ -49,19 +50,23 @@ Plan plan_of(const HstuPagedCache* c, const HstuPagedAttentionArgs* a) {
     // of 80 26, of 16 30), but none longer than 96 chunks, so that the last of them do not run alone (128 sequences of up to 16384 and eight heads:
     // whole sequences 291 us, runs of 384 chunks 281, of 103 264, of 33 281).  Sequences of a few chunks, more of them than fit, are a wave's each (1600 of
     // up to 10 chunks: 12 us, 16 by workgroups).
-    // Blocks of many rows: one workgroup of a CU, so whole sequences where there are 256 of them, for a run more is a partial sum of every row to write
-    // and read (32 sequences of 1280 .. 4352 positions, 256 rows, four heads: 106 us, of two runs 124); below that as many as there are CUs, none
-    // longer than 96 chunks (8 sequences of up to 8192, 512 rows, four heads: runs of 129 111 us, of 86 82).
+    // Blocks of many rows: two workgroups of a CU, for a run more is a partial sum of every row to write and read; parts of a sequence are equal, so that
+    // ranking the sequences balances them.
     const bool blocks = !p.step && p.rw == 4;
-    const int64_t slots = blocks ? 256 : 512, fill = (chunks * wgs + slots - 1) / slots;
+    const int64_t fill = (chunks * wgs + 511) / 512;
     int64_t run = a->kv_splits > 0 ? (chunks + a->kv_splits - 1) / a->kv_splits : (fill + 15) / 16 * 16;
-    if (!a->kv_splits && !blocks && run > 96) run = 96;
-    if (!a->kv_splits && blocks && wgs < 256 && run > 96) run = 96;
+    if (!a->kv_splits && run > 96) run = 96;
     if (run < 16) run = 16;
+    if (blocks) {
+        int64_t parts = a->kv_splits > 0 ? a->kv_splits : wgs > 0 ? (512 + wgs - 1) / wgs : 1;
+        if (parts > (chunks + 7) / 8) parts = (chunks + 7) / 8;
+        run = 8;
+        p.splits = (int)parts;
+    }
     if (p.step && chunks <= 17 && wgs > 1024) p.share = 1, run = chunks;
     if (run > chunks) run = chunks;
     p.run = (int)run;
-    p.splits = (int)((chunks + run - 1) / run);
+    if (!blocks) p.splits = (int)((chunks + run - 1) / run);
     if (p.splits > 1) p.workspace = p.splits * c->batch * a->delta_size * a->q_heads * (int64_t)c->dv * 4;
     return p;
 }
@@ -75,7 +80,7 @@ int launch_sized(const hstu::PagedAttentionParams& p, const Plan& plan, hipStrea
         hipLaunchKernelGGL((hstu::hstu_paged_attention_kernel<TT, DK, DV, decltype(mt)::value, 1>), dim3(blocks), dim3(256), 0, stream, p);
     };
     auto block = [&](auto mt) {
-        hipLaunchKernelGGL((hstu::hstu_paged_block_kernel<TT, DK, DV, decltype(mt)::value>), dim3(blocks), dim3(512), 0, stream, p);
+        hipLaunchKernelGGL((hstu::hstu_paged_block_kernel<TT, DK, DV, decltype(mt)::value>), dim3((unsigned)(p.items * (int64_t)plan.row_blocks)), dim3(256), 0, stream, p);
     };
     typedef std::integral_constant<int, 2> Two;
     typedef std::integral_constant<int, 4> Four;

@@ -73,8 +73,8 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttentionParams& p, i
     return s;
 }
 
-// Chunks of a run: `run`, or more where a sequence is longer than it should be.
-__device__ __forceinline__ int chunks_per_run(const PagedAttentionParams& p, int chunks) { return max(p.run, (chunks + p.splits - 1) / p.splits); }
+// Chunks of a run: `run`, or more where the splits would not do; an even number.
+__device__ __forceinline__ int chunks_per_run(const PagedAttentionParams& p, int chunks) { return (max(p.run, (chunks + p.splits - 1) / p.splits) + 1) & ~1; }
 
 // What one row sees: positions [lo, hi), [0, chi) and itself.
 struct RowSpan {
@@ -470,27 +470,51 @@ __global__ __launch_bounds__(256) void hstu_paged_attention_kernel(const PagedAt
     }
 }
 
-// The same for many rows: two teams of four waves; a team's waves take 16 MT rows each and share what unpacking yields.  A step is 32 CH positions
-// for each team; each wave unpacks its part of them -- a tile of 16 positions of K, a quarter of the columns of V -- into LDS, in the order in which the
+// Which part of the work this workgroup takes: sequence * each + (part of the sequence).  The longest sequences first, so that the last workgroups are
+// short ones; and where all of them run at once, two to a CU, the second of a CU's is as short as its first is long.  Every workgroup ranks the lengths
+// for itself, in LDS (256 of them take a microsecond); more sequences than that stay in their order.
+__device__ __forceinline__ int block_order(const PagedAttentionParams& p, int each, int* lengths) {
+    const int batch = p.cache.batch, total = batch * each;
+    int at = blockIdx.x;
+    if (batch > 256 || batch < 2) return at;
+    if (total <= 512 && at >= 256) at = total - 1 - (at - 256);  // (of 256 .. 511 the last first)
+    const int t = threadIdx.x;
+    if (t < batch) {
+        const int64_t n = index_at(p.lengths, p.lengths_i64, t);
+        lengths[t] = n < 0 ? 0 : n > (1 << 30) ? 1 << 30 : (int)n;
+    }
+    __syncthreads();
+    if (t < batch) {
+        const int n = lengths[t];
+        int rank = 0;
+        for (int i = 0; i < batch; ++i) rank += lengths[i] > n || (lengths[i] == n && i < t);
+        lengths[256 + rank] = t;
+    }
+    __syncthreads();
+    const int b = __builtin_amdgcn_readfirstlane(lengths[256 + at / each]);
+    __syncthreads();
+    return b * each + at % each;
+}
+
+// The same for many rows: the four waves of a workgroup take 16 MT rows each and share what unpacking yields.  A step is 32 CH positions;
+// each wave unpacks its part of them -- a tile of 16 positions of K, a quarter of the columns of V -- into LDS, in the order in which the
 // products' operands lie in registers (a lane's 16 bytes side by side: reads and writes without bank conflicts), and the pairs as four
 // floats a position: c1 s, c1 l of K, s, l + 7.5 s of V.  Two buffers, one barrier a step; the packed rows of the next step are on their way
-// while this one is worked on.  The teams' sums meet at the end: two waves to a SIMD, without the joining kernel that as many
-// workgroups of one team would need.  Unpacking per wave, as above, cost as much as half of the rest and the registers of a second wave.
+// while this one is worked on.  Two workgroups of a CU, out of step with each other, fill the gaps of one another: the same two
+// teams of waves in one workgroup, behind one barrier, took 106 us for attention_candidates.  Unpacking per wave, as above, cost as much as half of the rest and the registers of a second wave.
 template <class TT, int DK, int DV, int MT>
-__global__ __launch_bounds__(512, 2) void hstu_paged_block_kernel(const PagedAttentionParams p) {
+__global__ __launch_bounds__(256, 2) void hstu_paged_block_kernel(const PagedAttentionParams p) {
     typedef typename TT::elem T;
     typedef __attribute__((ext_vector_type(2))) T T2;
     constexpr int NK = DK / 32, NV = DV / 16, CH = DK == 256 ? 1 : 2, TILES = 2 * CH, HALVES = (NV + 3) / 4, KB = TILES * NK, VB = CH * NV;
-    constexpr int V_UNITS = CH * HALVES, ROWS = 64 * MT, STEP = 2 * CH;
+    constexpr int V_UNITS = CH * HALVES, ROWS = 64 * MT;
     static_assert(TILES <= 4 && V_UNITS <= 4, "one unit of K and one of V to a wave");
-    __shared__ u32x4_t frags_of[2][2][(KB + VB) * 64];  // [team][buffer]
-    __shared__ pa_f32x4 pairs_of[2][2][4][CH * 8];      // [team][buffer][which][position / 4]
+    __shared__ u32x4_t frags[2][(KB + VB) * 64];
+    __shared__ pa_f32x4 pairs[2][4][CH * 8];  // [buffer][which][position / 4]
     const PagedCache& c = p.cache;
-    const int xcd = blockIdx.x & 7, q8 = blockIdx.x >> 3;
-    const int rb = q8 % p.row_blocks, item = (q8 / p.row_blocks) * 8 + xcd;
-    if (item >= p.items) return;
-    const int hk = item % c.heads, b = (item / c.heads) % c.batch, split = item / (c.heads * c.batch);
-    const int wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), team = wave8 >> 2, wave = wave8 & 3, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+    const int each = c.heads * p.row_blocks * p.splits, part = block_order(p, each, (int*)&frags[0][0]);
+    const int b = part / each, rest = part - b * each, hk = rest % c.heads, rb = (rest / c.heads) % p.row_blocks, split = rest / (c.heads * p.row_blocks);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const int rows = p.delta * p.group, r_end = min((rb + 1) * ROWS, rows);
     const PagedSpan span = paged_span(p, b, rb * ROWS / p.group, (r_end - 1) / p.group + 1);
     const int chunks = span.na + span.nb, per = chunks_per_run(p, chunks), begin = split * per, end = min(begin + per, chunks);
@@ -498,8 +522,6 @@ __global__ __launch_bounds__(512, 2) void hstu_paged_block_kernel(const PagedAtt
     auto chunk_at = [&](int i) { return i < span.na ? span.a0 + i : span.b0 + (i - span.na); };
 
     // ---- unpacking ----
-    auto& frags = frags_of[team];
-    auto& pairs = pairs_of[team];
     const typename TT::codes k_codes;
     const CodesBf16 v_codes;
     const int in_page = (1 << c.page_shift) - 1;
@@ -588,7 +610,7 @@ __global__ __launch_bounds__(512, 2) void hstu_paged_block_kernel(const PagedAtt
         }
     };
 
-    if (begin < end) load(begin + team * CH);
+    if (begin < end) load(begin);
     // ---- rows ----
     u32x4_t qf[MT][NK];
     float qs[MT], qo[MT];
@@ -722,18 +744,17 @@ __global__ __launch_bounds__(512, 2) void hstu_paged_block_kernel(const PagedAtt
     }
     int buffer = 0;
     auto step = [&](int i, auto masked) __attribute__((always_inline)) {
-        const bool more = i + STEP < end;
-        const int mine = i + team * CH;
-        if (more) load(mine + STEP);
+        const bool more = i + CH < end;
+        if (more) load(i + CH);
 #pragma unroll
         for (int cc = 0; cc < CH; ++cc) {
             if constexpr (decltype(masked)::value) {
-                if (mine + cc < end) {
-                    const int chunk = chunk_at(mine + cc), first = chunk * 32;  // (not where this wave's rows see nothing of it)
+                if (i + cc < end) {
+                    const int chunk = chunk_at(i + cc), first = chunk * 32;  // (not where this wave's rows see nothing of it)
                     if ((first < any_hi && first + 32 > any_lo) || first < any_chi || (first <= self_hi && first + 32 > self_lo)) work_masked(buffer, cc, chunk, masked);
                 }
             } else {
-                work_masked(buffer, cc, chunk_at(mine + cc), masked);
+                work_masked(buffer, cc, chunk_at(i + cc), masked);
             }
         }
         if (more) unpack(buffer ^ 1);
@@ -743,44 +764,29 @@ __global__ __launch_bounds__(512, 2) void hstu_paged_block_kernel(const PagedAtt
     if (begin < end) unpack(0);
     __syncthreads();
     int i = begin;
-    for (; i < end && !(i >= whole0 && i + STEP <= whole1); i += STEP) step(i, std::true_type{});
-    for (; i + STEP <= min(end, whole1); i += STEP) step(i, std::false_type{});
-    for (; i < end; i += STEP) step(i, std::true_type{});
+    for (; i < end && !(i >= whole0 && i + CH <= whole1); i += CH) step(i, std::true_type{});
+    for (; i + CH <= min(end, whole1); i += CH) step(i, std::false_type{});
+    for (; i < end; i += CH) step(i, std::true_type{});
 
     // one wave's bad page is everyone's
-    int* said = (int*)&pairs_of[0][0][0][0];
+    int* said = (int*)&pairs[0][0][0];
     if (threadIdx.x == 0) *said = 0;
     __syncthreads();
     if (bad) *said = 1;
     __syncthreads();
     bad = *said != 0;
-    // the second team's sums through LDS, one tile of rows at a time
-    float* meet = (float*)&frags_of[0][0][0] + wave * (4 * NV * 64);
-    static_assert(sizeof(frags_of) >= 4 * 4 * NV * 64 * sizeof(float), "room for the sums of four waves");
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         float lower = plo[mt];
         lower += __shfl_xor(lower, 16, 64);
         lower += __shfl_xor(lower, 32, 64);
         if (bad) lower = __builtin_nanf("");
+        if (out_at[mt] < 0) continue;
         float o[4][NV];
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4)
 #pragma unroll
             for (int j = 0; j < NV; ++j) o[i4][j] = acc[mt][j][i4] - (CodesBf16::off(j & 3) + 7.5f) * psum[mt][i4] + lower;
-        if (mt > 0) __syncthreads();
-        if (team == 1) {
-#pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4)
-#pragma unroll
-                for (int j = 0; j < NV; ++j) meet[(i4 * NV + j) * 64 + lane] = o[i4][j];
-        }
-        __syncthreads();
-        if (team == 1 || out_at[mt] < 0) continue;
-#pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4)
-#pragma unroll
-            for (int j = 0; j < NV; ++j) o[i4][j] += meet[(i4 * NV + j) * 64 + lane];
         store_columns<T, NV>(p, split, out_at[mt] + NV * 4 * g, o);
     }
 }
