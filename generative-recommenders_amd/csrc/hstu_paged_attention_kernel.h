@@ -178,59 +178,35 @@ struct PagedChunk {
     static constexpr int VW = NV == 16 ? 2 : 1;
     unsigned k[2][NK], v[8][VW];
     u32x4_t ks[2], vs[2];
-};
-
-template <int DK, int DV>
-struct PagedReader {
-    static constexpr int NK = DK / 32, NV = DV / 16;
-    const PagedCache& c;
-    int64_t table_row;
-    int head, n, lane;
-    bool bad;
-
-    // Row of head `head` where 16 positions from `pos` on lie (pos a multiple of 16).  Positions that do not exist get the first page.
-    __device__ __forceinline__ int64_t row_of(int pos) {
-        int64_t page = 0;
-        if (pos < n) {
-            page = index_at(c.page_table, c.page_table_i64, table_row + (pos >> c.page_shift));
-            if (page < 0 || page >= c.pages) bad = true, page = 0;
-        }
-        return ((page * c.heads + head) << c.page_shift) + (pos & ((1 << c.page_shift) - 1));
-    }
-
-    __device__ __forceinline__ void load(PagedChunk<NK, NV>& x, int chunk) {
-        const int m = lane & 15, g = lane >> 4;
+    // Tile tt from `row` of the cache on.
+    __device__ __forceinline__ void load(const PagedCache& c, int64_t row, int tt, int lane) {
+        constexpr int KROW = 16 * NK, VROW = 8 * NV;  // bytes
+        const unsigned m = lane & 15, g = lane >> 4;
+        const UniformRows kr(c.k_codes + row * KROW, 16 * KROW), vr(c.v_codes + row * VROW, 16 * VROW), ksr(c.k_scales + row * 4, 64), vsr(c.v_scales + row * 4, 64);
+        const unsigned k_lane = m * KROW + g * (4 * NK), v_lane = 4 * g * VROW + m * (NV / 2);
+        if constexpr (NK == 1) {
+            k[tt][0] = kr.template at<unsigned>(k_lane);
+        } else if constexpr (NK == 2) {
+            const u32x2_t a = kr.template at<u32x2_t>(k_lane);
+            k[tt][0] = a.x, k[tt][1] = a.y;
+        } else {
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-            const int64_t row = row_of(chunk * 32 + tt * 16);
-            const char* k = c.k_codes + row * (DK / 2) + m * (DK / 2) + g * (4 * NK);
-            if constexpr (NK == 1) {
-                x.k[tt][0] = *(const unsigned*)k;
-            } else if constexpr (NK == 2) {
-                typedef __attribute__((ext_vector_type(2))) unsigned u2;
-                const u2 a = *(const u2*)k;
-                x.k[tt][0] = a.x, x.k[tt][1] = a.y;
-            } else {
-#pragma unroll
-                for (int j = 0; j < NK; j += 4) {
-                    const u32x4_t a = *(const u32x4_t*)(k + 4 * j);
-                    x.k[tt][j] = a.x, x.k[tt][j + 1] = a.y, x.k[tt][j + 2] = a.z, x.k[tt][j + 3] = a.w;
-                }
+            for (int j = 0; j < NK; j += 4) {
+                const u32x4_t a = kr.template at<u32x4_t>(k_lane + 4 * j);
+                k[tt][j] = a.x, k[tt][j + 1] = a.y, k[tt][j + 2] = a.z, k[tt][j + 3] = a.w;
             }
-            const char* v = c.v_codes + row * (DV / 2) + 4 * g * (DV / 2) + m * (NV / 2);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const char* vi = v + i * (DV / 2);
-                if constexpr (NV == 2) x.v[4 * tt + i][0] = *(const unsigned char*)vi;
-                else if constexpr (NV == 4) x.v[4 * tt + i][0] = *(const unsigned short*)vi;
-                else {
-#pragma unroll
-                    for (int j = 0; j < NV / 8; ++j) x.v[4 * tt + i][j] = *(const unsigned*)(vi + 4 * j);
-                }
-            }
-            x.ks[tt] = *(const u32x4_t*)(c.k_scales + (row + 4 * g) * 4);
-            x.vs[tt] = *(const u32x4_t*)(c.v_scales + (row + 4 * g) * 4);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned at = v_lane + i * VROW;
+            if constexpr (NV == 2) v[4 * tt + i][0] = vr.template at<unsigned char>(at);
+            else if constexpr (NV == 4) v[4 * tt + i][0] = vr.template at<unsigned short>(at);
+            else {
+#pragma unroll
+                for (int j = 0; j < VW; ++j) v[4 * tt + i][j] = vr.template at<unsigned>(at + 4 * j);
+            }
+        }
+        ks[tt] = ksr.template at<u32x4_t>(16 * g), vs[tt] = vsr.template at<u32x4_t>(16 * g);
     }
 };
 
@@ -254,21 +230,19 @@ __device__ __forceinline__ void store_columns(const PagedAttentionParams& p, int
     }
 }
 
-// grid: one workgroup of four waves per (block of 16 MT RW rows, head of the cache, run, sequence), numbered so that the row blocks
-// of one run, which read the same pages, are on one XCD.  RW waves share out the rows, the others the chunks of the run; the sums of
-// the latter meet in LDS.
-template <class TT, int DK, int DV, int MT, int RW>
+// grid: one workgroup of four waves per (block of 16 MT rows, head of the cache, run, sequence), numbered so that the row blocks of one
+// run, which read the same pages, are on one XCD.  The waves share out the chunks of the run; their sums meet in LDS.
+template <class TT, int DK, int DV, int MT>
 __global__ __launch_bounds__(256) void hstu_paged_attention_kernel(const PagedAttentionParams p) {
     typedef typename TT::elem T;
-    constexpr int NK = DK / 32, NV = DV / 16, KW = 4 / RW;
-    __shared__ float meet[KW > 1 ? 4 * NV * 4 * 64 : 1];
+    constexpr int NK = DK / 32, NV = DV / 16, KW = 4;
+    __shared__ float meet[KW * NV * 4 * 64];
     const int xcd = blockIdx.x & 7, q8 = blockIdx.x >> 3;
     const int rb = q8 % p.row_blocks, item = (q8 / p.row_blocks) * 8 + xcd;
     if (item >= p.items) return;
     const int hk = item % p.cache.heads, split = (item / p.cache.heads) % p.splits, b = item / (p.cache.heads * p.splits);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-    const int rw = wave / KW, kw = wave % KW;
-    constexpr int ROWS = 16 * MT * RW;
+    constexpr int ROWS = 16 * MT;
     const int rows = p.delta * p.group, r_end = min((rb + 1) * ROWS, rows);
     const PagedSpan span = paged_span(p, b, rb * ROWS / p.group, (r_end - 1) / p.group + 1);
     const int chunks = span.na + span.nb, per = chunks_per_run(p, chunks);
@@ -282,7 +256,7 @@ __global__ __launch_bounds__(256) void hstu_paged_attention_kernel(const PagedAt
     int lo_max = 0, hi_min = 1 << 30;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        const int r = rb * ROWS + (rw * MT + mt) * 16 + m;
+        const int r = rb * ROWS + mt * 16 + m;
         const int i = r / p.group, head = hk * p.group + (r - i * p.group);
         qs[mt] = qo[mt] = 0.f;
         see[mt].lo = see[mt].hi = see[mt].chi = 0, see[mt].self = -1;
@@ -325,10 +299,10 @@ __global__ __launch_bounds__(256) void hstu_paged_attention_kernel(const PagedAt
     }
     const typename TT::codes k_codes;
     const CodesBf16 v_codes;
-    PagedReader<DK, DV> reader{p.cache, b * p.cache.table_row_stride, hk, span.n, lane, span.bad};
+    bool bad = span.bad;
 
     auto chunk_at = [&](int i) { return i < span.na ? span.a0 + i : span.b0 + (i - span.na); };
-    auto work_masked = [&](const PagedChunk<NK, NV>& x, int chunk, auto masked) __attribute__((always_inline)) {
+    auto work = [&](const PagedChunk<NK, NV>& x, int chunk, auto masked) __attribute__((always_inline)) {
         const int pos0 = chunk * 32 + 4 * g;
         float ka[8], kb[8], va[8], vm[8];
 #pragma unroll
@@ -401,70 +375,71 @@ __global__ __launch_bounds__(256) void hstu_paged_attention_kernel(const PagedAt
         }
     };
 
-    // (code of their own for chunks that all rows see whole: a condition at each score would stand between them)
-    auto work = [&](const PagedChunk<NK, NV>& x, int chunk) __attribute__((always_inline)) {
-        if (chunk * 32 >= lo_max && chunk * 32 + 32 <= hi_min) work_masked(x, chunk, std::false_type{});
-        else work_masked(x, chunk, std::true_type{});
+    // Pages of the two tiles of 32 of this wave's chunks, KW apart from chunk i on, one to a lane; what does not exist has the first page.  Two
+    // sets: the next one has been loaded when its turn comes.
+    auto pages_of = [&](int i) __attribute__((always_inline)) {
+        int page = 0;
+        const int ci = i + KW * (lane >> 1), pos = ci < chunk_end ? chunk_at(ci) * 32 + (lane & 1) * 16 : span.n;
+        if (pos < span.n) {
+            const int64_t at = index_at(p.cache.page_table, p.cache.page_table_i64, b * p.cache.table_row_stride + (pos >> p.cache.page_shift));
+            if (at < 0 || at >= p.cache.pages) bad = true;
+            else page = (int)at;
+        }
+        return page;
     };
-
-    // two chunks in flight: the next one's loads are issued before the work on this one
-    PagedChunk<NK, NV> x0, x1;
-    int i = split * per + kw;
-    if (i < chunk_end) reader.load(x0, chunk_at(i));
-    while (i < chunk_end) {
-        if (i + KW < chunk_end) reader.load(x1, chunk_at(i + KW));
-        work(x0, chunk_at(i));
-        i += KW;
-        if (i >= chunk_end) break;
-        if (i + KW < chunk_end) reader.load(x0, chunk_at(i + KW));
-        work(x1, chunk_at(i));
-        i += KW;
-    }
+    PagedChunk<NK, NV> now, next;
+    int i = split * per + wave, k = 0, page = pages_of(i), page_next = pages_of(i + 32 * KW);
+    const int in_page = (1 << p.cache.page_shift) - 1;
+    auto load = [&](PagedChunk<NK, NV>& x, int i, int k) __attribute__((always_inline)) {
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+            const int64_t pg = __builtin_amdgcn_readlane(page, 2 * (k & 31) + tt);
+            x.load(p.cache, ((pg * p.cache.heads + hk) << p.cache.page_shift) + ((chunk_at(i) * 32 + tt * 16) & in_page), tt, lane);
+        }
+    };
+    // One chunk, the next one's loads on their way.  Code of their own for chunks that all rows see whole, in a loop of their own: a condition at each
+    // score would stand between them, and one around them would have the sums moved where its ways meet.
+    auto one = [&](auto masked) __attribute__((always_inline)) {
+        if (((k + 1) & 31) == 0) page = page_next, page_next = pages_of(i + KW + 32 * KW);
+        if (i + KW < chunk_end) load(next, i + KW, k + 1);
+        work(now, chunk_at(i), masked);
+        now = next;
+        i += KW, ++k;
+    };
+    const int whole0 = max(((lo_max + 31) >> 5) - span.a0, 0), whole1 = min((hi_min >> 5) - span.a0, span.na);
+    if (i < chunk_end) load(now, i, 0);
+    while (i < chunk_end && !(i >= whole0 && i < whole1)) one(std::true_type{});
+    while (i < min(chunk_end, whole1)) one(std::false_type{});
+    while (i < chunk_end) one(std::true_type{});
+    bad = __any(bad);
 
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         float lower = plo[mt];
         lower += __shfl_xor(lower, 16, 64);
         lower += __shfl_xor(lower, 32, 64);
-        if (reader.bad) lower = __builtin_nanf("");
+        if (bad) lower = __builtin_nanf("");
         float o[4][NV];  // [i][j]: column NV (4 g + i) + j
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4)
 #pragma unroll
             for (int j = 0; j < NV; ++j) o[i4][j] = acc[mt][j][i4] - (CodesBf16::off(j & 3) + 7.5f) * psum[mt][i4] + lower;
-        auto put = [&](int i4, const float (&x)[NV]) __attribute__((always_inline)) {
-            if (out_at[mt] < 0) return;
-            const int64_t at = out_at[mt] + NV * (4 * g + i4);
-            if (p.splits > 1) {
+        __syncthreads();
 #pragma unroll
-                for (int j = 0; j < NV; ++j) p.partial[split * p.partial_stride + at + j] = x[j];
-            } else {
+        for (int i4 = 0; i4 < 4; ++i4)
 #pragma unroll
-                for (int j = 0; j < NV; ++j) ((T*)p.out)[at + j] = (T)(x[j] * p.oscale);
-            }
-        };
-        if constexpr (KW == 1) {
+            for (int j = 0; j < NV; ++j) meet[((wave * 4 + i4) * NV + j) * 64 + lane] = o[i4][j];
+        __syncthreads();
+        // wave i4 adds up columns NV (4 g + i4) ..
+        if (out_at[mt] >= 0) {
+            const int64_t at = out_at[mt] + NV * (4 * g + wave);
 #pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4) put(i4, o[i4]);
-        } else {
-            __syncthreads();
+            for (int j = 0; j < NV; ++j) {
+                float x = 0.f;
 #pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4)
-#pragma unroll
-                for (int j = 0; j < NV; ++j) meet[((wave * 4 + i4) * NV + j) * 64 + lane] = o[i4][j];
-            __syncthreads();
-            // wave kw of the KW that share these rows adds up i4 = kw, kw + KW, ...
-#pragma unroll
-            for (int step = 0; step < 4 / KW; ++step) {
-                const int i4 = kw + step * KW;
-                float x[NV];
-#pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    x[j] = 0.f;
-#pragma unroll
-                    for (int w = 0; w < KW; ++w) x[j] += meet[(((rw * KW + w) * 4 + i4) * NV + j) * 64 + lane];
-                }
-                put(i4, x);
+                for (int w = 0; w < KW; ++w) x += meet[((w * 4 + wave) * NV + j) * 64 + lane];
+                if (p.splits > 1) p.partial[split * p.partial_stride + at + j] = x;
+                else ((T*)p.out)[at + j] = (T)(x * p.oscale);
             }
         }
     }
