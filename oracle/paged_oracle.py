@@ -118,7 +118,9 @@ def attention(max_seq_len, alpha, q, cache, page_table, lengths, targets=None, m
     bound = torch.zeros_like(out)
     # a code enters a product as 128 + code or 16 + code (fp16's scores: 64 + code)
     off_k, off_v = (128.0 if dtype == torch.bfloat16 else 64.0), 128.0
-    p_round = 2.0**-9 if dtype == torch.bfloat16 else 2.0**-16
+    # P times the step is rounded to bf16: 8 bits of significand, neighbours 2^-7 2^e apart around values of 2^e and more, so off by at most
+    # half of that, 2^-8 of the value (2^-9 holds just below 2^(e+1) alone).  Two words: 2^-8 of what the first left out, 2^-16.
+    p_round = 2.0**-8 if dtype == torch.bfloat16 else 2.0**-16
     for b in range(batch):
         n = int(lengths[b])
         if n <= 0:

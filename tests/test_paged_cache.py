@@ -459,6 +459,10 @@ ATTENTION = [
     ([40, 61, 35], 35, [5, 0, 12], 0, 10, 1, 1, 32, 32, 16, BF16),  # contextual rows among the newest
     ([3000, 2900, 31], 20, [20, 0, 20], 7, 0, 1, 1, 64, 128, 256, BF16),
     ([2100] * 3, 300, [300] * 3, 0, 0, 1, 1, 64, 64, 64, BF16),
+    ([700, 90, 333], 132, [0, 90, 132], 200, 5, 1, 1, 64, 128, 32, F16),
+    ([400, 97], 24, None, 90, 0, 1, 1, 128, 128, 16, BF16),
+    ([513, 512, 511, 1], 4, [4, 4, 0, 0], 0, 0, 4, 2, 128, 128, 64, F16),
+    ([2000, 33], 2, None, 0, 0, 4, 2, 128, 64, 16, BF16),
 ]
 
 
@@ -558,6 +562,67 @@ def test_attention_of_large_scores(pkg, dev):
         got = pkg.delta_hstu_mha_paged(200, 2.0, q.to(dev), tuple(c.to(dev) for c in cache), *_to(dev, table, lengths))
         torch.cuda.synchronize()
         _within(got, want, bound, str(dtype))
+
+
+@pytest.mark.gpu
+def test_a_cache_beyond_32_bit_offsets(pkg, dev):
+    """Pages that lie past 2^32 bytes of codes: appended, read and attended to as in a small cache."""
+    print("[case] a long cache", flush=True)
+    heads, dqk, dv, page, N = 1, 128, 64, 1024, 2048
+    pages = 70000  # 4.6 GB of K codes
+    big = (torch.empty((pages, heads, page, dqk // 2), dtype=torch.uint8, device=dev), torch.empty((pages, heads, page, 2), dtype=BF16, device=dev),
+           torch.empty((pages, heads, page, dv // 2), dtype=torch.uint8, device=dev), torch.empty((pages, heads, page, 2), dtype=BF16, device=dev))
+    small = pkg.allocate_paged_kv_cache(6, page, heads, dqk, dv, BF16, dev)
+    near = torch.tensor([[3, 0], [5, 1], [2, 4]], dtype=torch.int32)
+    far = near + (pages - 6)
+    lengths = torch.tensor([2048, 1500, 40])
+    offs = torch.cat([torch.zeros(1, dtype=torch.int64), lengths.cumsum(0)]).to(dev)
+    k, v = _rand(1, (int(lengths.sum()), heads, dqk), BF16).to(dev), _rand(2, (int(lengths.sum()), heads, dv), BF16).to(dev)
+    zero = torch.zeros(3, dtype=torch.int64, device=dev)
+    got = []
+    for cache, table in ((small, near), (big, far)):
+        table = table.to(dev)
+        pkg.append_paged_kv(cache, k, v, table, zero, offs)
+        out = list(pkg.read_paged_kv(cache, k.shape[0], table, zero, offs))
+        for delta in (1, 12, 100):
+            q = _rand(10 + delta, (3 * delta, 2, dqk), BF16).to(dev)
+            out.append(pkg.delta_hstu_mha_paged(N, 0.1, q, cache, table, lengths.to(dev)))
+        got.append(out)
+    torch.cuda.synchronize()
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert torch.isfinite(got[0][-1]).all()
+
+
+@pytest.mark.gpu
+def test_attention_of_many_sequences_and_tables_of_any_layout(pkg, dev):
+    """More sequences than a workgroup ranks, tables that are columns of a wider one, calls on two streams at once."""
+    print("[case] attention: many sequences", flush=True)
+    rng = torch.Generator().manual_seed(3)
+    lengths = torch.randint(0, 90, (300,), generator=rng).tolist()
+    for delta, hq in ((1, 1), (17, 1), (40, 2)):
+        case = (lengths, delta, None, 0, 0, hq, 1, 32, 32, 16, BF16)
+        q, cache, table, n, _ = _attention_inputs(case)
+        want, bound = O.attention(90, 0.2, q, cache, table, n)
+        wide = torch.full((300, 3 * table.shape[1]), 10**6, dtype=torch.int32)
+        wide[:, 2 : 2 + table.shape[1]] = table
+        wide, spread = wide.to(dev), torch.full((300, table.shape[1], 2), 10**6, dtype=torch.int64)
+        spread[:, :, 0] = table
+        on = tuple(c.to(dev) for c in cache)
+        first = pkg.delta_hstu_mha_paged(90, 0.2, q.to(dev), on, wide[:, 2 : 2 + table.shape[1]], n.to(dev))
+        second = pkg.delta_hstu_mha_paged(90, 0.2, q.to(dev), on, spread.to(dev)[:, :, 0], n.to(dev))
+        _within(first, want, bound, f"delta {delta}")
+        assert torch.equal(first, second)
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        args = (90, 0.2, q.to(dev), on, table.to(dev), n.to(dev))
+        torch.cuda.synchronize()
+        beside = []
+        for _ in range(3):
+            for st in streams:
+                with torch.cuda.stream(st):
+                    beside.append(pkg.delta_hstu_mha_paged(*args, kv_splits=3))
+        torch.cuda.synchronize()
+        assert all(torch.equal(b, beside[0]) for b in beside)
 
 
 # ---- together -----------------------------------------------------------------------------------------------------------
