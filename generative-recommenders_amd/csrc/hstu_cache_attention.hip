@@ -50,23 +50,33 @@ Plan plan_of(const HstuPagedCache* c, const HstuPagedAttentionArgs* a) {
     // of 80 26, of 16 30), but none longer than 96 chunks, so that the last of them do not run alone (128 sequences of up to 16384 and eight heads:
     // whole sequences 291 us, runs of 384 chunks 281, of 103 264, of 33 281).  Sequences of a few chunks, more of them than fit, are a wave's each (1600 of
     // up to 10 chunks: 12 us, 16 by workgroups).
-    // Blocks of many rows: two workgroups of a CU, for a run more is a partial sum of every row to write and read; parts of a sequence are equal, so that
-    // ranking the sequences balances them.
-    const bool blocks = !p.step && p.rw == 4;
+    // More rows are split into equal parts of each sequence, of at least 8 or 16 chunks: what a part more costs is a partial sum of every row to
+    // write and read.  Blocks: at least two workgroups of a CU, whose sequences are ranked.  Nine to 32 rows: parts that fill the card in one
+    // round, 512 workgroups of up to 16 rows or 256 of more, or in two rounds where one would leave much of it empty (24 rows, 160 workgroups
+    // for whole sequences of up to 8192: one part 88 us, two 74, three 64, four 67; 256 workgroups of up to 4096: one 49, two 57, four 66;
+    // 16 rows, 128 workgroups of up to 8192: two 41, four 34, eight 37).
     const int64_t fill = (chunks * wgs + 511) / 512;
-    int64_t run = a->kv_splits > 0 ? (chunks + a->kv_splits - 1) / a->kv_splits : (fill + 15) / 16 * 16;
-    if (!a->kv_splits && run > 96) run = 96;
-    if (run < 16) run = 16;
-    if (blocks) {
-        int64_t parts = a->kv_splits > 0 ? a->kv_splits : wgs > 0 ? (512 + wgs - 1) / wgs : 1;
-        if (parts > (chunks + 7) / 8) parts = (chunks + 7) / 8;
-        run = 8;
-        p.splits = (int)parts;
+    int64_t run = 16;
+    if (p.step) {
+        run = a->kv_splits > 0 ? (chunks + a->kv_splits - 1) / a->kv_splits : (fill + 15) / 16 * 16;
+        if (!a->kv_splits && run > 96) run = 96;
+        if (run < 16) run = 16;
+        if (run > chunks) run = chunks;
+    } else {
+        int64_t parts = a->kv_splits;
+        if (parts == 0 && wgs > 0) {
+            const int64_t slots = p.rw == 4 || p.mt == 1 ? 512 : 256;
+            parts = p.rw == 4 ? (slots + wgs - 1) / wgs : slots / wgs;
+            if (p.rw != 4 && parts <= 2 && 2 * slots / wgs > 2 * parts) parts = 2 * slots / wgs;
+        }
+        if (p.rw == 4) run = 8;
+        if (parts > (chunks + run - 1) / run) parts = (chunks + run - 1) / run;
+        p.splits = parts < 1 ? 1 : (int)parts;
+        if (run > chunks) run = chunks;
     }
     if (p.step && chunks <= 17 && wgs > 1024) p.share = 1, run = chunks;
-    if (run > chunks) run = chunks;
     p.run = (int)run;
-    if (!blocks) p.splits = (int)((chunks + run - 1) / run);
+    if (p.step) p.splits = (int)((chunks + run - 1) / run);
     if (p.splits > 1) p.workspace = p.splits * c->batch * a->delta_size * a->q_heads * (int64_t)c->dv * 4;
     return p;
 }
