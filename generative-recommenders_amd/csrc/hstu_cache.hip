@@ -12,9 +12,6 @@ namespace {
 
 thread_local char g_last_error[256] = "";
 
-// Largest grid that the row-wise kernels are launched with in x (a workgroup covers at least 4 rows: far more than fit the card).
-constexpr int64_t kMaxBlocks = 2147483647;
-
 int lanes_of(int dim) {
     int lanes = 4;
     while (lanes * 8 < dim) lanes *= 2;
@@ -162,11 +159,11 @@ int hstu_cache_norm_rope(const HstuNormRopeArgs* a, void* stream) {
     if (a->rows == 0 || heads == 0) return 0;
     for (const hstu::NormRopeSide& s : p.side)
         if (s.heads && !s.y) return HSTU_ERR_NULL_POINTER;
-    if (!hstu_cache_device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
     const int lanes = lanes_of(a->dim);
     p.heads_per_group = vectors_per_group(a->rows, lanes, heads, 2048);
     const int64_t blocks = (a->rows * lanes + 255) / 256, chunks = (heads + p.heads_per_group - 1) / p.heads_per_group;
     if (blocks > kMaxBlocks || chunks > 65535) return HSTU_ERR_UNSUPPORTED;
+    if (!hstu_cache_device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
     return with_type(a->dtype, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
         return with_lanes(lanes, [&](auto l) {
@@ -248,7 +245,6 @@ int hstu_cache_append(const HstuPagedCache* cache, const HstuAppendArgs* a, void
     if (!strides_fit(a->k_row_stride, a->k_head_stride, 8) || !strides_fit(a->v_row_stride, a->v_head_stride, 8)) return HSTU_ERR_MISALIGNED;
     for (const void* ptr : {a->k, a->v, a->k_weight})
         if (!hstu_cache_aligned(ptr)) return HSTU_ERR_MISALIGNED;
-    if (!hstu_cache_device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
     p.place = {a->start, a->seq_offsets, a->start_i64, a->seq_offsets_i64, a->rows, a->seq_offsets ? 0 : a->rows / cache->batch};
     p.k = (const char*)a->k, p.v = (const char*)a->v;
     p.k_rs = a->k_row_stride, p.k_hs = a->k_head_stride, p.v_rs = a->v_row_stride, p.v_hs = a->v_head_stride;
@@ -259,6 +255,7 @@ int hstu_cache_append(const HstuPagedCache* cache, const HstuAppendArgs* a, void
     p.vectors_per_group = vectors_per_group(a->rows, lanes, vectors, 2048);
     const int64_t blocks = (a->rows * lanes + 255) / 256, chunks = (vectors + p.vectors_per_group - 1) / p.vectors_per_group;
     if (blocks > kMaxBlocks || chunks > 65535) return HSTU_ERR_UNSUPPORTED;
+    if (!hstu_cache_device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
     auto launch = [&](auto* t, auto l) {
         typedef std::remove_pointer_t<decltype(t)> T;
         return with_turn(a->rotary, a->interleaved, [&](auto turn) {
@@ -279,13 +276,13 @@ int hstu_cache_read(const HstuPagedCache* cache, int64_t rows, const void* start
     if (rows == 0 || cache->batch == 0) return 0;
     if (!k || !v || !start) return HSTU_ERR_NULL_POINTER;
     if (!hstu_cache_aligned(k) || !hstu_cache_aligned(v)) return HSTU_ERR_MISALIGNED;
-    if (!hstu_cache_device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
     p.place = {start, seq_offsets, start_i64, seq_offsets_i64, rows, seq_offsets ? 0 : rows / cache->batch};
     p.k = (char*)k, p.v = (char*)v;
     const int lanes = lanes_of(cache->dqk > cache->dv ? cache->dqk : cache->dv), vectors = 2 * cache->heads;
     p.vectors_per_group = vectors_per_group(rows, lanes, vectors, 2048);
     const int64_t blocks = (rows * lanes + 255) / 256, chunks = (vectors + p.vectors_per_group - 1) / p.vectors_per_group;
     if (blocks > kMaxBlocks || chunks > 65535) return HSTU_ERR_UNSUPPORTED;
+    if (!hstu_cache_device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
     auto launch = [&](auto* t, auto l) {
         typedef std::remove_pointer_t<decltype(t)> T;
         hipLaunchKernelGGL((hstu::hstu_paged_read_kernel<T, decltype(l)::value>), dim3((unsigned)blocks, (unsigned)chunks), dim3(256), 0, (hipStream_t)stream, p);

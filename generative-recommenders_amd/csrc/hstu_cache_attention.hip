@@ -77,7 +77,7 @@ Plan plan_of(const HstuPagedCache* c, const HstuPagedAttentionArgs* a) {
     if (p.step && chunks <= 17 && wgs > 1024) p.share = 1, run = chunks;
     p.run = (int)run;
     if (p.step) p.splits = (int)((chunks + run - 1) / run);
-    if (p.splits > 1) p.workspace = p.splits * c->batch * a->delta_size * a->q_heads * (int64_t)c->dv * 4;
+    if (p.splits > 1) p.workspace = (int64_t)p.splits * c->batch * a->delta_size * a->q_heads * c->dv * 4;
     return p;
 }
 
@@ -164,7 +164,8 @@ int hstu_cache_attention(const HstuPagedCache* c, const HstuPagedAttentionArgs* 
         if (a->workspace_bytes < plan.workspace) return HSTU_ERR_BAD_SHAPE;
     }
     const int64_t items = (int64_t)c->batch * c->heads * plan.splits;
-    if (items * plan.row_blocks > (1ll << 30)) return HSTU_ERR_UNSUPPORTED;
+    const int64_t joined = plan.splits > 1 ? (int64_t)c->batch * a->delta_size * a->q_heads * c->dv / 8 * (plan.splits > 4 ? 8 : 1) : 0;
+    if (items * plan.row_blocks > kMaxBlocks || (joined + 255) / 256 > kMaxBlocks) return HSTU_ERR_UNSUPPORTED;
     if (!hstu_cache_device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
     p.q = (const char*)a->q, p.q_rs = a->q_row_stride, p.q_hs = a->q_head_stride, p.out = (char*)a->out;
     p.lengths = a->seq_lengths, p.lengths_i64 = a->seq_lengths_i64, p.targets = a->num_targets, p.targets_i64 = a->num_targets_i64;

@@ -15,6 +15,9 @@ int hstu_cache_device_is_gfx950(void);
 int hstu_cache_fill(const HstuPagedCache* cache, hstu::PagedCache& p);
 }
 
+// Largest grid in x: a launch has fewer than 2^32 threads in a dimension, and a workgroup 256 (rows of 128 columns: 2^28 of them).
+constexpr int64_t kMaxBlocks = (1 << 24) - 1;
+
 inline bool hstu_cache_aligned(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }
 
 // f(type pointer, lanes of a row) for a cache's type (bf16 or fp16) and 4 to 32 lanes.

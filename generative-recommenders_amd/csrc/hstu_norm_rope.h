@@ -164,7 +164,7 @@ __device__ __forceinline__ void lane_weights(const T* weight, int col0, float (&
     }
 }
 
-// 1 / sqrt(mean of squares + eps) of a vector, rounded as exactly as torch's mean and rsqrt over the last dimension give it (measured: the same
+// 1 / sqrt(mean of squares + eps) of a vector, rounded as a plain evaluation of the mean and the reciprocal root on this device gives it (measured: the same
 // bits): squares added pairwise, from sums of four on where a vector has 128 columns or more, and the instruction's root, good to a unit in
 // the last place, corrected once by its residual.
 template <int LPV>
@@ -227,7 +227,8 @@ struct NormRopeParams {
     float* partial;  // backward: [workgroups][2][dim]
 };
 
-// grid (rows / groups of a workgroup, heads / heads_per_group): heads count through q's, then k's.
+// grid (rows / groups of a workgroup, heads / heads_per_group): heads count through q's, then k's.  Bytes bound it: 151302 rows of eight
+// heads of q and four of k, 128 columns, 160 us (930 MB, 5.8 TB/s); 32 rows 5 us, which is one launch.
 template <class T, int LPV, int TURN>
 __global__ __launch_bounds__(256) void hstu_norm_rope_kernel(const NormRopeParams p) {
     constexpr int GROUPS = 256 / LPV, AHEAD = 4;
@@ -271,7 +272,8 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_kernel(const NormRopeParam
 }
 
 // The same grid, but a workgroup goes on to further rows, so that the sums for the weights stay in registers: each lane adds up its
-// columns, the groups of a workgroup meet in LDS, and the workgroups' sums are added by the kernel below.
+// columns, the groups of a workgroup meet in LDS, and the workgroups' sums are added by the kernel below.  151302 rows as above: 264 us
+// (1.39 GB, 5.3 TB/s), and 7 for the sums.
 template <class T, int LPV, int TURN>
 __global__ __launch_bounds__(256) void hstu_norm_rope_bwd_kernel(const NormRopeParams p) {
     constexpr int GROUPS = 256 / LPV, AHEAD = 2;

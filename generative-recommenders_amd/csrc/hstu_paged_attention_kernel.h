@@ -231,7 +231,9 @@ __device__ __forceinline__ void store_columns(const PagedAttentionParams& p, int
 }
 
 // grid: one workgroup of four waves per (block of 16 MT rows, head of the cache, run, sequence), numbered so that the row blocks of one
-// run, which read the same pages, are on one XCD.  The waves share out the chunks of the run; their sums meet in LDS.
+// run, which read the same pages, are on one XCD.  The waves share out the chunks of the run; their sums meet in LDS.  Unpacking and silu
+// bound it, the cache's bytes not far below: 12 rows, 256 sequences of 1000 .. 8192 positions and four heads of 128 182 us (629 MB, 121 us
+// of a copy); 24 rows, whose sums leave room for one wave of a SIMD, 318.
 template <class TT, int DK, int DV, int MT>
 __global__ __launch_bounds__(256) void hstu_paged_attention_kernel(const PagedAttentionParams p) {
     typedef typename TT::elem T;
@@ -475,8 +477,11 @@ __device__ __forceinline__ int block_order(const PagedAttentionParams& p, int ea
 // each wave unpacks its part of them -- a tile of 16 positions of K, a quarter of the columns of V -- into LDS, in the order in which the
 // products' operands lie in registers (a lane's 16 bytes side by side: reads and writes without bank conflicts), and the pairs as four
 // floats a position: c1 s, c1 l of K, s, l + 7.5 s of V.  Two buffers, one barrier a step; the packed rows of the next step are on their way
-// while this one is worked on.  Two workgroups of a CU, out of step with each other, fill the gaps of one another: the same two
-// teams of waves in one workgroup, behind one barrier, took 106 us for attention_candidates.  Unpacking per wave, as above, cost as much as half of the rest and the registers of a second wave.
+// while this one is worked on.  Unpacking per wave, as above, cost as much as half of the rest and the registers of a second wave.
+// What bounds it is silu: 8 operations and two of a quarter's rate for each score, 62 clocks of a SIMD for 64 scores, beside which the
+// products take 34 and unpacking 14.  32 sequences of 1280 .. 4352 positions with 256 rows and four heads of 128 (39 GFLOP, 32 us of the
+// matrix cores as a large library product uses them, 33 of silu alone): 88 us.  Two workgroups of a CU, out of step with each other, fill the gaps of one another: the same
+// two teams of waves in one workgroup, behind one barrier, took 106.
 template <class TT, int DK, int DV, int MT>
 __global__ __launch_bounds__(256, 2) void hstu_paged_block_kernel(const PagedAttentionParams p) {
     typedef typename TT::elem T;
@@ -771,8 +776,9 @@ __global__ __launch_bounds__(256, 2) void hstu_paged_block_kernel(const PagedAtt
 // it where the chunk is its own.  silu and what surrounds it then run once for F chunks, on full lanes, and so do the loads of the pairs
 // (step, lowest value).  For the second product each chunk's columns alone have P, the others zero: its sums land in columns of their own,
 // which are added up over the chunks at the end.
-// Waves of a SIMD: three in 168 registers each took 281 us for attention_step's 1.45 GB where two in 172 took 290; heads of 256 need
-// the registers of one.
+// Waves of a SIMD: three in 168 registers each took 281 us where two in 172 took 290 (128 sequences of 4096 .. 16384 positions, eight
+// heads of 128, 1.45 GB); heads of 256 need the registers of one.  The cache's bytes bound it: the same sequences in runs of up to 96
+// chunks take 265 us, 5.4 TB/s where a copy of 1 GiB reaches 5.2.  One short sequence is launches and loads that wait for each other: 8 us.
 template <int DK, int DV>
 constexpr int STEP_WAVES = DK == 256 ? 1 : DK + DV >= 256 ? 2 : DK + DV >= 128 ? 3 : 4;
 
@@ -1056,6 +1062,7 @@ __global__ __launch_bounds__(256, (STEP_WAVES<DK, DV>)) void hstu_paged_step_ker
 }
 
 // out = oscale * the sum of the runs there are: eight columns to PARTS threads, which share out the runs and add up in a fixed order.
+// The loads of a thread's runs wait for nothing, and a launch bounds it: 3 to 6 us.
 template <class TT, int PARTS>
 __global__ __launch_bounds__(256) void hstu_paged_join_kernel(const PagedAttentionParams p, int block_rows, int64_t total8) {
     typedef typename TT::elem T;

@@ -146,8 +146,10 @@ __device__ __forceinline__ unsigned to_four_bits(const float (&x)[8], unsigned& 
 }
 
 // grid (rows / groups of a workgroup, vectors / vectors_per_group): a row's vectors count through its heads of K, then of V.
-// (16 columns to a lane, which do what a row takes once in half as many lanes, came to a third fewer instructions and to the same time: 98 us
-// for append_prefill, four waves of a SIMD in 107 registers where six have 78.  So did the first loads in front of the lookups.)
+// (16 columns to a lane, which do what a row takes once in half as many lanes, came to a third fewer instructions and to the same time,
+// four waves of a SIMD in 107 registers where six have 78.  So did the first loads in front of the lookups.)  Vector operations
+// bound it, with the bytes close below: 256 sequences of 64 .. 1024 rows, four heads of 128, normed and turned, 97 us (337 MB, 65 us of a
+// copy; 51 million operations, 83 us of the SIMDs).  64 single rows take 4.5 us, one launch and three loads that wait for each other.
 template <class T, int LPV, int TURN>
 __global__ __launch_bounds__(256) void hstu_paged_append_kernel(const AppendParams p) {
     constexpr int GROUPS = 256 / LPV, AHEAD = 4;
@@ -204,6 +206,7 @@ __global__ __launch_bounds__(256) void hstu_paged_append_kernel(const AppendPara
     }
 }
 
+// The inverse, value = lowest + step code, rounded once.  Bytes bound it: the rows of the sequences above 69 us, 4.9 TB/s.
 template <class T, int LPV>
 __global__ __launch_bounds__(256) void hstu_paged_read_kernel(const ReadParams p) {
     constexpr int GROUPS = 256 / LPV, AHEAD = 4;

@@ -262,8 +262,8 @@ def append_paged_kv(
     if hip_backend.contract_checks_enabled():
         _check_places(cache, page_table, start, seq_offsets, rows)
         if rotary_table is not None:
-            _check_positions(positions if positions is not None else start + (rows // batch if seq_offsets is None else seq_offsets[1:] - seq_offsets[:-1]) - 1,
-                             rotary_table)
+            count = torch.full_like(start, rows // batch) if seq_offsets is None else seq_offsets[1:] - seq_offsets[:-1]
+            _check_positions(positions if positions is not None else (start + count - 1)[count > 0], rotary_table)
     _served(native.front.append_paged_kv(cache, _copied(k), _copied(v), _pages(page_table), start, seq_offsets, rotary_table, positions,
                                          k_weight, eps, interleaved, True), "append_paged_kv")
 
@@ -342,11 +342,11 @@ def delta_hstu_mha_paged(
         return torch.empty((delta_q.shape[0], delta_q.shape[1], 2 * cache[2].shape[3]), dtype=delta_q.dtype, device=delta_q.device)
     if hip_backend.contract_checks_enabled():
         _check_places(cache, page_table, torch.zeros_like(seq_lengths), torch.nn.functional.pad(seq_lengths.cumsum(0), (1, 0)), int(seq_lengths.sum()))
-        if bool((seq_lengths > max_seq_len).any()) or bool((seq_lengths < delta_q.shape[0] // batch).any()):
-            raise ValueError("hstu_cache: a sequence is longer than max_seq_len or shorter than its newest positions")
+        if bool((seq_lengths > max_seq_len).any()):
+            raise ValueError("hstu_cache: a sequence is longer than max_seq_len")
         if num_targets is not None and bool(((num_targets < 0) | (num_targets > seq_lengths)).any()):
             raise ValueError("hstu_cache: num_targets outside [0, length]")
-        if bool((seq_lengths - (0 if num_targets is None else num_targets) < contextual_seq_len).any()):
+        if bool(((seq_lengths - (0 if num_targets is None else num_targets) < contextual_seq_len) & (seq_lengths > 0)).any()):
             raise ValueError("hstu_cache: fewer non-target positions than contextual_seq_len")
     return _served(native.front.delta_hstu_mha_paged(max_seq_len, alpha, _copied(delta_q), cache, _pages(page_table), seq_lengths, num_targets,
                                                      max_attn_len, contextual_seq_len, kv_splits, True), "delta_hstu_mha_paged")

@@ -81,6 +81,59 @@ def test_statuses_of_the_c_abi():
     assert lib.hstu_cache_last_error() == b""
 
 
+def _abi():
+    """The library and its argument structures, read from the header."""
+    import ctypes
+    import os
+    import re
+
+    from generative_recommenders_amd import build
+
+    lib = ctypes.CDLL(build.CACHE_LIB_PATH)
+    header = re.sub(r"/\*.*?\*/", "", open(os.path.join(build.INCLUDE, "hstu_cache.h")).read(), flags=re.S)
+    types = {"int64_t": ctypes.c_int64, "int32_t": ctypes.c_int32, "float": ctypes.c_float}
+    made = {}
+    for body, name in re.findall(r"typedef struct \w+ \{(.*?)\} (\w+);", header, flags=re.S):
+        fields = []
+        for line in body.split(";"):
+            if line.strip():
+                kind, names = line.strip().removeprefix("const ").split(None, 1)
+                for n in names.split(","):
+                    fields.append((n.strip().lstrip("* "), ctypes.c_void_p if "*" in line else types[kind]))
+        made[name] = type(name, (ctypes.Structure,), {"_fields_": fields})
+    for name in ("attention", "norm_rope_bwd"):
+        getattr(lib, f"hstu_cache_{name}_workspace_bytes").restype = ctypes.c_size_t
+    return lib, ctypes.byref, made
+
+
+def test_sizes_past_32_bits_in_the_c_abi():
+    """Scratch memory of more than 2^31 values is asked for in full, and what no launch can number is refused (pointers are never followed)."""
+    lib, ref, made = _abi()
+    at = 1 << 20
+    cache = made["HstuPagedCache"](k_codes=at, k_scales=at, v_codes=at, v_scales=at, pages=1 << 20, heads=1, page_size=1024, dqk=128, dv=128, dtype=0, page_table=at,
+                                   table_row_stride=1024, table_columns=1024, batch=256)
+    call = made["HstuPagedAttentionArgs"](q=at, q_row_stride=1024, q_head_stride=128, out=at, seq_lengths=at, q_heads=8, delta_size=512, max_seq_len=1 << 20, alpha=1.0, kv_splits=4096,
+                                          workspace=at)
+    need = lib.hstu_cache_attention_workspace_bytes(ref(cache), ref(call))
+    assert need == 4096 * 256 * 512 * 8 * 128 * 4
+    call.workspace_bytes = need - 1
+    assert lib.hstu_cache_attention(ref(cache), ref(call), None) == -5
+    call.workspace_bytes = need
+    assert lib.hstu_cache_attention(ref(cache), ref(call), None) == -6
+    call.kv_splits = 1
+    assert lib.hstu_cache_attention_workspace_bytes(ref(cache), ref(call)) == 0
+    rows = 1 << 28
+    for name, start in (("append", made["HstuAppendArgs"](k=at, v=at, rows=rows, k_row_stride=128, k_head_stride=128, v_row_stride=128, v_head_stride=128, start=at)),):
+        assert getattr(lib, f"hstu_cache_{name}")(ref(cache), ref(start), None) == -6
+    import ctypes
+
+    assert lib.hstu_cache_read(ref(cache), ctypes.c_int64(rows), ctypes.c_void_p(at), 0, None, 0, ctypes.c_void_p(at), ctypes.c_void_p(at), None) == -6
+    turn = made["HstuNormRopeArgs"](q=at, q_row_stride=128, q_head_stride=128, q_out=at, q_weight=at, rows=rows, q_heads=1, dim=128, dtype=0)
+    assert lib.hstu_cache_norm_rope(ref(turn), None) == -6
+    turn.rows = 1 << 40
+    assert 0 < lib.hstu_cache_norm_rope_bwd_workspace_bytes(ref(turn)) <= 2048 * 2 * 128 * 4
+
+
 def test_no_vector_instruction_reads_a_matrix_result_too_early(tmp_path):
     import os
     import shutil
@@ -265,6 +318,55 @@ def test_norm_rope_leaves_an_infinity_where_it_is(pkg, dev, interleaved):
     pair = [4, 5 if interleaved else 20]
     rest = [i for i in range(32) if i not in pair]
     assert not torch.isfinite(got[3, 0, pair]).any() and torch.isfinite(got[3, 0, rest]).all() and torch.isfinite(got[2, 1, :32]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_norm_rope_of_odd_rows(pkg, dev, dtype):
+    """Rows of zeros, tiny and huge rows, a NaN: what the formula gives in fp32, rounded once, and the row's neighbours as they are without it."""
+    print(f"[case] norm and rotation: odd rows {dtype}", flush=True)
+    x = _rand(1, (8, 2, 64), dtype)
+    x[0] = 0
+    x[1] = x[1] * 1e-30  # squares below all numbers
+    x[2] = x[2] * 1e25  # squares above all numbers
+    x[3, 0, 7] = float("nan")
+    x[4] = x[4] * 1e12
+    w = 1 + 0.1 * _rand(2, (64,), dtype)
+    for eps in (1e-6, 0.0):
+        got = pkg.qk_norm_rope(x.to(dev), None, None, None, w.to(dev), eps=eps)[0].float().cpu()
+        f = x.float()
+        mean = (f * f).mean(-1, keepdim=True) + eps
+        want = f * mean.rsqrt() * w.float()
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        # the mean of 64 squares: 7 additions and 2 products; its root twice half of that; two products; the rounding to the type
+        bound = (4.5 + 2 + 2) * 2.0**-24 + torch.finfo(dtype).eps / 2
+        near = torch.isfinite(want)
+        assert ((got - want).abs()[near] <= 1.01 * bound * want.abs()[near] + 1e-37).all()
+        assert torch.equal(got[~near & ~torch.isnan(want)], want[~near & ~torch.isnan(want)])
+
+
+@pytest.mark.gpu
+def test_norm_rope_gradients_against_differences_of_the_kernel(pkg, dev):
+    """<gradient, direction> against central differences of the kernel's own results, fp32.  With h = 2^-6 and directions of size one: the third
+    derivative leaves h^2 / 6 of some units, 2^-12 of the sum's size; the roundings 2^-22 / 2h of it, less."""
+    print("[case] norm and rotation: differences", flush=True)
+    rows, dim, h = 23, 48, 2.0**-6
+    q, k, qw, kw = (_rand(i, shape, F32).to(dev) for i, shape in enumerate(((rows, 3, dim), (rows, 1, dim), (dim,), (dim,))))
+    turns, at = pkg.make_rotary_table(50, 32, device=dev), torch.arange(rows, device=dev) * 2
+    up = [_rand(9 + i, x.shape, F32).to(dev) for i, x in enumerate((q, k))]
+    leaves = [x.clone().requires_grad_() for x in (q, k, qw, kw)]
+
+    def value(q, k, qw, kw):
+        a, b = pkg.qk_norm_rope(q, k, at, turns, qw, kw, interleaved=True)
+        return (a.double() * up[0]).sum() + (b.double() * up[1]).sum()
+
+    grads = torch.autograd.grad(value(*leaves), leaves)
+    for i, g in enumerate(grads):
+        way = _rand(20 + i, g.shape, F32).to(dev)
+        moved = [[x + s * h * way if j == i else x for j, x in enumerate((q, k, qw, kw))] for s in (1, -1)]
+        slope = (value(*moved[0]) - value(*moved[1])) / (2 * h)
+        size = (g.double() * way).abs().sum()
+        assert abs(float(slope - (g.double() * way).sum())) <= 2.0**-10 * float(size), i
 
 
 @pytest.mark.gpu
@@ -548,6 +650,29 @@ def test_attention_of_sequences_shorter_than_the_newest_rows(pkg, dev):
         torch.cuda.synchronize()
         _within(got, want, bound, f"delta {delta}")
         assert (got[: delta - 3] == 0).all() and (got[delta : 2 * delta] == 0).all()
+
+
+@pytest.mark.gpu
+def test_padded_batches_pass_the_contract_checks(pkg, dev, monkeypatch):
+    """Sequences without new rows, of no length at all, or shorter than the newest rows are allowed calls; checks on, they give the same."""
+    print("[case] padded batches", flush=True)
+    heads, dim, page = 1, 32, 16
+    cache = pkg.allocate_paged_kv_cache(6, page, heads, dim, dim, BF16, dev)
+    table = torch.tensor([[0, 1], [2, 3], [4, -1], [-1, -1]], dtype=torch.int32, device=dev)
+    k, v = _rand(1, (34, heads, dim), BF16).to(dev), _rand(2, (34, heads, dim), BF16).to(dev)
+    turns = pkg.make_rotary_table(20, 16, device=dev)
+    offs, zero = torch.tensor([0, 20, 20, 34, 34], device=dev), torch.zeros(4, dtype=torch.int64, device=dev)
+    lengths, targets = torch.tensor([20, 0, 14, 0], device=dev), torch.tensor([3, 0, 3, 0], device=dev)
+    q = _rand(3, (4 * 16, 2, dim), BF16).to(dev)
+    got = []
+    for check in ("0", "1"):
+        monkeypatch.setenv("HSTU_HIP_CHECK_CONTRACT", check)
+        pkg.append_paged_kv(cache, k, v, table, zero, offs, turns)
+        got.append([*pkg.read_paged_kv(cache, 34, table, zero, offs), pkg.delta_hstu_mha_paged(20, 0.2, q, cache, table, lengths, targets, 0, 2)])
+    torch.cuda.synchronize()
+    for a, b in zip(*got):
+        assert torch.equal(a, b) and torch.isfinite(a).all()
+    assert (got[0][2][16:32] == 0).all() and (got[0][2][32:34] == 0).all() and (got[0][2][48:] == 0).all()
 
 
 @pytest.mark.gpu
