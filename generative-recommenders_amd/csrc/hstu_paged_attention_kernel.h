@@ -478,10 +478,12 @@ __device__ __forceinline__ int block_order(const PagedAttentionParams& p, int ea
 // products' operands lie in registers (a lane's 16 bytes side by side: reads and writes without bank conflicts), and the pairs as four
 // floats a position: c1 s, c1 l of K, s, l + 7.5 s of V.  Two buffers, one barrier a step; the packed rows of the next step are on their way
 // while this one is worked on.  Unpacking per wave, as above, cost as much as half of the rest and the registers of a second wave.
-// What bounds it is silu: 8 operations and two of a quarter's rate for each score, 62 clocks of a SIMD for 64 scores, beside which the
-// products take 34 and unpacking 14.  32 sequences of 1280 .. 4352 positions with 256 rows and four heads of 128 (39 GFLOP, 32 us of the
-// matrix cores as a large library product uses them, 33 of silu alone): 88 us.  Two workgroups of a CU, out of step with each other, fill the gaps of one another: the same
-// two teams of waves in one workgroup, behind one barrier, took 106.
+// Vector operations bound it: for 32 positions and 32 rows a wave has 204 of them, 152 for silu, its masks and roundings, and 34 products.
+// 32 sequences of 1280 .. 4352 positions with 256 rows and four heads of 128 (39 GFLOP, 32 us of the matrix cores as a large library
+// product uses them): 88 us, 10 of them for joining two parts of each sequence; of 177 thousand clocks a SIMD has 71 of vector operations
+// and 41 of products (counted), and what is left is waits, and the longest sequence's end.  Two workgroups of a CU, out of step with each
+// other, fill the gaps of one another: the same two teams of waves in one workgroup, behind one barrier, took 106 us.  Three of 64 rows and
+// one chunk a step took 91: more operations, nothing gained from a third wave.
 template <class TT, int DK, int DV, int MT>
 __global__ __launch_bounds__(256, 2) void hstu_paged_block_kernel(const PagedAttentionParams p) {
     typedef typename TT::elem T;

@@ -4,6 +4,8 @@
 // extremes of a row are log2(LPV) lane exchanges.  Codes are found by a quotient that is rounded as IEEE says, so that a tie between
 // two codes (K and V have 8 or 11 bits, a step too: ties do occur) falls the same way on any machine.
 #pragma once
+#include <type_traits>
+
 #include "hstu_norm_rope.h"
 
 namespace hstu {
@@ -137,19 +139,25 @@ __device__ __forceinline__ unsigned to_four_bits(const float (&x)[8], unsigned& 
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float a = __builtin_fmaf(x[i], by, from), q = a * y;
-        code[i] = __builtin_amdgcn_fmed3f(__builtin_rintf(__builtin_fmaf(__builtin_fmaf(-q, b, a), y, q)), 0.f, 15.f);
+        code[i] = __builtin_fmaf(__builtin_fmaf(-q, b, a), y, q);
     }
-    // four codes are one number below 2^16, exact in a float
-    const float low = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(code[3], 16.f, code[2]), 16.f, code[1]), 16.f, code[0]);
-    const float high = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(code[7], 16.f, code[6]), 16.f, code[5]), 16.f, code[4]);
-    return step > 0.f ? (unsigned)low | ((unsigned)high << 16) : 0u;
+    // No quotient is below 0; one above 15 1/2 there is only where the step, below the type's normal numbers, has lost bits in its rounding.
+    if (__ballot(step < (std::is_same<T, __bf16>::value ? 0x1p-126f : 0x1p-14f)) != 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) code[i] = fminf(code[i], 15.f);
+    }
+    // rounded to the nearest, ties to even, into a byte each: the even columns' word, the odd ones'
+    unsigned even = 0, odd = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) even = __builtin_amdgcn_cvt_pk_u8_f32(code[2 * i], i, even), odd = __builtin_amdgcn_cvt_pk_u8_f32(code[2 * i + 1], i, odd);
+    return step > 0.f ? even | (odd << 4) : 0u;
 }
 
 // grid (rows / groups of a workgroup, vectors / vectors_per_group): a row's vectors count through its heads of K, then of V.
 // (16 columns to a lane, which do what a row takes once in half as many lanes, came to a third fewer instructions and to the same time,
 // four waves of a SIMD in 107 registers where six have 78.  So did the first loads in front of the lookups.)  Vector operations
-// bound it, with the bytes close below: 256 sequences of 64 .. 1024 rows, four heads of 128, normed and turned, 97 us (337 MB, 65 us of a
-// copy; 51 million operations, 83 us of the SIMDs).  64 single rows take 4.5 us, one launch and three loads that wait for each other.
+// bound it, with the bytes close below: 256 sequences of 64 .. 1024 rows, four heads of 128, normed and turned, 93 us (337 MB, 65 us of a
+// copy; the loads and stores alone 68); fp16 rows that are only turned, 146378 of eight heads, 175 (761 MB; alone 163).  64 single rows take 4.5 us, one launch and three loads that wait for each other.
 template <class T, int LPV, int TURN>
 __global__ __launch_bounds__(256) void hstu_paged_append_kernel(const AppendParams p) {
     constexpr int GROUPS = 256 / LPV, AHEAD = 4;
