@@ -45,11 +45,14 @@ Plan plan_of(const HstuPagedCache* c, const HstuPagedAttentionArgs* a) {
     if (a->max_attn_len > 0 && (int64_t)a->max_attn_len + a->delta_size + a->contextual_seq_len < longest)
         longest = (int64_t)a->max_attn_len + a->delta_size + a->contextual_seq_len;
     const int64_t chunks = (longest + 31) / 32 + 1, wgs = (int64_t)p.row_blocks * c->heads * c->batch;
-    // Runs of a step: as many workgroups as the card holds at once (two of a CU), for each begins with some microseconds of loads that wait
-    // for each other (64 sequences of 1024 .. 4096 positions and four heads, 256 workgroups for whole sequences: runs of 130 chunks, all of one, 28 us,
-    // of 80 26, of 16 30), but none longer than 96 chunks, so that the last of them do not run alone (128 sequences of up to 16384 and eight heads:
-    // whole sequences 291 us, runs of 384 chunks 281, of 103 264, of 33 281).  Sequences of a few chunks, more of them than fit, are a wave's each (1600 of
-    // up to 10 chunks: 12 us, 16 by workgroups).
+    // Runs of a step.  Joining costs 3 us, so sequences of up to 40 chunks are one run each (one of 512 positions: 8.2 us, in two runs 11.4; of 1024:
+    // 10.2, in three 11.6), and so are those of up to 96 where they fill half of what the card holds, two workgroups of a CU (100 of up to 2048
+    // positions and four heads: 22 us, in two runs 25).  Else runs that fill it once, for each begins with some microseconds of loads that wait for
+    // each other (64 sequences of 1024 .. 4096 positions and four heads, 256 workgroups for whole sequences: in two runs 26 us, one 28, eight 30);
+    // in eights, two chunks to each wave (33 sequences of up to 2048, four rows: runs of 16 15 us, of 18 or 32 18); none that leaves a short second
+    // or third; and none longer than 96, so that the last of them do not run alone (128 sequences of up to 16384 and eight heads: whole
+    // sequences 291 us, runs of 384 chunks 281, of 96 264, of 33 281).  Sequences of a few chunks, more of them than fit, are a wave's each
+    // (1600 of up to 10 chunks: 12 us, 16 by workgroups).
     // More rows are split into equal parts of each sequence, of at least 8 or 16 chunks: what a part more costs is a partial sum of every row to
     // write and read.  Blocks: at least two workgroups of a CU, whose sequences are ranked.  Nine to 32 rows: parts that fill the card in one
     // round, 512 workgroups of up to 16 rows or 256 of more, or in two rounds where one would leave much of it empty (24 rows, 160 workgroups
@@ -58,8 +61,16 @@ Plan plan_of(const HstuPagedCache* c, const HstuPagedAttentionArgs* a) {
     const int64_t fill = (chunks * wgs + 511) / 512;
     int64_t run = 16;
     if (p.step) {
-        run = a->kv_splits > 0 ? (chunks + a->kv_splits - 1) / a->kv_splits : (fill + 15) / 16 * 16;
-        if (!a->kv_splits && run > 96) run = 96;
+        if (a->kv_splits > 0) {
+            run = (chunks + a->kv_splits - 1) / a->kv_splits;
+        } else if (chunks <= 40 || (wgs >= 256 && chunks <= 96)) {
+            run = chunks;
+        } else {
+            run = (fill + 4) / 8 * 8;
+            if (run > 96) run = 96;
+            if (run < 16) run = 16;
+            if (chunks > run && chunks / run <= 2 && chunks % run <= run / 4) run = (chunks / (chunks / run) + 8) / 8 * 8;
+        }
         if (run < 16) run = 16;
         if (run > chunks) run = chunks;
     } else {
