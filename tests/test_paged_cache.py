@@ -370,6 +370,38 @@ def test_norm_rope_gradients_against_differences_of_the_kernel(pkg, dev):
 
 
 @pytest.mark.gpu
+def test_rows_past_32_bit_offsets(pkg, dev):
+    """More than 2^31 values in q and in K: the last rows are those that a call on them alone gives, forward, backward and in the cache."""
+    print("[case] rows past 2^31 values", flush=True)
+    heads, dim, page, tail = 8, 128, 1024, 300
+    rows = 2**31 // (heads * dim) + 77
+    x = torch.empty((rows, heads, dim), dtype=BF16, device=dev)
+    x[: rows - tail] = 1
+    x[rows - tail :] = _rand(1, (tail, heads, dim), BF16).to(dev)
+    w, turns = (1 + 0.1 * _rand(2, (dim,), BF16)).to(dev), pkg.make_rotary_table(4096, dim, device=dev)
+    at = torch.arange(rows, device=dev) % 4096
+    got = []
+    for q, pos in ((x, at), (x[rows - tail :].clone(), at[rows - tail :].clone())):
+        q = q.detach().requires_grad_()
+        y = pkg.qk_norm_rope(q, None, pos, turns, w)[0]
+        dq = torch.autograd.grad(y, q, q.detach())[0]
+        got.append((y.detach()[-tail:].clone(), dq[-tail:].clone()))
+        del y, dq, q
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    pages = -(-rows // page)
+    cache = pkg.allocate_paged_kv_cache(pages, page, heads, dim, 32, BF16, dev)
+    v = x[:, :, 32:64]
+    table, zero = torch.arange(pages, dtype=torch.int32, device=dev).view(1, -1), torch.zeros(1, dtype=torch.int64, device=dev)
+    pkg.append_paged_kv(cache, x, v, table, zero, None, turns, at, w)
+    k_all, v_all = pkg.read_paged_kv(cache, rows, table, zero)
+    few = pkg.allocate_paged_kv_cache(1, page, heads, dim, 32, BF16, dev)
+    pkg.append_paged_kv(few, x[rows - tail :], v[rows - tail :], zero.int().view(1, 1), zero, None, turns, at[rows - tail :].clone(), w)
+    k_few, v_few = pkg.read_paged_kv(few, tail, zero.int().view(1, 1), zero)
+    torch.cuda.synchronize()
+    assert torch.equal(k_all[-tail:], k_few) and torch.equal(v_all[-tail:], v_few)
+
+
+@pytest.mark.gpu
 def test_norm_rope_refusals(pkg, dev):
     q, k, pos, table, qw, kw, _ = _norm_rope_inputs((12, 2, 1, 32, 32, False, True, BF16))
     q, k, pos, table, qw, kw = _to(dev, q, k, pos, table, qw, kw)
@@ -592,6 +624,29 @@ def test_attention_over_the_cache(pkg, dev, case):
         torch.cuda.synchronize()
         assert torch.equal(got, again), "two runs differ"
         _within(got, want, bound, f"splits {splits}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dqk,dv,dtype", [(128, 128, BF16), (64, 128, F16), (32, 64, BF16), (128, 32, F16), (256, 256, BF16), (64, 64, F16)])
+def test_attention_around_the_kernels_numbers_of_rows(pkg, dev, dqk, dv, dtype):
+    """Every number of rows at which another kernel, or another tile of one, takes over; ragged lengths around chunks and pages."""
+    for i, rows in enumerate((2, 3, 4, 5, 8, 9, 12, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 193)):
+        print(f"[case] attention, {rows} rows {dqk} {dv} {dtype}", flush=True)
+        group = 2 if rows % 2 == 0 and i % 3 else 1
+        delta = rows // group
+        lengths = [delta + 31 * i, delta, 1100 + 7 * i, delta + 512 - 32 * (i % 3)]
+        targets, w, c = ([delta, 0, delta // 2, 1], 0, 0) if i % 2 else (None, 150 + i, 3 if delta < 60 else 0)
+        case = (lengths, delta, targets, w, c, group, 1, dqk, dv, 16 << (i % 4), dtype)
+        q, cache, table, n, t = _attention_inputs(case, seed=10 * i)
+        if c and targets is None:
+            n = n.clamp(min=c)
+        N = max(lengths)
+        want, bound = O.attention(N, dqk**-0.5, q, cache, table, n, t, w, c, dtype)
+        args = (N, dqk**-0.5, q.to(dev), tuple(x.to(dev) for x in cache), table.to(dev), n.to(dev), None if t is None else t.to(dev), w, c)
+        for splits in (0, 2):
+            got = pkg.delta_hstu_mha_paged(*args, kv_splits=splits)
+            torch.cuda.synchronize()
+            _within(got, want, bound, f"{rows} rows, splits {splits}")
 
 
 @pytest.mark.gpu
