@@ -55,9 +55,9 @@ Plan plan_of(const HstuPagedCache* c, const HstuPagedAttentionArgs* a) {
     // (1600 of up to 10 chunks: 12 us, 16 by workgroups).
     // More rows are split into equal parts of each sequence, of at least 8 or 16 chunks: what a part more costs is a partial sum of every row to
     // write and read.  Blocks: at least two workgroups of a CU, whose sequences are ranked.  Nine to 32 rows: parts that fill the card in one
-    // round, 512 workgroups of up to 16 rows or 256 of more, or in two rounds where one would leave much of it empty (24 rows, 160 workgroups
+    // round, 512 workgroups, or 256 of more than 16 rows of wide heads, whose waves need a SIMD each, or in two rounds where one would leave much of it empty (24 rows, 160 workgroups
     // for whole sequences of up to 8192: one part 88 us, two 74, three 64, four 67; 256 workgroups of up to 4096: one 49, two 57, four 66;
-    // 16 rows, 128 workgroups of up to 8192: two 41, four 34, eight 37).
+    // 16 rows, 128 workgroups of up to 8192: two 41, four 34, eight 37; 24 rows of 64 columns, the same: two 45, four 34, eight 35).
     const int64_t fill = (chunks * wgs + 511) / 512;
     int64_t run = 16;
     if (p.step) {
@@ -76,7 +76,7 @@ Plan plan_of(const HstuPagedCache* c, const HstuPagedAttentionArgs* a) {
     } else {
         int64_t parts = a->kv_splits;
         if (parts == 0 && wgs > 0) {
-            const int64_t slots = p.rw == 4 || p.mt == 1 ? 512 : 256;
+            const int64_t slots = p.rw == 4 || p.mt == 1 || c->dqk + c->dv < 256 ? 512 : 256;
             parts = p.rw == 4 ? (slots + wgs - 1) / wgs : slots / wgs;
             if (p.rw != 4 && parts <= 2 && 2 * slots / wgs > 2 * parts) parts = 2 * slots / wgs;
         }

@@ -233,9 +233,10 @@ __device__ __forceinline__ void store_columns(const PagedAttentionParams& p, int
 // grid: one workgroup of four waves per (block of 16 MT rows, head of the cache, run, sequence), numbered so that the row blocks of one
 // run, which read the same pages, are on one XCD.  The waves share out the chunks of the run; their sums meet in LDS.  Unpacking and silu
 // bound it, the cache's bytes not far below: 12 rows, 256 sequences of 1000 .. 8192 positions and four heads of 128 182 us (629 MB, 121 us
-// of a copy); 24 rows, whose sums leave room for one wave of a SIMD, 318.
+// of a copy); 24 rows, whose registers leave room for one wave of a SIMD, 318.  Held to two waves, with 85 registers spilled, the latter took 361;
+// heads of 64 and 128, with seven, gained: 64 sequences of 512 .. 4096 46 us by one wave, 36 by two.
 template <class TT, int DK, int DV, int MT>
-__global__ __launch_bounds__(256) void hstu_paged_attention_kernel(const PagedAttentionParams p) {
+__global__ __launch_bounds__(256, (MT == 2 && DK + DV < 256 ? 2 : 1)) void hstu_paged_attention_kernel(const PagedAttentionParams p) {
     typedef typename TT::elem T;
     constexpr int NK = DK / 32, NV = DV / 16, KW = 4;
     __shared__ float meet[KW * NV * 4 * 64];
