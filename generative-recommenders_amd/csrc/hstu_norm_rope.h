@@ -200,6 +200,10 @@ __device__ __forceinline__ void norm_and_turn(const LaneTurn& t, const Cols<T>& 
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = y[i] * t.c[i] + p[i] * t.s[i];
     }
+    // What comes next rounds an fp32 number.  (The compiler may otherwise make one instruction of the last product and its conversion to fp16, which
+    // rounds once where the other form of the step rounds twice: a byte or two in a million of a cache's.)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm("" : "+v"(y[i]));
 }
 
 // One side (q or k) of the step.
