@@ -164,16 +164,17 @@ __device__ __forceinline__ void lane_weights(const T* weight, int col0, float (&
     }
 }
 
-// 1 / sqrt(mean of squares + eps) of a vector, rounded as a plain evaluation of the mean and the reciprocal root on this device gives it (measured: the same
-// bits): squares added pairwise, from sums of four on where a vector has 128 columns or more, and the instruction's root, good to a unit in
-// the last place, corrected once by its residual.
+// 1 / sqrt(mean of squares + eps) of a vector: squares added pairwise, in vectors of more than 64 columns (`wide`) from sums of four on, and the
+// instruction's root, good to a unit in the last place, corrected once by its residual.  The order goes by the vector's width and not by the lanes
+// it is given, so that K comes out the same beside any width of V.  At 16, 32, 64, 128 and 256 columns that is also, bit by bit, what PyTorch's mean
+// and reciprocal root gave on this device; at 48, 80, 104 and 512 a fifth of the rows differed in the last place.
 template <int LPV>
-__device__ __forceinline__ float inverse_rms(const float (&x)[8], bool there, float inv_dim, float eps) {
+__device__ __forceinline__ float inverse_rms(const float (&x)[8], bool there, bool wide, float inv_dim, float eps) {
 #pragma clang fp contract(off)
     float q[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) q[i] = x[i] * x[i];
-    const float sum = LPV >= 16 ? (q[0] + q[1] + q[2] + q[3]) + (q[4] + q[5] + q[6] + q[7]) : ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+    const float sum = LPV >= 16 && wide ? (q[0] + q[1] + q[2] + q[3]) + (q[4] + q[5] + q[6] + q[7]) : ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
     const float v = group_sum<LPV>(there ? sum : 0.f) * inv_dim + eps;
     const float r = __builtin_amdgcn_rsqf(v), h = v * r, low = __builtin_fmaf(v, r, -h);
     const float fixed = __builtin_fmaf(0.5f * r, __builtin_fmaf(-low, r, __builtin_fmaf(-h, r, 1.f)), r);
@@ -185,12 +186,12 @@ __device__ __forceinline__ float inverse_rms(const float (&x)[8], bool there, fl
 // to codes, where a value that comes out a unit in the last place off now and then is a whole step off.  (Weights multiplied into cosines and
 // sines, and sums by fused operations, gave twenty such codes in 18 million; this costs no more.)
 template <class T, int LPV, int TURN>
-__device__ __forceinline__ void norm_and_turn(const LaneTurn& t, const Cols<T>& in, const float (&w)[8], bool there, bool norm, float inv_dim, float eps,
-                                              float (&y)[8]) {
+__device__ __forceinline__ void norm_and_turn(const LaneTurn& t, const Cols<T>& in, const float (&w)[8], bool there, bool norm, bool wide, float inv_dim,
+                                              float eps, float (&y)[8]) {
 #pragma clang fp contract(off)
     in.get(y);
     if (norm) {
-        const float r = inverse_rms<LPV>(y, there, inv_dim, eps);
+        const float r = inverse_rms<LPV>(y, there, wide, inv_dim, eps);
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = y[i] * r * w[i];
     }
@@ -266,7 +267,7 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_kernel(const NormRopeParam
             for (int a = 0; a < AHEAD; ++a) {
                 if (h + a >= h1) break;  // (the same for the whole workgroup)
                 float y[8];
-                norm_and_turn<T, LPV, TURN>(t, in[a], w, cols, s.weight != nullptr, p.inv_dim, p.eps, y);
+                norm_and_turn<T, LPV, TURN>(t, in[a], w, cols, s.weight != nullptr, true, p.inv_dim, p.eps, y);
                 Cols<T> o;
                 o.put(y);
                 if (there) o.store(out + (h + a) * p.dim);
@@ -332,7 +333,7 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_bwd_kernel(const NormRopeP
                     }
                     if (s.weight) {
                         in[a].get(x);
-                        const float r = inverse_rms<LPV>(x, cols, p.inv_dim, p.eps);
+                        const float r = inverse_rms<LPV>(x, cols, true, p.inv_dim, p.eps);
                         float dot = 0.f;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {

@@ -198,7 +198,7 @@ __global__ __launch_bounds__(256) void hstu_paged_append_kernel(const AppendPara
                 float x[8];
                 if (changed) {
                     float y[8];
-                    norm_and_turn<T, LPV, TURN>(t, in[a], w, cols, p.k_weight != nullptr, p.inv_dim, p.eps, y);
+                    norm_and_turn<T, LPV, TURN>(t, in[a], w, cols, p.k_weight != nullptr, dim > 64, p.inv_dim, p.eps, y);
                     Cols<T> rounded;
                     rounded.put(y);
                     rounded.get(x);

@@ -38,3 +38,20 @@ def _two_ways(pkg, dev, dqk, dv):
 @pytest.mark.parametrize("dim", [32, 64, 128, 256])
 def test_codes_do_not_depend_on_who_normed_and_turned(pkg, dev, dim):
     _two_ways(pkg, dev, dim, dim)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dqk,dv", [(32, 64), (32, 128), (32, 256), (64, 128), (64, 256), (128, 32), (128, 256), (256, 128)])
+def test_codes_do_not_depend_on_the_width_of_v(pkg, dev, dqk, dv):
+    _two_ways(pkg, dev, dqk, dv)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+def test_norms_of_a_caches_widths_are_those_of_plain_operators(pkg, dev, dim):
+    """At the widths a cache has, the norm in fp32 is bit by bit that of PyTorch's mean, reciprocal root and products, as this image has them (at
+    48, 80, 104 or 512 columns it is not: other orders of the sum)."""
+    print(f"[case] norm beside plain operators {dim}", flush=True)
+    x, w = _rand(1, (20000, 2, dim), F32).to(dev), (1 + 0.1 * _rand(2, (dim,), F32)).to(dev)
+    want = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + 1e-6) * w
+    assert torch.equal(pkg.qk_norm_rope(x, None, None, None, w)[0], want)
