@@ -45,6 +45,7 @@ struct PagedAttentionParams {
 struct PagedSpan {
     int n, u;  // length and its part that is no target
     int a0, na, b0, nb;
+    int seen;  // the first position that a row sees: pages that end in front of it need not be there
     bool bad;  // the sequence has no room in the page table
 };
 
@@ -58,13 +59,15 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttentionParams& p, i
     t = t < 0 ? 0 : t > s.n ? s.n : t;
     s.u = s.n - (int)t;
     const int first = max(s.n - p.delta + i0, 0), end = s.n - p.delta + i1;  // positions of the rows
-    s.a0 = s.na = s.b0 = s.nb = 0;
+    s.a0 = s.na = s.b0 = s.nb = s.seen = 0;
     if (end <= first) return s;
     const bool contextual = first < p.c;
     const int a_end = contextual ? max(s.u, min(end, s.u)) : min(end, s.u);
     const int id = min(p.c ? first - p.c + 1 : first, p.c ? s.u - p.c + 1 : s.u);  // of the first row: the others' are not less
     const int from = p.w > 0 && !contextual && id > p.w ? max(0, id - p.w + (p.c ? p.c - 1 : 0)) : 0;
+    s.seen = from;
     if (a_end > from) s.a0 = from >> 5, s.na = ((a_end + 31) >> 5) - s.a0;
+    else s.seen = max(s.u, first);
     if (end > s.u) {  // targets: the positions that only they themselves see
         const int self = max(s.u, first), done = s.a0 + s.na;
         s.b0 = max(self >> 5, s.na ? done : 0);
@@ -378,12 +381,12 @@ __global__ __launch_bounds__(256, (MT == 2 && DK + DV < 256 ? 2 : 1)) void hstu_
         }
     };
 
-    // Pages of the two tiles of 32 of this wave's chunks, KW apart from chunk i on, one to a lane; what does not exist has the first page.  Two
+    // Pages of the two tiles of 32 of this wave's chunks, KW apart from chunk i on, one to a lane; what does not exist, or lies in front of all that is seen, has the first page.  Two
     // sets: the next one has been loaded when its turn comes.
     auto pages_of = [&](int i) __attribute__((always_inline)) {
         int page = 0;
         const int ci = i + KW * (lane >> 1), pos = ci < chunk_end ? chunk_at(ci) * 32 + (lane & 1) * 16 : span.n;
-        if (pos < span.n) {
+        if (pos < span.n && pos + 16 > span.seen) {
             const int64_t at = index_at(p.cache.page_table, p.cache.page_table_i64, b * p.cache.table_row_stride + (pos >> p.cache.page_shift));
             if (at < 0 || at >= p.cache.pages) bad = true;
             else page = (int)at;
@@ -513,12 +516,12 @@ __global__ __launch_bounds__(256, 2) void hstu_paged_block_kernel(const PagedAtt
     const unsigned v_lane = 4 * g * (DV / 2) + m * (NV / 2) + 2 * v_half;
     bool bad = span.bad;
     unsigned raw_k[NK], raw_v[8], raw_ks = 0, raw_vs = 0;
-    // Pages of the 64 tiles of 16 positions from chunk ci on, one to a lane; what does not exist has the first page.  Two sets: the next one
+    // Pages of the 64 tiles of 16 positions from chunk ci on, one to a lane; what does not exist, or lies in front of all that is seen, has the first page.  Two sets: the next one
     // has been loaded when its turn comes.  (A page looked up where it is needed is two loads that the wave waits for, three times a step.)
     auto pages_of = [&](int ci) __attribute__((always_inline)) {
         int page = 0;
         const int pos = ci + (lane >> 1) < end ? chunk_at(ci + (lane >> 1)) * 32 + (lane & 1) * 16 : span.n;
-        if (pos < span.n) {
+        if (pos < span.n && pos + 16 > span.seen) {
             const int64_t at = index_at(c.page_table, c.page_table_i64, b * c.table_row_stride + (pos >> c.page_shift));
             if (at < 0 || at >= c.pages) bad = true;
             else page = (int)at;
@@ -850,11 +853,11 @@ __global__ __launch_bounds__(256, (STEP_WAVES<DK, DV>)) void hstu_paged_step_ker
     const int in_page = (1 << c.page_shift) - 1;
     const unsigned k_lane = n * (DK / 2) + g * (4 * NK), v_lane = 4 * g * (DV / 2) + n * (NV / 2);
 
-    // Pages of the tiles of 16 of the F chunks from s0 on, one to a lane; what does not exist has the first page.
+    // Pages of the tiles of 16 of the F chunks from s0 on, one to a lane; what does not exist, or lies in front of all that is seen, has the first page.
     auto pages_of = [&](int s0) __attribute__((always_inline)) {
         int page = 0;
         const int pos = chunk_at(min(s0 + ((lane >> 1) & (F - 1)), end - 1)) * 32 + (lane & 1) * 16;
-        if (pos < span.n) {
+        if (pos < span.n && pos + 16 > span.seen) {
             const int64_t at = index_at(c.page_table, c.page_table_i64, b * c.table_row_stride + (pos >> c.page_shift));
             if (at < 0 || at >= c.pages) bad = true;
             else page = (int)at;

@@ -211,6 +211,18 @@ def _check_places(cache, page_table: torch.Tensor, start: torch.Tensor, offsets:
         raise ValueError("hstu_cache: page_table names a page that the cache does not have")
 
 
+def _first_seen(lengths: torch.Tensor, targets: Optional[torch.Tensor], delta: int, max_attn_len: int, contextual: int) -> torch.Tensor:
+    """The first position that any of the newest ``delta`` positions of each sequence sees."""
+    top = (lengths - delta).clamp(min=0)
+    history = lengths if targets is None else lengths - targets.long()
+    ids = torch.minimum(top, history) - (contextual - 1 if contextual else 0)
+    lowest = (ids - max_attn_len + (contextual - 1 if contextual else 0)) if max_attn_len else torch.zeros_like(ids)
+    first = torch.where(ids > max_attn_len, lowest, torch.zeros_like(ids))
+    if contextual:
+        return torch.where(top < contextual, torch.zeros_like(ids), first)
+    return torch.where(ids > 0, first, top)
+
+
 def append_paged_kv(
     cache: Sequence[torch.Tensor],
     k: torch.Tensor,
@@ -314,8 +326,10 @@ def delta_hstu_mha_paged(
 
     The masks are those of ``delta_hstu_mha``.  K and V enter as they are stored, unrounded (``lowest + step * code``); sums are in
     fp32.  A sequence shorter than ``delta`` has zeros in the rows in front of its first position; one that does not fit its row
-    of the page table, or one of whose pages the cache does not have, comes back NaN (``HSTU_HIP_CHECK_CONTRACT=1`` raises
-    instead).  ``kv_splits``: at most so many runs per row block (0 = automatic); it changes the order of the fp32 sums.
+    of the page table comes back NaN, and so does every row that sees a position on a page that the cache does not have (other rows
+    of its sequence may; ``HSTU_HIP_CHECK_CONTRACT=1`` raises instead).  Pages that end in front of the first position that any of
+    the ``delta`` rows sees, behind a window, may be gone: they are not looked at.  ``kv_splits``: at most so many runs per row block
+    (0 = automatic); it changes the order of the fp32 sums.
     """
     out = native.front.delta_hstu_mha_paged(max_seq_len, alpha, delta_q, tuple(cache), page_table, seq_lengths, num_targets, max_attn_len,
                                             contextual_seq_len, kv_splits, False)
@@ -341,7 +355,9 @@ def delta_hstu_mha_paged(
     if delta_q.numel() == 0:
         return torch.empty((delta_q.shape[0], delta_q.shape[1], 2 * cache[2].shape[3]), dtype=delta_q.dtype, device=delta_q.device)
     if hip_backend.contract_checks_enabled():
-        _check_places(cache, page_table, torch.zeros_like(seq_lengths), torch.nn.functional.pad(seq_lengths.cumsum(0), (1, 0)), int(seq_lengths.sum()))
+        first = _first_seen(seq_lengths.long(), num_targets, delta_q.shape[0] // batch, max_attn_len, contextual_seq_len)
+        count = seq_lengths - first
+        _check_places(cache, page_table, first, torch.nn.functional.pad(count.cumsum(0), (1, 0)), int(count.sum()))
         if bool((seq_lengths > max_seq_len).any()):
             raise ValueError("hstu_cache: a sequence is longer than max_seq_len")
         if num_targets is not None and bool(((num_targets < 0) | (num_targets > seq_lengths)).any()):

@@ -147,8 +147,9 @@ int hstu_cache_read(const HstuPagedCache* cache, int64_t rows, const void* start
  * p = seq_lengths[b] - delta_size + i of every sequence, with the masks of the cached form (hstu_hip.h).  Head h of q reads head
  * h / (q_heads / heads) of the cache.  K and V enter as lowest + step * code, unrounded; silu(.) times a V row's step is rounded to
  * bf16 for the second product (to two bf16 words, 16 bits, where the type is fp16), sums are in fp32 and rounded once.
- * A row at a position before the first is zero.  A sequence that is longer than its row of the page table, or one of whose pages
- * is not one of the cache's, gives NaN.
+ * A row at a position before the first is zero.  A sequence that is longer than its row of the page table gives NaN.  Where one of its
+ * pages is not one of the cache's, every row that sees a position on that page is NaN, and other rows of the sequence may be; pages that end
+ * in front of the first position that any row of the call sees (behind a window) are not looked at.
  * The positions of a row block are cut into runs that `workspace` joins (kv_splits: 0 = automatic, else at most that many); the
  * order of the sums depends on the sizes of the call and the lengths alone.
  */

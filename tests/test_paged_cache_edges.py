@@ -11,6 +11,77 @@ from test_paged_cache import _abi, _append_inputs, _norm_rope_inputs, _rand, _to
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
+# ---- pages that are none ------------------------------------------------------------------------------------------------
+
+
+def _first_seen(n, delta, targets, w, c):
+    """First position that any of the newest ``delta`` rows of a sequence of ``n`` sees."""
+    seen = hstu_oracle._seq_mask_rows(n, max(n - delta, 0), n, targets, w, c, 0)
+    return int(seen.any(0).nonzero()[0]) if n else 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("delta", [1, 3, 12, 24, 40, 150])
+@pytest.mark.parametrize("page,dtype", [(16, BF16), (64, F16)])
+def test_pages_in_front_of_the_window_may_be_gone(pkg, dev, delta, page, dtype, monkeypatch):
+    """Pages that lie whole in front of the first position a row sees are not looked at: the table may name anything there, with the contract checks
+    on too.  Windows that end anywhere in a chunk of 32 positions."""
+    print(f"[case] attention: pages in front of the window {delta} {page} {dtype}", flush=True)
+    dim = 32
+    for c, w, t in ((0, 41, None), (0, 56, 1), (3, 63, 0), (2, 77, delta)):
+        lengths = [700 + 17 * b for b in range(9)] + [delta + c + 20, 0]
+        targets = None if t is None else torch.tensor([min(t, n) for n in lengths])
+        table, pages = O.page_table(delta, lengths, page)
+        cache = tuple(x.to(dev) for x in O.fill_cache(delta + 1, pages, 1, page, dim, dim, dtype))
+        q = _rand(delta + 2, (len(lengths) * delta, 1, dim), dtype).to(dev)
+        n, tg = torch.tensor(lengths).to(dev), None if targets is None else targets.to(dev)
+        gone = table.clone()
+        for b, length in enumerate(lengths):
+            first = _first_seen(length, delta, None if t is None else int(targets[b]), w, c)
+            gone[b, : first // page] = torch.tensor([-1, 10**6, pages], dtype=torch.int32).repeat(100)[: first // page]
+        assert int((gone != table).sum()) > 5
+        want, bound = O.attention(900, 0.2, q.cpu(), tuple(x.cpu() for x in cache), table, n.cpu(), targets, w, c, dtype)
+        for splits in (0, 3):
+            for check in ("0", "1"):
+                monkeypatch.setenv("HSTU_HIP_CHECK_CONTRACT", check)
+                whole = pkg.delta_hstu_mha_paged(900, 0.2, q, cache, table.to(dev), n, tg, w, c, kv_splits=splits)
+                got = pkg.delta_hstu_mha_paged(900, 0.2, q, cache, gone.to(dev), n, tg, w, c, kv_splits=splits)
+                torch.cuda.synchronize()
+                assert torch.equal(got, whole), (c, w, t, splits, check)
+                _within(got, want, bound, f"{c} {w} {t}")
+        # one page further on is one that a row sees
+        b = 4
+        first = _first_seen(lengths[b], delta, None if t is None else int(targets[b]), w, c)
+        gone[b, first // page] = -1
+        monkeypatch.setenv("HSTU_HIP_CHECK_CONTRACT", "1")
+        with pytest.raises(ValueError, match="page"):
+            pkg.delta_hstu_mha_paged(900, 0.2, q, cache, gone.to(dev), n, tg, w, c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("delta", [5, 20, 300])
+def test_rows_that_see_a_bad_page_are_nan(pkg, dev, delta):
+    """A page that is none, among the history or among the targets: every row that sees a position on it is NaN, whatever block it is in, and the
+    other sequences are what they were."""
+    print(f"[case] attention: bad pages, {delta} rows", flush=True)
+    lengths = [delta + 500, delta + 333, delta + 64]
+    table, pages = O.page_table(1, lengths, 32)
+    cache = tuple(x.to(dev) for x in O.fill_cache(2, pages, 2, 32, 64, 64, BF16))
+    q = _rand(3, (3 * delta, 2, 64), BF16).to(dev)
+    for t in (0, delta):
+        n, tg = torch.tensor(lengths).to(dev), torch.tensor([t] * 3).to(dev)
+        good = pkg.delta_hstu_mha_paged(900, 0.2, q, cache, table.to(dev), n, tg)
+        for place in (100, lengths[1] - delta, lengths[1] - 1):
+            bad = table.clone()
+            bad[1, place // 32] = -7
+            got = pkg.delta_hstu_mha_paged(900, 0.2, q, cache, bad.to(dev), n, tg)
+            torch.cuda.synchronize()
+            seen = hstu_oracle._seq_mask_rows(lengths[1], lengths[1] - delta, lengths[1], t, 0, 0, 0)
+            on_page = seen[:, place // 32 * 32 : place // 32 * 32 + 32].any(1).to(dev)
+            assert torch.isnan(got[delta : 2 * delta][on_page]).all() and bool(on_page.any())
+            assert torch.equal(got[:delta], good[:delta]) and torch.equal(got[2 * delta :], good[2 * delta :])
+
+
 # ---- two ways to one cache ----------------------------------------------------------------------------------------------
 
 
