@@ -1,5 +1,8 @@
 // C ABI of the attention over a 4-bit paged cache (include/hstu_cache.h): checks, the cut into runs, launches.
 #include "hstu_cache.h"
+
+#include <algorithm>
+
 #include "hstu_cache_host.h"
 #include "hstu_paged_attention_kernel.h"
 
@@ -41,7 +44,8 @@ Plan plan_of(const HstuPagedCache* c, const HstuPagedAttentionArgs* a) {
         p.block = 16 * p.mt * p.rw;
     }
     p.row_blocks = (int)((rows + p.block - 1) / p.block);
-    int64_t longest = a->max_seq_len;
+    // (max_seq_len divides the result and may be far above what a row of the page table has room for)
+    int64_t longest = std::min((int64_t)a->max_seq_len, (int64_t)c->table_columns * c->page_size);
     if (a->max_attn_len > 0 && (int64_t)a->max_attn_len + a->delta_size + a->contextual_seq_len < longest)
         longest = (int64_t)a->max_attn_len + a->delta_size + a->contextual_seq_len;
     const int64_t chunks = (longest + 31) / 32 + 1, wgs = (int64_t)p.row_blocks * c->heads * c->batch;

@@ -11,6 +11,44 @@ from test_paged_cache import _abi, _append_inputs, _norm_rope_inputs, _rand, _to
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
+# ---- a divisor larger than the table's room -----------------------------------------------------------------------------
+
+
+def test_scratch_goes_by_the_tables_room():
+    """``max_seq_len`` divides the result; no sequence has more positions than its row of the page table has room for.  Scratch memory does not
+    grow with a divisor past that room, whichever kernel the number of rows takes (pointers are never followed)."""
+    lib, ref, made = _abi()
+    at = 1 << 20
+    for batch, heads, columns, page in ((64, 8, 128, 64), (32, 4, 8, 64), (1, 1, 1000, 16), (300, 2, 1, 1024)):
+        for delta in (1, 8, 12, 24, 64, 257):
+            need = []
+            for divisor in (columns * page, columns * page + 1, 1 << 20, 2**31 - 1):
+                cache = made["HstuPagedCache"](k_codes=at, k_scales=at, v_codes=at, v_scales=at, pages=1 << 16, heads=heads, page_size=page, dqk=128, dv=128, dtype=0, page_table=at,
+                                               table_row_stride=columns, table_columns=columns, batch=batch)
+                call = made["HstuPagedAttentionArgs"](q=at, q_row_stride=128 * heads, q_head_stride=128, out=at, seq_lengths=at, q_heads=heads, delta_size=delta, max_seq_len=divisor,
+                                                      alpha=1.0)
+                need.append(lib.hstu_cache_attention_workspace_bytes(ref(cache), ref(call)))
+            assert len(set(need)) == 1, (batch, heads, columns, page, delta, need)
+
+
+@pytest.mark.gpu
+def test_any_divisor_is_served(pkg, dev):
+    """Divisors of 2^20 and 2^31 - 1 (2^31 in fp32) with a table of 512 positions: the result is that of the divisor 512, scaled by a power of two, in
+    the same order of the sums."""
+    print("[case] attention: divisors past the table's room", flush=True)
+    batch, heads, dim, page, columns = 32, 4, 64, 64, 8
+    for delta, hq in ((1, 4), (3, 8), (12, 4), (40, 4)):
+        lengths = [delta + (37 * b) % (513 - delta) for b in range(batch)]
+        table, pages = O.page_table(delta, lengths, page, columns)
+        cache = tuple(c.to(dev) for c in O.fill_cache(delta + 1, pages, heads, page, dim, dim, BF16))
+        q, table, n = _to(dev, _rand(delta + 2, (batch * delta, hq, dim), BF16), table, torch.tensor(lengths))
+        want = pkg.delta_hstu_mha_paged(512, 0.125, q, cache, table, n)
+        for divisor, power in ((1 << 20, 20 - 9), (2**31 - 1, 31 - 9)):
+            got = pkg.delta_hstu_mha_paged(divisor, 0.125, q, cache, table, n)
+            torch.cuda.synchronize()
+            assert torch.equal(got.double(), want.double() * 2.0**-power), (delta, divisor)
+
+
 # ---- pages that are none ------------------------------------------------------------------------------------------------
 
 
