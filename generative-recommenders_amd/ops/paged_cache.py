@@ -147,7 +147,8 @@ def qk_norm_rope(
         raise NotImplementedError("head dims are multiples of 8 up to 512")
     if q.numel() == 0 or (k is not None and k.numel() == 0):
         if q.numel() == 0 and (k is None or k.numel() == 0):
-            return q * 1, None if k is None else k * 1  # (nothing in them; the graph, if there is one, goes on)
+            # nothing in them; the graph, if there is one, goes on, to gradients of zero for the weights too
+            return q * (1 if q_weight is None else q_weight), None if k is None else k * (1 if k_weight is None else k_weight)
         raise NotImplementedError("q and k must both have heads")
     q = _copied(q)
     k = None if k is None else _copied(k)

@@ -164,3 +164,24 @@ def test_norms_of_a_caches_widths_are_those_of_plain_operators(pkg, dev, dim):
     x, w = _rand(1, (20000, 2, dim), F32).to(dev), (1 + 0.1 * _rand(2, (dim,), F32)).to(dev)
     want = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + 1e-6) * w
     assert torch.equal(pkg.qk_norm_rope(x, None, None, None, w)[0], want)
+
+
+# ---- an empty batch, forward mode ---------------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+def test_an_empty_batch_gives_gradients_of_zero(pkg, dev):
+    """No rows: outputs without rows, and gradients of zero, of the inputs' shapes, for everything that wants one."""
+    print("[case] norm and rotation of no rows, backward", flush=True)
+    turns = pkg.make_rotary_table(8, 32, device=dev)
+    for dtype in (BF16, F32):
+        q, k = (torch.empty((0, h, 32), dtype=dtype, device=dev, requires_grad=True) for h in (4, 2))
+        qw, kw = (torch.ones(32, dtype=dtype, device=dev, requires_grad=True) for _ in range(2))
+        at = torch.empty(0, dtype=torch.int64, device=dev)
+        for args, leaves in (((q, k, at, turns, qw, kw), (q, k, qw, kw)), ((q, None, None, None, qw), (q, qw)), ((q, k, None, None, None, kw), (q, k, kw)),
+                             ((q.detach(), k.detach(), at, turns, qw, kw), (qw, kw)), ((q, k, at, turns), (q, k))):
+            out = pkg.qk_norm_rope(*args)
+            assert [None if y is None else (y.shape, y.dtype) for y in out] == [None if x is None else (x.shape, x.dtype) for x in args[:2]]
+            grads = torch.autograd.grad([y.sum() for y in out if y is not None and y.requires_grad], leaves)
+            for x, g in zip(leaves, grads):
+                assert g.shape == x.shape and g.dtype == x.dtype and bool((g == 0).all())
