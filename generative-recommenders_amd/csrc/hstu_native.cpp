@@ -749,6 +749,15 @@ void fill_k(HstuNormRopeArgs& a, const Tensor& x, const OptTensor& w) {
     a.k_weight = w ? w->const_data_ptr() : nullptr;
 }
 
+// Whether forward-mode differentiation has a tangent for any of these: the Python operator refuses them.
+bool has_tangent(std::initializer_list<const Tensor*> ts, std::initializer_list<const OptTensor*> others = {}) {
+    for (const Tensor* t : ts)
+        if (t->_fw_grad(0).defined()) return true;
+    for (const OptTensor* t : others)
+        if (*t && (*t)->_fw_grad(0).defined()) return true;
+    return false;
+}
+
 typedef std::tuple<Tensor, OptTensor> QAndK;
 
 QAndK norm_rope_result(const Tensor& q, const OptTensor& k, const OptTensor& positions, const OptTensor& table, const OptTensor& qw, const OptTensor& kw,
@@ -842,7 +851,7 @@ std::optional<QAndK> qk_norm_rope(const Tensor& q, const OptTensor& k, const Opt
     if (k && (!head_rows(*k, q.device()) || k->scalar_type() != type || k->size(0) != q.size(0) || k->size(2) != q.size(2))) return {};
     if (!rotary_table(table, q) || !norm_weight_of(qw, q) || !norm_weight_of(kw, q) || (kw && !k) || (!table && !qw && !kw)) return {};
     if (table && (!positions || !index_vector(*positions, q.size(0), q.device()) || table->size(1) > q.size(2))) return {};
-    if (!checked && contract_checks() && table) return {};
+    if ((!checked && contract_checks() && table) || has_tangent({&q}, {&k, &qw, &kw, &table})) return {};
     const NormRopeCall c{q.size(0), q.size(2), eps, interleaved};
     bool grad = wants_grad({&q});
     for (const OptTensor* t : {&k, &qw, &kw}) grad = grad || (*t && wants_grad({&**t}));
@@ -893,7 +902,7 @@ bool append_paged_kv(const CacheTensors& cache, const Tensor& k, const Tensor& v
     if (!placing(start, offsets, k.size(0), c.batch, k.device()) || !rotary_table(table, k) || !norm_weight_of(kw, k)) return false;
     if (table && table->size(1) > k.size(2)) return false;
     if (positions && !index_vector(*positions, k.size(0), k.device())) return false;
-    if (wants_grad({&k, &v}) || (kw && wants_grad({&*kw}))) return false;
+    if (wants_grad({&k, &v}) || (kw && wants_grad({&*kw})) || has_tangent({&k, &v}, {&kw, &table})) return false;
     HstuAppendArgs a{};
     a.k = k.const_data_ptr(), a.v = v.const_data_ptr(), a.rows = k.size(0);
     a.k_row_stride = row_pitch(k), a.k_head_stride = head_pitch(k), a.v_row_stride = row_pitch(v), a.v_head_stride = head_pitch(v);
@@ -929,7 +938,7 @@ OptTensor delta_hstu_mha_paged(int64_t max_seq_len, double alpha, const Tensor& 
     const Tensor& scales = std::get<1>(cache);
     if (!head_rows(q, scales.device()) || q.scalar_type() != scales.scalar_type() || q.size(2) != c.dqk || q.size(1) % c.heads != 0) return {};
     if (q.size(0) % c.batch != 0 || !index_vector(lengths, c.batch, q.device()) || (targets && !index_vector(*targets, c.batch, q.device()))) return {};
-    if (w < 0 || w > INT32_MAX || ctx < 0 || ctx > INT32_MAX || kv_splits < 0 || kv_splits > INT32_MAX || wants_grad({&q})) return {};
+    if (w < 0 || w > INT32_MAX || ctx < 0 || ctx > INT32_MAX || kv_splits < 0 || kv_splits > INT32_MAX || wants_grad({&q}) || has_tangent({&q})) return {};
     HstuPagedAttentionArgs a{};
     a.q = q.const_data_ptr(), a.q_row_stride = row_pitch(q), a.q_head_stride = head_pitch(q);
     a.seq_lengths = lengths.const_data_ptr(), a.seq_lengths_i64 = is_i64(lengths);

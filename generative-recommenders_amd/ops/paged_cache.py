@@ -15,6 +15,7 @@ check what it leaves: tensors that need a copy first, and calls that are refused
 from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import hip_backend, native
 from .hstu_attention import _check_forward_only, _kernel_layout, _require_device
@@ -92,6 +93,11 @@ def _rotary(table: Optional[torch.Tensor], dim: int, interleaved: bool, device: 
     return _dense(table)
 
 
+def _check_no_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("the HIP backend has no forward-mode derivatives; pass tensors without tangents")
+
+
 def _check_positions(positions: torch.Tensor, table: torch.Tensor) -> None:
     if positions.numel() and not bool(((positions >= 0) & (positions < table.shape[0])).all()):
         raise ValueError("hstu_cache: positions outside of the rotary table")
@@ -120,7 +126,7 @@ def qk_norm_rope(
     how many columns of a head turn: pairs ``(i, i + width / 2)``, or ``(2 i, 2 i + 1)`` with ``interleaved``.  fp32 inside, one
     rounding at the end.  ``positions``: ``[L]``; a row whose position is not in the table comes back NaN
     (``HSTU_HIP_CHECK_CONTRACT=1`` raises instead).  Gradients for q, k and both weights; a weight's are summed in fp32 in an
-    order that only depends on the sizes.
+    order that only depends on the sizes.  Tensors with forward-mode tangents are refused.
     """
     out = native.front.qk_norm_rope(q, k, positions, rotary_table, q_weight, k_weight, eps, interleaved, False)
     if out is not None:
@@ -136,6 +142,7 @@ def qk_norm_rope(
         torch._assert(k.dtype == q.dtype and k.device == q.device, "q and k must have the same dtype and device")
     torch._assert(k is not None or k_weight is None, "k_weight without k")
     torch._assert(rotary_table is not None or q_weight is not None or k_weight is not None, "neither a norm weight nor a rotary table")
+    _check_no_tangents(q, k, q_weight, k_weight, rotary_table)
     q_weight, k_weight = _parameter(q_weight, "q_weight", dim, q), _parameter(k_weight, "k_weight", dim, q)
     rotary_table = _rotary(rotary_table, dim, interleaved, q.device)
     if rotary_table is not None:
@@ -270,6 +277,7 @@ def append_paged_kv(
     if positions is not None:
         positions = _index(positions, "positions", rows, k.device)
     _check_forward_only(k, v, *([] if k_weight is None else [k_weight]))
+    _check_no_tangents(k, v, k_weight, rotary_table)
     if rows == 0:
         return
     if hip_backend.contract_checks_enabled():
@@ -353,6 +361,7 @@ def delta_hstu_mha_paged(
     if num_targets is not None:
         num_targets = _index(num_targets, "num_targets", batch, delta_q.device)
     _check_forward_only(delta_q)
+    _check_no_tangents(delta_q)
     if delta_q.numel() == 0:
         return torch.empty((delta_q.shape[0], delta_q.shape[1], 2 * cache[2].shape[3]), dtype=delta_q.dtype, device=delta_q.device)
     if hip_backend.contract_checks_enabled():

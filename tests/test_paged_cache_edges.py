@@ -185,3 +185,32 @@ def test_an_empty_batch_gives_gradients_of_zero(pkg, dev):
             grads = torch.autograd.grad([y.sum() for y in out if y is not None and y.requires_grad], leaves)
             for x, g in zip(leaves, grads):
                 assert g.shape == x.shape and g.dtype == x.dtype and bool((g == 0).all())
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused(pkg, dev):
+    """There is no forward derivative: a tensor with a tangent is refused by each operator, with and without grad mode, not answered without it."""
+    import torch.autograd.forward_ad as fwd
+
+    print("[case] tensors with tangents", flush=True)
+    q, k, pos, table, qw, kw, _ = _norm_rope_inputs((12, 2, 1, 32, 32, False, True, BF16))
+    q, k, pos, table, qw, kw = _to(dev, q, k, pos, table, qw, kw)
+    cache = pkg.allocate_paged_kv_cache(1, 16, 1, 32, 32, device=dev)
+    pages, zero = torch.zeros((1, 1), dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int64, device=dev)
+    v, n = torch.zeros_like(k), zero + 12
+    pkg.append_paged_kv(cache, k, v, pages, zero)
+    held = [x.clone() for x in cache]
+    want = pkg.qk_norm_rope(q, k, pos, table, qw, kw)
+    for grad in (False, True):
+        with torch.set_grad_enabled(grad), fwd.dual_level():
+            assert torch.equal(pkg.qk_norm_rope(q, k, pos, table, qw, kw)[0], want[0])  # (no tangents: served)
+            calls = [(pkg.qk_norm_rope, [q, k, pos, table, qw, kw], i) for i in (0, 1, 3, 4, 5)]
+            calls += [(pkg.append_paged_kv, [cache, k, v, pages, zero, None, table, pos, kw], i) for i in (1, 2, 6, 8)]
+            calls += [(pkg.delta_hstu_mha_paged, [16, 0.2, q, cache, pages, n], 2)]
+            for f, args, i in calls:
+                args = list(args)
+                args[i] = fwd.make_dual(args[i], torch.ones_like(args[i]))
+                with pytest.raises(NotImplementedError):
+                    f(*args)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(held, cache))
