@@ -284,7 +284,10 @@ def append_paged_kv(
         _check_places(cache, page_table, start, seq_offsets, rows)
         if rotary_table is not None:
             count = torch.full_like(start, rows // batch) if seq_offsets is None else seq_offsets[1:] - seq_offsets[:-1]
-            _check_positions(positions if positions is not None else (start + count - 1)[count > 0], rotary_table)
+            if positions is None:
+                _check_positions((start + count - 1)[count > 0], rotary_table)
+            else:  # (rows behind the last sequence are no one's)
+                _check_positions(positions if seq_offsets is None else positions[: int(seq_offsets[-1])], rotary_table)
     _served(native.front.append_paged_kv(cache, _copied(k), _copied(v), _pages(page_table), start, seq_offsets, rotary_table, positions,
                                          k_weight, eps, interleaved, True), "append_paged_kv")
 

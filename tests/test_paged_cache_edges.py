@@ -214,3 +214,28 @@ def test_forward_mode_is_refused(pkg, dev):
                     f(*args)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(held, cache))
+
+
+# ---- contract checks ----------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+def test_positions_of_rows_behind_the_last_sequence_are_no_ones(pkg, dev, monkeypatch):
+    """With the contract checks on, positions outside of the table are refused for rows of a sequence and for those alone."""
+    print("[case] positions behind the last sequence", flush=True)
+    cache = pkg.allocate_paged_kv_cache(4, 16, 1, 32, 32, device=dev)
+    k, v = _rand(1, (20, 1, 32), BF16).to(dev), _rand(2, (20, 1, 32), BF16).to(dev)
+    pages, zero = torch.tensor([[0, 1], [2, 3]], device=dev), torch.zeros(2, dtype=torch.int64, device=dev)
+    offs, turns = torch.tensor([0, 7, 15], device=dev), pkg.make_rotary_table(16, 32, device=dev)
+    pos = torch.arange(20, device=dev) % 8
+    pos[15:] = torch.tensor([-1, 16, 10**9, 99, -5], device=dev)
+    held = []
+    for check in ("0", "1"):
+        monkeypatch.setenv("HSTU_HIP_CHECK_CONTRACT", check)
+        pkg.append_paged_kv(cache, k, v, pages, zero, offs, turns, pos)
+        held.append([x.clone() for x in cache])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(*held))
+    pos[14] = 16
+    with pytest.raises(ValueError, match="positions"):
+        pkg.append_paged_kv(cache, k, v, pages, zero, offs, turns, pos)
