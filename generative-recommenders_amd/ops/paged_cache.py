@@ -219,6 +219,16 @@ def _check_places(cache, page_table: torch.Tensor, start: torch.Tensor, offsets:
         raise ValueError("hstu_cache: page_table names a page that the cache does not have")
 
 
+def _check_once(cache, page_table: torch.Tensor, start: torch.Tensor, count: torch.Tensor) -> None:
+    """No two of the rows start[b] .. start[b] + count[b] - 1, whose places there are, have one (synchronises)."""
+    page, count = cache[0].shape[2], count.long()
+    of = torch.repeat_interleave(torch.arange(count.numel(), device=count.device), count)
+    place = start.long()[of] + torch.arange(of.numel(), device=count.device) - (count.cumsum(0) - count)[of]
+    row = page_table[of, place // page].long() * page + place % page
+    if row.unique().numel() != row.numel():
+        raise ValueError("hstu_cache: two rows of the call have one place")
+
+
 def _first_seen(lengths: torch.Tensor, targets: Optional[torch.Tensor], delta: int, max_attn_len: int, contextual: int) -> torch.Tensor:
     """The first position that any of the newest ``delta`` positions of each sequence sees."""
     top = (lengths - delta).clamp(min=0)
@@ -253,8 +263,9 @@ def append_paged_kv(
     stand behind the same history).  A row is kept as (step, lowest value) in K's type and codes 0 .. 15: half a step off at
     most, and the rounding of the step.  A row with a NaN or an infinity becomes NaN.
 
-    Caller contract: every place has a page, no two rows of a call have one place.  Rows without a page are not stored
-    (``HSTU_HIP_CHECK_CONTRACT=1`` raises instead); rows behind the last sequence are no one's and not stored either.
+    Caller contract: every place has a page, no two rows of a call have one place (``HSTU_HIP_CHECK_CONTRACT=1`` raises where
+    either does not hold).  Rows without a page are not stored; what two rows leave in one place is neither's; rows behind the
+    last sequence are no one's and not stored either.
     No gradients.
     """
     if native.front.append_paged_kv(tuple(cache), k, v, page_table, start, seq_offsets, rotary_table, positions, k_weight, eps, interleaved, False):
@@ -282,8 +293,9 @@ def append_paged_kv(
         return
     if hip_backend.contract_checks_enabled():
         _check_places(cache, page_table, start, seq_offsets, rows)
+        count = torch.full_like(start, rows // batch) if seq_offsets is None else seq_offsets[1:] - seq_offsets[:-1]
+        _check_once(cache, page_table, start, count)
         if rotary_table is not None:
-            count = torch.full_like(start, rows // batch) if seq_offsets is None else seq_offsets[1:] - seq_offsets[:-1]
             if positions is None:
                 _check_positions((start + count - 1)[count > 0], rotary_table)
             else:  # (rows behind the last sequence are no one's)

@@ -239,3 +239,20 @@ def test_positions_of_rows_behind_the_last_sequence_are_no_ones(pkg, dev, monkey
     pos[14] = 16
     with pytest.raises(ValueError, match="positions"):
         pkg.append_paged_kv(cache, k, v, pages, zero, offs, turns, pos)
+
+
+@pytest.mark.gpu
+def test_two_rows_for_one_place_are_refused_by_the_checks(pkg, dev, monkeypatch):
+    """No two rows of a call may have one place: two sequences that share a page, or one page twice in a sequence.  A shared page that only one of
+    them writes to is allowed."""
+    print("[case] two rows for one place", flush=True)
+    cache = pkg.allocate_paged_kv_cache(6, 16, 1, 32, 32, device=dev)
+    k, v = _rand(1, (24, 1, 32), BF16).to(dev), _rand(2, (24, 1, 32), BF16).to(dev)
+    monkeypatch.setenv("HSTU_HIP_CHECK_CONTRACT", "1")
+    index = lambda *x: torch.tensor(x, device=dev)  # noqa: E731
+    for pages, start, offs in ((index([0, 1], [0, 2]), index(0, 0), None), (index([3, 3], [4, 5]), index(0, 0), index(0, 24, 24)), (index([1, 2], [4, 2]), index(16, 20), index(0, 6, 12))):
+        with pytest.raises(ValueError, match="one place"):
+            pkg.append_paged_kv(cache, k, v, pages, start, offs)
+    for pages, start, offs in ((index([0, 1], [0, 2]), index(16, 16), index(0, 10, 20)), (index([0, 1], [0, 2]), index(0, 3), index(0, 3, 8)), (index([5, 1], [5, 2]), index(0, 4), index(0, 4, 9))):
+        pkg.append_paged_kv(cache, k, v, pages, start, offs)
+    torch.cuda.synchronize()
