@@ -256,3 +256,83 @@ def test_two_rows_for_one_place_are_refused_by_the_checks(pkg, dev, monkeypatch)
     for pages, start, offs in ((index([0, 1], [0, 2]), index(16, 16), index(0, 10, 20)), (index([0, 1], [0, 2]), index(0, 3), index(0, 3, 8)), (index([5, 1], [5, 2]), index(0, 4), index(0, 4, 9))):
         pkg.append_paged_kv(cache, k, v, pages, start, offs)
     torch.cuda.synchronize()
+
+
+# ---- how a call is cut into workgroups ----------------------------------------------------------------------------------
+
+
+def _attend(pkg, dev, lengths, delta, hq, heads, dqk, dv, page, dtype, seed, targets=None, w=0, c=0, splits=(0,), N=None):
+    """The attention of random rows against the oracle; results' memory holds NaN before, so that what is not written shows."""
+    table, pages = O.page_table(seed, lengths, page)
+    cache = O.fill_cache(seed + 1, pages, heads, page, dqk, dv, dtype)
+    q, n = _rand(seed + 2, (len(lengths) * delta, hq, dqk), dtype), torch.tensor(lengths)
+    t = None if targets is None else torch.tensor(targets)
+    N = N or max(lengths)
+    want, bound = O.attention(N, dqk**-0.5, q, cache, table, n, t, w, c, dtype)
+    on = _to(dev, q, table, n, t)
+    cache = tuple(x.to(dev) for x in cache)
+    for s in splits:
+        for big in (1 << 20, 1 << 26):  # (what the allocator hands out next, for results and for scratch)
+            del_me = torch.full((big,), float("nan"), device=dev)
+            del del_me
+        poison = torch.full((q.shape[0], hq, dv), float("nan"), dtype=dtype, device=dev)
+        del poison
+        got = pkg.delta_hstu_mha_paged(N, dqk**-0.5, on[0], cache, on[1], on[2], on[3], w, c, kv_splits=s)
+        again = pkg.delta_hstu_mha_paged(N, dqk**-0.5, on[0], cache, on[1], on[2], on[3], w, c, kv_splits=s)
+        torch.cuda.synchronize()
+        _within(got, want, bound, f"splits {s}")
+        assert torch.equal(got, again)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 2, 4])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_few_rows_against_long_sequences(pkg, dev, rows, dtype):
+    """One to four rows of a head, where a wave goes over several groups of chunks: whole groups that every row sees, the last one short by any
+    number of chunks, the next group's loads ahead; with and without a window, a prefix and targets."""
+    print(f"[case] attention: {rows} rows, long sequences {dtype}", flush=True)
+    group, delta = (2, rows // 2) if rows > 1 else (1, 1)
+    for i, (w, c, t) in enumerate(((0, 0, 0), (0, 0, delta), (4700, 0, 0), (2500, 5, delta))):
+        # around whole numbers of groups for four waves (16, 8 or 4 chunks of 32 positions each), and anywhere
+        lengths = [8192, 8192 + 1, 8192 - 31, 6144 + 32, 5000 + 13 * i, 9000 - i]
+        _attend(pkg, dev, lengths, delta, group, 1, 64, 32, 64, dtype, 100 * i + rows, [t] * 6, w, c, (1, 0, 2))
+    _attend(pkg, dev, [5120, 7001], delta, group, 1, 128, 128, 16, dtype, 7 + rows, None, 0, 0, (1, 0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("delta", [12, 24])
+def test_nine_to_32_rows_against_long_sequences(pkg, dev, delta):
+    """Runs in which each of the four waves looks its pages up three times over (32 of its chunks at a time, 4096 positions of the run)."""
+    print(f"[case] attention: {delta} rows, long sequences", flush=True)
+    for dqk, dv, page, dtype in ((64, 64, 16, F16), (128, 128, 64, BF16)):
+        _attend(pkg, dev, [9000, 8193, 8500], delta, 1, 1, dqk, dv, page, dtype, delta + dqk, [delta, 0, 3], 0, 0, (1, 0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 3, 8])
+def test_a_wave_for_each_of_many_short_sequences(pkg, dev, rows):
+    """More than 1024 (sequence, head) pairs of at most 17 chunks: a wave each, the last workgroup not full, some sequences empty."""
+    print(f"[case] attention: {rows} rows of many short sequences", flush=True)
+    lengths = [0 if b % 11 == 3 else 1 + (b * 97) % 500 for b in range(257)]
+    for dtype, targets in ((BF16, None), (F16, [min(n, 2) for n in lengths])):
+        _attend(pkg, dev, lengths, rows, 5, 5, 32, 32, 16, dtype, rows, targets)
+
+
+@pytest.mark.gpu
+def test_automatic_runs_of_many_long_sequences(pkg, dev):
+    """One row each: runs held to 96 chunks, runs of 40, and runs made longer so that no short one is left over."""
+    for batch, heads, top in ((48, 4, 9000), (16, 4, 9000), (64, 4, 3080)):
+        print(f"[case] attention: runs of {batch} x {heads} up to {top}", flush=True)
+        lengths = [top] + [1 + (b * 7919) % top for b in range(1, batch)]
+        _attend(pkg, dev, lengths, 1, heads, heads, 32, 32, 64, BF16, batch, N=top)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,heads", [(86, 3), (73, 7), (128, 4), (171, 3), (200, 5), (256, 1), (256, 2), (2, 255)])
+def test_blocks_of_every_number_of_workgroups(pkg, dev, batch, heads):
+    """More than 32 rows: sequences ranked by length, ties among them, and the second 256 workgroups in reverse where at most 512 run."""
+    print(f"[case] attention: {batch * heads} workgroups", flush=True)
+    lengths = [40 + (b * 53) % 90 if b % 5 else 77 for b in range(batch)]
+    if batch > 2:
+        lengths[3], lengths[batch - 1] = 0, 33
+    _attend(pkg, dev, lengths, 33, heads, heads, 32, 32, 16, BF16, batch, [min(n, 20) for n in lengths] if heads % 2 else None, splits=(1,))
