@@ -100,9 +100,8 @@ typedef std::integral_constant<int, 1> One;
 
 template <class TT, int DK, int DV>
 int launch_sized(const hstu::PagedAttentionParams& p, const Plan& plan, hipStream_t stream) {
-    const unsigned blocks = (unsigned)((p.items + 7) / 8 * 8 * (int64_t)plan.row_blocks);
     auto go = [&](auto mt) {
-        hipLaunchKernelGGL((hstu::hstu_paged_attention_kernel<TT, DK, DV, decltype(mt)::value>), dim3(blocks), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((hstu::hstu_paged_attention_kernel<TT, DK, DV, decltype(mt)::value>), dim3((unsigned)p.items), dim3(256), 0, stream, p);
     };
     auto block = [&](auto mt) {
         hipLaunchKernelGGL((hstu::hstu_paged_block_kernel<TT, DK, DV, decltype(mt)::value>), dim3((unsigned)(p.items * (int64_t)plan.row_blocks)), dim3(256), 0, stream, p);

@@ -233,8 +233,8 @@ __device__ __forceinline__ void store_columns(const PagedAttentionParams& p, int
     }
 }
 
-// grid: one workgroup of four waves per (block of 16 MT rows, head of the cache, run, sequence), numbered so that the row blocks of one
-// run, which read the same pages, are on one XCD.  The waves share out the chunks of the run; their sums meet in LDS.  Unpacking and silu
+// grid: one workgroup of four waves per (head of the cache, run, sequence); its 16 MT rows are all that share a head.  The waves share out the
+// chunks of the run; their sums meet in LDS.  Unpacking and silu
 // bound it, the cache's bytes not far below: 12 rows, 256 sequences of 1000 .. 8192 positions and four heads of 128 182 us (629 MB, 121 us
 // of a copy); 24 rows, whose registers leave room for one wave of a SIMD, 318.  Held to two waves, with 85 registers spilled, the latter took 361;
 // heads of 64 and 128, with seven, gained: 64 sequences of 512 .. 4096 46 us by one wave, 36 by two.
@@ -243,14 +243,11 @@ __global__ __launch_bounds__(256, (MT == 2 && DK + DV < 256 ? 2 : 1)) void hstu_
     typedef typename TT::elem T;
     constexpr int NK = DK / 32, NV = DV / 16, KW = 4;
     __shared__ float meet[KW * NV * 4 * 64];
-    const int xcd = blockIdx.x & 7, q8 = blockIdx.x >> 3;
-    const int rb = q8 % p.row_blocks, item = (q8 / p.row_blocks) * 8 + xcd;
-    if (item >= p.items) return;
+    const int item = blockIdx.x;
     const int hk = item % p.cache.heads, split = (item / p.cache.heads) % p.splits, b = item / (p.cache.heads * p.splits);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-    constexpr int ROWS = 16 * MT;
-    const int rows = p.delta * p.group, r_end = min((rb + 1) * ROWS, rows);
-    const PagedSpan span = paged_span(p, b, rb * ROWS / p.group, (r_end - 1) / p.group + 1);
+    const int rows = p.delta * p.group;
+    const PagedSpan span = paged_span(p, b, 0, p.delta);
     const int chunks = span.na + span.nb, per = chunks_per_run(p, chunks);
     const int chunk_end = min((split + 1) * per, chunks);
     if (p.splits > 1 && split * per >= chunks) return;  // (the joining kernel knows)
@@ -262,7 +259,7 @@ __global__ __launch_bounds__(256, (MT == 2 && DK + DV < 256 ? 2 : 1)) void hstu_
     int lo_max = 0, hi_min = 1 << 30;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        const int r = rb * ROWS + mt * 16 + m;
+        const int r = mt * 16 + m;
         const int i = r / p.group, head = hk * p.group + (r - i * p.group);
         qs[mt] = qo[mt] = 0.f;
         see[mt].lo = see[mt].hi = see[mt].chi = 0, see[mt].self = -1;
