@@ -336,3 +336,57 @@ def test_blocks_of_every_number_of_workgroups(pkg, dev, batch, heads):
     if batch > 2:
         lengths[3], lengths[batch - 1] = 0, 33
     _attend(pkg, dev, lengths, 33, heads, heads, 32, 32, 16, BF16, batch, [min(n, 20) for n in lengths] if heads % 2 else None, splits=(1,))
+
+
+# ---- the smallest numbers, one weight -----------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_rows_of_the_smallest_numbers(pkg, dev, dtype):
+    """Rows whose values, or whose steps, are below the type's normal numbers or at the border: codes, steps and lowest values are the definition's,
+    bit by bit, codes above 15 held there, and reading them rounds once."""
+    print(f"[case] rows of the smallest numbers {dtype}", flush=True)
+    rows, heads, dim, page = 640, 2, 64, 64
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps  # the smallest number there is
+    g = torch.Generator().manual_seed(1)
+    whole = torch.randint(0, 40, (rows, heads, dim), generator=g).double() * torch.logspace(0, 9, rows, 2, dtype=torch.float64).floor().view(-1, 1, 1)
+    k = (whole * tiny).to(dtype)
+    v = k - k[:, :, :1] + (torch.randn((rows, heads, 1), generator=g) * 300 * tiny).to(dtype)
+    pages = rows // page
+    table, zero = torch.randperm(pages, generator=g).to(torch.int32).view(1, -1), torch.zeros(1, dtype=torch.int64, device=dev)
+    cache = pkg.allocate_paged_kv_cache(pages, page, heads, dim, dim, dtype, dev)
+    pkg.append_paged_kv(cache, k.to(dev), v.to(dev), table.to(dev), zero)
+    got = pkg.read_paged_kv(cache, rows, table.to(dev), zero)
+    torch.cuda.synchronize()
+    places = torch.arange(rows)
+    at = (table[0].long()[places // page], slice(None), places % page)
+    for i, x in ((0, k), (2, v)):
+        code, step, low = O.four_bits(x)
+        assert 0 < int((step < torch.finfo(dtype).smallest_normal).sum()) and 0 < int((step > torch.finfo(dtype).smallest_normal).sum())
+        scales = torch.cat([step, low], -1).to(dtype)
+        assert torch.equal(cache[i].cpu()[at], O.pack(code)) and torch.equal(cache[i + 1].cpu()[at], scales)
+        assert torch.equal(got[i // 2].cpu(), O.values(O.pack(code), scales).to(dtype))
+
+
+@pytest.mark.gpu
+def test_one_norm_weight_of_two(pkg, dev):
+    """A norm of k alone or of q alone, with and without the rotation: the gradients of what there is."""
+    print("[case] norm and rotation: one weight", flush=True)
+    q, k, pos, table, qw, kw, _ = _norm_rope_inputs((50, 3, 2, 64, 32, False, True, BF16))
+    up = _rand(8, q.shape, BF16), _rand(9, k.shape, BF16)
+    for a, b in ((None, kw), (qw, None)):
+        for turned in (False, True):
+            at, tab = (pos, table) if turned else (None, None)
+            on = _to(dev, q, k, at, tab, a, b)
+            leaves = [t.requires_grad_() for t in (on[0], on[1], on[4], on[5]) if t is not None]
+            y = pkg.qk_norm_rope(*on)
+            grads = torch.autograd.grad(y, leaves, _to(dev, *up))
+            torch.cuda.synchronize()
+            for i, (x, w, dy) in enumerate(((q, a, up[0]), (k, b, up[1]))):
+                args = (w, 1e-6, tab, at, False)
+                _within(y[i], O.norm_rope(x, *args), O.norm_rope_bound(x, BF16, *args), "qk"[i])
+                (dx, dw, _), (dx_bound, dw_bound) = O.norm_rope_grad(x, dy, *args), O.norm_rope_grad_bounds(x, dy, BF16, *args)
+                _within(grads[i], dx, dx_bound, "d" + "qk"[i])
+                if w is not None:
+                    _within(grads[2], dw, dw_bound, "dw of " + "qk"[i])
