@@ -363,49 +363,55 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_bwd_kernel(const NormRopeP
         for (int i = 0; i < 8; ++i) meet[(threadIdx.x / LPV) * (LPV * 8) + 8 * l + i] = sum[which][i];
         __syncthreads();
         for (int col = threadIdx.x; col < p.dim; col += 256) {
-            float v = 0.f;
+            double v = 0;
             for (int g = 0; g < GROUPS; ++g) v += meet[g * (LPV * 8) + col];
-            p.partial[(wg * 2 + which) * p.dim + col] = v;
+            p.partial[(wg * 2 + which) * p.dim + col] = (float)v;
         }
     }
 }
 
 // dw[col] = sum over workgroups of partial[workgroup][which][col]: 16 columns to a workgroup, as four lanes of four, and 64 parts of
 // the workgroups' sums, four of them in flight.  (With 16 parts of single columns, one load in flight, 2048 sums took 53 us.)
+// Here and where groups meet the additions are in 64 bits: they are few, and with all of them in 32 a gradient in fp32 of 5679 terms a column was
+// more than 1.2e-7 of its size off, where it is 0.6e-7 to 0.75e-7.
 template <class T>
 __global__ __launch_bounds__(256) void hstu_norm_rope_dw_kernel(const float* partial, int64_t workgroups, int dim, T* dq_weight, T* dk_weight) {
     typedef __attribute__((ext_vector_type(4))) float f4;
-    __shared__ float meet[64][17];
+    __shared__ double meet[64][17];
     const int c = threadIdx.x & 3, part = threadIdx.x >> 2, which = blockIdx.y;
     const int col = blockIdx.x * 16 + 4 * c;
     T* out = which ? dk_weight : dq_weight;
     if (!out) return;
-    f4 v = {0, 0, 0, 0};
+    double v[4] = {0, 0, 0, 0};
     if (col < dim) {  // (a multiple of 8)
         const float* from = partial + which * dim + col;
+        auto add = [&](f4 x) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] += x[k];
+        };
         int64_t w = part;
         for (; w + 192 < workgroups; w += 256) {
             f4 x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = *(const f4*)(from + (w + 64 * i) * 2 * dim);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v += x[i];
+            for (int i = 0; i < 4; ++i) add(x[i]);
         }
-        for (; w < workgroups; w += 64) v += *(const f4*)(from + w * 2 * dim);
+        for (; w < workgroups; w += 64) add(*(const f4*)(from + w * 2 * dim));
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) meet[part][4 * c + i] = v[i];
     __syncthreads();
     const int one = threadIdx.x & 15, lane16 = threadIdx.x >> 4;
-    float total = meet[lane16][one] + meet[lane16 + 16][one] + meet[lane16 + 32][one] + meet[lane16 + 48][one];
+    double total = meet[lane16][one] + meet[lane16 + 16][one] + meet[lane16 + 32][one] + meet[lane16 + 48][one];
     __syncthreads();
     meet[lane16][one] = total;
     __syncthreads();
     if (threadIdx.x < 16 && blockIdx.x * 16 + threadIdx.x < dim) {
-        total = 0.f;
+        total = 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) total += meet[i][threadIdx.x];
-        out[blockIdx.x * 16 + threadIdx.x] = (T)total;
+        out[blockIdx.x * 16 + threadIdx.x] = (T)(float)total;
     }
 }
 

@@ -125,8 +125,8 @@ def qk_norm_rope(
     by the heads) that is None leaves its norm out; no ``rotary_table`` (``make_rotary_table``), no rotation.  The table's width is
     how many columns of a head turn: pairs ``(i, i + width / 2)``, or ``(2 i, 2 i + 1)`` with ``interleaved``.  fp32 inside, one
     rounding at the end.  ``positions``: ``[L]``; a row whose position is not in the table comes back NaN
-    (``HSTU_HIP_CHECK_CONTRACT=1`` raises instead).  Gradients for q, k and both weights; a weight's are summed in fp32 in an
-    order that only depends on the sizes.  Tensors with forward-mode tangents are refused.
+    (``HSTU_HIP_CHECK_CONTRACT=1`` raises instead).  Gradients for q, k and both weights; a weight's are summed in fp32 and,
+    over the lanes, in 64 bits, in an order that only depends on the sizes.  Tensors with forward-mode tangents are refused.
     """
     out = native.front.qk_norm_rope(q, k, positions, rotary_table, q_weight, k_weight, eps, interleaved, False)
     if out is not None:

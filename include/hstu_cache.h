@@ -63,7 +63,8 @@ typedef struct HstuNormRopeArgs {
 int hstu_cache_norm_rope(const HstuNormRopeArgs* args, void* stream);
 
 /* Gradients from those of the outputs; statistics are recomputed from q and k.  A weight's gradient is summed over rows and
- * heads in fp32, in an order that depends on the sizes alone, and rounded once; its workspace is needed where either is asked for. */
+ * heads, by each lane in fp32 and over the lanes in 64 bits, in an order that depends on the sizes alone; its workspace is needed where
+ * either is asked for. */
 typedef struct HstuNormRopeGrads {
     const void* dq_out;        /* [rows, q_heads, dim]; NULL where q is */
     const void* dk_out;

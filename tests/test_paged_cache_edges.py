@@ -390,3 +390,20 @@ def test_one_norm_weight_of_two(pkg, dev):
                 _within(grads[i], dx, dx_bound, "d" + "qk"[i])
                 if w is not None:
                     _within(grads[2], dw, dw_bound, "dw of " + "qk"[i])
+
+
+@pytest.mark.gpu
+def test_norm_weights_gradients_keep_their_bits_in_fp32(pkg, dev):
+    """A weight's gradient in fp32, 5679 terms a column, relative to its size over the columns.  A term goes through some nine roundings (the mean,
+    its root, their product, the turn's three operations, the product, the sum of six in a lane, the partial sum), each off by 0.3 to 0.6 of
+    2^-24 in the mean square, independently: three times 0.42, 1.3 of 2^-24 together; sums of hundreds in 32 bits would add three more."""
+    print("[case] norm weights' gradients in fp32", flush=True)
+    q, k, pos, table, qw, kw, _ = _norm_rope_inputs((1893, 3, 3, 32, 32, False, True, F32), 40)
+    up = _rand(8, q.shape, F32), _rand(9, k.shape, F32)
+    on = _to(dev, q, k, pos, table, qw, kw)
+    leaves = [on[4].requires_grad_(), on[5].requires_grad_()]
+    grads = torch.autograd.grad(pkg.qk_norm_rope(*on), leaves, _to(dev, *up))
+    torch.cuda.synchronize()
+    for x, w, dy, got in ((q, qw, up[0], grads[0]), (k, kw, up[1], grads[1])):
+        _, want, _ = O.norm_rope_grad(x, dy, w, 1e-6, table, pos)
+        assert float((got.double().cpu() - want).norm() / want.norm()) <= 2 * 2.0**-24
