@@ -363,9 +363,12 @@ __global__ __launch_bounds__(256) void hstu_norm_rope_bwd_kernel(const NormRopeP
         for (int i = 0; i < 8; ++i) meet[(threadIdx.x / LPV) * (LPV * 8) + 8 * l + i] = sum[which][i];
         __syncthreads();
         for (int col = threadIdx.x; col < p.dim; col += 256) {
-            double v = 0;
-            for (int g = 0; g < GROUPS; ++g) v += meet[g * (LPV * 8) + col];
-            p.partial[(wg * 2 + which) * p.dim + col] = (float)v;
+            double v[4] = {0, 0, 0, 0};
+#pragma unroll 4
+            for (int g = 0; g < GROUPS; g += 4)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] += meet[(g + i) * (LPV * 8) + col];
+            p.partial[(wg * 2 + which) * p.dim + col] = (float)((v[0] + v[1]) + (v[2] + v[3]));
         }
     }
 }
