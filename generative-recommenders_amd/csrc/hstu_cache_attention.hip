@@ -54,7 +54,7 @@ Plan plan_of(const HstuPagedCache* c, const HstuPagedAttentionArgs* a) {
     // positions and four heads: 22 us, in two runs 25).  Else runs that fill it once, for each begins with some microseconds of loads that wait for
     // each other (64 sequences of 1024 .. 4096 positions and four heads, 256 workgroups for whole sequences: in two runs 26 us, one 28, eight 30);
     // in eights, two chunks to each wave (33 sequences of up to 2048, four rows: runs of 16 15 us, of 18 or 32 18); none that leaves a short second
-    // or third; and none longer than 96, so that the last of them do not run alone (128 sequences of up to 16384 and eight heads: whole
+    // or third, which makes some of them up to 120 long; and else none longer than 96, so that the last of them do not run alone (128 sequences of up to 16384 and eight heads: whole
     // sequences 291 us, runs of 384 chunks 281, of 96 264, of 33 281).  Sequences of a few chunks, more of them than fit, are a wave's each
     // (1600 of up to 10 chunks: 12 us, 16 by workgroups).
     // More rows are split into equal parts of each sequence, of at least 8 or 16 chunks: what a part more costs is a partial sum of every row to

@@ -16,7 +16,9 @@
 // rounded P as one more product sees it (a row of ones).  With step s and lowest value l of a row
 //     <q, k> = s (acc) + l sum(q),     O = sum_pos (P s) (c - 7.5) + sum_pos P (l + 7.5 s),
 // the first sum on the matrix cores with P s rounded to bf16, the second in fp32: around the middle code the rounding of P s weighs
-// a third of what it would around the lowest value.  For fp16 results P s is kept in two bf16 words (16 bits, and bf16's range).
+// a third of what it would around the lowest value.  For fp16 results P s is kept in two bf16 words (16 bits, and bf16's range).  In bf16 one word
+// leaves results 0.0024 of their size from 64 bits, where rounding them alone leaves 0.0017.  Two are not free there either: one row of 128
+// sequences of 4096 .. 16384, eight heads of 128, 271 -> 308 us, eight rows of 128 of up to 8192 94 -> 113.
 #pragma once
 #include "hstu_paged_rows.h"
 
@@ -235,8 +237,10 @@ __device__ __forceinline__ void store_columns(const PagedAttentionParams& p, int
 
 // grid: one workgroup of four waves per (head of the cache, run, sequence); its 16 MT rows are all that share a head.  The waves share out the
 // chunks of the run; their sums meet in LDS.  Unpacking and silu
-// bound it, the cache's bytes not far below: 12 rows, 256 sequences of 1000 .. 8192 positions and four heads of 128 182 us (629 MB, 121 us
-// of a copy); 24 rows, whose registers leave room for one wave of a SIMD, 318.  Held to two waves, with 85 registers spilled, the latter took 361;
+// take most of it, the cache's bytes not far below: 12 rows, 256 sequences of 1000 .. 8192 positions and four heads of 128 187 us (640 MB, 124 us
+// of a copy), of whose 371 thousand clocks a SIMD has 173 of vector operations and 39 of products (counted): no unit is full, waves wait for
+// 45 % of their time and 28 % of the room for them stands empty, most of it while the longest sequences end.  24 rows, whose registers leave room for one
+// wave of a SIMD, 350 (711 thousand, 240 and 77).  Held to two waves, with 85 registers spilled, they took a seventh longer;
 // heads of 64 and 128, with seven, gained: 64 sequences of 512 .. 4096 46 us by one wave, 36 by two.
 template <class TT, int DK, int DV, int MT>
 __global__ __launch_bounds__(256, (MT == 2 && DK + DV < 256 ? 2 : 1)) void hstu_paged_attention_kernel(const PagedAttentionParams p) {
@@ -479,10 +483,12 @@ __device__ __forceinline__ int block_order(const PagedAttentionParams& p, int ea
 // products' operands lie in registers (a lane's 16 bytes side by side: reads and writes without bank conflicts), and the pairs as four
 // floats a position: c1 s, c1 l of K, s, l + 7.5 s of V.  Two buffers, one barrier a step; the packed rows of the next step are on their way
 // while this one is worked on.  Unpacking per wave, as above, cost as much as half of the rest and the registers of a second wave.
-// Vector operations bound it: for 32 positions and 32 rows a wave has 204 of them, 152 for silu, its masks and roundings, and 34 products.
+// For 32 positions and 32 rows a wave has 204 vector operations, 152 of them for silu, its masks and roundings, and 34 products.
 // 32 sequences of 1280 .. 4352 positions with 256 rows and four heads of 128 (39 GFLOP, 32 us of the matrix cores as a large library
-// product uses them): 88 us, 10 of them for joining two parts of each sequence; of 177 thousand clocks a SIMD has 71 of vector operations
-// and 41 of products (counted), and what is left is waits, and the longest sequence's end.  Two workgroups of a CU, out of step with each
+// product uses them): 88 us, 8 of them for joining two parts of each sequence.  No unit bounds it: of the kernel's 177 thousand clocks a SIMD has 71
+// of vector operations and 41 of products (counted).  A wave lives 135 of them in the mean, because parts are parts of a sequence and the longest
+// sequence has the longest, so that a quarter of the waves' room stands empty; the rest is waits, for which two waves of a SIMD
+// are few.  Two workgroups of a CU, out of step with each
 // other, fill the gaps of one another: the same two teams of waves in one workgroup, behind one barrier, took 106 us.  Three of 64 rows and
 // one chunk a step took 91: more operations, nothing gained from a third wave.
 template <class TT, int DK, int DV, int MT>

@@ -156,8 +156,9 @@ __device__ __forceinline__ unsigned to_four_bits(const float (&x)[8], unsigned& 
 // grid (rows / groups of a workgroup, vectors / vectors_per_group): a row's vectors count through its heads of K, then of V.
 // (16 columns to a lane, which do what a row takes once in half as many lanes, came to a third fewer instructions and to the same time,
 // four waves of a SIMD in 107 registers where six have 78.  So did the first loads in front of the lookups.)  Vector operations
-// bound it, with the bytes close below: 256 sequences of 64 .. 1024 rows, four heads of 128, normed and turned, 93 us (337 MB, 65 us of a
-// copy; the loads and stores alone 68); fp16 rows that are only turned, 146378 of eight heads, 175 (761 MB; alone 163).  64 single rows take 4.5 us, one launch and three loads that wait for each other.
+// bound it, with the bytes close below: 256 sequences of 64 .. 1024 rows, four heads of 128, normed and turned, 97 us (337 MB, 65 us of a
+// copy; the loads and stores alone 68), of whose 200 thousand clocks a SIMD has 187 of vector operations (counted); fp16 rows that are only
+// turned, 146378 of eight heads, 166 again and again, 180 to 197 with their reading between (761 MB; 321 of 410).  64 single rows take 4.5 us, one launch and three loads that wait for each other.
 template <class T, int LPV, int TURN>
 __global__ __launch_bounds__(256) void hstu_paged_append_kernel(const AppendParams p) {
     constexpr int GROUPS = 256 / LPV, AHEAD = 4;

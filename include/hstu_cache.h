@@ -87,7 +87,7 @@ int hstu_cache_norm_rope_bwd(const HstuNormRopeArgs* args, const HstuNormRopeGra
  * 4 bits, two to a byte, the even column in the low half, and a pair (step, lowest value) in the type of K and V; the value
  * of a column is  lowest + step * code.  Row x in that type becomes
  *     lowest = min x,  step = (max x - min x) / 15 rounded to the type,  code = (x - lowest) / step rounded to the nearest
- * (ties to even) and held within 0 .. 15; code 0 throughout where step is 0.  A row with a NaN or an infinity, or whose step
+ * (ties to even) and held within 0 .. 15; code 0 throughout where step is 0.  The difference and the quotient are rounded to fp32.  A row with a NaN or an infinity, or whose step
  * the type does not hold, becomes NaN: step and lowest value both.
  * Position i of sequence b lies in page page_table[b][i / page_size].
  */
@@ -147,7 +147,9 @@ int hstu_cache_read(const HstuPagedCache* cache, int64_t rows, const void* start
  * out[b * delta_size + i] = sum_s M(p, s) * silu(alpha * <q, k_s>) / max_seq_len * v_s  for the newest delta_size positions
  * p = seq_lengths[b] - delta_size + i of every sequence, with the masks of the cached form (hstu_hip.h).  Head h of q reads head
  * h / (q_heads / heads) of the cache.  K and V enter as lowest + step * code, unrounded; silu(.) times a V row's step is rounded to
- * bf16 for the second product (to two bf16 words, 16 bits, where the type is fp16), sums are in fp32 and rounded once.
+ * bf16 for the second product (to two bf16 words, 16 bits, where the type is fp16), sums are in fp32 and rounded once.  Codes enter the
+ * products with an offset of up to 128: sums over a row of |q|, or over the positions of |silu(.)| times a V row's step, of 2^120 and
+ * more may overflow.
  * A row at a position before the first is zero.  A sequence that is longer than its row of the page table gives NaN.  Where one of its
  * pages is not one of the cache's, every row that sees a position on that page is NaN, and other rows of the sequence may be; pages that end
  * in front of the first position that any row of the call sees (behind a window) are not looked at.
