@@ -16,9 +16,10 @@
 // rounded P as one more product sees it (a row of ones).  With step s and lowest value l of a row
 //     <q, k> = s (acc) + l sum(q),     O = sum_pos (P s) (c - 7.5) + sum_pos P (l + 7.5 s),
 // the first sum on the matrix cores with P s rounded to bf16, the second in fp32: around the middle code the rounding of P s weighs
-// a third of what it would around the lowest value.  For fp16 results P s is kept in two bf16 words (16 bits, and bf16's range).  In bf16 one word
-// leaves results 0.0024 of their size from 64 bits, where rounding them alone leaves 0.0017.  Two are not free there either: one row of 128
-// sequences of 4096 .. 16384, eight heads of 128, 271 -> 308 us, eight rows of 128 of up to 8192 94 -> 113.
+// a third of what it would around the lowest value.  For fp16 results, and for few rows, P s is kept in two bf16 words (16 bits, and bf16's
+// range): results are then as far from 64 bits as rounding them leaves them.  For more rows in bf16 it is one word, as in the attention on 16-bit K and V: results
+// are 0.0024 of their size from 64 bits, where rounding them alone leaves 0.0017.  Two words are twice the second product's instructions there:
+// 12 rows of 256 sequences of 1000 .. 8192, four heads of 128, 189 -> 202 us, 24 rows 349 -> 387, 256 rows of 32 sequences of 1280 .. 4352 92 -> 107.
 #pragma once
 #include "hstu_paged_rows.h"
 
@@ -783,13 +784,15 @@ __global__ __launch_bounds__(256, 2) void hstu_paged_block_kernel(const PagedAtt
 // The same for few rows (at most 8 of one head of the cache), where a product of 16 columns would waste most of them: F = 16 / RP chunks
 // side by side.  Column n of a score tile stands for row n % RP and chunk n / RP of F: a chunk's product fills all columns, and each lane keeps
 // it where the chunk is its own.  silu and what surrounds it then run once for F chunks, on full lanes, and so do the loads of the pairs
-// (step, lowest value).  For the second product each chunk's columns alone have P, the others zero: its sums land in columns of their own,
-// which are added up over the chunks at the end.
+// (step, lowest value).  For the second product a chunk's own columns have the first words of P, the columns of the chunk F / 2 away the second words, the
+// others zero: its sums land in columns that nothing else uses, which are added up over the chunks at the end, and two words take no more products than
+// one.  (A product for each word took 308 us below, where this takes 270.)
 // Waves of a SIMD: three in 168 registers each took 281 us where two in 172 took 290 (128 sequences of 4096 .. 16384 positions, eight
-// heads of 128, 1.45 GB); heads of 256 need the registers of one.  The cache's bytes bound it: the same sequences in runs of up to 96
+// heads of 128, 1.45 GB); four rows of 128 sequences of up to 8192 88 where two in 214 took 103, but of 33 of up to 2048 16.5 where two took 14.5;
+// heads of 256 need the registers of one.  The cache's bytes bound it: the same sequences in runs of up to 96
 // chunks take 265 us, 5.4 TB/s where a copy of 1 GiB reaches 5.2.  One short sequence is launches and loads that wait for each other: 8 us.
 template <int DK, int DV>
-constexpr int STEP_WAVES = DK == 256 ? 1 : DK + DV >= 256 ? 2 : DK + DV >= 128 ? 3 : 4;
+constexpr int STEP_WAVES = DK == 256 ? 1 : DK + DV >= 128 ? 3 : 4;
 
 template <class TT, int DK, int DV, int RP>
 __global__ __launch_bounds__(256, (STEP_WAVES<DK, DV>)) void hstu_paged_step_kernel(const PagedAttentionParams p) {
@@ -812,11 +815,10 @@ __global__ __launch_bounds__(256, (STEP_WAVES<DK, DV>)) void hstu_paged_step_ker
     const int begin = silent ? 0 : min(split * per + part * each, run_end), end = silent ? 0 : min(begin + each, run_end);
     auto chunk_at = [&](int i) { return i < span.na ? span.a0 + i : span.b0 + (i - span.na); };
 
-    RowSpan see{0, 0, 0, -1};
     int lo_max = 0, hi_min = 1 << 30;
     const int row_i = r / p.group, head = hk * p.group + (r - row_i * p.group);
     if (r < rows) {
-        see = row_span(p, span, span.n - p.delta + row_i);
+        const RowSpan see = row_span(p, span, span.n - p.delta + row_i);
         lo_max = see.lo, hi_min = see.hi;
     }
     u32x4_t qf[NK];
@@ -965,9 +967,12 @@ __global__ __launch_bounds__(256, (STEP_WAVES<DK, DV>)) void hstu_paged_step_ker
             scores(k_now, c0);
             __builtin_memcpy(k_now, k_next, sizeof(k_now));
         }
-        u32x4_t ph, pl;
+        u32x4_t ph, pl;  // P s of this lane's chunk, in two words: the second in the lane half of the chunks away
         auto silu = [&](auto masked) __attribute__((always_inline)) {
             const int own_pos = chunk_at(min(s0 + own, end - 1)) * 32 + 4 * g;
+            int pos = r < rows ? span.n - p.delta + row_i : -1;
+            asm volatile("" : "+v"(pos));  // what the row sees is worked out where it is needed: four registers that the loads ahead have instead
+            const RowSpan see = row_span(p, span, pos);
             float ps[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -982,29 +987,23 @@ __global__ __launch_bounds__(256, (STEP_WAVES<DK, DV>)) void hstu_paged_step_ker
                 }
                 plo += lower;
             }
-            pa_bf16x8 high;
+            pa_bf16x8 high, rest;
 #pragma unroll
             for (int e = 0; e < 8; ++e) high[e] = (__bf16)ps[e], psum += (float)high[e];
-            ph = __builtin_bit_cast(u32x4_t, high);
-            if constexpr (TT::P_WORDS == 2) {
-                pa_bf16x8 rest;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) rest[e] = (__bf16)(ps[e] - (float)high[e]), psum += (float)rest[e];
-                pl = __builtin_bit_cast(u32x4_t, rest);
-            }
+            for (int e = 0; e < 8; ++e) rest[e] = (__bf16)(ps[e] - (float)high[e]), psum += (float)rest[e];
+            ph = __builtin_bit_cast(u32x4_t, high), pl = __builtin_bit_cast(u32x4_t, rest);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pl[i] = (unsigned)__builtin_amdgcn_update_dpp(0, (int)pl[i], 0x128, 0xf, 0xf, true);  // (rotated by 8 of 16 lanes)
         };
         if (nc == F && s0 + F <= span.na && chunk_at(s0) * 32 >= lo_max && chunk_at(s0 + F - 1) * 32 + 32 <= hi_min) silu(std::false_type{});
         else silu(std::true_type{});
         auto sums = [&](const unsigned (&x)[U][8][VW], int c0) __attribute__((always_inline)) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const bool mine = own == c0 + u;
-                u32x4_t bh, bl;
+                u32x4_t b;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    bh[i] = mine ? ph[i] : 0u;
-                    if constexpr (TT::P_WORDS == 2) bl[i] = mine ? pl[i] : 0u;
-                }
+                for (int i = 0; i < 4; ++i) b[i] = own == c0 + u ? ph[i] : own == ((c0 + u) ^ (F / 2)) ? pl[i] : 0u;
 #pragma unroll
                 for (int h = 0; h < (NV + 3) / 4; ++h) {
                     u32x4_t vf[4];
@@ -1020,8 +1019,7 @@ __global__ __launch_bounds__(256, (STEP_WAVES<DK, DV>)) void hstu_paged_step_ker
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         if (4 * h + k >= NV) break;
-                        acc[4 * h + k] = PagedBf16::mma(vf[k], bh, acc[4 * h + k]);
-                        if constexpr (TT::P_WORDS == 2) acc[4 * h + k] = PagedBf16::mma(vf[k], bl, acc[4 * h + k]);
+                        acc[4 * h + k] = PagedBf16::mma(vf[k], b, acc[4 * h + k]);
                     }
                 }
             }

@@ -147,7 +147,8 @@ int hstu_cache_read(const HstuPagedCache* cache, int64_t rows, const void* start
  * out[b * delta_size + i] = sum_s M(p, s) * silu(alpha * <q, k_s>) / max_seq_len * v_s  for the newest delta_size positions
  * p = seq_lengths[b] - delta_size + i of every sequence, with the masks of the cached form (hstu_hip.h).  Head h of q reads head
  * h / (q_heads / heads) of the cache.  K and V enter as lowest + step * code, unrounded; silu(.) times a V row's step is rounded to
- * bf16 for the second product (to two bf16 words, 16 bits, where the type is fp16), sums are in fp32 and rounded once.  Codes enter the
+ * bf16 for the second product (to two bf16 words, 16 bits, where the type is fp16 or no more than eight rows of q, delta_size times
+ * q_heads / heads, share a head), sums are in fp32 and rounded once.  Codes enter the
  * products with an offset of up to 128: sums over a row of |q|, or over the positions of |silu(.)| times a V row's step, of 2^120 and
  * more may overflow.
  * A row at a position before the first is zero.  A sequence that is longer than its row of the page table gives NaN.  Where one of its

@@ -108,8 +108,9 @@ def sequence_rows(cache, table_row, n, which):
     return c, s[..., :1], s[..., 1:]
 
 
-def attention(max_seq_len, alpha, q, cache, page_table, lengths, targets=None, max_attn_len=0, contextual_seq_len=0, dtype=torch.bfloat16):
-    """(out, bound) of the cached form on CPU copies of a cache, ``[batch * delta, q heads, dv]``."""
+def attention(max_seq_len, alpha, q, cache, page_table, lengths, targets=None, max_attn_len=0, contextual_seq_len=0, dtype=torch.bfloat16, p_words=None):
+    """(out, bound) of the cached form on CPU copies of a cache, ``[batch * delta, q heads, dv]``.  ``p_words``: bf16 words that P times the step is
+    kept in (by default one for bf16, two for fp16)."""
     batch = page_table.shape[0]
     delta, hq, heads = q.shape[0] // batch, q.shape[1], cache[0].shape[1]
     group = hq // heads
@@ -120,7 +121,7 @@ def attention(max_seq_len, alpha, q, cache, page_table, lengths, targets=None, m
     off_k, off_v = (128.0 if dtype == torch.bfloat16 else 64.0), 128.0
     # P times the step is rounded to bf16: 8 bits of significand, neighbours 2^-7 2^e apart around values of 2^e and more, so off by at most
     # half of that, 2^-8 of the value (2^-9 holds just below 2^(e+1) alone).  Two words: 2^-8 of what the first left out, 2^-16.
-    p_round = 2.0**-8 if dtype == torch.bfloat16 else 2.0**-16
+    p_round = 2.0**-8 if (p_words or (1 if dtype == torch.bfloat16 else 2)) == 1 else 2.0**-16
     for b in range(batch):
         n = int(lengths[b])
         if n <= 0:

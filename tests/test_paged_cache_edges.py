@@ -407,3 +407,23 @@ def test_norm_weights_gradients_keep_their_bits_in_fp32(pkg, dev):
     for x, w, dy, got in ((q, qw, up[0], grads[0]), (k, kw, up[1], grads[1])):
         _, want, _ = O.norm_rope_grad(x, dy, w, 1e-6, table, pos)
         assert float((got.double().cpu() - want).norm() / want.norm()) <= 2 * 2.0**-24
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,hq", [(1, 1), (2, 1), (1, 3), (4, 1), (5, 1), (4, 2)])
+@pytest.mark.parametrize("dqk,dv", [(128, 128), (32, 64), (64, 32), (256, 256)])
+def test_few_rows_are_as_exact_as_their_type(pkg, dev, rows, hq, dqk, dv):
+    """Up to eight rows of a head in bf16: P times the step is kept to 16 bits, so that nothing but the result's own rounding is left of bf16."""
+    print(f"[case] attention: {rows} x {hq} rows of {dqk} and {dv}, exact", flush=True)
+    lengths = [777, 31, 1500, 512, rows]
+    table, pages = O.page_table(rows, lengths, 32)
+    cache = O.fill_cache(rows + 1, pages, 1, 32, dqk, dv, BF16)
+    q, n = _rand(rows + 2, (5 * rows, hq, dqk), BF16), torch.tensor(lengths)
+    for targets, w, c in ((None, 0, 0), ([min(m, rows) for m in lengths], 200, 0)):
+        t = None if targets is None else torch.tensor(targets)
+        want, bound = O.attention(1500, dqk**-0.5, q, cache, table, n, t, w, c, BF16, p_words=2)
+        on = _to(dev, q, table, n, t)
+        for splits in (0, 1):
+            got = pkg.delta_hstu_mha_paged(1500, dqk**-0.5, on[0], tuple(x.to(dev) for x in cache), on[1], on[2], on[3], w, c, kv_splits=splits)
+            torch.cuda.synchronize()
+            _within(got, want, bound, f"window {w}, splits {splits}")
