@@ -790,7 +790,7 @@ __global__ __launch_bounds__(256, 2) void hstu_paged_block_kernel(const PagedAtt
 // Waves of a SIMD: three in 168 registers each took 281 us where two in 172 took 290 (128 sequences of 4096 .. 16384 positions, eight
 // heads of 128, 1.45 GB); four rows of 128 sequences of up to 8192 88 where two in 214 took 103, but of 33 of up to 2048 16.5 where two took 14.5;
 // heads of 256 need the registers of one.  The cache's bytes bound it: the same sequences in runs of up to 96
-// chunks take 265 us, 5.4 TB/s where a copy of 1 GiB reaches 5.2.  One short sequence is launches and loads that wait for each other: 8 us.
+// chunks take 267 us, 5.4 TB/s where a copy of 1 GiB reaches 5.2.  One short sequence is launches and loads that wait for each other: 8 us.
 template <int DK, int DV>
 constexpr int STEP_WAVES = DK == 256 ? 1 : DK + DV >= 128 ? 3 : 4;
 
