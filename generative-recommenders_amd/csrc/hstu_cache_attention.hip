@@ -49,14 +49,14 @@ Plan plan_of(const HstuPagedCache* c, const HstuPagedAttentionArgs* a) {
     if (a->max_attn_len > 0 && (int64_t)a->max_attn_len + a->delta_size + a->contextual_seq_len < longest)
         longest = (int64_t)a->max_attn_len + a->delta_size + a->contextual_seq_len;
     const int64_t chunks = (longest + 31) / 32 + 1, wgs = (int64_t)p.row_blocks * c->heads * c->batch;
-    // Runs of a step.  Joining costs 3 us, so sequences of up to 40 chunks are one run each (one of 512 positions: 8.2 us, in two runs 11.4; of 1024:
-    // 10.2, in three 11.6), and so are those of up to 96 where they fill half of what the card holds, two workgroups of a CU (100 of up to 2048
-    // positions and four heads: 22 us, in two runs 25).  Else runs that fill it once, for each begins with some microseconds of loads that wait for
-    // each other (64 sequences of 1024 .. 4096 positions and four heads, 256 workgroups for whole sequences: in two runs 26 us, one 28, eight 30);
-    // in eights, two chunks to each wave (33 sequences of up to 2048, four rows: runs of 16 15 us, of 18 or 32 18); none that leaves a short second
-    // or third, which makes some of them up to 120 long; and else none longer than 96, so that the last of them do not run alone (128 sequences of up to 16384 and eight heads: whole
-    // sequences 291 us, runs of 384 chunks 281, of 96 264, of 33 281).  Sequences of a few chunks, more of them than fit, are a wave's each
-    // (1600 of up to 10 chunks: 12 us, 16 by workgroups).
+    // Runs of a step.  Joining costs 3 us, so sequences of up to 40 chunks are one run each (one of 512 positions: 8.0 us, in two runs 10.8; of 1024:
+    // 10.3, in three 11.2), and so are those of up to 96 where they fill half of what the card holds, two workgroups of a CU (100 of up to 2048
+    // positions and four heads: 22.3 us, in two runs 24.1).  Else runs that fill it once, for each begins with some microseconds of loads that wait
+    // for each other (64 sequences of 1024 .. 4096 positions and four heads, 256 workgroups for whole sequences: in two runs 26.6 us, one 28.1, eight
+    // 32.1); in eights, two chunks to each wave (33 sequences of up to 2048, four rows: runs of 16 17 us, of 18 18, whole sequences 20); none that
+    // leaves a short second or third, which makes some of them up to 120 long; and else none longer than 96, so that the last of them do not run
+    // alone (128 sequences of up to 16384 and eight heads: whole sequences 307 us, runs of 257 chunks 276, of 96 269, of 33 284).  Sequences of a few
+    // chunks, more of them than fit, are a wave's each (1600 of up to 10 chunks, by workgroups, took a third longer).
     // More rows are split into equal parts of each sequence, of at least 8 or 16 chunks: what a part more costs is a partial sum of every row to
     // write and read.  Blocks: at least two workgroups of a CU, whose sequences are ranked.  Nine to 32 rows: parts that fill the card in one
     // round, 512 workgroups, or 256 of more than 16 rows of wide heads, whose waves need a SIMD each, or in two rounds where one would leave much of it empty (24 rows, 160 workgroups
