@@ -1,5 +1,5 @@
 // Native front of the operators: a Python module (`hstu_native`) that takes torch tensors, checks them, allocates the
-// result and the scratch memory and calls the C ABI (hstu_hip.h, hstu_linear.h, hstu_cache.h) -- the work that ops/*.py does through
+// result and the scratch memory and calls the C ABI (hstu_hip.h, hstu_linear.h, hstu_cache.h, hstu_recurrent.h) -- the work that ops/*.py does through
 // ctypes for every argument it has to look at, in a few microseconds instead of ten to thirty.
 //
 // The operators that are differentiable record a backward node of their own here (torch::autograd::Function): nothing but inputs
@@ -15,6 +15,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <array>
 #include <cstdlib>
 #include <optional>
 #include <tuple>
@@ -22,6 +23,7 @@
 #include "hstu_cache.h"
 #include "hstu_hip.h"
 #include "hstu_linear.h"
+#include "hstu_recurrent.h"
 
 namespace {
 
@@ -958,6 +960,276 @@ OptTensor delta_hstu_mha_paged(int64_t max_seq_len, double alpha, const Tensor& 
     return out;
 }
 
+// ---- the gated recurrence, and what stands between two blocks -----------------------------------------------------------
+
+void check_recurrent(int rc) {
+    if (rc == 0) return;
+    const std::string what = c10::str("hstu_recurrent: ", hstu_hip_status_string(rc), " (", hstu_recurrent_last_error(), ") [status ", rc, "]");
+    TORCH_CHECK_VALUE(rc != HSTU_ERR_NULL_POINTER && rc != HSTU_ERR_BAD_SHAPE, what);
+    TORCH_CHECK_NOT_IMPLEMENTED(rc != HSTU_ERR_UNSUPPORTED, what);
+    TORCH_CHECK(false, what);
+}
+
+bool float_type(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kFloat; }
+
+// [rows, width] or [rows, heads, dim] with the columns of a row side by side, at any distance between rows.
+bool flat_rows(const Tensor& t) {
+    if (!t.is_cuda() || t.numel() == 0 || (t.dim() != 2 && t.dim() != 3)) return false;
+    const int64_t last = t.dim() - 1;
+    if (t.size(last) > 1 && t.stride(last) != 1) return false;
+    if (last == 2 && t.size(1) > 1 && t.stride(1) != t.size(2)) return false;
+    return t.size(0) == 1 || t.stride(0) >= 0;
+}
+int64_t flat_pitch(const Tensor& t) { return t.size(0) == 1 ? 0 : t.stride(0); }
+int64_t flat_width(const Tensor& t) { return t.dim() == 3 ? t.size(1) * t.size(2) : t.size(1); }
+Tensor to_flat_rows(const Tensor& t) { return flat_rows(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+Tensor to_dense(const Tensor& t) { return t.is_contiguous() ? t : t.clone(at::MemoryFormat::Contiguous); }
+
+// A tensor like x in shape, type and device, as the kernels read it.
+bool alike(const Tensor& t, const Tensor& x) { return flat_rows(t) && t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type() && t.device() == x.device(); }
+
+bool decay_of(const Tensor& decay, const Tensor& x) {
+    return decay.is_cuda() && decay.dim() == 1 && decay.size(0) == flat_width(x) && decay.is_contiguous() && decay.device() == x.device() &&
+           (decay.scalar_type() == at::kFloat || decay.scalar_type() == x.scalar_type());
+}
+
+// [count, width] of fp32, dense
+bool state_rows(const Tensor& t, int64_t count, const Tensor& x) {
+    return t.is_cuda() && t.dim() == 2 && t.size(0) == count && t.size(1) == flat_width(x) && t.scalar_type() == at::kFloat && t.is_contiguous() &&
+           t.device() == x.device();
+}
+
+Tensor bytes_like(size_t bytes, const Tensor& like, void** ptr) {
+    Tensor t = at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+    *ptr = bytes ? t.data_ptr() : nullptr;
+    return t;
+}
+
+void fill_scan(HstuRecurrenceArgs& a, const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& decay, const OptTensor& initial, const Tensor& offsets,
+               double rate) {
+    a.x = x.const_data_ptr(), a.decay_gate = r.const_data_ptr(), a.input_gate = i.const_data_ptr();
+    a.x_row_stride = flat_pitch(x), a.decay_gate_row_stride = flat_pitch(r), a.input_gate_row_stride = flat_pitch(i);
+    a.decay = decay.const_data_ptr(), a.decay_f32 = decay.scalar_type() == at::kFloat, a.rate = (float)rate;
+    a.seq_offsets = offsets.const_data_ptr(), a.seq_offsets_i64 = is_i64(offsets), a.batch = (int32_t)(offsets.numel() - 1);
+    a.rows = x.size(0), a.width = (int32_t)flat_width(x), a.dtype = attention_dtype(x.scalar_type());
+    a.initial_state = initial ? (const float*)initial->const_data_ptr() : nullptr;
+}
+
+struct ScanResult {
+    Tensor out, final_state, saved;  // the last two: where asked for
+};
+
+ScanResult scan_result(const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& decay, const OptTensor& initial, const Tensor& offsets, double rate,
+                       bool want_state, bool want_saved) {
+    HstuRecurrenceArgs a{};
+    fill_scan(a, x, r, i, decay, initial, offsets, rate);
+    ScanResult got{at::empty(x.sizes(), x.options()), Tensor(), Tensor()};
+    a.out = got.out.data_ptr();
+    if (want_state) {
+        got.final_state = at::empty({a.batch, a.width}, x.options().dtype(at::kFloat));
+        a.final_state = (float*)got.final_state.data_ptr();
+    }
+    void* ptr;
+    if (want_saved) got.saved = bytes_like(hstu_recurrent_scan_saved_bytes(&a), x, &ptr), a.saved = (float*)ptr;
+    a.workspace_bytes = (int64_t)hstu_recurrent_scan_workspace_bytes(&a);
+    Tensor scratch;
+    if (a.workspace_bytes > 0) scratch = bytes_like(a.workspace_bytes, x, &a.workspace);
+    const c10::DeviceGuard on_device(x.device());
+    check_recurrent(hstu_recurrent_scan(&a, stream_of(x)));
+    return got;
+}
+
+struct ScanFunction : torch::autograd::Function<ScanFunction> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& decay, const OptTensor& initial,
+                                 const Tensor& offsets, double rate, bool want_state) {
+        const ScanResult got = scan_result(x, r, i, decay, initial, offsets, rate, want_state, true);
+        ctx->save_for_backward({x, r, i, decay, initial ? *initial : Tensor(), offsets, got.saved});
+        ctx->saved_data["rate"] = rate;
+        ctx->set_materialize_grads(false);
+        if (want_state) return {got.out, got.final_state};
+        return {got.out};
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const BackwardScope scope;
+        const auto saved = ctx->get_saved_variables();
+        variable_list got(8);
+        const bool any_out = grads[0].defined(), any_state = grads.size() > 1 && grads[1].defined();
+        if (!any_out && !any_state) return got;
+        const Tensor x = to_flat_rows(saved[0]), r = to_flat_rows(saved[1]), i = to_flat_rows(saved[2]), decay = to_dense(saved[3]), offsets = to_dense(saved[5]),
+                     entry = to_dense(saved[6]);
+        const OptTensor initial = saved[4].defined() ? OptTensor(to_dense(saved[4])) : OptTensor();
+        HstuRecurrenceArgs a{};
+        HstuRecurrenceGrads g{};
+        fill_scan(a, x, r, i, decay, initial, offsets, ctx->saved_data["rate"].toDouble());
+        a.saved = entry.numel() ? (float*)entry.data_ptr() : nullptr;
+        Tensor dout, dstate;
+        if (any_out) dout = to_flat_rows(grads[0].to(x.scalar_type())), g.d_out = dout.const_data_ptr(), g.d_out_row_stride = flat_pitch(dout);
+        if (any_state) dstate = to_dense(grads[1].to(at::kFloat)), g.d_final_state = (const float*)dstate.const_data_ptr();
+        auto make = [&](size_t k, const Tensor& like) {
+            if (!ctx->needs_input_grad(k)) return (void*)nullptr;
+            got[k] = at::empty(like.sizes(), like.options());
+            return got[k].data_ptr();
+        };
+        g.d_x = make(0, x), g.d_decay_gate = make(1, r), g.d_input_gate = make(2, i), g.d_decay = make(3, decay);
+        if (initial) g.d_initial_state = (float*)make(4, *initial);
+        g.workspace_bytes = (int64_t)hstu_recurrent_scan_bwd_workspace_bytes(&a);
+        Tensor scratch;
+        if (g.workspace_bytes > 0) scratch = bytes_like(g.workspace_bytes, x, &g.workspace);
+        const c10::DeviceGuard on_device(x.device());
+        check_recurrent(hstu_recurrent_scan_bwd(&a, &g, stream_of(x)));
+        return got;
+    }
+};
+
+std::optional<std::tuple<Tensor, OptTensor>> gated_recurrence(const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& decay, const Tensor& offsets,
+                                                              const OptTensor& initial, double rate, bool want_state, bool checked) {
+    if (!flat_rows(x) || !float_type(x) || !alike(r, x) || !alike(i, x) || !decay_of(decay, x) || !(rate > 0) || !((float)rate > 0.f)) return {};
+    if (!offsets.is_cuda() || offsets.dim() != 1 || offsets.numel() < 2 || !index_vector(offsets, offsets.numel(), x.device())) return {};
+    if (initial && !state_rows(*initial, offsets.numel() - 1, x)) return {};
+    if ((!checked && contract_checks()) || has_tangent({&x, &r, &i, &decay}, {&initial})) return {};
+    RECORD_USER_SCOPE("gated_recurrence");
+    const bool grad = wants_grad({&x, &r, &i, &decay}) || (initial && wants_grad({&*initial}));
+    if (!grad) {
+        const ScanResult got = scan_result(x, r, i, decay, initial, offsets, rate, want_state, false);
+        return std::make_tuple(got.out, want_state ? OptTensor(got.final_state) : OptTensor());
+    }
+    const variable_list o = ScanFunction::apply(x, r, i, decay, initial, offsets, rate, want_state);
+    return std::make_tuple(o[0], want_state ? OptTensor(o[1]) : OptTensor());
+}
+
+OptTensor gated_recurrence_step(const Tensor& states, const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& decay, const OptTensor& slots,
+                                const OptTensor& new_slots, double rate, bool checked) {
+    if (!flat_rows(x) || !float_type(x) || !alike(r, x) || !alike(i, x) || !decay_of(decay, x) || !(rate > 0) || !((float)rate > 0.f)) return {};
+    if (!states.is_cuda() || states.dim() != 2 || states.size(1) != flat_width(x) || states.scalar_type() != at::kFloat || states.device() != x.device()) return {};
+    if ((states.size(1) > 1 && states.stride(1) != 1) || (states.size(0) > 1 && states.stride(0) < states.size(1))) return {};
+    if ((!slots && states.size(0) != x.size(0)) || (slots && !index_vector(*slots, x.size(0), x.device()))) return {};
+    if (new_slots && !index_vector(*new_slots, x.size(0), x.device())) return {};
+    if ((!checked && contract_checks()) || wants_grad({&states, &x, &r, &i, &decay}) || has_tangent({&states, &x, &r, &i, &decay})) return {};
+    HstuRecurrenceStepArgs a{};
+    a.x = x.const_data_ptr(), a.decay_gate = r.const_data_ptr(), a.input_gate = i.const_data_ptr();
+    a.x_row_stride = flat_pitch(x), a.decay_gate_row_stride = flat_pitch(r), a.input_gate_row_stride = flat_pitch(i);
+    a.decay = decay.const_data_ptr(), a.decay_f32 = decay.scalar_type() == at::kFloat, a.rate = (float)rate;
+    a.state_rows = states.size(0), a.state_row_stride = states.size(0) > 1 ? states.stride(0) : 0;
+    if (slots) a.slots = slots->const_data_ptr(), a.slots_i64 = is_i64(*slots);
+    if (new_slots) a.new_slots = new_slots->const_data_ptr(), a.new_slots_i64 = is_i64(*new_slots);
+    a.rows = x.size(0), a.width = (int32_t)flat_width(x), a.dtype = attention_dtype(x.scalar_type());
+    RECORD_USER_SCOPE("gated_recurrence_step");
+    Tensor out = at::empty(x.sizes(), x.options());
+    a.out = out.data_ptr(), a.states = (float*)states.data_ptr();
+    const c10::DeviceGuard on_device(x.device());
+    states.unsafeGetTensorImpl()->bump_version();  // (in place)
+    check_recurrent(hstu_recurrent_step(&a, stream_of(x)));
+    return out;
+}
+
+// Parameters in the order of HstuResidualNormArgs: post_weight, post_bias, scale, pre_weight, pre_bias.
+typedef std::array<OptTensor, 5> NormParameters;
+
+struct ResidualNormCall {
+    double eps;
+    bool layer_norm;
+    int64_t activation;
+    double dropout;
+    uint64_t seed, offset;
+};
+
+void fill_residual_norm(HstuResidualNormArgs& a, const Tensor& x, const Tensor& y, const OptTensor& gate, const NormParameters& p, const ResidualNormCall& c) {
+    a.x = x.const_data_ptr(), a.y = y.const_data_ptr(), a.x_row_stride = flat_pitch(x), a.y_row_stride = flat_pitch(y);
+    if (gate) a.gate = gate->const_data_ptr(), a.gate_row_stride = flat_pitch(*gate);
+    const void** to[5] = {&a.post_weight, &a.post_bias, &a.scale, &a.pre_weight, &a.pre_bias};
+    for (int k = 0; k < 5; ++k) *to[k] = p[k] ? p[k]->const_data_ptr() : nullptr;
+    a.eps = (float)c.eps, a.layer_norm = c.layer_norm, a.gate_activation = (int32_t)c.activation, a.dtype = attention_dtype(x.scalar_type());
+    a.rows = x.size(0), a.width = (int32_t)flat_width(x);
+    a.dropout_ratio = c.dropout, a.dropout_seed = c.seed, a.dropout_offset = c.offset;
+}
+
+typedef std::tuple<Tensor, OptTensor> OutAndNormed;
+
+OutAndNormed residual_norm_result(const Tensor& x, const Tensor& y, const OptTensor& gate, const NormParameters& p, const ResidualNormCall& c) {
+    HstuResidualNormArgs a{};
+    fill_residual_norm(a, x, y, gate, p, c);
+    Tensor out = at::empty(x.sizes(), x.options());
+    OptTensor normed;
+    a.out = out.data_ptr();
+    if (p[3]) normed = at::empty(x.sizes(), x.options()), a.normed = normed->data_ptr();
+    const c10::DeviceGuard on_device(x.device());
+    check_recurrent(hstu_recurrent_residual_norm(&a, stream_of(x)));
+    return {out, normed};
+}
+
+struct ResidualNormFunction : torch::autograd::Function<ResidualNormFunction> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& y, const OptTensor& gate, const OptTensor& post_weight,
+                                 const OptTensor& post_bias, const OptTensor& scale, const OptTensor& pre_weight, const OptTensor& pre_bias,
+                                 const ResidualNormCall& c) {
+        auto [out, normed] = residual_norm_result(x, y, gate, {post_weight, post_bias, scale, pre_weight, pre_bias}, c);
+        variable_list keep{x, y};
+        for (const OptTensor* t : {&gate, &post_weight, &post_bias, &scale, &pre_weight, &pre_bias}) keep.push_back(*t ? **t : Tensor());
+        ctx->save_for_backward(keep);
+        ctx->saved_data["call"] = std::vector<int64_t>{c.layer_norm, c.activation, (int64_t)c.seed, (int64_t)c.offset};
+        ctx->saved_data["floats"] = std::vector<double>{c.eps, c.dropout};
+        ctx->set_materialize_grads(false);
+        if (normed) return {out, *normed};
+        return {out};
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const BackwardScope scope;
+        const auto saved = ctx->get_saved_variables();
+        const auto n = ctx->saved_data["call"].toIntVector();
+        const auto f = ctx->saved_data["floats"].toDoubleVector();
+        const ResidualNormCall c{f[0], n[0] != 0, n[1], f[1], (uint64_t)n[2], (uint64_t)n[3]};
+        variable_list got(9);
+        const bool any_out = grads[0].defined(), any_normed = grads.size() > 1 && grads[1].defined();
+        if (!any_out && !any_normed) return got;
+        const Tensor x = to_flat_rows(saved[0]), y = to_flat_rows(saved[1]);
+        const OptTensor gate = saved[2].defined() ? OptTensor(to_flat_rows(saved[2])) : OptTensor();
+        NormParameters p;
+        for (int k = 0; k < 5; ++k)
+            if (saved[3 + k].defined()) p[k] = to_dense(saved[3 + k]);
+        HstuResidualNormArgs a{};
+        HstuResidualNormGrads g{};
+        fill_residual_norm(a, x, y, gate, p, c);
+        Tensor dout, dnormed;
+        if (any_out) dout = to_flat_rows(grads[0].to(x.scalar_type())), g.d_out = dout.const_data_ptr(), g.d_out_row_stride = flat_pitch(dout);
+        if (any_normed) dnormed = to_flat_rows(grads[1].to(x.scalar_type())), g.d_normed = dnormed.const_data_ptr(), g.d_normed_row_stride = flat_pitch(dnormed);
+        size_t edge = 0;  // inputs as autograd counts them: those that there are
+        auto make = [&](size_t k, const Tensor& like) {
+            if (!like.defined() || !ctx->needs_input_grad(edge++)) return (void*)nullptr;
+            got[k] = at::empty(like.sizes(), x.options());
+            return got[k].data_ptr();
+        };
+        g.d_x = make(0, x), g.d_y = make(1, y), g.d_gate = make(2, saved[2]);
+        void** to[5] = {&g.d_post_weight, &g.d_post_bias, &g.d_scale, &g.d_pre_weight, &g.d_pre_bias};
+        for (int k = 0; k < 5; ++k) *to[k] = make(3 + k, saved[3 + k]);
+        // (without a gradient of normed its norm's parameters have none to give: zeros)
+        g.workspace_bytes = (int64_t)hstu_recurrent_residual_norm_bwd_workspace_bytes(&a);
+        Tensor scratch = bytes_like(g.workspace_bytes, x, &g.workspace);
+        const c10::DeviceGuard on_device(x.device());
+        check_recurrent(hstu_recurrent_residual_norm_bwd(&a, &g, stream_of(x)));
+        return got;
+    }
+};
+
+std::optional<OutAndNormed> gated_residual_norm(const Tensor& x, const Tensor& y, const OptTensor& gate, const OptTensor& post_weight, const OptTensor& post_bias,
+                                                const OptTensor& scale, const OptTensor& pre_weight, const OptTensor& pre_bias, double eps, bool layer_norm,
+                                                int64_t activation, double dropout, uint64_t seed, uint64_t offset) {
+    if (!flat_rows(x) || !float_type(x) || !alike(y, x) || (gate && !alike(*gate, x)) || activation < 0) return {};
+    const NormParameters p{post_weight, post_bias, scale, pre_weight, pre_bias};
+    const int64_t width = flat_width(x);
+    bool grad = wants_grad({&x, &y}) || (gate && wants_grad({&*gate}));
+    for (const OptTensor& t : p) {
+        if (!t) continue;
+        if (!t->is_cuda() || t->dim() != 1 || t->size(0) != width || !t->is_contiguous() || t->scalar_type() != x.scalar_type() || t->device() != x.device()) return {};
+        grad = grad || wants_grad({&*t});
+    }
+    if ((post_bias && !post_weight) || (pre_bias && !pre_weight) || !(dropout >= 0 && dropout < 1) || width > 8192) return {};
+    if (has_tangent({&x, &y}, {&gate, &post_weight, &post_bias, &scale, &pre_weight, &pre_bias})) return {};
+    const ResidualNormCall c{eps, layer_norm, activation, dropout, seed, offset};
+    RECORD_USER_SCOPE("gated_residual_norm");
+    if (!grad) return residual_norm_result(x, y, gate, p, c);
+    const variable_list o = ResidualNormFunction::apply(x, y, gate, post_weight, post_bias, scale, pre_weight, pre_bias, c);
+    return OutAndNormed(o[0], pre_weight ? OptTensor(o[1]) : OptTensor());
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -975,4 +1247,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("append_paged_kv", &append_paged_kv, nogil);
     m.def("read_paged_kv", &read_paged_kv, nogil);
     m.def("delta_hstu_mha_paged", &delta_hstu_mha_paged, nogil);
+    m.def("gated_recurrence", &gated_recurrence, nogil);
+    m.def("gated_recurrence_step", &gated_recurrence_step, nogil);
+    m.def("gated_residual_norm", &gated_residual_norm, nogil);
 }

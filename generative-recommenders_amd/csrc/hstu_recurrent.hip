@@ -1,0 +1,311 @@
+// C ABI of libhstu_recurrent.so (include/hstu_recurrent.h): checks and launches.
+#include "hstu_recurrent.h"
+
+#include <hip/hip_runtime.h>
+
+#include <atomic>
+#include <cstdio>
+#include <cstring>
+#include <type_traits>
+
+#include "hstu_hip.h"
+#include "hstu_recurrence_kernel.h"
+#include "hstu_residual_norm_kernel.h"
+
+namespace {
+
+thread_local char g_last_error[256] = "";
+
+int launch_status(const char* what) {
+    const hipError_t e = hipGetLastError();
+    if (e == hipSuccess) return 0;
+    snprintf(g_last_error, sizeof(g_last_error), "%s: %s", what, hipGetErrorString(e));
+    return HSTU_ERR_LAUNCH;
+}
+
+bool device_is_gfx950() {
+    static std::atomic<int> known[64];  // 0 unknown, 1 yes, 2 no; racing threads store the same value
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return false;
+    if (known[dev] == 0) {
+        hipDeviceProp_t prop;
+        if (hipGetDeviceProperties(&prop, dev) != hipSuccess) return false;
+        known[dev] = strncmp(prop.gcnArchName, "gfx950", 6) == 0 ? 1 : 2;
+    }
+    return known[dev] == 1;
+}
+
+template <class F>
+int with_type(int dtype, F&& f) {
+    if (dtype == HSTU_BF16) return f((__bf16*)nullptr);
+    if (dtype == HSTU_FP16) return f((_Float16*)nullptr);
+    return f((float*)nullptr);
+}
+
+bool known_type(int dtype) { return dtype == HSTU_BF16 || dtype == HSTU_FP16 || dtype == HSTU_FP32; }
+int bytes_of(int dtype) { return dtype == HSTU_FP32 ? 4 : 2; }
+bool aligned_to(const void* ptr, int bytes) { return (reinterpret_cast<uintptr_t>(ptr) & (bytes - 1)) == 0; }
+
+constexpr int64_t kMaxBlocks = (1 << 22) - 1;  // a launch has fewer than 2^32 threads in a dimension, and a workgroup at most 1024
+
+// ---- the recurrence ----
+
+// 0, or the status.  What only one direction needs is its own to check.
+int check_scan(const HstuRecurrenceArgs* a) {
+    if (!a) return HSTU_ERR_NULL_POINTER;
+    if (!known_type(a->dtype)) return HSTU_ERR_BAD_DTYPE;
+    if (a->rows < 0 || a->width <= 0 || a->batch <= 0 || !(a->rate > 0.f)) return HSTU_ERR_BAD_SHAPE;
+    if (a->x_row_stride < 0 || a->decay_gate_row_stride < 0 || a->input_gate_row_stride < 0) return HSTU_ERR_BAD_SHAPE;
+    if (!a->seq_offsets || !a->decay) return HSTU_ERR_NULL_POINTER;
+    if (a->rows > 0 && (!a->x || !a->decay_gate || !a->input_gate)) return HSTU_ERR_NULL_POINTER;
+    const int es = bytes_of(a->dtype);
+    if (!aligned_to(a->x, es) || !aligned_to(a->decay_gate, es) || !aligned_to(a->input_gate, es) || !aligned_to(a->out, es)) return HSTU_ERR_MISALIGNED;
+    if (!aligned_to(a->decay, a->decay_f32 ? 4 : es) || !aligned_to(a->initial_state, 4) || !aligned_to(a->final_state, 4) || !aligned_to(a->saved, 4))
+        return HSTU_ERR_MISALIGNED;
+    if (!aligned_to(a->seq_offsets, a->seq_offsets_i64 ? 8 : 4)) return HSTU_ERR_MISALIGNED;
+    return 0;
+}
+
+hstu::ScanParams scan_params(const HstuRecurrenceArgs* a) {
+    hstu::ScanParams p{};
+    p.x = (const char*)a->x, p.r = (const char*)a->decay_gate, p.i = (const char*)a->input_gate;
+    p.x_rs = a->x_row_stride, p.r_rs = a->decay_gate_row_stride, p.i_rs = a->input_gate_row_stride;
+    p.decay = a->decay, p.decay_f32 = a->decay_f32, p.rate = a->rate;
+    p.offsets = a->seq_offsets, p.offsets_i64 = a->seq_offsets_i64, p.batch = a->batch;
+    p.rows = a->rows, p.width = a->width, p.initial = a->initial_state;
+    return p;
+}
+
+}  // namespace
+
+extern "C" {
+
+int hstu_recurrent_version(void) { return 100; }
+const char* hstu_recurrent_last_error(void) { return g_last_error; }
+
+size_t hstu_recurrent_scan_workspace_bytes(const HstuRecurrenceArgs*) { return 0; }
+size_t hstu_recurrent_scan_saved_bytes(const HstuRecurrenceArgs*) { return 0; }
+
+int hstu_recurrent_scan(const HstuRecurrenceArgs* a, void* stream) {
+    const int rc = check_scan(a);
+    if (rc) return rc;
+    if (a->rows > 0 && !a->out) return HSTU_ERR_NULL_POINTER;
+    if (a->batch >= 65535) return HSTU_ERR_UNSUPPORTED;
+    if (!device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
+    hstu::ScanParams p = scan_params(a);
+    p.out = (char*)a->out, p.final_state = a->final_state;
+    return with_type(a->dtype, [&](auto* t) {
+        hipLaunchKernelGGL((hstu::hstu_scan_kernel<std::remove_pointer_t<decltype(t)>>), dim3((a->width + 255) / 256, a->batch + 1), dim3(256), 0, (hipStream_t)stream, p);
+        return launch_status("recurrence kernel launch");
+    });
+}
+
+size_t hstu_recurrent_scan_bwd_workspace_bytes(const HstuRecurrenceArgs* a) {
+    if (check_scan(a)) return 0;
+    return (size_t)(a->rows + a->batch) * a->width * sizeof(float);
+}
+
+int hstu_recurrent_scan_bwd(const HstuRecurrenceArgs* a, const HstuRecurrenceGrads* g, void* stream) {
+    const int rc = check_scan(a);
+    if (rc) return rc;
+    if (!g) return HSTU_ERR_NULL_POINTER;
+    if (g->d_out_row_stride < 0) return HSTU_ERR_BAD_SHAPE;
+    const int es = bytes_of(a->dtype);
+    for (const void* ptr : {g->d_out, (const void*)g->d_x, (const void*)g->d_decay_gate, (const void*)g->d_input_gate})
+        if (!aligned_to(ptr, es)) return HSTU_ERR_MISALIGNED;
+    if (!aligned_to(g->d_final_state, 4) || !aligned_to(g->d_initial_state, 4) || !aligned_to(g->d_decay, a->decay_f32 ? 4 : es) || !aligned_to(g->workspace, 16))
+        return HSTU_ERR_MISALIGNED;
+    if (a->batch >= 65535) return HSTU_ERR_UNSUPPORTED;
+    if (!g->workspace) return HSTU_ERR_NULL_POINTER;
+    if (g->workspace_bytes < (int64_t)hstu_recurrent_scan_bwd_workspace_bytes(a)) return HSTU_ERR_BAD_SHAPE;
+    if (!device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
+    hstu::ScanParams p = scan_params(a);
+    p.dout = (const char*)g->d_out, p.dout_rs = g->d_out_row_stride, p.dfinal = g->d_final_state;
+    p.dx = (char*)g->d_x, p.dr = (char*)g->d_decay_gate, p.di = (char*)g->d_input_gate, p.dinitial = g->d_initial_state;
+    p.states = (float*)g->workspace, p.partial = g->d_decay ? p.states + a->rows * a->width : nullptr;
+    return with_type(a->dtype, [&](auto* t) {
+        typedef std::remove_pointer_t<decltype(t)> T;
+        hipLaunchKernelGGL((hstu::hstu_scan_bwd_kernel<T>), dim3((a->width + 255) / 256, a->batch + 1), dim3(256), 0, (hipStream_t)stream, p);
+        const int status = launch_status("recurrence backward kernel launch");
+        if (status || !g->d_decay) return status;
+        hipLaunchKernelGGL((hstu::hstu_scan_decay_kernel<T>), dim3((a->width + 255) / 256), dim3(256), 0, (hipStream_t)stream, p.partial, a->batch, a->width, a->decay,
+                           a->decay_f32, a->rate, g->d_decay);
+        return launch_status("recurrence decay gradient kernel launch");
+    });
+}
+
+int hstu_recurrent_step(const HstuRecurrenceStepArgs* a, void* stream) {
+    if (!a) return HSTU_ERR_NULL_POINTER;
+    if (!known_type(a->dtype)) return HSTU_ERR_BAD_DTYPE;
+    if (a->rows < 0 || a->width <= 0 || a->state_rows < 0 || a->state_row_stride < 0 || !(a->rate > 0.f)) return HSTU_ERR_BAD_SHAPE;
+    if (a->x_row_stride < 0 || a->decay_gate_row_stride < 0 || a->input_gate_row_stride < 0) return HSTU_ERR_BAD_SHAPE;
+    if (a->rows == 0) return 0;
+    if (!a->x || !a->decay_gate || !a->input_gate || !a->out || !a->decay || (a->state_rows > 0 && !a->states)) return HSTU_ERR_NULL_POINTER;
+    const int es = bytes_of(a->dtype);
+    for (const void* ptr : {a->x, a->decay_gate, a->input_gate, (const void*)a->out})
+        if (!aligned_to(ptr, es)) return HSTU_ERR_MISALIGNED;
+    if (!aligned_to(a->decay, a->decay_f32 ? 4 : es) || !aligned_to(a->states, 4)) return HSTU_ERR_MISALIGNED;
+    if (!aligned_to(a->slots, a->slots_i64 ? 8 : 4) || !aligned_to(a->new_slots, a->new_slots_i64 ? 8 : 4)) return HSTU_ERR_MISALIGNED;
+    if (a->rows > (int64_t)65535 * 65535) return HSTU_ERR_UNSUPPORTED;
+    if (!device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
+    hstu::StepParams p{};
+    p.x = (const char*)a->x, p.r = (const char*)a->decay_gate, p.i = (const char*)a->input_gate;
+    p.x_rs = a->x_row_stride, p.r_rs = a->decay_gate_row_stride, p.i_rs = a->input_gate_row_stride;
+    p.out = (char*)a->out, p.decay = a->decay, p.decay_f32 = a->decay_f32, p.rate = a->rate;
+    p.states = a->states, p.state_rows = a->state_rows, p.state_rs = a->state_row_stride;
+    p.slots = a->slots, p.new_slots = a->new_slots, p.slots_i64 = a->slots_i64, p.new_slots_i64 = a->new_slots_i64;
+    p.rows = a->rows, p.width = a->width;
+    const unsigned y = (unsigned)(a->rows < 65535 ? a->rows : 65535), z = (unsigned)((a->rows + 65534) / 65535);
+    return with_type(a->dtype, [&](auto* t) {
+        hipLaunchKernelGGL((hstu::hstu_scan_step_kernel<std::remove_pointer_t<decltype(t)>>), dim3((a->width + 255) / 256, y, z), dim3(256), 0, (hipStream_t)stream, p);
+        return launch_status("recurrence step kernel launch");
+    });
+}
+
+}  // extern "C"
+
+namespace {
+
+// ---- between two blocks ----
+
+int residual_lanes(int width) {
+    int lanes = 8;
+    while (lanes * 8 < width) lanes *= 2;
+    return lanes;
+}
+int residual_groups(int lanes) { return lanes > 256 ? 1 : 256 / lanes; }
+
+int64_t residual_workgroups(const HstuResidualNormArgs* a, int64_t most) {
+    const int groups = residual_groups(residual_lanes(a->width));
+    const int64_t all = (a->rows + groups - 1) / groups;
+    return all < most ? all : most;
+}
+
+// Forward and backward: 0, or the status.  `wide`: whether all that `p` points to may be read and written in 16-byte pieces.
+int fill_residual(const HstuResidualNormArgs* a, hstu::ResidualNormParams& p, bool& wide) {
+    if (!a) return HSTU_ERR_NULL_POINTER;
+    if (!known_type(a->dtype)) return HSTU_ERR_BAD_DTYPE;
+    if (a->rows < 0 || a->width <= 0 || a->x_row_stride < 0 || a->y_row_stride < 0 || a->gate_row_stride < 0) return HSTU_ERR_BAD_SHAPE;
+    if (a->gate_activation < 0 || a->gate_activation > 2 || !(a->dropout_ratio >= 0. && a->dropout_ratio < 1.)) return HSTU_ERR_BAD_SHAPE;
+    if ((a->post_bias && !a->post_weight) || (a->pre_bias && !a->pre_weight)) return HSTU_ERR_NULL_POINTER;
+    if (a->width > 8192) return HSTU_ERR_UNSUPPORTED;
+    if (a->rows > 0 && (!a->x || !a->y)) return HSTU_ERR_NULL_POINTER;
+    p = hstu::ResidualNormParams{};
+    const int es = bytes_of(a->dtype), per16 = 16 / es;
+    const void* param[hstu::P_COUNT] = {a->post_weight, a->post_bias, a->scale, a->pre_weight, a->pre_bias};
+    wide = a->width % 8 == 0;
+    auto take = [&](const void* ptr, int64_t rs) {
+        if (ptr && (!aligned_to(ptr, 16) || rs % per16 != 0)) wide = false;
+        return aligned_to(ptr, es);
+    };
+    if (!take(a->x, a->x_row_stride) || !take(a->y, a->y_row_stride) || !take(a->gate, a->gate_row_stride)) return HSTU_ERR_MISALIGNED;
+    for (int k = 0; k < hstu::P_COUNT; ++k) {
+        if (!take(param[k], 0)) return HSTU_ERR_MISALIGNED;
+        p.param[k] = (const char*)param[k];
+    }
+    p.x = (const char*)a->x, p.y = (const char*)a->y, p.gate = (const char*)a->gate;
+    p.x_rs = a->x_row_stride, p.y_rs = a->y_row_stride, p.gate_rs = a->gate_row_stride;
+    p.eps = a->eps, p.inv_width = 1.f / a->width, p.layer_norm = a->layer_norm, p.act = a->gate_activation;
+    p.rows = a->rows, p.width = a->width;
+    p.drop.seed = a->dropout_seed, p.drop.offset = a->dropout_offset;
+    p.drop.thresh = (uint32_t)(a->dropout_ratio * 4294967296.0), p.drop.scale = (float)(1. / (1. - a->dropout_ratio));
+    return 0;
+}
+
+template <class F>
+int with_row(int lanes, bool wide, F&& f) {
+    auto sized = [&](auto l) { return wide ? f(l, std::true_type{}) : f(l, std::false_type{}); };
+    switch (lanes) {
+        case 8: return sized(std::integral_constant<int, 8>{});
+        case 16: return sized(std::integral_constant<int, 16>{});
+        case 32: return sized(std::integral_constant<int, 32>{});
+        case 64: return sized(std::integral_constant<int, 64>{});
+        case 128: return sized(std::integral_constant<int, 128>{});
+        case 256: return sized(std::integral_constant<int, 256>{});
+        case 512: return sized(std::integral_constant<int, 512>{});
+        default: return sized(std::integral_constant<int, 1024>{});
+    }
+}
+
+constexpr int64_t kForwardWorkgroups = 4096, kBackwardWorkgroups = 1024;
+
+}  // namespace
+
+extern "C" {
+
+int hstu_recurrent_residual_norm(const HstuResidualNormArgs* a, void* stream) {
+    hstu::ResidualNormParams p;
+    bool wide;
+    const int rc = fill_residual(a, p, wide);
+    if (rc) return rc;
+    if (a->rows == 0) return 0;
+    if (!a->out || (a->pre_weight && !a->normed)) return HSTU_ERR_NULL_POINTER;
+    if (!aligned_to(a->out, bytes_of(a->dtype)) || !aligned_to(a->normed, bytes_of(a->dtype))) return HSTU_ERR_MISALIGNED;
+    wide = wide && aligned_to(a->out, 16) && aligned_to(a->normed, 16);
+    if (!device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
+    p.out = (char*)a->out, p.normed = (char*)a->normed;
+    const int lanes = residual_lanes(a->width);
+    const unsigned blocks = (unsigned)residual_workgroups(a, kForwardWorkgroups);
+    return with_type(a->dtype, [&](auto* t) {
+        typedef std::remove_pointer_t<decltype(t)> T;
+        return with_row(lanes, wide, [&](auto l, auto w) {
+            constexpr int LPR = decltype(l)::value;
+            hipLaunchKernelGGL((hstu::hstu_residual_norm_kernel<T, LPR, decltype(w)::value>), dim3(blocks), dim3(LPR > 256 ? LPR : 256), 0, (hipStream_t)stream, p);
+            return launch_status("residual norm kernel launch");
+        });
+    });
+}
+
+size_t hstu_recurrent_residual_norm_bwd_workspace_bytes(const HstuResidualNormArgs* a) {
+    if (!a || a->rows <= 0 || a->width <= 0 || a->width > 8192) return 0;
+    return (size_t)residual_workgroups(a, kBackwardWorkgroups) * hstu::P_COUNT * a->width * sizeof(float);
+}
+
+int hstu_recurrent_residual_norm_bwd(const HstuResidualNormArgs* a, const HstuResidualNormGrads* g, void* stream) {
+    hstu::ResidualNormParams p;
+    bool wide;
+    const int rc = fill_residual(a, p, wide);
+    if (rc) return rc;
+    if (!g) return HSTU_ERR_NULL_POINTER;
+    if (g->d_out_row_stride < 0 || g->d_normed_row_stride < 0) return HSTU_ERR_BAD_SHAPE;
+    if (a->rows == 0) return HSTU_ERR_BAD_SHAPE;  // (the parameters' gradients would have to be cleared: the caller's to do)
+    const int es = bytes_of(a->dtype), per16 = 16 / es;
+    for (const void* ptr : {g->d_out, g->d_normed, (const void*)g->d_x, (const void*)g->d_y, (const void*)g->d_gate}) {
+        if (!aligned_to(ptr, es)) return HSTU_ERR_MISALIGNED;
+        wide = wide && aligned_to(ptr, 16);
+    }
+    wide = wide && g->d_out_row_stride % per16 == 0 && g->d_normed_row_stride % per16 == 0;
+    p.dout = (const char*)g->d_out, p.dout_rs = g->d_out_row_stride;
+    p.dnormed = a->pre_weight ? (const char*)g->d_normed : nullptr, p.dnormed_rs = g->d_normed_row_stride;
+    p.dx = (char*)g->d_x, p.dy = (char*)g->d_y, p.dgate = a->gate ? (char*)g->d_gate : nullptr;
+    void* to[hstu::P_COUNT] = {g->d_post_weight, g->d_post_bias, g->d_scale, g->d_pre_weight, g->d_pre_bias};
+    hstu::ParameterGrads grads{};
+    for (int k = 0; k < hstu::P_COUNT; ++k)
+        if (to[k] && p.param[k]) {
+            if (!aligned_to(to[k], es)) return HSTU_ERR_MISALIGNED;
+            p.wanted |= 1 << k, grads.out[k] = to[k];
+        }
+    if (p.wanted) {
+        if (!g->workspace) return HSTU_ERR_NULL_POINTER;
+        if (!aligned_to(g->workspace, 16)) return HSTU_ERR_MISALIGNED;
+        if (g->workspace_bytes < (int64_t)hstu_recurrent_residual_norm_bwd_workspace_bytes(a)) return HSTU_ERR_BAD_SHAPE;
+        p.partial = (float*)g->workspace;
+    }
+    if (!device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
+    const int lanes = residual_lanes(a->width);
+    const int64_t blocks = residual_workgroups(a, kBackwardWorkgroups);
+    return with_type(a->dtype, [&](auto* t) {
+        typedef std::remove_pointer_t<decltype(t)> T;
+        const int status = with_row(lanes, wide, [&](auto l, auto w) {
+            constexpr int LPR = decltype(l)::value;
+            hipLaunchKernelGGL((hstu::hstu_residual_norm_bwd_kernel<T, LPR, decltype(w)::value>), dim3((unsigned)blocks), dim3(LPR > 256 ? LPR : 256), 0, (hipStream_t)stream, p);
+            return launch_status("residual norm backward kernel launch");
+        });
+        if (status || !p.wanted) return status;
+        hipLaunchKernelGGL((hstu::hstu_residual_norm_sum_kernel<T>), dim3((a->width + 15) / 16, hstu::P_COUNT), dim3(256), 0, (hipStream_t)stream, p.partial, blocks,
+                           a->width, grads);
+        return launch_status("residual norm parameter gradient kernel launch");
+    });
+}
+
+}  // extern "C"

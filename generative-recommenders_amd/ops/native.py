@@ -8,7 +8,7 @@ import importlib.machinery
 import importlib.util
 import os
 
-from ..build import CACHE_LIB_PATH, LIB_PATH, LINEAR_LIB_PATH, NATIVE_PATH
+from ..build import CACHE_LIB_PATH, LIB_PATH, LINEAR_LIB_PATH, NATIVE_PATH, RECURRENT_LIB_PATH
 
 
 class _Unloaded:
@@ -16,7 +16,7 @@ class _Unloaded:
 
     def __getattr__(self, name):
         global front
-        for path in (NATIVE_PATH, LIB_PATH, LINEAR_LIB_PATH, CACHE_LIB_PATH):
+        for path in (NATIVE_PATH, LIB_PATH, LINEAR_LIB_PATH, CACHE_LIB_PATH, RECURRENT_LIB_PATH):
             if not os.path.exists(path):
                 raise RuntimeError(f"{path} is missing: build it with __graft_entry__.build().  There is no fallback.")
         loader = importlib.machinery.ExtensionFileLoader("hstu_native", NATIVE_PATH)
