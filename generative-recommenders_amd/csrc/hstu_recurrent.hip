@@ -76,6 +76,53 @@ hstu::ScanParams scan_params(const HstuRecurrenceArgs* a) {
     return p;
 }
 
+// Whether rows are read two columns at a time (in 16 bits).
+bool scan_in_pairs(const HstuRecurrenceArgs* a, const HstuRecurrenceGrads* g) {
+    if (a->dtype == HSTU_FP32 || a->width % 2 != 0) return false;
+    int64_t odd = a->x_row_stride | a->decay_gate_row_stride | a->input_gate_row_stride;
+    bool pairs = true;
+    for (const void* ptr : {a->x, a->decay_gate, a->input_gate, (const void*)(g ? nullptr : a->out)}) pairs = pairs && aligned_to(ptr, 4);
+    if (g) {
+        odd |= g->d_out ? g->d_out_row_stride : 0;
+        for (const void* ptr : {g->d_out, (const void*)g->d_x, (const void*)g->d_decay_gate, (const void*)g->d_input_gate}) pairs = pairs && aligned_to(ptr, 4);
+    }
+    return pairs && odd % 2 == 0;
+}
+
+constexpr int kRows = 16, kWaves = 8;           // of a tile of the forward
+constexpr int kBackRows = 8, kBackWaves = 8;    // ... and of the backward
+constexpr int kShortRows = 2, kShortWaves = 8;  // at a time, where sequences are short
+
+// Few rows to a sequence, and no state to save: a workgroup for each sequence.
+bool scan_is_short(const HstuRecurrenceArgs* a) { return !a->saved && a->rows <= 16 * (int64_t)a->batch + 48 && a->rows <= 4096 && a->batch < 65535; }
+
+int64_t scan_tiles(const HstuRecurrenceArgs* a, int rows_of_tile) { return (a->rows + rows_of_tile - 1) / rows_of_tile; }
+
+// Words that tiles leave for each other, 64 bits each, the ticket's included: one tile needs none.
+size_t scan_words(int64_t tiles, int width) { return tiles > 1 ? (size_t)(tiles + tiles / hstu::kGroup) * width + 2 : 0; }
+
+// Sets `p` for so many tiles: 0, or the status.
+int set_tiles(hstu::ScanParams& p, int64_t tiles, int cols, void* words) {
+    p.col_blocks = (p.width + cols - 1) / cols;
+    if (tiles > kMaxBlocks / p.col_blocks) return HSTU_ERR_UNSUPPORTED;
+    p.tiles = (int)tiles;
+    const size_t n = scan_words(tiles, p.width);
+    if (n) {
+        p.words = (unsigned long long*)words;
+        p.clear = (int64_t)n - 2;
+        p.ticket = (unsigned*)(p.words + p.clear);
+    }
+    return 0;
+}
+
+int launch_clear(const hstu::ScanParams& p, hipStream_t stream) {
+    const int64_t states = p.final_state ? (int64_t)p.batch * p.width : 0, most = p.clear > states ? p.clear : states;
+    if (most == 0) return 0;
+    const int64_t blocks = (most + 1023) / 1024;
+    hipLaunchKernelGGL(hstu::hstu_scan_clear_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, stream, p);
+    return launch_status("recurrence clearing kernel launch");
+}
+
 }  // namespace
 
 extern "C" {
@@ -83,26 +130,57 @@ extern "C" {
 int hstu_recurrent_version(void) { return 100; }
 const char* hstu_recurrent_last_error(void) { return g_last_error; }
 
-size_t hstu_recurrent_scan_workspace_bytes(const HstuRecurrenceArgs*) { return 0; }
-size_t hstu_recurrent_scan_saved_bytes(const HstuRecurrenceArgs*) { return 0; }
+size_t hstu_recurrent_scan_workspace_bytes(const HstuRecurrenceArgs* a) {
+    if (check_scan(a) || scan_is_short(a)) return 0;
+    return scan_words(scan_tiles(a, kRows * kWaves), a->width) * sizeof(unsigned long long);
+}
+
+size_t hstu_recurrent_scan_saved_bytes(const HstuRecurrenceArgs* a) {
+    if (check_scan(a)) return 0;
+    return (size_t)((a->rows + 63) / 64) * a->width * sizeof(float);
+}
 
 int hstu_recurrent_scan(const HstuRecurrenceArgs* a, void* stream) {
     const int rc = check_scan(a);
     if (rc) return rc;
     if (a->rows > 0 && !a->out) return HSTU_ERR_NULL_POINTER;
-    if (a->batch >= 65535) return HSTU_ERR_UNSUPPORTED;
-    if (!device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
     hstu::ScanParams p = scan_params(a);
-    p.out = (char*)a->out, p.final_state = a->final_state;
+    p.out = (char*)a->out, p.final_state = a->final_state, p.saved = a->saved;
+    if (scan_is_short(a)) {
+        if (!device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
+        return with_type(a->dtype, [&](auto* t) {
+            hipLaunchKernelGGL((hstu::hstu_scan_short_kernel<std::remove_pointer_t<decltype(t)>, kShortRows, kShortWaves>), dim3((a->width + 63) / 64, a->batch + 1),
+                               dim3(64 * kShortWaves), 0, (hipStream_t)stream, p);
+            return launch_status("recurrence kernel launch, short sequences");
+        });
+    }
+    const size_t need = hstu_recurrent_scan_workspace_bytes(a);
+    if (need && !a->workspace) return HSTU_ERR_NULL_POINTER;
+    if (!aligned_to(a->workspace, 16)) return HSTU_ERR_MISALIGNED;
+    if (a->workspace_bytes < (int64_t)need) return HSTU_ERR_BAD_SHAPE;
+    const bool pairs = scan_in_pairs(a, nullptr);
+    const int status = set_tiles(p, scan_tiles(a, kRows * kWaves), pairs ? 128 : 64, a->workspace);
+    if (status) return status;
+    if (!device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
+    const int cleared = launch_clear(p, (hipStream_t)stream);
+    if (cleared || a->rows == 0) return cleared;
     return with_type(a->dtype, [&](auto* t) {
-        hipLaunchKernelGGL((hstu::hstu_scan_kernel<std::remove_pointer_t<decltype(t)>>), dim3((a->width + 255) / 256, a->batch + 1), dim3(256), 0, (hipStream_t)stream, p);
-        return launch_status("recurrence kernel launch");
+        typedef std::remove_pointer_t<decltype(t)> T;
+        auto launch = [&](auto v) {
+            hipLaunchKernelGGL((hstu::hstu_scan_kernel<T, decltype(v)::value, kRows, kWaves>), dim3((unsigned)(p.tiles * p.col_blocks)), dim3(64 * kWaves), 0,
+                               (hipStream_t)stream, p);
+            return launch_status("recurrence kernel launch");
+        };
+        if constexpr (sizeof(T) == 2)
+            if (pairs) return launch(std::integral_constant<int, 2>{});
+        return launch(std::integral_constant<int, 1>{});
     });
 }
 
 size_t hstu_recurrent_scan_bwd_workspace_bytes(const HstuRecurrenceArgs* a) {
     if (check_scan(a)) return 0;
-    return (size_t)(a->rows + a->batch) * a->width * sizeof(float);
+    const int64_t tiles = scan_tiles(a, kBackRows * kBackWaves);
+    return scan_words(tiles, a->width) * sizeof(unsigned long long) + (size_t)tiles * a->width * sizeof(float);
 }
 
 int hstu_recurrent_scan_bwd(const HstuRecurrenceArgs* a, const HstuRecurrenceGrads* g, void* stream) {
@@ -110,25 +188,44 @@ int hstu_recurrent_scan_bwd(const HstuRecurrenceArgs* a, const HstuRecurrenceGra
     if (rc) return rc;
     if (!g) return HSTU_ERR_NULL_POINTER;
     if (g->d_out_row_stride < 0) return HSTU_ERR_BAD_SHAPE;
+    if (a->rows > 0 && (!a->saved || !g->workspace)) return HSTU_ERR_NULL_POINTER;
     const int es = bytes_of(a->dtype);
     for (const void* ptr : {g->d_out, (const void*)g->d_x, (const void*)g->d_decay_gate, (const void*)g->d_input_gate})
         if (!aligned_to(ptr, es)) return HSTU_ERR_MISALIGNED;
     if (!aligned_to(g->d_final_state, 4) || !aligned_to(g->d_initial_state, 4) || !aligned_to(g->d_decay, a->decay_f32 ? 4 : es) || !aligned_to(g->workspace, 16))
         return HSTU_ERR_MISALIGNED;
-    if (a->batch >= 65535) return HSTU_ERR_UNSUPPORTED;
-    if (!g->workspace) return HSTU_ERR_NULL_POINTER;
     if (g->workspace_bytes < (int64_t)hstu_recurrent_scan_bwd_workspace_bytes(a)) return HSTU_ERR_BAD_SHAPE;
-    if (!device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
     hstu::ScanParams p = scan_params(a);
+    p.saved = a->saved;
     p.dout = (const char*)g->d_out, p.dout_rs = g->d_out_row_stride, p.dfinal = g->d_final_state;
     p.dx = (char*)g->d_x, p.dr = (char*)g->d_decay_gate, p.di = (char*)g->d_input_gate, p.dinitial = g->d_initial_state;
-    p.states = (float*)g->workspace, p.partial = g->d_decay ? p.states + a->rows * a->width : nullptr;
+    const bool pairs = scan_in_pairs(a, g);
+    const int64_t tiles = scan_tiles(a, kBackRows * kBackWaves);
+    const int status = set_tiles(p, tiles, pairs ? 128 : 64, g->workspace);
+    if (status) return status;
+    if (g->d_decay) p.partial = (float*)((unsigned long long*)g->workspace + scan_words(tiles, a->width));
+    if (!device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
+    hstu::ScanParams clear = p;
+    clear.final_state = p.dinitial, clear.initial = p.dfinal;  // the gradient of a state that no row changes
+    const int cleared = launch_clear(clear, (hipStream_t)stream);
+    if (cleared) return cleared;
     return with_type(a->dtype, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
-        hipLaunchKernelGGL((hstu::hstu_scan_bwd_kernel<T>), dim3((a->width + 255) / 256, a->batch + 1), dim3(256), 0, (hipStream_t)stream, p);
-        const int status = launch_status("recurrence backward kernel launch");
-        if (status || !g->d_decay) return status;
-        hipLaunchKernelGGL((hstu::hstu_scan_decay_kernel<T>), dim3((a->width + 255) / 256), dim3(256), 0, (hipStream_t)stream, p.partial, a->batch, a->width, a->decay,
+        auto launch = [&](auto v) {
+            hipLaunchKernelGGL((hstu::hstu_scan_bwd_kernel<T, decltype(v)::value, kBackRows, kBackWaves>), dim3((unsigned)(p.tiles * p.col_blocks)),
+                               dim3(64 * kBackWaves), 0, (hipStream_t)stream, p);
+            return launch_status("recurrence backward kernel launch");
+        };
+        int rows = 0;
+        if (a->rows > 0) {
+            rows = [&] {
+                if constexpr (sizeof(T) == 2)
+                    if (pairs) return launch(std::integral_constant<int, 2>{});
+                return launch(std::integral_constant<int, 1>{});
+            }();
+        }
+        if (rows || !g->d_decay) return rows;
+        hipLaunchKernelGGL((hstu::hstu_scan_decay_kernel<T>), dim3((a->width + 15) / 16), dim3(256), 0, (hipStream_t)stream, p.partial, tiles, a->width, a->decay,
                            a->decay_f32, a->rate, g->d_decay);
         return launch_status("recurrence decay gradient kernel launch");
     });

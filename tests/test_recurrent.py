@@ -219,6 +219,16 @@ def test_scan_widths(pkg, dev, dtype, width):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("lengths", [[4700], [2047, 0, 2050, 3, 4500], [64] * 70, [5, 0, 9, 1, 0, 0, 2] * 300, [0] * 1500 + [3000] + [0] * 1500],
+                         ids=["one", "some", "whole-tiles", "many", "many-without-rows"])
+def test_scan_over_many_tiles(pkg, dev, dtype, lengths):
+    """Tiles that go back over groups of others, sequences that begin and end at their borders, more sequences than a workgroup has threads."""
+    case, dout, dfinal = scan_case(lengths, 6, dtype, seed=21, behind=200)
+    check_scan(pkg, dev, case, dout, dfinal)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF, FP, F32])
 def test_scan_reads_slices_in_place(pkg, dev, dtype):
     """Column slices of one buffer, odd distances between rows, addresses off every boundary, heads, rows that repeat, int32 offsets."""
@@ -307,6 +317,18 @@ def test_step(pkg, dev, dtype):
         within(here, put, put_err, "states")
         untouched = put_err.sum(1) == 0
         assert torch.equal(here.cpu()[untouched], held[untouched])
+
+
+@pytest.mark.gpu
+def test_results_are_the_same_from_call_to_call(pkg, dev):
+    """Whichever tile comes first, and whatever was in the scratch memory."""
+    case, dout, dfinal = scan_case([9000, 40, 3000], 256, BF, seed=22)
+    first = run_scan(pkg, dev, case, dout, dfinal)
+    for _ in range(5):
+        junk = torch.full((1 << 22,), 0x7FC00001, dtype=torch.int32, device=dev)
+        del junk
+        again = run_scan(pkg, dev, case, dout, dfinal)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1]) and all(torch.equal(first[2][k], again[2][k]) for k in first[2])
 
 
 @pytest.mark.gpu
