@@ -19,8 +19,8 @@ constexpr float kLog2e = 1.44269504088896340736f;
 
 __device__ __forceinline__ float sigmoid_of(float x) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * x)); }
 
-// log(1 + exp(d)), and its derivative.
-__device__ __forceinline__ float softplus_of(float d) { return fmaxf(d, 0.f) + log1pf(expf(-fabsf(d))); }
+// rate softplus(d) log2(e)
+__device__ __forceinline__ float strength_of(float d, float rate) { return rate * (fmaxf(d, 0.f) + log1pf(expf(-fabsf(d)))) * kLog2e; }
 
 // What a row's gates make of it.  1 - a and 1 - a^2 are wanted to their own last places: a is close to one in layers that remember, and what it
 // is off by counts once for each of the 1 / (1 - a) rows that h goes back over.  So for small z both come from the series of
@@ -30,21 +30,20 @@ template <class T>
 struct Gates {
     float s, a, m, si;
     __device__ __forceinline__ Gates() {}
+    // `strength` has the log2(e) in it, so that a = 2^-z; the series' terms have powers of log(2) for it.
     __device__ __forceinline__ Gates(float r, float i, float strength) {
+        constexpr float k1 = 0.69314718056f, k2 = -k1 * k1 / 2, k3 = k1 * k1 * k1 / 6, k4 = k2 * k2 / -6, k5 = k3 * k1 * k1 / 20, k6 = k3 * k3 / -20;
         s = sigmoid_of(r), si = sigmoid_of(i);
-        const float z = strength * s;
-        const float far = __builtin_amdgcn_exp2f(-kLog2e * z);
-        float series, e;
-        if constexpr (sizeof(T) == 4) {
-            series = __builtin_fmaf(z, -1.f / 720, 1.f / 120);
-            series = __builtin_fmaf(z, series, -1.f / 24);
-        } else {
-            series = -1.f / 24;
-        }
-        series = __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, series, 1.f / 6), -.5f), 1.f);
-        const bool near = z < (sizeof(T) == 4 ? .25f : .0625f);
-        e = near ? z * series : 1.f - far;
-        a = near ? 1.f - e : far;
+        const float z = strength * s, far = __builtin_amdgcn_exp2f(-z);
+        float series;
+        if constexpr (sizeof(T) == 4)
+            series = __builtin_fmaf(z, __builtin_fmaf(z, k6, k5), k4);
+        else
+            series = k4;
+        series = z * __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, series, k3), k2), k1);
+        const bool near = z < (sizeof(T) == 4 ? .25f : .0625f) * kLog2e;
+        const float e = near ? series : 1.f - far;
+        a = near ? 1.f - series : far;
         m = __builtin_amdgcn_sqrtf(e * (2.f - e));
     }
 };
@@ -53,6 +52,18 @@ template <class T>
 __device__ __forceinline__ float decay_at(const void* decay, int f32, int col) {
     return f32 ? ((const float*)decay)[col] : (float)((const T*)decay)[col];
 }
+
+// Tiles of kTile rows: whole sequences, one or more short ones, make a segment, and a segment's rows are cut into tiles from its first on.
+constexpr int kTile = 64;
+
+// A tile: where it is and which of its segment's it is.  The backward counts a segment's tiles from its last.
+struct Tile {
+    int64_t first;    // row
+    int64_t behind;   // the row behind its segment's last
+    int segment, at;  // -1: none
+    int slot;         // where its segment's places in the lists of words and saved states begin; its own are `at` further
+    int in_front;     // how many tiles of its segment lie in front of it (what the forward calls `at`)
+};
 
 struct ScanParams {
     const char *x, *r, *i;
@@ -67,18 +78,24 @@ struct ScanParams {
     int width;
     const float* initial;
     float* final_state;
-    float* saved;                // [rows / 64][width]: h in front of every 64th row
-    int tiles, col_blocks;
-    unsigned long long* words;   // [tiles][width], then [tiles / kGroup][width]: what tiles, and groups of them, make of h; 0: not there yet
-    unsigned* ticket;
-    int64_t clear;               // how many words, and the ticket behind them
+    float* saved;               // [slots][width]: h in front of each tile
+    int col_blocks;
+    // what the tiles share, in scratch memory
+    int segments, per_segment;  // sequences to a segment; rows behind the last sequence are one more
+    int slots;
+    Tile* tiles;                // [slots], in the order in which they are begun
+    float* strength;            // [width]: rate softplus(decay) log2(e)
+    unsigned long long *sums, *states, *groups;  // [slots][width], [slots][width], [slots / kGroup + 1][width]
+    unsigned* tickets;          // one for each block of columns, kTicketPitch apart, behind the words
+    int64_t clear;              // how many words to clear, the tickets' included
+    int backward;
     // backward
     const char* dout;
     int64_t dout_rs;
     const float* dfinal;
     char *dx, *dr, *di;
     float* dinitial;
-    float* partial;  // [tiles][width], or null
+    float* partial;  // [slots][width], or null
 };
 
 // V neighbouring columns of a row, four bytes at most.
@@ -110,29 +127,46 @@ struct Piece {
     }
 };
 
+// ROWS rows of a tensor from row w0 on, the last one in front of `behind` again where there are no more.  Row addresses are the wave's, not the
+// lane's (`off`: bytes).
+template <class T, int V, int ROWS>
+__device__ __forceinline__ void load_rows(Piece<T, V> (&to)[ROWS], const char* base, int64_t rs, int64_t w0, int64_t behind, unsigned off) {
+    const char* row = base + min(w0, behind - 1) * rs * (int64_t)sizeof(T);
+    const int left = (int)min(behind - w0, (int64_t)ROWS);
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) {
+        to[j].load((const T*)(row + off));
+        row += j + 1 < left ? rs * (int64_t)sizeof(T) : 0;
+    }
+}
+
 // Rows behind the last sequence, or 0.
 __device__ __forceinline__ int64_t rows_end(const ScanParams& p) {
     const int64_t end = index_at(p.offsets, p.offsets_i64, p.batch);
     return end < 0 ? 0 : end > p.rows ? p.rows : end;
 }
 
-// Where sequences begin and end in a tile of R rows.
-template <int R>
+// The same in all lanes, for the compiler to know.
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    return (int64_t)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)x));
+}
+
+// Where sequences begin and end in a tile.
 struct TileRows {
-    int begins[R], ends[R];  // the sequence whose first, whose last row it is, or -1
-    int64_t first, behind;   // first row of the sequence that the tile's first row is of; the row behind the one that its last row is of
+    int begins[kTile], ends[kTile];  // the sequence whose first, whose last row it is, or -1
     int low;
-    template <int THREADS>
     __device__ __forceinline__ void clear() {
-        for (int k = threadIdx.x; k < R; k += THREADS) begins[k] = ends[k] = -1;
-        if (threadIdx.x == 0) first = behind = -1, low = 0;
+        if (threadIdx.x < kTile) begins[threadIdx.x] = ends[threadIdx.x] = -1;
+        if (threadIdx.x == 0) low = 0;
     }
-    // After a barrier behind clear(); needs one behind it.  The sequences' offsets are narrowed down by THREADS at a time and then looked at side by
-    // side, from the one that row t0 is of to those that begin behind the tile.  Where offsets are not in order every index stays in bounds and every loop
-    // ends all the same.
+    // After a barrier behind clear(); needs one behind it.  The segment's sequences are narrowed down by THREADS at a time and then looked at side by
+    // side, from one that begins in front of the tile to those that begin behind it.  Where offsets are not in order every index stays in bounds and every
+    // loop ends all the same.
     template <int THREADS>
-    __device__ __forceinline__ void find(const ScanParams& p, int64_t t0, int64_t end) {
-        int lo = 0, hi = p.batch;
+    __device__ __forceinline__ void find(const ScanParams& p, const Tile& tile) {
+        const int64_t t0 = tile.first;
+        int lo = min(tile.segment * p.per_segment, p.batch), hi = min(lo + p.per_segment, p.batch);
+        const int last = hi;
         while (hi - lo >= THREADS) {
             const int step = (hi - lo + THREADS - 1) / THREADS, at = lo + (int)threadIdx.x * step;
             if (at <= hi && index_at(p.offsets, p.offsets_i64, at) <= t0) atomicMax(&low, at);
@@ -140,185 +174,326 @@ struct TileRows {
             lo = max(lo, low), hi = min(hi, lo + step);
             __syncthreads();
         }
-        for (int base = lo; base < p.batch; base += THREADS) {
+        for (int base = lo; base < last; base += THREADS) {
             const int b = base + threadIdx.x;
-            if (b < p.batch) {
-                const int64_t v = index_at(p.offsets, p.offsets_i64, b), e = min(index_at(p.offsets, p.offsets_i64, b + 1), end);
+            if (b < last) {
+                const int64_t v = index_at(p.offsets, p.offsets_i64, b), e = min(index_at(p.offsets, p.offsets_i64, b + 1), tile.behind);
                 if (e > v) {
-                    if (v >= t0 && v < t0 + R) begins[v - t0] = b;
-                    if (e > t0 && e <= t0 + R) ends[e - 1 - t0] = b;
-                    if (v <= t0 && e > t0) first = v;
-                    if (v < t0 + R && e >= t0 + R) behind = e;
+                    if (v >= t0 && v < t0 + kTile) begins[v - t0] = b;
+                    if (e > t0 && e <= t0 + kTile) ends[e - 1 - t0] = b;
                 }
             }
-            if (base + THREADS < p.batch && index_at(p.offsets, p.offsets_i64, base + THREADS) >= t0 + R) break;  // (the same for all)
+            if (base + THREADS < last && index_at(p.offsets, p.offsets_i64, base + THREADS) >= t0 + kTile) break;  // (the same for all)
         }
     }
 };
 
 // Bit k: whether rows[k] is a sequence's; the same in all lanes.
-template <int R>
-__device__ __forceinline__ void marks(const int (&rows)[R], uint64_t (&bits)[R / 64]) {
-#pragma unroll
-    for (int k = 0; k < R / 64; ++k) bits[k] = __ballot(rows[64 * k + (threadIdx.x & 63)] >= 0);
-}
-template <int ROWS, int N>
-__device__ __forceinline__ unsigned marks_of(const uint64_t (&bits)[N], int wave) {
-    const int at = wave * ROWS;
-    return (unsigned)(bits[at >> 6] >> (at & 63)) & ((1u << ROWS) - 1);
+__device__ __forceinline__ uint64_t marks(const int (&rows)[kTile]) { return __ballot(rows[threadIdx.x & 63] >= 0); }
+template <int ROWS>
+__device__ __forceinline__ unsigned marks_of(uint64_t bits, int wave) {
+    return (unsigned)(bits >> (wave * ROWS)) & ((1u << ROWS) - 1);
 }
 
 // ---- tiles joined along the rows ----
 //
-// What a run of rows makes of the h in front of it is A h + H.  Each tile works out its (A, H), puts them down as one word for each column, and takes
-// up those of the tiles in front of it, back to the first of its sequence.  A word is written and read as a whole, and is never 0 once written (A's sign bit
-// is set: A is not negative), so it needs no flag and no fence beside it.  Every kGroup-th tile also joins its group's words into one, so
-// that a tile of a long sequence takes up tiles / kGroup + 2 kGroup words and nothing waits for more than two others one behind another.  Tiles are
-// numbered by a ticket as workgroups begin: those in front have been begun and wait for no tile behind them, so each wait ends.  (The limit on it only
-// keeps a broken device from hanging.)  Which words are joined in which order goes by the tile's number and its sequence's first row alone.
-constexpr int kGroup = 16;
+// What a tile makes of the h in front of it is A h + H, or H alone where a sequence begins in it (it is cut off).  Each tile puts its (A, H) down as
+// one word for each column, and the h behind it, its state, as another once it knows it: state = A (state in front) + H.  A tile that finds no
+// state in front of it yet takes up (A, H)s back to one.  A word is written and read as a whole and is never 0 once written, so it needs no flag and no
+// fence beside it.
+//
+// Tiles are begun in the order of p.tiles, all segments' first ones in front of their second ones (64 segments at a time), by tickets that a
+// workgroup takes when it runs: those in front have been begun and wait for none behind them, so each wait ends.  (The limit on it only keeps a broken
+// device from hanging.)  With many segments the tile in front has nearly always been done; a single long one has hundreds of its tiles under way at
+// once, and for those every kGroup-th joins the (A, H) of its kGroup into one word, and its state is defined by that: A_group (state in front of the
+// group) + H_group.  So every state has one definition, and results do not depend on which tile was first.
+//
+// (Tiles of rows regardless of sequences, begun one after another and each taking up all (A, H) of its sequence in front of it, waited a third of the time:
+// five histories of up to 16000 rows, 1024 columns, 137 us; 98 without the waits.)
+// A block of columns has a ticket of its own: all workgroups at one counter were 18 ns each.
+constexpr int kGroup = 16, kGroupsBack = 8, kTicketPitch = 64;
+constexpr unsigned kCut = 0x7f800000u;  // A's bits where there is none
 
-__device__ __forceinline__ void put_word(unsigned long long* at, float A, float H) {
-    const unsigned long long w = (unsigned long long)__float_as_uint(H) << 32 | (__float_as_uint(A) | 0x80000000u);
+__device__ __forceinline__ void put_word(unsigned long long* at, float A, bool cut, float H) {
+    const unsigned long long w = (unsigned long long)__float_as_uint(H) << 32 | ((cut ? kCut : __float_as_uint(A)) | 0x80000000u);
     __hip_atomic_store(at, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+__device__ __forceinline__ unsigned long long get_word(const unsigned long long* at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float word_h(unsigned long long w) { return __uint_as_float((unsigned)(w >> 32)); }
+__device__ __forceinline__ float word_a(unsigned long long w) { return __uint_as_float((unsigned)w & 0x7fffffffu); }
+__device__ __forceinline__ bool word_cut(unsigned long long w) { return ((unsigned)w & 0x7fffffffu) == kCut; }
+// H behind what `w` says, from H in front of it.
+__device__ __forceinline__ float apply(unsigned long long w, float H) { return word_cut(w) ? word_h(w) : __builtin_fmaf(word_a(w), H, word_h(w)); }
 
-// Joins n words, word k at at(k), into (A, H): earlier ones are applied first.
-template <int V, class AT>
-__device__ __forceinline__ void join_words(int from, int to, AT&& at, float (&A)[V], float (&H)[V]) {
-    constexpr int AHEAD = 4;
+// V words, all lanes', when they are there; NaN if they never are.
+template <int V>
+__device__ __forceinline__ void await(const unsigned long long* at, unsigned long long (&w)[V]) {
+    for (int tries = 0; tries < (1 << 20); ++tries) {
+        bool there = true;
 #pragma unroll
-    for (int v = 0; v < V; ++v) A[v] = 1.f, H[v] = 0.f;
-    for (int k = from; k < to; k += AHEAD) {
-        unsigned long long w[AHEAD][V];
-        bool there = false;
-        for (int tries = 0; tries < (1 << 22) && !there; ++tries) {
-            if (tries) __builtin_amdgcn_s_sleep(1);
-            bool mine = true;
+        for (int v = 0; v < V; ++v) there = there && w[v] != 0;
+        if (__all(there)) return;
+        __builtin_amdgcn_s_sleep(1);
 #pragma unroll
-            for (int q = 0; q < AHEAD; ++q)
+        for (int v = 0; v < V; ++v) w[v] = get_word(at + v);
+    }
 #pragma unroll
-                for (int v = 0; v < V; ++v) w[q][v] = __hip_atomic_load(at(min(k + q, to - 1)) + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int v = 0; v < V; ++v) w[v] = 0x7fc00000ull << 32 | 0x80000000u | kCut;
+}
+
+// What the waves of a workgroup share while they go back.
+template <int V, int WAVES>
+struct Back {
+    unsigned long long sums[kGroup + kGroupsBack][64 * V];
+    float states[2 * WAVES][64 * V];
+    int found[2 * WAVES];  // 0 no, 1 cut off, 2 a state
+};
+
+// Goes back over `count` sums, two to a wave at a time: sum(i) is that of the i-th from here (from 1 on), state(i) the state in front of it
+// (in front of here for 0; NULL: there is none).  True: H is a state, or not needed, and the `n` sums from here to it, in back.sums[row + i - 1], go on from it.
+// `all`: takes every sum, and looks for no state.  Every thread of the workgroup calls.
+template <int V, int WAVES, class SUM, class STATE>
+__device__ __forceinline__ bool go_back(int count, bool all, int row, SUM&& sum, STATE&& state, Back<V, WAVES>& back, int wave, int& n, float (&H)[V]) {
+    const int lane = threadIdx.x & 63;
+    for (int from = 0; from <= count; from += 2 * WAVES) {
+        unsigned long long s[2][V], t[2][V];
 #pragma unroll
-            for (int q = 0; q < AHEAD; ++q)
+        for (int q = 0; q < 2; ++q) {
+            const int i = min(from + 2 * wave + q, count);
+            const unsigned long long* front = all ? nullptr : state(i);
 #pragma unroll
-                for (int v = 0; v < V; ++v) mine = mine && w[q][v] != 0;
-            there = __all(mine);
+            for (int v = 0; v < V; ++v) s[q][v] = i ? get_word(sum(i) + v) : 1, t[q][v] = front ? get_word(front + v) : 0;
         }
 #pragma unroll
-        for (int q = 0; q < AHEAD; ++q) {
-            if (k + q >= to) break;  // (the same for the wave)
+        for (int q = 0; q < 2; ++q) {
+            const int i = from + 2 * wave + q;
+            if (i > count) continue;  // (the same for the wave)
+            bool cut = i > 0, known = true;
+            if (i) await<V>(sum(i), s[q]);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const float a = __uint_as_float((unsigned)w[q][v] & 0x7fffffffu), h = there ? __uint_as_float((unsigned)(w[q][v] >> 32)) : __builtin_nanf("");
-                H[v] = k + q == from ? h : __builtin_fmaf(a, H[v], h);
-                A[v] = k + q == from ? a : a * A[v];
+                if (i) back.sums[row + i - 1][lane * V + v] = s[q][v], cut = cut && word_cut(s[q][v]);
+                known = known && t[q][v] != 0;
+                back.states[2 * wave + q][lane * V + v] = word_h(t[q][v]);
             }
+            const int found = __all(known) ? 2 : __all(cut) ? 1 : 0;
+            if (lane == 0) back.found[2 * wave + q] = found;
         }
+        __syncthreads();
+        for (int k = 0; k < 2 * WAVES && from + k <= count && !all; ++k) {
+            const int found = back.found[k];  // (the same for all)
+            if (!found) continue;
+            n = from + k;
+#pragma unroll
+            for (int v = 0; v < V; ++v) H[v] = found == 2 ? back.states[k][lane * V + v] : 0.f;
+            return true;
+        }
+        __syncthreads();
     }
+    n = count;
+    return false;
 }
 
-// The waves of a workgroup join n words: each a part of them, in LDS the parts.  Every thread of the workgroup calls; `meet` is free before and after.
-template <int V, int WAVES, class AT>
-__device__ __forceinline__ void join_together(int n, AT&& at, float2 (*meet)[64 * V], int wave, float (&A)[V], float (&H)[V]) {
-    const int lane = threadIdx.x & 63, per = (n + WAVES - 1) / WAVES, from = min(wave * per, n), to = min(from + per, n);
-    if (from < to) {
-        join_words<V>(from, to, at, A, H);
-#pragma unroll
-        for (int v = 0; v < V; ++v) meet[wave][lane * V + v] = float2{A[v], H[v]};
-    }
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < V; ++v) A[v] = 1.f, H[v] = 0.f;
-    for (int w = 0; w * per < n; ++w)
+// H in front of tile `at` of a segment whose words begin at `slot`; and where the tile is the last of a group and not cut off (`closes`), what the tiles in
+// front of it in its group make of h, (A, G) or G alone (`off`), and in `base` the h in front of the group.  Every thread of the workgroup calls.
+template <int V, int WAVES>
+__device__ __forceinline__ void look_back(const ScanParams& p, int slot, int at, int col, bool closes, Back<V, WAVES>& back, int wave, float (&H)[V], float (&A)[V],
+                                          float (&G)[V], bool& off, float (&base)[V]) {
+    const int lane = threadIdx.x & 63, lo = at / kGroup * kGroup, group = at / kGroup;
+    const int64_t width = p.width;
+    auto sum_of = [&](int i) { return p.sums + (slot + at - i) * width + col; };
+    auto state_of = [&](int tile) { return tile < 0 ? nullptr : p.states + (slot + tile) * width + col; };
+    int n;
+    bool known = go_back<V, WAVES>(at - lo, closes, 0, sum_of, [&](int i) { return state_of(at - i - 1); }, back, wave, n, H);
+    off = false;
+    if (closes) {
+        for (int k = 0; k < n; ++k) off = off || word_cut(back.sums[k][0]);  // (the same in all columns)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const float2 s = meet[w][lane * V + v];
-            H[v] = w ? __builtin_fmaf(s.x, H[v], s.y) : s.y;
-            A[v] = w ? s.x * A[v] : s.x;
+            A[v] = 1.f, G[v] = H[v] = 0.f;
+            for (int k = n - 1; k >= 0; --k) {
+                const unsigned long long w = back.sums[k][lane * V + v];
+                G[v] = apply(w, G[v]), A[v] *= word_a(w);
+            }
         }
+        known = off;
+    }
+    if (!known) {  // the state behind the group in front (there is one: a segment's first tile is cut off)
+        // (a segment's groups end kGroup slots from each other, and no nearer to those of the segments beside it)
+        auto group_of = [&](int i) { return p.groups + (slot + (group - i) * kGroup + kGroup - 1) / kGroup * width + col; };
+        const int count = min(group, kGroupsBack);
+        int m;
+        if (!go_back<V, WAVES>(count, false, kGroup, group_of, [&](int i) { return state_of((group - i) * kGroup - 1); }, back, wave, m, H)) {
+            const unsigned long long* far = state_of((group - count) * kGroup - 1);
+            unsigned long long w[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) w[v] = get_word(far + v);
+            await<V>(far, w);
+#pragma unroll
+            for (int v = 0; v < V; ++v) H[v] = word_h(w[v]);
+        }
+        for (int k = m - 1; k >= 0; --k)
+#pragma unroll
+            for (int v = 0; v < V; ++v) H[v] = apply(back.sums[kGroup + k][lane * V + v], H[v]);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) base[v] = H[v];
+    for (int k = n - 1; k >= 0; --k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) H[v] = apply(back.sums[k][lane * V + v], H[v]);
+}
+
+// What a tile has to do with the others.  `me`: the wave that has its (A, H), which it puts down; `front`: the h in front of the tile, where it `needs` it.
+// Every thread of the workgroup calls.
+template <int V, int WAVES>
+__device__ __forceinline__ void join_tile(const ScanParams& p, int slot, int at, int col, bool mine, bool me, bool cut, bool needs, const float (&A)[V],
+                                          const float (&H)[V], Back<V, WAVES>& back, int wave, float (&front)[V]) {
+    const bool closes = at % kGroup == kGroup - 1;
+    const int64_t word = (int64_t)(slot + at) * p.width + col;
+    unsigned long long* group = p.groups + (int64_t)((slot + at) / kGroup) * p.width + col;
+    if (me && mine)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            put_word(p.sums + word + v, A[v], cut, H[v]);
+            if (cut) put_word(p.states + word + v, 0.f, true, H[v]);
+            if (cut && closes) put_word(group + v, 0.f, true, H[v]);
+        }
+    if (!needs) return;  // (needs, where it is not cut off)
+    float by[V], G[V], base[V];
+    bool off;
+    look_back<V, WAVES>(p, slot, at, col, closes && !cut, back, wave, front, by, G, off, base);
+    if (!me || !mine || cut) return;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        float state = __builtin_fmaf(A[v], front[v], H[v]);
+        if (closes) {
+            by[v] *= A[v], G[v] = __builtin_fmaf(A[v], G[v], H[v]);
+            put_word(group + v, by[v], off, G[v]);
+            state = off ? G[v] : __builtin_fmaf(by[v], base[v], G[v]);
+        }
+        put_word(p.states + word + v, 0.f, true, state);
+    }
+}
+
+// Which block of columns a workgroup takes: each as often as there are tiles, and each of the eight dies, which workgroups go to in turn, all of them
+// in turn (1024 columns, one die always at the same 256 bytes of a row: 1261 us where others take 1105).
+__device__ __forceinline__ int column_block(const ScanParams& p) { return (int)((blockIdx.x + blockIdx.x / p.col_blocks) % p.col_blocks); }
+
+// The tile that a workgroup takes up, to LDS: one thread's work, with a barrier behind it.
+__device__ __forceinline__ void take_tile(const ScanParams& p, int block, Tile& tile) { tile = p.tiles[atomicAdd(p.tickets + block * kTicketPitch, 1u)]; }
+
+// The list of 64 segments' tiles, by workgroups that share its entries out.  Segment s has the rows from F(s) up to F(s + 1): F(0) is 0, F(s) where its
+// first sequence begins, or where any in front of it does if offsets are not in order; its slots begin at F(s) / kTile + s, so that nobody has to count
+// the tiles in front.  Tile k of segment s comes behind all with a lower k and those of the segments in front with the same: its place is the sum of
+// min(tiles, k + 1) over the segments in front and of min(tiles, k) over the others.
+struct PlanPart {
+    int tiles[64], before[64], slot[64];  // before: tiles of the segments in front
+    int64_t first[64], behind[64];
+};
+__device__ __forceinline__ void plan_tiles(const ScanParams& p, int batch, int part, int parts, PlanPart& plan) {
+    const int lane = threadIdx.x & 63, s0 = 64 * batch, s = s0 + lane;
+    auto bound = [&](int64_t segment) {
+        if (segment > p.segments) return p.rows;
+        if (segment == 0) return (int64_t)0;
+        const int64_t at = index_at(p.offsets, p.offsets_i64, min(segment * p.per_segment, (int64_t)p.batch));
+        return at < 0 ? (int64_t)0 : at > p.rows ? p.rows : at;
+    };
+    if (threadIdx.x < 64) {
+        int64_t first = bound(s), behind = bound(s0 + 64), top = 0;
+#pragma unroll 4
+        for (int k = lane; k < s0; k += 64) top = max(top, bound(k));
+        if (s0)
+            for (int d = 32; d; d >>= 1) top = max(top, (int64_t)__shfl_xor((long long)top, d, 64));
+        first = max(first, top);
+        for (int d = 1; d < 64; d <<= 1) {
+            const int64_t other = __shfl_up((long long)first, d, 64);
+            if (lane >= d) first = max(first, other);
+        }
+        const int64_t next = __shfl_down((long long)first, 1, 64);
+        behind = lane == 63 ? max(first, behind) : next;
+        const int tiles = s <= p.segments ? (int)((behind - first + kTile - 1) / kTile) : 0;
+        int upto = tiles;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int other = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += other;
+        }
+        plan.tiles[lane] = tiles, plan.before[lane] = upto - tiles, plan.slot[lane] = (int)(first / kTile) + s;
+        plan.first[lane] = first, plan.behind[lane] = behind;
+    }
     __syncthreads();
+    const int base = plan.slot[0], total = plan.before[63] + plan.tiles[63];
+    const int end = s0 + 64 <= p.segments ? (int)(plan.behind[63] / kTile) + s0 + 64 : p.slots;
+    for (int e = part * 256 + (int)threadIdx.x; e < end - base; e += parts * 256) {
+        Tile t{};
+        int at = e;
+        t.at = -1;  // a slot without a tile
+        if (e < total) {
+            int of = 0;  // the last segment with before <= e that has tiles: e is one of its
+            for (int d = 32; d; d >>= 1)
+                if (plan.before[of + d] <= e) of += d;
+            const int k = e - plan.before[of];
+            at = 0;
+            for (int q = 0; q < 64; ++q) at += min(plan.tiles[q], k + (q < of ? 1 : 0));
+            t.segment = s0 + of, t.at = k, t.slot = plan.slot[of], t.in_front = p.backward ? plan.tiles[of] - 1 - k : k;
+            t.first = plan.first[of] + (int64_t)kTile * t.in_front, t.behind = plan.behind[of];
+        }
+        p.tiles[base + at] = t;
+    }
 }
 
-// Takes up what the tiles from `from` up to `tile` make of a column's h.
-template <int V, int WAVES>
-__device__ __forceinline__ void join_tiles(const ScanParams& p, int from, int tile, int col, float2 (*meet)[64 * V], int wave, float (&H)[V]) {
-    const unsigned long long* words = p.words + col;
-    const unsigned long long* groups = words + (int64_t)p.tiles * p.width;
-    const int group = tile / kGroup, whole = (from + kGroup - 1) / kGroup;  // groups [whole, group) lie behind `from`
-    const int singles = whole < group ? whole * kGroup - from : tile - from, joined = whole < group ? group - whole : 0;
-    const int n = singles + joined + (whole < group ? tile - group * kGroup : 0);
-    float A[V];
-    join_together<V, WAVES>(
-        n,
-        [&](int k) {
-            const unsigned long long* base = k >= singles && k < singles + joined ? groups : words;
-            const int64_t at = k < singles ? from + k : k < singles + joined ? whole + k - singles : group * kGroup + k - singles - joined;
-            return base + at * p.width;
-        },
-        meet, wave, A, H);
-}
-
-// A tile's own (A, H), by its last wave to come, and its group's by the last tile of one.  Every thread calls; `meet` is free before and after.
-template <int V, int WAVES>
-__device__ __forceinline__ void put_tile(const ScanParams& p, int tile, int col, bool mine, bool me, const float (&A)[V], const float (&H)[V], float2 (*meet)[64 * V],
-                                         int wave) {
-    if (me && mine)
-#pragma unroll
-        for (int v = 0; v < V; ++v) put_word(p.words + (int64_t)tile * p.width + col + v, A[v], H[v]);
-    if (tile % kGroup != kGroup - 1) return;
-    float a[V], h[V];
-    const unsigned long long* first = p.words + (int64_t)(tile - (kGroup - 1)) * p.width + col;
-    join_together<V, WAVES>(kGroup - 1, [&](int k) { return first + (int64_t)k * p.width; }, meet, wave, a, h);
-    if (me && mine)
-#pragma unroll
-        for (int v = 0; v < V; ++v) put_word(p.words + (int64_t)(p.tiles + tile / kGroup) * p.width + col + v, A[v] * a[v], __builtin_fmaf(A[v], h[v], H[v]));
-}
-
-// No word is there yet; states of sequences without rows are what they were.
-__global__ __launch_bounds__(256) void hstu_scan_clear_kernel(const ScanParams p) {
+// What the tiles find: their list, no words yet, columns' strengths, and the states of sequences without rows as they were.
+template <class T>
+__global__ __launch_bounds__(256) void hstu_scan_begin_kernel(const ScanParams p) {
+    __shared__ PlanPart plan;
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
-    for (int64_t k = at; k < p.clear; k += step) p.words[k] = 0;
-    if (at == 0 && p.ticket) *p.ticket = 0;
+    typedef __attribute__((ext_vector_type(4))) unsigned u4;
+    for (int64_t k = 2 * at; k < p.clear; k += 2 * step) *(u4*)(p.sums + k) = u4{0, 0, 0, 0};  // (an even number of words)
+    for (int64_t k = at; k < p.width; k += step) p.strength[k] = strength_of(decay_at<T>(p.decay, p.decay_f32, k), p.rate);
+    if (p.partial)  // (there are slots without a tile)
+        for (int64_t k = at; k < (int64_t)p.slots * p.width; k += step) p.partial[k] = 0.f;
     if (p.final_state)
         for (int64_t k = at; k < (int64_t)p.batch * p.width; k += step) p.final_state[k] = p.initial ? p.initial[k] : 0.f;
+    const int batches = p.segments / 64 + 1, parts = min(max((int)gridDim.x / batches, 1), 16);
+    for (int q = blockIdx.x; q < batches * parts; q += gridDim.x) {
+        if (q != (int)blockIdx.x) __syncthreads();
+        plan_tiles(p, q % batches, q / batches, parts, plan);
+    }
 }
 
 template <class T, int V, int ROWS, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 4) void hstu_scan_kernel(const ScanParams p) {
-    constexpr int R = ROWS * WAVES, COLS = 64 * V;
-    __shared__ TileRows<R> map;
-    __shared__ float2 sums[WAVES][COLS], meet[WAVES][COLS];
-    __shared__ unsigned number;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    map.template clear<64 * WAVES>();
-    if (threadIdx.x == 0) number = p.words ? atomicAdd(p.ticket, 1u) : blockIdx.x;
+    constexpr int COLS = 64 * V;
+    static_assert(ROWS * WAVES == kTile, "a row for each");
+    __shared__ TileRows map;
+    __shared__ float2 sums[WAVES][COLS];
+    __shared__ Back<V, WAVES> back;
+    __shared__ Tile taken;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, block = column_block(p);
+    map.clear();
+    if (threadIdx.x == 0) take_tile(p, block, taken);
     __syncthreads();
-    const int n = __builtin_amdgcn_readfirstlane(number), tile = n / p.col_blocks, col0 = (n % p.col_blocks) * COLS + lane * V, col = min(col0, p.width - V);
+    const int at = __builtin_amdgcn_readfirstlane(taken.at), slot = __builtin_amdgcn_readfirstlane(taken.slot);
+    if (at < 0) return;
+    const int64_t t0 = uniform(taken.first), behind = uniform(taken.behind), w0 = t0 + wave * ROWS, pitch = p.width * (int64_t)sizeof(T);
+    const int col0 = block * COLS + lane * V, col = min(col0, p.width - V);
     const bool mine = col0 < p.width;
-    const int64_t t0 = (int64_t)tile * R, w0 = t0 + wave * ROWS, end = rows_end(p);
-    T* out = (T*)p.out + w0 * p.width + col;
-    if (t0 >= end) {  // rows behind the last sequence (no tile in front of it waits for this one)
-#pragma unroll
-        for (int j = 0; j < ROWS; ++j)
-            if (mine && w0 + j < p.rows) {
-                const float zero[V] = {};
-                Piece<T, V>::put(zero, out + (int64_t)j * p.width);
-            }
+    const unsigned off = col * (unsigned)sizeof(T);
+    char* out = p.out + w0 * pitch;
+    if (__builtin_amdgcn_readfirstlane(taken.segment) == p.segments) {  // rows behind the last sequence
+        for (int j = 0; j < ROWS && w0 + j < behind; ++j, out += pitch) {
+            const float zero[V] = {};
+            if (mine) Piece<T, V>::put(zero, (T*)(out + off));
+        }
         return;
     }
     Piece<T, V> x[ROWS], r[ROWS], i[ROWS];
-#pragma unroll
-    for (int j = 0; j < ROWS; ++j) {
-        const int64_t row = min(w0 + j, p.rows - 1);
-        x[j].load((const T*)p.x + row * p.x_rs + col);
-        r[j].load((const T*)p.r + row * p.r_rs + col);
-        i[j].load((const T*)p.i + row * p.i_rs + col);
-    }
+    load_rows<T, V, ROWS>(r, p.r, p.r_rs, w0, behind, off);
+    load_rows<T, V, ROWS>(i, p.i, p.i_rs, w0, behind, off);
+    load_rows<T, V, ROWS>(x, p.x, p.x_rs, w0, behind, off);
     float strength[V], a[ROWS][V], b[ROWS][V], A[V], H[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) strength[v] = p.rate * softplus_of(decay_at<T>(p.decay, p.decay_f32, col + v)), A[v] = 1.f, H[v] = 0.f;
-    map.template find<64 * WAVES>(p, t0, end);
+    for (int v = 0; v < V; ++v) strength[v] = p.strength[col + v], A[v] = 1.f, H[v] = 0.f;
+    map.template find<64 * WAVES>(p, taken);
 #pragma unroll
     for (int j = 0; j < ROWS; ++j)
 #pragma unroll
@@ -327,9 +502,8 @@ __global__ __launch_bounds__(64 * WAVES, 4) void hstu_scan_kernel(const ScanPara
             a[j][v] = g.a, b[j][v] = g.m * g.si * x[j].get(v);
         }
     __syncthreads();
-    uint64_t bits[R / 64];
-    marks(map.begins, bits);
-    const unsigned begins = marks_of<ROWS>(bits, wave);
+    const uint64_t bits = marks(map.begins);
+    const unsigned begins = marks_of<ROWS>(bits, wave), ends = marks_of<ROWS>(marks(map.ends), wave);
     if (begins && p.initial)
 #pragma unroll
         for (int j = 0; j < ROWS; ++j)
@@ -362,109 +536,106 @@ __global__ __launch_bounds__(64 * WAVES, 4) void hstu_scan_kernel(const ScanPara
     bool cut = false;    // whether a sequence begins in one of them
 #pragma unroll
     for (int v = 0; v < V; ++v) fA[v] = 1.f, fH[v] = 0.f;
-#pragma unroll
-    for (int w = 0; w < WAVES - 1; ++w) {
-        if (w >= wave) break;
+#pragma unroll 1  // (all parts at once would take the registers of the rows)
+    for (int w = 0; w < wave; ++w) {
         const bool begun = marks_of<ROWS>(bits, w) != 0;
         cut = cut || begun;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const float2 s = sums[w][lane * V + v];
             fH[v] = begun ? s.y : __builtin_fmaf(s.x, fH[v], s.y);
-            fA[v] = begun ? 0.f : s.x * fA[v];
+            fA[v] = s.x * fA[v];
         }
     }
-    if (p.words) {
+    const bool needs = at > 0 && !(bits & 1);
+    float front[V] = {};
 #pragma unroll
-        for (int v = 0; v < V; ++v) H[v] = begins ? H[v] : __builtin_fmaf(A[v], fH[v], H[v]), A[v] = begins ? 0.f : A[v] * fA[v];
-        put_tile<V, WAVES>(p, tile, col, mine, wave == WAVES - 1, A, H, meet, wave);
-        const int64_t first = map.first < 0 ? 0 : map.first;
-        if (first < t0) {
-            join_tiles<V, WAVES>(p, (int)(first / R), tile, col, meet, wave, H);
+    for (int v = 0; v < V; ++v) H[v] = begins ? H[v] : __builtin_fmaf(A[v], fH[v], H[v]), A[v] *= fA[v];
+    join_tile<V, WAVES>(p, slot, at, col, mine, wave == WAVES - 1, at == 0 || bits, needs, A, H, back, wave, front);
+    if (p.saved && wave == 0 && mine)
 #pragma unroll
-            for (int v = 0; v < V; ++v) fH[v] = cut ? fH[v] : __builtin_fmaf(fA[v], H[v], fH[v]);
-        }
-    }
+        for (int v = 0; v < V; ++v) p.saved[(int64_t)(slot + at) * p.width + col + v] = front[v];
+    if (needs)
+#pragma unroll
+        for (int v = 0; v < V; ++v) fH[v] = cut ? fH[v] : __builtin_fmaf(fA[v], front[v], fH[v]);
 #pragma unroll
     for (int v = 0; v < V; ++v) H[v] = fH[v];
-    if (p.saved && w0 % 64 == 0 && w0 < p.rows && mine)
+    if (!begins && !(ends && p.final_state) && w0 + ROWS <= behind) {
+        if (mine)
+            rows(std::false_type{}, [&](int) {
+                Piece<T, V>::put(H, (T*)(out + off));
+                out += pitch;
+            });
+        return;
+    }
+    rows(std::true_type{}, [&](int j) {
+        if (w0 + j < behind && mine) {
+            Piece<T, V>::put(H, (T*)(out + off));
+            if (p.final_state && ends >> j & 1)
 #pragma unroll
-        for (int v = 0; v < V; ++v) p.saved[w0 / 64 * p.width + col + v] = H[v];
-    auto store = [&](int j) {
-        if (w0 + j < p.rows && mine) {
-            float h[V];
-#pragma unroll
-            for (int v = 0; v < V; ++v) h[v] = w0 + j < end ? H[v] : 0.f;
-            Piece<T, V>::put(h, out + (int64_t)j * p.width);
-            const int b = p.final_state ? map.ends[wave * ROWS + j] : -1;
-            if (b >= 0)
-#pragma unroll
-                for (int v = 0; v < V; ++v) p.final_state[(int64_t)b * p.width + col + v] = H[v];
+                for (int v = 0; v < V; ++v) p.final_state[(int64_t)map.ends[wave * ROWS + j] * p.width + col + v] = H[v];
         }
-    };
-    if (begins)
-        rows(std::true_type{}, store);
-    else
-        rows(std::false_type{}, store);
+        out += pitch;
+    });
 }
 
 // The same from the last row to the first: G is to dh what h is to b, with a row's a on the way to the row in front of it.  h in front of each row is
 // worked out again from the state that the forward saved for the tile.  c = a G is what a row passes on.
 template <class T, int V, int ROWS, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 4) void hstu_scan_bwd_kernel(const ScanParams p) {
-    constexpr int R = ROWS * WAVES, COLS = 64 * V;
-    static_assert(R == 64, "the forward saves h in front of every 64th row");
-    __shared__ TileRows<R> map;
-    __shared__ float2 sums[WAVES][COLS], meet[WAVES][COLS];
-    __shared__ float back[WAVES][COLS];
-    __shared__ unsigned number;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    map.template clear<64 * WAVES>();
-    if (threadIdx.x == 0) number = p.words ? atomicAdd(p.ticket, 1u) : blockIdx.x;
+    constexpr int COLS = 64 * V;
+    static_assert(ROWS * WAVES == kTile, "a row for each");
+    __shared__ TileRows map;
+    __shared__ float2 sums[WAVES][COLS];
+    __shared__ float passed[WAVES][COLS];
+    __shared__ Back<V, WAVES> back;
+    __shared__ Tile taken;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, block = column_block(p);
+    map.clear();
+    if (threadIdx.x == 0) take_tile(p, block, taken);
     __syncthreads();
-    const int n = __builtin_amdgcn_readfirstlane(number), turned = n / p.col_blocks, tile = p.tiles - 1 - turned;
-    const int col0 = (n % p.col_blocks) * COLS + lane * V, col = min(col0, p.width - V);
+    const int turned = __builtin_amdgcn_readfirstlane(taken.at), slot = __builtin_amdgcn_readfirstlane(taken.slot);
+    if (turned < 0) return;
+    const int64_t t0 = uniform(taken.first), behind = uniform(taken.behind), w0 = t0 + wave * ROWS, pitch = p.width * (int64_t)sizeof(T);
+    const int64_t same = slot + __builtin_amdgcn_readfirstlane(taken.in_front);  // the slot that the forward had for this tile
+    const int col0 = block * COLS + lane * V, col = min(col0, p.width - V);
     const bool mine = col0 < p.width;
-    const int64_t t0 = (int64_t)tile * R, w0 = t0 + wave * ROWS, end = rows_end(p), out0 = w0 * p.width + col;
-    auto put = [&](char* to, int j, const float (&d)[V]) {
-        if (to) Piece<T, V>::put(d, (T*)to + out0 + (int64_t)j * p.width);
-    };
-    if (t0 >= end) {
+    const unsigned off = col * (unsigned)sizeof(T);
+    int64_t at = w0 * pitch;  // of a row of the results
+    auto put = [&](char* to, const float (&d)[V]) { Piece<T, V>::put(d, (T*)(to + at + off)); };
+    if (__builtin_amdgcn_readfirstlane(taken.segment) == p.segments) {  // rows behind the last sequence
         const float zero[V] = {};
-#pragma unroll
-        for (int j = 0; j < ROWS; ++j)
-            if (mine && w0 + j < p.rows) put(p.dx, j, zero), put(p.dr, j, zero), put(p.di, j, zero);
-        if (p.partial && wave == 0 && mine)
-#pragma unroll
-            for (int v = 0; v < V; ++v) p.partial[(int64_t)tile * p.width + col + v] = 0.f;
+        for (int j = 0; j < ROWS && w0 + j < behind; ++j, at += pitch)
+            if (mine) {
+                if (p.dx) put(p.dx, zero);
+                if (p.dr) put(p.dr, zero);
+                if (p.di) put(p.di, zero);
+            }
         return;
     }
     Piece<T, V> x[ROWS], r[ROWS], i[ROWS], d[ROWS];
+    load_rows<T, V, ROWS>(r, p.r, p.r_rs, w0, behind, off);
+    load_rows<T, V, ROWS>(i, p.i, p.i_rs, w0, behind, off);
+    load_rows<T, V, ROWS>(x, p.x, p.x_rs, w0, behind, off);
+    if (p.dout)
+        load_rows<T, V, ROWS>(d, p.dout, p.dout_rs, w0, behind, off);
+    else
 #pragma unroll
-    for (int j = 0; j < ROWS; ++j) {
-        const int64_t row = min(w0 + j, p.rows - 1);
-        x[j].load((const T*)p.x + row * p.x_rs + col);
-        r[j].load((const T*)p.r + row * p.r_rs + col);
-        i[j].load((const T*)p.i + row * p.i_rs + col);
-        d[j].w = 0;
-        if (p.dout) d[j].load((const T*)p.dout + row * p.dout_rs + col);
-    }
+        for (int j = 0; j < ROWS; ++j) d[j].w = 0;
     float strength[V], h[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) strength[v] = p.rate * softplus_of(decay_at<T>(p.decay, p.decay_f32, col + v)), h[v] = p.saved[(int64_t)tile * p.width + col + v];
-    map.template find<64 * WAVES>(p, t0, end);
+    for (int v = 0; v < V; ++v) strength[v] = p.strength[col + v], h[v] = p.saved[same * p.width + col + v];
+    map.template find<64 * WAVES>(p, taken);
     Gates<T> g[ROWS][V];
 #pragma unroll
     for (int j = 0; j < ROWS; ++j)
 #pragma unroll
         for (int v = 0; v < V; ++v) g[j][v] = Gates<T>(r[j].get(v), i[j].get(v), strength[v]);
     __syncthreads();
-    uint64_t bits[1], end_bits[1];
-    marks(map.begins, bits);
-    marks(map.ends, end_bits);
+    const uint64_t bits = marks(map.begins), end_bits = marks(map.ends);
     const unsigned begins = marks_of<ROWS>(bits, wave), ends = marks_of<ROWS>(end_bits, wave);
     // Waves whose rows all lie within one sequence have nothing to ask at each.
-    const bool plain = !begins && !ends && w0 + ROWS <= end;
+    const bool plain = !begins && !ends && w0 + ROWS <= behind && p.dx && p.dr && p.di;
     auto either = [&](auto&& pass) {
         if (plain)
             pass(std::true_type{});
@@ -475,12 +646,12 @@ __global__ __launch_bounds__(64 * WAVES, 4) void hstu_scan_bwd_kernel(const Scan
         if (decltype(all)::value || !(begins >> j & 1)) return now;
         return p.initial ? p.initial[(int64_t)map.begins[wave * ROWS + j] * p.width + col + v] : 0.f;
     };
-    auto behind = [&](auto all, int j, float now) { return decltype(all)::value || !(ends >> j & 1) ? now : 0.f; };  // c from behind row j
+    auto from_behind = [&](auto all, int j, float now) { return decltype(all)::value || !(ends >> j & 1) ? now : 0.f; };  // c from behind row j
     float A[V], H[V], C[V], G[ROWS][V];  // G: dh as yet
 #pragma unroll
     for (int j = 0; j < ROWS; ++j)
 #pragma unroll
-        for (int v = 0; v < V; ++v) G[j][v] = w0 + j < end ? d[j].get(v) : 0.f;
+        for (int v = 0; v < V; ++v) G[j][v] = w0 + j < behind ? d[j].get(v) : 0.f;
     if (p.dfinal && ends)
 #pragma unroll
         for (int j = 0; j < ROWS; ++j)
@@ -497,16 +668,15 @@ __global__ __launch_bounds__(64 * WAVES, 4) void hstu_scan_bwd_kernel(const Scan
                 A[v] *= g[j][v].a;
             }
 #pragma unroll
-            for (int j = ROWS - 1; j >= 0; --j) C[v] = g[j][v].a * (G[j][v] + behind(all, j, C[v]));
+            for (int j = ROWS - 1; j >= 0; --j) C[v] = g[j][v].a * (G[j][v] + from_behind(all, j, C[v]));
         }
     });
 #pragma unroll
-    for (int v = 0; v < V; ++v) sums[wave][lane * V + v] = float2{A[v], H[v]}, back[wave][lane * V + v] = C[v];
+    for (int v = 0; v < V; ++v) sums[wave][lane * V + v] = float2{A[v], H[v]}, passed[wave][lane * V + v] = C[v];
     __syncthreads();
     // h in front of the wave's rows
-#pragma unroll
-    for (int w = 0; w < WAVES - 1; ++w) {
-        if (w >= wave) break;
+#pragma unroll 1  // (all parts at once would take the registers of the rows)
+    for (int w = 0; w < wave; ++w) {
         const bool begun = marks_of<ROWS>(bits, w) != 0;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -519,73 +689,82 @@ __global__ __launch_bounds__(64 * WAVES, 4) void hstu_scan_bwd_kernel(const Scan
     bool cut = false;
 #pragma unroll
     for (int v = 0; v < V; ++v) fA[v] = 1.f, fC[v] = 0.f;
-#pragma unroll
-    for (int w = WAVES - 1; w > 0; --w) {
-        if (w <= wave) break;
+#pragma unroll 1
+    for (int w = WAVES - 1; w > wave; --w) {
         const bool ended = marks_of<ROWS>(end_bits, w) != 0;
         cut = cut || ended;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const float by = sums[w][lane * V + v].x, c = back[w][lane * V + v];
+            const float by = sums[w][lane * V + v].x, c = passed[w][lane * V + v];
             fC[v] = ended ? c : __builtin_fmaf(by, fC[v], c);
-            fA[v] = ended ? 0.f : by * fA[v];
+            fA[v] = by * fA[v];
         }
     }
-    if (p.words) {
+    const bool needs = turned > 0 && !(end_bits >> (kTile - 1));
+    float from[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) C[v] = ends ? C[v] : __builtin_fmaf(A[v], fC[v], C[v]), A[v] = ends ? 0.f : A[v] * fA[v];
-        put_tile<V, WAVES>(p, turned, col, mine, wave == 0, A, C, meet, wave);
-        if (map.behind > t0 + R) {
-            join_tiles<V, WAVES>(p, p.tiles - 1 - (int)((map.behind - 1) / R), turned, col, meet, wave, C);
+    for (int v = 0; v < V; ++v) C[v] = ends ? C[v] : __builtin_fmaf(A[v], fC[v], C[v]), A[v] *= fA[v];
+    join_tile<V, WAVES>(p, slot, turned, col, mine, wave == 0, turned == 0 || end_bits, needs, A, C, back, wave, from);
+    if (needs)
 #pragma unroll
-            for (int v = 0; v < V; ++v) fC[v] = cut ? fC[v] : __builtin_fmaf(fA[v], C[v], fC[v]);
-        }
-    }
+        for (int v = 0; v < V; ++v) fC[v] = cut ? fC[v] : __builtin_fmaf(fA[v], from[v], fC[v]);
     // G of every row from the last to the first, then the results along with h from the first to the last
-    float sum[V] = {};
+    float sum[V] = {}, natural[V];
 #pragma unroll
-    for (int j = 0; j < ROWS; ++j) asm("" : "+v"(x[j].w));  // products with x are worked out again: kept from above they would take 32 registers that there are not
+    for (int v = 0; v < V; ++v) natural[v] = strength[v] * (1 / kLog2e);
+    // Products of gates and x are worked out again below: kept from above they would take 32 registers that there are not.
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) {
+        asm("" : "+v"(x[j].w));
+#pragma unroll
+        for (int v = 0; v < V; ++v) asm("" : "+v"(g[j][v].si));
+    }
     either([&](auto all) {
         constexpr bool ALL = decltype(all)::value;
 #pragma unroll
         for (int v = 0; v < V; ++v)
 #pragma unroll
             for (int j = ROWS - 1; j >= 0; --j) {
-                G[j][v] += behind(all, j, fC[v]);
+                G[j][v] += from_behind(all, j, fC[v]);
                 fC[v] = g[j][v].a * G[j][v];
                 if (!ALL && p.dinitial && mine && begins >> j & 1) p.dinitial[(int64_t)map.begins[wave * ROWS + j] * p.width + col + v] = fC[v];
             }
 #pragma unroll
         for (int j = 0; j < ROWS; ++j) {
             float dx[V], dr[V], di[V];
-            const bool there = ALL || w0 + j < end;
+            const bool there = ALL || w0 + j < behind;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const Gates<T>& q = g[j][v];
-                const float Gm = G[j][v] * q.m, u = q.si * x[j].get(v), old = before(all, j, v, h[v]);
+                const float u = q.si * x[j].get(v), old = before(all, j, v, h[v]);
                 const float share = q.m > 0.f ? q.s * __builtin_amdgcn_rcpf(q.m) : 0.f;
                 const float dq = G[j][v] * q.a * (u * q.a * share - q.s * old);
-                dx[v] = there ? Gm * q.si : 0.f;
-                dr[v] = there ? strength[v] * (1.f - q.s) * dq : 0.f;
-                di[v] = there ? Gm * u * (1.f - q.si) : 0.f;
+                dx[v] = there ? G[j][v] * (q.m * q.si) : 0.f;
+                dr[v] = there ? natural[v] * (1.f - q.s) * dq : 0.f;
+                di[v] = there ? dx[v] * x[j].get(v) * (1.f - q.si) : 0.f;
                 sum[v] += there ? dq : 0.f;
                 h[v] = __builtin_fmaf(q.a, old, q.m * u);
             }
-            if (mine && (ALL || w0 + j < p.rows)) put(p.dx, j, dx), put(p.dr, j, dr), put(p.di, j, di);
+            if (mine && (ALL || w0 + j < behind)) {
+                if (ALL || p.dx) put(p.dx, dx);
+                if (ALL || p.dr) put(p.dr, dr);
+                if (ALL || p.di) put(p.di, di);
+            }
+            at += pitch;
         }
     });
     if (!p.partial) return;
     __syncthreads();
 #pragma unroll
-    for (int v = 0; v < V; ++v) back[wave][lane * V + v] = sum[v];
+    for (int v = 0; v < V; ++v) passed[wave][lane * V + v] = sum[v];
     __syncthreads();
     if (wave == 0 && mine)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float all = 0.f;
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) all += back[w][lane * V + v];
-            p.partial[(int64_t)tile * p.width + col + v] = all;
+            for (int w = 0; w < WAVES; ++w) all += passed[w][lane * V + v];
+            p.partial[same * p.width + col + v] = all;
         }
 }
 
@@ -633,7 +812,7 @@ __global__ __launch_bounds__(64 * WAVES) void hstu_scan_short_kernel(const ScanP
         return;
     }
     const int64_t first = max(index_at(p.offsets, p.offsets_i64, b), (int64_t)0), end = min(index_at(p.offsets, p.offsets_i64, b + 1), last);
-    const float strength = p.rate * softplus_of(decay_at<T>(p.decay, p.decay_f32, col));
+    const float strength = strength_of(decay_at<T>(p.decay, p.decay_f32, col), p.rate);
     float carry = p.initial ? p.initial[(int64_t)b * p.width + col] : 0.f;
     int turn = 0;
     for (int64_t t0 = first; t0 < end; t0 += R, turn ^= 1) {
@@ -688,7 +867,7 @@ __global__ __launch_bounds__(256) void hstu_scan_step_kernel(const StepParams p)
     if (col >= p.width || t >= p.rows) return;
     const int64_t from = p.slots ? index_at(p.slots, p.slots_i64, t) : t, to = p.new_slots ? index_at(p.new_slots, p.new_slots_i64, t) : from;
     const bool known = from >= -1 && from < p.state_rows;
-    const float strength = p.rate * softplus_of(decay_at<T>(p.decay, p.decay_f32, col));
+    const float strength = strength_of(decay_at<T>(p.decay, p.decay_f32, col), p.rate);
     float h = from >= 0 && known ? p.states[from * p.state_rs + col] : 0.f;
     const Gates<T> g((float)((const T*)p.r)[t * p.r_rs + col], (float)((const T*)p.i)[t * p.i_rs + col], strength);
     h = __builtin_fmaf(g.a, h, g.m * g.si * (float)((const T*)p.x)[t * p.x_rs + col]);

@@ -54,7 +54,7 @@ constexpr int64_t kMaxBlocks = (1 << 22) - 1;  // a launch has fewer than 2^32 t
 int check_scan(const HstuRecurrenceArgs* a) {
     if (!a) return HSTU_ERR_NULL_POINTER;
     if (!known_type(a->dtype)) return HSTU_ERR_BAD_DTYPE;
-    if (a->rows < 0 || a->width <= 0 || a->batch <= 0 || !(a->rate > 0.f)) return HSTU_ERR_BAD_SHAPE;
+    if (a->rows < 0 || a->width <= 0 || a->batch <= 0 || a->batch > (1 << 30) || !(a->rate > 0.f)) return HSTU_ERR_BAD_SHAPE;
     if (a->x_row_stride < 0 || a->decay_gate_row_stride < 0 || a->input_gate_row_stride < 0) return HSTU_ERR_BAD_SHAPE;
     if (!a->seq_offsets || !a->decay) return HSTU_ERR_NULL_POINTER;
     if (a->rows > 0 && (!a->x || !a->decay_gate || !a->input_gate)) return HSTU_ERR_NULL_POINTER;
@@ -89,38 +89,54 @@ bool scan_in_pairs(const HstuRecurrenceArgs* a, const HstuRecurrenceGrads* g) {
     return pairs && odd % 2 == 0;
 }
 
-constexpr int kRows = 16, kWaves = 8;           // of a tile of the forward
-constexpr int kBackRows = 8, kBackWaves = 8;    // ... and of the backward
+constexpr int kRows = 16, kWaves = 4;           // of a tile, in the forward
+constexpr int kBackRows = 8, kBackWaves = 8;    // ... and in the backward
 constexpr int kShortRows = 2, kShortWaves = 8;  // at a time, where sequences are short
 
 // Few rows to a sequence, and no state to save: a workgroup for each sequence.
 bool scan_is_short(const HstuRecurrenceArgs* a) { return !a->saved && a->rows <= 16 * (int64_t)a->batch + 48 && a->rows <= 4096 && a->batch < 65535; }
 
-int64_t scan_tiles(const HstuRecurrenceArgs* a, int rows_of_tile) { return (a->rows + rows_of_tile - 1) / rows_of_tile; }
+// How the tiles of a call are counted, and what they share, behind one another in the scratch memory.
+struct ScanPlan {
+    int64_t per_segment, segments, slots, words;
+    size_t tiles_at, strength_at, partial_at, bytes;
+};
 
-// Words that tiles leave for each other, 64 bits each, the ticket's included: one tile needs none.
-size_t scan_words(int64_t tiles, int width) { return tiles > 1 ? (size_t)(tiles + tiles / hstu::kGroup) * width + 2 : 0; }
+// A segment is a sequence, or as many as have 512 rows on the average: half a tile is lost at its end.
+ScanPlan scan_plan(const HstuRecurrenceArgs* a, bool backward) {
+    ScanPlan s{};
+    s.per_segment = a->rows > 0 ? (512 * (int64_t)a->batch + a->rows - 1) / a->rows : a->batch;
+    if (s.per_segment > a->batch) s.per_segment = a->batch;
+    if (s.per_segment < 1) s.per_segment = 1;
+    s.segments = (a->batch + s.per_segment - 1) / s.per_segment;
+    s.slots = a->rows / hstu::kTile + s.segments + 2;
+    s.words = (2 * s.slots + s.slots / hstu::kGroup + 1) * a->width + (int64_t)(a->width + 63) / 64 * (hstu::kTicketPitch / 2);
+    s.words += s.words & 1;
+    s.tiles_at = (size_t)s.words * 8;
+    s.strength_at = s.tiles_at + (size_t)s.slots * sizeof(hstu::Tile) + 8;
+    s.partial_at = s.strength_at + (size_t)a->width * 4;
+    s.bytes = s.partial_at + (backward ? (size_t)s.slots * a->width * 4 : 0);
+    return s;
+}
 
-// Sets `p` for so many tiles: 0, or the status.
-int set_tiles(hstu::ScanParams& p, int64_t tiles, int cols, void* words) {
+// Sets `p` for a call: 0, or the status.
+int set_plan(hstu::ScanParams& p, const ScanPlan& s, int cols, bool backward, void* scratch) {
     p.col_blocks = (p.width + cols - 1) / cols;
-    if (tiles > kMaxBlocks / p.col_blocks) return HSTU_ERR_UNSUPPORTED;
-    p.tiles = (int)tiles;
-    const size_t n = scan_words(tiles, p.width);
-    if (n) {
-        p.words = (unsigned long long*)words;
-        p.clear = (int64_t)n - 2;
-        p.ticket = (unsigned*)(p.words + p.clear);
-    }
+    if (s.slots > kMaxBlocks / p.col_blocks) return HSTU_ERR_UNSUPPORTED;
+    p.segments = (int)s.segments, p.per_segment = (int)s.per_segment, p.slots = (int)s.slots, p.backward = backward;
+    p.sums = (unsigned long long*)scratch, p.states = p.sums + s.slots * p.width, p.groups = p.states + s.slots * p.width;
+    p.tickets = (unsigned*)(p.groups + (s.slots / hstu::kGroup + 1) * p.width), p.clear = s.words;
+    p.tiles = (hstu::Tile*)((char*)scratch + s.tiles_at), p.strength = (float*)((char*)scratch + s.strength_at);
     return 0;
 }
 
-int launch_clear(const hstu::ScanParams& p, hipStream_t stream) {
-    const int64_t states = p.final_state ? (int64_t)p.batch * p.width : 0, most = p.clear > states ? p.clear : states;
-    if (most == 0) return 0;
-    const int64_t blocks = (most + 1023) / 1024;
-    hipLaunchKernelGGL(hstu::hstu_scan_clear_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, stream, p);
-    return launch_status("recurrence clearing kernel launch");
+int launch_begin(int dtype, const hstu::ScanParams& p, hipStream_t stream) {
+    const int64_t states = p.final_state ? (int64_t)p.batch * p.width : 0, most = p.clear > states ? p.clear : states, wide = (most + p.width + 1023) / 1024, planned = p.segments / 64 + 1,
+                  blocks = wide < 2048 ? wide : 2048;
+    return with_type(dtype, [&](auto* t) {
+        hipLaunchKernelGGL((hstu::hstu_scan_begin_kernel<std::remove_pointer_t<decltype(t)>>), dim3((unsigned)(blocks > planned ? blocks : planned < 2048 ? planned : 2048)), dim3(256), 0, stream, p);
+        return launch_status("recurrence beginning kernel launch");
+    });
 }
 
 }  // namespace
@@ -132,12 +148,12 @@ const char* hstu_recurrent_last_error(void) { return g_last_error; }
 
 size_t hstu_recurrent_scan_workspace_bytes(const HstuRecurrenceArgs* a) {
     if (check_scan(a) || scan_is_short(a)) return 0;
-    return scan_words(scan_tiles(a, kRows * kWaves), a->width) * sizeof(unsigned long long);
+    return scan_plan(a, false).bytes;
 }
 
 size_t hstu_recurrent_scan_saved_bytes(const HstuRecurrenceArgs* a) {
     if (check_scan(a)) return 0;
-    return (size_t)((a->rows + 63) / 64) * a->width * sizeof(float);
+    return (size_t)scan_plan(a, false).slots * a->width * sizeof(float);
 }
 
 int hstu_recurrent_scan(const HstuRecurrenceArgs* a, void* stream) {
@@ -155,19 +171,19 @@ int hstu_recurrent_scan(const HstuRecurrenceArgs* a, void* stream) {
         });
     }
     const size_t need = hstu_recurrent_scan_workspace_bytes(a);
-    if (need && !a->workspace) return HSTU_ERR_NULL_POINTER;
+    if (!a->workspace) return HSTU_ERR_NULL_POINTER;
     if (!aligned_to(a->workspace, 16)) return HSTU_ERR_MISALIGNED;
     if (a->workspace_bytes < (int64_t)need) return HSTU_ERR_BAD_SHAPE;
     const bool pairs = scan_in_pairs(a, nullptr);
-    const int status = set_tiles(p, scan_tiles(a, kRows * kWaves), pairs ? 128 : 64, a->workspace);
+    const int status = set_plan(p, scan_plan(a, false), pairs ? 128 : 64, false, a->workspace);
     if (status) return status;
     if (!device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
-    const int cleared = launch_clear(p, (hipStream_t)stream);
+    const int cleared = launch_begin(a->dtype, p, (hipStream_t)stream);
     if (cleared || a->rows == 0) return cleared;
     return with_type(a->dtype, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
         auto launch = [&](auto v) {
-            hipLaunchKernelGGL((hstu::hstu_scan_kernel<T, decltype(v)::value, kRows, kWaves>), dim3((unsigned)(p.tiles * p.col_blocks)), dim3(64 * kWaves), 0,
+            hipLaunchKernelGGL((hstu::hstu_scan_kernel<T, decltype(v)::value, kRows, kWaves>), dim3((unsigned)(p.slots * p.col_blocks)), dim3(64 * kWaves), 0,
                                (hipStream_t)stream, p);
             return launch_status("recurrence kernel launch");
         };
@@ -179,8 +195,7 @@ int hstu_recurrent_scan(const HstuRecurrenceArgs* a, void* stream) {
 
 size_t hstu_recurrent_scan_bwd_workspace_bytes(const HstuRecurrenceArgs* a) {
     if (check_scan(a)) return 0;
-    const int64_t tiles = scan_tiles(a, kBackRows * kBackWaves);
-    return scan_words(tiles, a->width) * sizeof(unsigned long long) + (size_t)tiles * a->width * sizeof(float);
+    return scan_plan(a, true).bytes;
 }
 
 int hstu_recurrent_scan_bwd(const HstuRecurrenceArgs* a, const HstuRecurrenceGrads* g, void* stream) {
@@ -188,7 +203,7 @@ int hstu_recurrent_scan_bwd(const HstuRecurrenceArgs* a, const HstuRecurrenceGra
     if (rc) return rc;
     if (!g) return HSTU_ERR_NULL_POINTER;
     if (g->d_out_row_stride < 0) return HSTU_ERR_BAD_SHAPE;
-    if (a->rows > 0 && (!a->saved || !g->workspace)) return HSTU_ERR_NULL_POINTER;
+    if (!g->workspace || (a->rows > 0 && !a->saved)) return HSTU_ERR_NULL_POINTER;
     const int es = bytes_of(a->dtype);
     for (const void* ptr : {g->d_out, (const void*)g->d_x, (const void*)g->d_decay_gate, (const void*)g->d_input_gate})
         if (!aligned_to(ptr, es)) return HSTU_ERR_MISALIGNED;
@@ -200,19 +215,19 @@ int hstu_recurrent_scan_bwd(const HstuRecurrenceArgs* a, const HstuRecurrenceGra
     p.dout = (const char*)g->d_out, p.dout_rs = g->d_out_row_stride, p.dfinal = g->d_final_state;
     p.dx = (char*)g->d_x, p.dr = (char*)g->d_decay_gate, p.di = (char*)g->d_input_gate, p.dinitial = g->d_initial_state;
     const bool pairs = scan_in_pairs(a, g);
-    const int64_t tiles = scan_tiles(a, kBackRows * kBackWaves);
-    const int status = set_tiles(p, tiles, pairs ? 128 : 64, g->workspace);
+    const ScanPlan plan = scan_plan(a, true);
+    const int status = set_plan(p, plan, pairs ? 128 : 64, true, g->workspace);
     if (status) return status;
-    if (g->d_decay) p.partial = (float*)((unsigned long long*)g->workspace + scan_words(tiles, a->width));
+    if (g->d_decay) p.partial = (float*)((char*)g->workspace + plan.partial_at);
     if (!device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
     hstu::ScanParams clear = p;
     clear.final_state = p.dinitial, clear.initial = p.dfinal;  // the gradient of a state that no row changes
-    const int cleared = launch_clear(clear, (hipStream_t)stream);
+    const int cleared = launch_begin(a->dtype, clear, (hipStream_t)stream);
     if (cleared) return cleared;
     return with_type(a->dtype, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
         auto launch = [&](auto v) {
-            hipLaunchKernelGGL((hstu::hstu_scan_bwd_kernel<T, decltype(v)::value, kBackRows, kBackWaves>), dim3((unsigned)(p.tiles * p.col_blocks)),
+            hipLaunchKernelGGL((hstu::hstu_scan_bwd_kernel<T, decltype(v)::value, kBackRows, kBackWaves>), dim3((unsigned)(p.slots * p.col_blocks)),
                                dim3(64 * kBackWaves), 0, (hipStream_t)stream, p);
             return launch_status("recurrence backward kernel launch");
         };
@@ -225,7 +240,7 @@ int hstu_recurrent_scan_bwd(const HstuRecurrenceArgs* a, const HstuRecurrenceGra
             }();
         }
         if (rows || !g->d_decay) return rows;
-        hipLaunchKernelGGL((hstu::hstu_scan_decay_kernel<T>), dim3((a->width + 15) / 16), dim3(256), 0, (hipStream_t)stream, p.partial, tiles, a->width, a->decay,
+        hipLaunchKernelGGL((hstu::hstu_scan_decay_kernel<T>), dim3((a->width + 15) / 16), dim3(256), 0, (hipStream_t)stream, p.partial, plan.slots, a->width, a->decay,
                            a->decay_f32, a->rate, g->d_decay);
         return launch_status("recurrence decay gradient kernel launch");
     });
