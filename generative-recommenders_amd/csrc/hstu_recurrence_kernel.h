@@ -85,9 +85,10 @@ struct ScanParams {
     int slots;
     Tile* tiles;                // [slots], in the order in which they are begun
     float* strength;            // [width]: rate softplus(decay) log2(e)
-    unsigned long long *sums, *states, *groups;  // [slots][width], [slots][width], [slots / kGroup + 1][width]
-    unsigned* tickets;          // one for each block of columns, kTicketPitch apart, behind the words
-    int64_t clear;              // how many words to clear, the tickets' included
+    unsigned long long *sums, *groups;  // [slots][width], [slots / kGroup + 1][width]
+    unsigned* states;           // [slots][width]
+    unsigned* tickets;          // one for each block of columns, kTicketPitch apart
+    int64_t clear;              // how many pairs of words to clear from `sums` on: all of the four above
     int backward;
     // backward
     const char* dout;
@@ -98,44 +99,15 @@ struct ScanParams {
     float* partial;  // [slots][width], or null
 };
 
-// V neighbouring columns of a row, four bytes at most.
-template <class T, int V>
-struct Piece {
-    static_assert(V * sizeof(T) <= 4, "one register");
-    unsigned w;
-    __device__ __forceinline__ void load(const T* p) {
-        if constexpr (V * sizeof(T) == 4)
-            w = *(const unsigned*)p;
-        else
-            w = *(const uint16_t*)p;
-    }
-    __device__ __forceinline__ float get(int v) const {
-        if constexpr (sizeof(T) == 4)
-            return __uint_as_float(w);
-        else
-            return (float)__builtin_bit_cast(T, (uint16_t)(v ? w >> 16 : w));
-    }
-    __device__ __forceinline__ static void put(const float (&x)[V], T* p) {
-        if constexpr (V == 1) {
-            *p = (T)x[0];
-        } else {
-            typedef __attribute__((ext_vector_type(2))) T T2;
-            T2 v;
-            v[0] = (T)x[0], v[1] = (T)x[1];
-            *(T2*)p = v;
-        }
-    }
-};
-
-// ROWS rows of a tensor from row w0 on, the last one in front of `behind` again where there are no more.  Row addresses are the wave's, not the
-// lane's (`off`: bytes).
-template <class T, int V, int ROWS>
-__device__ __forceinline__ void load_rows(Piece<T, V> (&to)[ROWS], const char* base, int64_t rs, int64_t w0, int64_t behind, unsigned off) {
+// ROWS rows of a column of a tensor from row w0 on, the last one in front of `behind` again where there are no more.  Row addresses are the wave's, not
+// the lane's (`off`: bytes).
+template <class T, int ROWS>
+__device__ __forceinline__ void load_rows(T (&to)[ROWS], const char* base, int64_t rs, int64_t w0, int64_t behind, unsigned off) {
     const char* row = base + min(w0, behind - 1) * rs * (int64_t)sizeof(T);
     const int left = (int)min(behind - w0, (int64_t)ROWS);
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) {
-        to[j].load((const T*)(row + off));
+        to[j] = *(const T*)(row + off);
         row += j + 1 < left ? rs * (int64_t)sizeof(T) : 0;
     }
 }
@@ -198,94 +170,91 @@ __device__ __forceinline__ unsigned marks_of(uint64_t bits, int wave) {
 // ---- tiles joined along the rows ----
 //
 // What a tile makes of the h in front of it is A h + H, or H alone where a sequence begins in it (it is cut off).  Each tile puts its (A, H) down as
-// one word for each column, and the h behind it, its state, as another once it knows it: state = A (state in front) + H.  A tile that finds no
-// state in front of it yet takes up (A, H)s back to one.  A word is written and read as a whole and is never 0 once written, so it needs no flag and no
+// one word for each column, its sum, and the h behind it, its state, as another once it knows it: state = A (state in front) + H.  A tile that finds no
+// state in front of it yet takes up sums back to one.  A word is written and read as a whole and is never 0 once written, so it needs no flag and no
 // fence beside it.
 //
 // Tiles are begun in the order of p.tiles, all segments' first ones in front of their second ones (64 segments at a time), by tickets that a
 // workgroup takes when it runs: those in front have been begun and wait for none behind them, so each wait ends.  (The limit on it only keeps a broken
 // device from hanging.)  With many segments the tile in front has nearly always been done; a single long one has hundreds of its tiles under way at
-// once, and for those every kGroup-th joins the (A, H) of its kGroup into one word, and its state is defined by that: A_group (state in front of the
+// once, and for those every kGroup-th joins the sums of its kGroup into one, and its state is defined by that: A_group (state in front of the
 // group) + H_group.  So every state has one definition, and results do not depend on which tile was first.
 //
-// (Tiles of rows regardless of sequences, begun one after another and each taking up all (A, H) of its sequence in front of it, waited a third of the time:
-// five histories of up to 16000 rows, 1024 columns, 137 us; 98 without the waits.)
-// A block of columns has a ticket of its own: all workgroups at one counter were 18 ns each.
+// What was measured.  Tiles of rows regardless of sequences, each taking up all sums of its sequence in front of it: a third of the time went into waits
+// (five histories of up to 16000 rows, 1024 columns, 137 us; 98 without them).  A pass for the sums and another for the rows reads everything twice.  Two
+// columns to a lane: 231 us where one takes 206 (a training step of 48 histories, 512 columns), since half as many waves fit; eight rows to a lane 222.
+// All workgroups at one ticket counter were 18 ns each, so a block of columns has one of its own.
 constexpr int kGroup = 16, kGroupsBack = 8, kTicketPitch = 64;
 constexpr unsigned kCut = 0x7f800000u;  // A's bits where there is none
 
-__device__ __forceinline__ void put_word(unsigned long long* at, float A, bool cut, float H) {
-    const unsigned long long w = (unsigned long long)__float_as_uint(H) << 32 | ((cut ? kCut : __float_as_uint(A)) | 0x80000000u);
+__device__ __forceinline__ void put_sum(unsigned long long* at, float A, bool cut, float H) {
+    const unsigned long long w = (unsigned long long)__float_as_uint(H) << 32 | ((cut ? kCut : __float_as_uint(A)) | 0x80000000u);  // (A is not negative)
     __hip_atomic_store(at, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ unsigned long long get_word(const unsigned long long* at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ float word_h(unsigned long long w) { return __uint_as_float((unsigned)(w >> 32)); }
-__device__ __forceinline__ float word_a(unsigned long long w) { return __uint_as_float((unsigned)w & 0x7fffffffu); }
-__device__ __forceinline__ bool word_cut(unsigned long long w) { return ((unsigned)w & 0x7fffffffu) == kCut; }
-// H behind what `w` says, from H in front of it.
-__device__ __forceinline__ float apply(unsigned long long w, float H) { return word_cut(w) ? word_h(w) : __builtin_fmaf(word_a(w), H, word_h(w)); }
-
-// V words, all lanes', when they are there; NaN if they never are.
-template <int V>
-__device__ __forceinline__ void await(const unsigned long long* at, unsigned long long (&w)[V]) {
-    for (int tries = 0; tries < (1 << 20); ++tries) {
-        bool there = true;
-#pragma unroll
-        for (int v = 0; v < V; ++v) there = there && w[v] != 0;
-        if (__all(there)) return;
-        __builtin_amdgcn_s_sleep(1);
-#pragma unroll
-        for (int v = 0; v < V; ++v) w[v] = get_word(at + v);
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) w[v] = 0x7fc00000ull << 32 | 0x80000000u | kCut;
+__device__ __forceinline__ void put_state(unsigned* at, float h) {
+    const unsigned w = __float_as_uint(h);
+    __hip_atomic_store(at, w ? w : 0x80000000u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // (zero as the other zero)
 }
+template <class W>
+__device__ __forceinline__ W get_word(const W* at) {
+    return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float sum_h(unsigned long long w) { return __uint_as_float((unsigned)(w >> 32)); }
+__device__ __forceinline__ float sum_a(unsigned long long w) { return __uint_as_float((unsigned)w & 0x7fffffffu); }
+__device__ __forceinline__ bool is_cut(unsigned long long w) { return ((unsigned)w & 0x7fffffffu) == kCut; }
+// h behind what `w` says, from h in front of it.
+__device__ __forceinline__ float apply(unsigned long long w, float h) { return is_cut(w) ? sum_h(w) : __builtin_fmaf(sum_a(w), h, sum_h(w)); }
+
+// All lanes' words, when they are there; `never` if they never are.
+template <class W>
+__device__ __forceinline__ W await(const W* at, W w, W never) {
+    for (int tries = 0; tries < (1 << 20); ++tries) {
+        if (__all(w != 0)) return w;
+        __builtin_amdgcn_s_sleep(1);
+        w = get_word(at);
+    }
+    return never;
+}
+constexpr unsigned kNoState = 0x7fc00000u;
+constexpr unsigned long long kNoSum = (unsigned long long)kNoState << 32 | 0x80000000u | kCut;
 
 // What the waves of a workgroup share while they go back.
-template <int V, int WAVES>
+template <int WAVES>
 struct Back {
-    unsigned long long sums[kGroup + kGroupsBack][64 * V];
-    float states[2 * WAVES][64 * V];
+    unsigned long long sums[kGroup + kGroupsBack][64];
+    float states[2 * WAVES][64];
     int found[2 * WAVES];  // 0 no, 1 cut off, 2 a state
 };
 
 // Goes back over `count` sums, two to a wave at a time: sum(i) is that of the i-th from here (from 1 on), state(i) the state in front of it
-// (in front of here for 0; NULL: there is none).  True: H is a state, or not needed, and the `n` sums from here to it, in back.sums[row + i - 1], go on from it.
+// (in front of here for 0; NULL: there is none).  True: h is a state, or not needed, and the `n` sums from here to it, in back.sums[row + i - 1], go on from it.
 // `all`: takes every sum, and looks for no state.  Every thread of the workgroup calls.
-template <int V, int WAVES, class SUM, class STATE>
-__device__ __forceinline__ bool go_back(int count, bool all, int row, SUM&& sum, STATE&& state, Back<V, WAVES>& back, int wave, int& n, float (&H)[V]) {
+template <int WAVES, class SUM, class STATE>
+__device__ __forceinline__ bool go_back(int count, bool all, int row, SUM&& sum, STATE&& state, Back<WAVES>& back, int wave, int& n, float& h) {
     const int lane = threadIdx.x & 63;
     for (int from = 0; from <= count; from += 2 * WAVES) {
-        unsigned long long s[2][V], t[2][V];
+        unsigned long long s[2];
+        unsigned t[2];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const int i = min(from + 2 * wave + q, count);
-            const unsigned long long* front = all ? nullptr : state(i);
-#pragma unroll
-            for (int v = 0; v < V; ++v) s[q][v] = i ? get_word(sum(i) + v) : 1, t[q][v] = front ? get_word(front + v) : 0;
+            const unsigned* front = all ? nullptr : state(i);
+            s[q] = i ? get_word(sum(i)) : 1, t[q] = front ? get_word(front) : 0;
         }
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const int i = from + 2 * wave + q;
             if (i > count) continue;  // (the same for the wave)
-            bool cut = i > 0, known = true;
-            if (i) await<V>(sum(i), s[q]);
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                if (i) back.sums[row + i - 1][lane * V + v] = s[q][v], cut = cut && word_cut(s[q][v]);
-                known = known && t[q][v] != 0;
-                back.states[2 * wave + q][lane * V + v] = word_h(t[q][v]);
-            }
-            const int found = __all(known) ? 2 : __all(cut) ? 1 : 0;
+            if (i) back.sums[row + i - 1][lane] = s[q] = await(sum(i), s[q], kNoSum);
+            back.states[2 * wave + q][lane] = __uint_as_float(t[q]);
+            const int found = __all(t[q] != 0) ? 2 : __all(i && is_cut(s[q])) ? 1 : 0;
             if (lane == 0) back.found[2 * wave + q] = found;
         }
         __syncthreads();
         for (int k = 0; k < 2 * WAVES && from + k <= count && !all; ++k) {
             const int found = back.found[k];  // (the same for all)
             if (!found) continue;
-            n = from + k;
-#pragma unroll
-            for (int v = 0; v < V; ++v) H[v] = found == 2 ? back.states[k][lane * V + v] : 0.f;
+            n = from + k, h = found == 2 ? back.states[k][lane] : 0.f;
             return true;
         }
         __syncthreads();
@@ -294,27 +263,24 @@ __device__ __forceinline__ bool go_back(int count, bool all, int row, SUM&& sum,
     return false;
 }
 
-// H in front of tile `at` of a segment whose words begin at `slot`; and where the tile is the last of a group and not cut off (`closes`), what the tiles in
-// front of it in its group make of h, (A, G) or G alone (`off`), and in `base` the h in front of the group.  Every thread of the workgroup calls.
-template <int V, int WAVES>
-__device__ __forceinline__ void look_back(const ScanParams& p, int slot, int at, int col, bool closes, Back<V, WAVES>& back, int wave, float (&H)[V], float (&A)[V],
-                                          float (&G)[V], bool& off, float (&base)[V]) {
-    const int lane = threadIdx.x & 63, lo = at / kGroup * kGroup, group = at / kGroup;
+// h in front of tile `at` of a segment whose words begin at `slot`; and where the tile is the last of a group and not cut off (`closes`), what the tiles in
+// front of it in its group make of h, (A, H) or H alone (`off`), and in `base` the h in front of the group.  Every thread of the workgroup calls.
+template <int WAVES>
+__device__ __forceinline__ float look_back(const ScanParams& p, int slot, int at, int col, bool closes, Back<WAVES>& back, int wave, float& A, float& H, bool& off,
+                                           float& base) {
+    const int lane = threadIdx.x & 63, group = at / kGroup;
     const int64_t width = p.width;
     auto sum_of = [&](int i) { return p.sums + (slot + at - i) * width + col; };
     auto state_of = [&](int tile) { return tile < 0 ? nullptr : p.states + (slot + tile) * width + col; };
     int n;
-    bool known = go_back<V, WAVES>(at - lo, closes, 0, sum_of, [&](int i) { return state_of(at - i - 1); }, back, wave, n, H);
+    float h;
+    bool known = go_back<WAVES>(at % kGroup, closes, 0, sum_of, [&](int i) { return state_of(at - i - 1); }, back, wave, n, h);
     off = false;
     if (closes) {
-        for (int k = 0; k < n; ++k) off = off || word_cut(back.sums[k][0]);  // (the same in all columns)
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            A[v] = 1.f, G[v] = H[v] = 0.f;
-            for (int k = n - 1; k >= 0; --k) {
-                const unsigned long long w = back.sums[k][lane * V + v];
-                G[v] = apply(w, G[v]), A[v] *= word_a(w);
-            }
+        A = 1.f, H = h = 0.f;
+        for (int k = n - 1; k >= 0; --k) {
+            const unsigned long long w = back.sums[k][lane];
+            off = off || is_cut(w), H = apply(w, H), A *= sum_a(w);  // (cut off in all columns or none)
         }
         known = off;
     }
@@ -323,60 +289,47 @@ __device__ __forceinline__ void look_back(const ScanParams& p, int slot, int at,
         auto group_of = [&](int i) { return p.groups + (slot + (group - i) * kGroup + kGroup - 1) / kGroup * width + col; };
         const int count = min(group, kGroupsBack);
         int m;
-        if (!go_back<V, WAVES>(count, false, kGroup, group_of, [&](int i) { return state_of((group - i) * kGroup - 1); }, back, wave, m, H)) {
-            const unsigned long long* far = state_of((group - count) * kGroup - 1);
-            unsigned long long w[V];
-#pragma unroll
-            for (int v = 0; v < V; ++v) w[v] = get_word(far + v);
-            await<V>(far, w);
-#pragma unroll
-            for (int v = 0; v < V; ++v) H[v] = word_h(w[v]);
+        if (!go_back<WAVES>(count, false, kGroup, group_of, [&](int i) { return state_of((group - i) * kGroup - 1); }, back, wave, m, h)) {
+            const unsigned* far = state_of((group - count) * kGroup - 1);
+            h = __uint_as_float(await(far, get_word(far), kNoState));
         }
-        for (int k = m - 1; k >= 0; --k)
-#pragma unroll
-            for (int v = 0; v < V; ++v) H[v] = apply(back.sums[kGroup + k][lane * V + v], H[v]);
+        for (int k = m - 1; k >= 0; --k) h = apply(back.sums[kGroup + k][lane], h);
     }
-#pragma unroll
-    for (int v = 0; v < V; ++v) base[v] = H[v];
-    for (int k = n - 1; k >= 0; --k)
-#pragma unroll
-        for (int v = 0; v < V; ++v) H[v] = apply(back.sums[k][lane * V + v], H[v]);
+    base = h;
+    for (int k = n - 1; k >= 0; --k) h = apply(back.sums[k][lane], h);
+    return h;
 }
 
-// What a tile has to do with the others.  `me`: the wave that has its (A, H), which it puts down; `front`: the h in front of the tile, where it `needs` it.
-// Every thread of the workgroup calls.
-template <int V, int WAVES>
-__device__ __forceinline__ void join_tile(const ScanParams& p, int slot, int at, int col, bool mine, bool me, bool cut, bool needs, const float (&A)[V],
-                                          const float (&H)[V], Back<V, WAVES>& back, int wave, float (&front)[V]) {
+// What a tile has to do with the others.  `me`: the wave that has its (A, H), which it puts down.  Returns the h in front of the tile, where it
+// `needs` it.  Every thread of the workgroup calls.
+template <int WAVES>
+__device__ __forceinline__ float join_tile(const ScanParams& p, int slot, int at, int col, bool mine, bool me, bool cut, bool needs, float A, float H,
+                                           Back<WAVES>& back, int wave) {
     const bool closes = at % kGroup == kGroup - 1;
     const int64_t word = (int64_t)(slot + at) * p.width + col;
     unsigned long long* group = p.groups + (int64_t)((slot + at) / kGroup) * p.width + col;
-    if (me && mine)
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            put_word(p.sums + word + v, A[v], cut, H[v]);
-            if (cut) put_word(p.states + word + v, 0.f, true, H[v]);
-            if (cut && closes) put_word(group + v, 0.f, true, H[v]);
-        }
-    if (!needs) return;  // (needs, where it is not cut off)
-    float by[V], G[V], base[V];
-    bool off;
-    look_back<V, WAVES>(p, slot, at, col, closes && !cut, back, wave, front, by, G, off, base);
-    if (!me || !mine || cut) return;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        float state = __builtin_fmaf(A[v], front[v], H[v]);
-        if (closes) {
-            by[v] *= A[v], G[v] = __builtin_fmaf(A[v], G[v], H[v]);
-            put_word(group + v, by[v], off, G[v]);
-            state = off ? G[v] : __builtin_fmaf(by[v], base[v], G[v]);
-        }
-        put_word(p.states + word + v, 0.f, true, state);
+    if (me && mine) {
+        put_sum(p.sums + word, A, cut, H);
+        if (cut) put_state(p.states + word, H);
+        if (cut && closes) put_sum(group, 0.f, true, H);
     }
+    if (!needs) return 0.f;  // (needs, where it is not cut off)
+    float by, from, base;
+    bool off;
+    const float front = look_back<WAVES>(p, slot, at, col, closes && !cut, back, wave, by, from, off, base);
+    if (!me || !mine || cut) return front;
+    float state = __builtin_fmaf(A, front, H);
+    if (closes) {
+        by *= A, from = __builtin_fmaf(A, from, H);
+        put_sum(group, by, off, from);
+        state = off ? from : __builtin_fmaf(by, base, from);
+    }
+    put_state(p.states + word, state);
+    return front;
 }
 
 // Which block of columns a workgroup takes: each as often as there are tiles, and each of the eight dies, which workgroups go to in turn, all of them
-// in turn (1024 columns, one die always at the same 256 bytes of a row: 1261 us where others take 1105).
+// in turn (1024 columns, one die always at the same part of a row: 1261 us where others take 1105).
 __device__ __forceinline__ int column_block(const ScanParams& p) { return (int)((blockIdx.x + blockIdx.x / p.col_blocks) % p.col_blocks); }
 
 // The tile that a workgroup takes up, to LDS: one thread's work, with a barrier behind it.
@@ -447,7 +400,7 @@ __global__ __launch_bounds__(256) void hstu_scan_begin_kernel(const ScanParams p
     __shared__ PlanPart plan;
     const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
     typedef __attribute__((ext_vector_type(4))) unsigned u4;
-    for (int64_t k = 2 * at; k < p.clear; k += 2 * step) *(u4*)(p.sums + k) = u4{0, 0, 0, 0};  // (an even number of words)
+    for (int64_t k = at; k < p.clear; k += step) ((u4*)p.sums)[k] = u4{0, 0, 0, 0};
     for (int64_t k = at; k < p.width; k += step) p.strength[k] = strength_of(decay_at<T>(p.decay, p.decay_f32, k), p.rate);
     if (p.partial)  // (there are slots without a tile)
         for (int64_t k = at; k < (int64_t)p.slots * p.width; k += step) p.partial[k] = 0.f;
@@ -460,13 +413,13 @@ __global__ __launch_bounds__(256) void hstu_scan_begin_kernel(const ScanParams p
     }
 }
 
-template <class T, int V, int ROWS, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 4) void hstu_scan_kernel(const ScanParams p) {
-    constexpr int COLS = 64 * V;
-    static_assert(ROWS * WAVES == kTile, "a row for each");
+// A workgroup takes a tile of 64 columns, a lane one of them, ROWS rows to a wave.  Bytes and waits bound it: see above.
+template <class T, int ROWS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 6) void hstu_scan_kernel(const ScanParams p) {
+    static_assert(ROWS * WAVES == kTile && ROWS <= 16, "a row for each");
     __shared__ TileRows map;
-    __shared__ float2 sums[WAVES][COLS];
-    __shared__ Back<V, WAVES> back;
+    __shared__ float2 sums[WAVES][64];
+    __shared__ Back<WAVES> back;
     __shared__ Tile taken;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, block = column_block(p);
     map.clear();
@@ -475,52 +428,43 @@ __global__ __launch_bounds__(64 * WAVES, 4) void hstu_scan_kernel(const ScanPara
     const int at = __builtin_amdgcn_readfirstlane(taken.at), slot = __builtin_amdgcn_readfirstlane(taken.slot);
     if (at < 0) return;
     const int64_t t0 = uniform(taken.first), behind = uniform(taken.behind), w0 = t0 + wave * ROWS, pitch = p.width * (int64_t)sizeof(T);
-    const int col0 = block * COLS + lane * V, col = min(col0, p.width - V);
-    const bool mine = col0 < p.width;
+    const int col = min(block * 64 + lane, p.width - 1);  // (a lane without a column goes along with the last)
+    const bool mine = block * 64 + lane < p.width;
     const unsigned off = col * (unsigned)sizeof(T);
     char* out = p.out + w0 * pitch;
     if (__builtin_amdgcn_readfirstlane(taken.segment) == p.segments) {  // rows behind the last sequence
-        for (int j = 0; j < ROWS && w0 + j < behind; ++j, out += pitch) {
-            const float zero[V] = {};
-            if (mine) Piece<T, V>::put(zero, (T*)(out + off));
-        }
+        for (int j = 0; j < ROWS && w0 + j < behind; ++j, out += pitch)
+            if (mine) *(T*)(out + off) = (T)0.f;
         return;
     }
-    Piece<T, V> x[ROWS], r[ROWS], i[ROWS];
-    load_rows<T, V, ROWS>(r, p.r, p.r_rs, w0, behind, off);
-    load_rows<T, V, ROWS>(i, p.i, p.i_rs, w0, behind, off);
-    load_rows<T, V, ROWS>(x, p.x, p.x_rs, w0, behind, off);
-    float strength[V], a[ROWS][V], b[ROWS][V], A[V], H[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) strength[v] = p.strength[col + v], A[v] = 1.f, H[v] = 0.f;
+    T x[ROWS], r[ROWS], i[ROWS];
+    load_rows(r, p.r, p.r_rs, w0, behind, off);
+    load_rows(i, p.i, p.i_rs, w0, behind, off);
+    load_rows(x, p.x, p.x_rs, w0, behind, off);
+    const float strength = p.strength[col];
     map.template find<64 * WAVES>(p, taken);
+    float a[ROWS], b[ROWS];
 #pragma unroll
-    for (int j = 0; j < ROWS; ++j)
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const Gates<T> g(r[j].get(v), i[j].get(v), strength[v]);
-            a[j][v] = g.a, b[j][v] = g.m * g.si * x[j].get(v);
-        }
+    for (int j = 0; j < ROWS; ++j) {
+        const Gates<T> g((float)r[j], (float)i[j], strength);
+        a[j] = g.a, b[j] = g.m * g.si * (float)x[j];
+    }
     __syncthreads();
     const uint64_t bits = marks(map.begins);
     const unsigned begins = marks_of<ROWS>(bits, wave), ends = marks_of<ROWS>(marks(map.ends), wave);
     if (begins && p.initial)
 #pragma unroll
         for (int j = 0; j < ROWS; ++j)
-            if (begins >> j & 1)
-#pragma unroll
-                for (int v = 0; v < V; ++v) b[j][v] = __builtin_fmaf(a[j][v], p.initial[(int64_t)map.begins[wave * ROWS + j] * p.width + col + v], b[j][v]);
-    // (a, b) row by row; a row that begins a sequence knows nothing of what is in front of it, whatever that is
+            if (begins >> j & 1) b[j] = __builtin_fmaf(a[j], p.initial[(int64_t)map.begins[wave * ROWS + j] * p.width + col], b[j]);
+    // Row by row; a row that begins a sequence knows nothing of what is in front of it, whatever that is.
+    float A = 1.f, H = 0.f;
     auto rows = [&](auto any, auto&& each) {
 #pragma unroll
         for (int j = 0; j < ROWS; ++j) {
-            if (decltype(any)::value && begins >> j & 1) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) H[v] = b[j][v], A[v] = 0.f;
-            } else {
-#pragma unroll
-                for (int v = 0; v < V; ++v) H[v] = __builtin_fmaf(a[j][v], H[v], b[j][v]), A[v] *= a[j][v];
-            }
+            if (decltype(any)::value && begins >> j & 1)
+                H = b[j];
+            else
+                H = __builtin_fmaf(a[j], H, b[j]), A *= a[j];
             each(j);
         }
     };
@@ -529,66 +473,48 @@ __global__ __launch_bounds__(64 * WAVES, 4) void hstu_scan_kernel(const ScanPara
         rows(std::true_type{}, nothing);
     else
         rows(std::false_type{}, nothing);
-#pragma unroll
-    for (int v = 0; v < V; ++v) sums[wave][lane * V + v] = float2{A[v], H[v]};
+    sums[wave][lane] = float2{A, H};
     __syncthreads();
-    float fA[V], fH[V];  // of the waves in front
-    bool cut = false;    // whether a sequence begins in one of them
-#pragma unroll
-    for (int v = 0; v < V; ++v) fA[v] = 1.f, fH[v] = 0.f;
+    float fA = 1.f, fH = 0.f;  // of the waves in front
+    bool cut = false;          // whether a sequence begins in one of them
 #pragma unroll 1  // (all parts at once would take the registers of the rows)
     for (int w = 0; w < wave; ++w) {
         const bool begun = marks_of<ROWS>(bits, w) != 0;
+        const float2 s = sums[w][lane];
         cut = cut || begun;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const float2 s = sums[w][lane * V + v];
-            fH[v] = begun ? s.y : __builtin_fmaf(s.x, fH[v], s.y);
-            fA[v] = s.x * fA[v];
-        }
+        fH = begun ? s.y : __builtin_fmaf(s.x, fH, s.y), fA *= s.x;
     }
     const bool needs = at > 0 && !(bits & 1);
-    float front[V] = {};
-#pragma unroll
-    for (int v = 0; v < V; ++v) H[v] = begins ? H[v] : __builtin_fmaf(A[v], fH[v], H[v]), A[v] *= fA[v];
-    join_tile<V, WAVES>(p, slot, at, col, mine, wave == WAVES - 1, at == 0 || bits, needs, A, H, back, wave, front);
-    if (p.saved && wave == 0 && mine)
-#pragma unroll
-        for (int v = 0; v < V; ++v) p.saved[(int64_t)(slot + at) * p.width + col + v] = front[v];
-    if (needs)
-#pragma unroll
-        for (int v = 0; v < V; ++v) fH[v] = cut ? fH[v] : __builtin_fmaf(fA[v], front[v], fH[v]);
-#pragma unroll
-    for (int v = 0; v < V; ++v) H[v] = fH[v];
+    const float front = join_tile<WAVES>(p, slot, at, col, mine, wave == WAVES - 1, at == 0 || bits, needs, A * fA, begins ? H : __builtin_fmaf(A, fH, H), back, wave);
+    if (p.saved && wave == 0 && mine) p.saved[(int64_t)(slot + at) * p.width + col] = front;
+    H = needs && !cut ? __builtin_fmaf(fA, front, fH) : fH;
     if (!begins && !(ends && p.final_state) && w0 + ROWS <= behind) {
         if (mine)
             rows(std::false_type{}, [&](int) {
-                Piece<T, V>::put(H, (T*)(out + off));
+                *(T*)(out + off) = (T)H;
                 out += pitch;
             });
         return;
     }
     rows(std::true_type{}, [&](int j) {
         if (w0 + j < behind && mine) {
-            Piece<T, V>::put(H, (T*)(out + off));
-            if (p.final_state && ends >> j & 1)
-#pragma unroll
-                for (int v = 0; v < V; ++v) p.final_state[(int64_t)map.ends[wave * ROWS + j] * p.width + col + v] = H[v];
+            *(T*)(out + off) = (T)H;
+            if (p.final_state && ends >> j & 1) p.final_state[(int64_t)map.ends[wave * ROWS + j] * p.width + col] = H;
         }
         out += pitch;
     });
 }
 
 // The same from the last row to the first: G is to dh what h is to b, with a row's a on the way to the row in front of it.  h in front of each row is
-// worked out again from the state that the forward saved for the tile.  c = a G is what a row passes on.
-template <class T, int V, int ROWS, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 4) void hstu_scan_bwd_kernel(const ScanParams p) {
-    constexpr int COLS = 64 * V;
-    static_assert(ROWS * WAVES == kTile, "a row for each");
+// worked out again from the state that the forward saved for the tile.  c = a G is what a row passes on.  Three waves of a SIMD, whose registers hold a row's gates
+// from the first pass to the last: with four they did not (232 us where this takes 216, a training step of 48 histories).
+template <class T, int ROWS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 3) void hstu_scan_bwd_kernel(const ScanParams p) {
+    static_assert(ROWS * WAVES == kTile && ROWS <= 16, "a row for each");
     __shared__ TileRows map;
-    __shared__ float2 sums[WAVES][COLS];
-    __shared__ float passed[WAVES][COLS];
-    __shared__ Back<V, WAVES> back;
+    __shared__ float2 sums[WAVES][64];
+    __shared__ float passed[WAVES][64];
+    __shared__ Back<WAVES> back;
     __shared__ Tile taken;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, block = column_block(p);
     map.clear();
@@ -598,39 +524,35 @@ __global__ __launch_bounds__(64 * WAVES, 4) void hstu_scan_bwd_kernel(const Scan
     if (turned < 0) return;
     const int64_t t0 = uniform(taken.first), behind = uniform(taken.behind), w0 = t0 + wave * ROWS, pitch = p.width * (int64_t)sizeof(T);
     const int64_t same = slot + __builtin_amdgcn_readfirstlane(taken.in_front);  // the slot that the forward had for this tile
-    const int col0 = block * COLS + lane * V, col = min(col0, p.width - V);
-    const bool mine = col0 < p.width;
+    const int col = min(block * 64 + lane, p.width - 1);
+    const bool mine = block * 64 + lane < p.width;
     const unsigned off = col * (unsigned)sizeof(T);
     int64_t at = w0 * pitch;  // of a row of the results
-    auto put = [&](char* to, const float (&d)[V]) { Piece<T, V>::put(d, (T*)(to + at + off)); };
+    auto put = [&](char* to, float d) { *(T*)(to + at + off) = (T)d; };
     if (__builtin_amdgcn_readfirstlane(taken.segment) == p.segments) {  // rows behind the last sequence
-        const float zero[V] = {};
         for (int j = 0; j < ROWS && w0 + j < behind; ++j, at += pitch)
             if (mine) {
-                if (p.dx) put(p.dx, zero);
-                if (p.dr) put(p.dr, zero);
-                if (p.di) put(p.di, zero);
+                if (p.dx) put(p.dx, 0.f);
+                if (p.dr) put(p.dr, 0.f);
+                if (p.di) put(p.di, 0.f);
             }
         return;
     }
-    Piece<T, V> x[ROWS], r[ROWS], i[ROWS], d[ROWS];
-    load_rows<T, V, ROWS>(r, p.r, p.r_rs, w0, behind, off);
-    load_rows<T, V, ROWS>(i, p.i, p.i_rs, w0, behind, off);
-    load_rows<T, V, ROWS>(x, p.x, p.x_rs, w0, behind, off);
+    T x[ROWS], r[ROWS], i[ROWS], d[ROWS];
+    load_rows(r, p.r, p.r_rs, w0, behind, off);
+    load_rows(i, p.i, p.i_rs, w0, behind, off);
+    load_rows(x, p.x, p.x_rs, w0, behind, off);
     if (p.dout)
-        load_rows<T, V, ROWS>(d, p.dout, p.dout_rs, w0, behind, off);
+        load_rows(d, p.dout, p.dout_rs, w0, behind, off);
     else
 #pragma unroll
-        for (int j = 0; j < ROWS; ++j) d[j].w = 0;
-    float strength[V], h[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) strength[v] = p.strength[col + v], h[v] = p.saved[same * p.width + col + v];
+        for (int j = 0; j < ROWS; ++j) d[j] = (T)0.f;
+    const float strength = p.strength[col], natural = strength * (1 / kLog2e);
+    float h = p.saved[same * p.width + col];
     map.template find<64 * WAVES>(p, taken);
-    Gates<T> g[ROWS][V];
+    Gates<T> g[ROWS];
 #pragma unroll
-    for (int j = 0; j < ROWS; ++j)
-#pragma unroll
-        for (int v = 0; v < V; ++v) g[j][v] = Gates<T>(r[j].get(v), i[j].get(v), strength[v]);
+    for (int j = 0; j < ROWS; ++j) g[j] = Gates<T>((float)r[j], (float)i[j], strength);
     __syncthreads();
     const uint64_t bits = marks(map.begins), end_bits = marks(map.ends);
     const unsigned begins = marks_of<ROWS>(bits, wave), ends = marks_of<ROWS>(end_bits, wave);
@@ -642,154 +564,115 @@ __global__ __launch_bounds__(64 * WAVES, 4) void hstu_scan_bwd_kernel(const Scan
         else
             pass(std::false_type{});
     };
-    auto before = [&](auto all, int j, int v, float now) {  // h in front of row j
+    auto before = [&](auto all, int j, float now) {  // h in front of row j
         if (decltype(all)::value || !(begins >> j & 1)) return now;
-        return p.initial ? p.initial[(int64_t)map.begins[wave * ROWS + j] * p.width + col + v] : 0.f;
+        return p.initial ? p.initial[(int64_t)map.begins[wave * ROWS + j] * p.width + col] : 0.f;
     };
-    auto from_behind = [&](auto all, int j, float now) { return decltype(all)::value || !(ends >> j & 1) ? now : 0.f; };  // c from behind row j
-    float A[V], H[V], C[V], G[ROWS][V];  // G: dh as yet
+    auto from_behind = [&](auto all, int j, float now) { return decltype(all)::value || !(ends >> j & 1) ? now : 0.f; };  // c
+    float A = 1.f, H = 0.f, C = 0.f, G[ROWS];  // G: dh as yet
 #pragma unroll
-    for (int j = 0; j < ROWS; ++j)
-#pragma unroll
-        for (int v = 0; v < V; ++v) G[j][v] = w0 + j < behind ? d[j].get(v) : 0.f;
+    for (int j = 0; j < ROWS; ++j) G[j] = w0 + j < behind ? (float)d[j] : 0.f;
     if (p.dfinal && ends)
 #pragma unroll
         for (int j = 0; j < ROWS; ++j)
-            if (ends >> j & 1)
-#pragma unroll
-                for (int v = 0; v < V; ++v) G[j][v] += p.dfinal[(int64_t)map.ends[wave * ROWS + j] * p.width + col + v];
+            if (ends >> j & 1) G[j] += p.dfinal[(int64_t)map.ends[wave * ROWS + j] * p.width + col];
     either([&](auto all) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            A[v] = 1.f, H[v] = C[v] = 0.f;
-#pragma unroll
-            for (int j = 0; j < ROWS; ++j) {
-                H[v] = __builtin_fmaf(g[j][v].a, before(all, j, v, H[v]), g[j][v].m * g[j][v].si * x[j].get(v));
-                A[v] *= g[j][v].a;
-            }
-#pragma unroll
-            for (int j = ROWS - 1; j >= 0; --j) C[v] = g[j][v].a * (G[j][v] + from_behind(all, j, C[v]));
+        for (int j = 0; j < ROWS; ++j) {
+            H = __builtin_fmaf(g[j].a, before(all, j, H), g[j].m * g[j].si * (float)x[j]);
+            A *= g[j].a;
         }
-    });
 #pragma unroll
-    for (int v = 0; v < V; ++v) sums[wave][lane * V + v] = float2{A[v], H[v]}, passed[wave][lane * V + v] = C[v];
+        for (int j = ROWS - 1; j >= 0; --j) C = g[j].a * (G[j] + from_behind(all, j, C));
+    });
+    sums[wave][lane] = float2{A, H}, passed[wave][lane] = C;
     __syncthreads();
     // h in front of the wave's rows
 #pragma unroll 1  // (all parts at once would take the registers of the rows)
     for (int w = 0; w < wave; ++w) {
-        const bool begun = marks_of<ROWS>(bits, w) != 0;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const float2 s = sums[w][lane * V + v];
-            h[v] = begun ? s.y : __builtin_fmaf(s.x, h[v], s.y);
-        }
+        const float2 s = sums[w][lane];
+        h = marks_of<ROWS>(bits, w) ? s.y : __builtin_fmaf(s.x, h, s.y);
     }
     // c from the waves behind
-    float fA[V], fC[V];
+    float fA = 1.f, fC = 0.f;
     bool cut = false;
-#pragma unroll
-    for (int v = 0; v < V; ++v) fA[v] = 1.f, fC[v] = 0.f;
 #pragma unroll 1
     for (int w = WAVES - 1; w > wave; --w) {
         const bool ended = marks_of<ROWS>(end_bits, w) != 0;
+        const float by = sums[w][lane].x, c = passed[w][lane];
         cut = cut || ended;
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const float by = sums[w][lane * V + v].x, c = passed[w][lane * V + v];
-            fC[v] = ended ? c : __builtin_fmaf(by, fC[v], c);
-            fA[v] = by * fA[v];
-        }
+        fC = ended ? c : __builtin_fmaf(by, fC, c), fA *= by;
     }
     const bool needs = turned > 0 && !(end_bits >> (kTile - 1));
-    float from[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) C[v] = ends ? C[v] : __builtin_fmaf(A[v], fC[v], C[v]), A[v] *= fA[v];
-    join_tile<V, WAVES>(p, slot, turned, col, mine, wave == 0, turned == 0 || end_bits, needs, A, C, back, wave, from);
-    if (needs)
-#pragma unroll
-        for (int v = 0; v < V; ++v) fC[v] = cut ? fC[v] : __builtin_fmaf(fA[v], from[v], fC[v]);
+    const float front = join_tile<WAVES>(p, slot, turned, col, mine, wave == 0, turned == 0 || end_bits, needs, A * fA, ends ? C : __builtin_fmaf(A, fC, C), back, wave);
+    if (needs && !cut) fC = __builtin_fmaf(fA, front, fC);
     // G of every row from the last to the first, then the results along with h from the first to the last
-    float sum[V] = {}, natural[V];
+    float sum = 0.f;
+    // Products of gates and x are worked out again below: kept from above they would take registers that there are not.
 #pragma unroll
-    for (int v = 0; v < V; ++v) natural[v] = strength[v] * (1 / kLog2e);
-    // Products of gates and x are worked out again below: kept from above they would take 32 registers that there are not.
-#pragma unroll
-    for (int j = 0; j < ROWS; ++j) {
-        asm("" : "+v"(x[j].w));
-#pragma unroll
-        for (int v = 0; v < V; ++v) asm("" : "+v"(g[j][v].si));
-    }
+    for (int j = 0; j < ROWS; ++j) asm("" : "+v"(g[j].si));
     either([&](auto all) {
         constexpr bool ALL = decltype(all)::value;
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-#pragma unroll
-            for (int j = ROWS - 1; j >= 0; --j) {
-                G[j][v] += from_behind(all, j, fC[v]);
-                fC[v] = g[j][v].a * G[j][v];
-                if (!ALL && p.dinitial && mine && begins >> j & 1) p.dinitial[(int64_t)map.begins[wave * ROWS + j] * p.width + col + v] = fC[v];
-            }
+        for (int j = ROWS - 1; j >= 0; --j) {
+            G[j] += from_behind(all, j, fC);
+            fC = g[j].a * G[j];
+            if (!ALL && p.dinitial && mine && begins >> j & 1) p.dinitial[(int64_t)map.begins[wave * ROWS + j] * p.width + col] = fC;
+        }
 #pragma unroll
         for (int j = 0; j < ROWS; ++j) {
-            float dx[V], dr[V], di[V];
             const bool there = ALL || w0 + j < behind;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const Gates<T>& q = g[j][v];
-                const float u = q.si * x[j].get(v), old = before(all, j, v, h[v]);
-                const float share = q.m > 0.f ? q.s * __builtin_amdgcn_rcpf(q.m) : 0.f;
-                const float dq = G[j][v] * q.a * (u * q.a * share - q.s * old);
-                dx[v] = there ? G[j][v] * (q.m * q.si) : 0.f;
-                dr[v] = there ? natural[v] * (1.f - q.s) * dq : 0.f;
-                di[v] = there ? dx[v] * x[j].get(v) * (1.f - q.si) : 0.f;
-                sum[v] += there ? dq : 0.f;
-                h[v] = __builtin_fmaf(q.a, old, q.m * u);
-            }
-            if (mine && (ALL || w0 + j < behind)) {
+            const Gates<T>& q = g[j];
+            const float u = q.si * (float)x[j], old = before(all, j, h);
+            const float share = q.m > 0.f ? q.s * __builtin_amdgcn_rcpf(q.m) : 0.f;
+            const float dq = G[j] * q.a * (u * q.a * share - q.s * old), dx = G[j] * (q.m * q.si);
+            sum += there ? dq : 0.f;
+            h = __builtin_fmaf(q.a, old, q.m * u);
+            if (mine && there) {
                 if (ALL || p.dx) put(p.dx, dx);
-                if (ALL || p.dr) put(p.dr, dr);
-                if (ALL || p.di) put(p.di, di);
+                if (ALL || p.dr) put(p.dr, natural * (1.f - q.s) * dq);
+                if (ALL || p.di) put(p.di, dx * (float)x[j] * (1.f - q.si));
             }
             at += pitch;
         }
     });
     if (!p.partial) return;
     __syncthreads();
-#pragma unroll
-    for (int v = 0; v < V; ++v) passed[wave][lane * V + v] = sum[v];
+    passed[wave][lane] = sum;
     __syncthreads();
-    if (wave == 0 && mine)
+    if (wave || !mine) return;
+    float total = 0.f;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            float all = 0.f;
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) all += passed[w][lane * V + v];
-            p.partial[same * p.width + col + v] = all;
-        }
+    for (int w = 0; w < WAVES; ++w) total += passed[w][lane];
+    p.partial[same * p.width + col] = total;
 }
 
-// d decay = rate sigmoid(decay) * the sum of `count` partial sums, in 64 bits: 16 columns to a workgroup, 16 parts of the sums.
+// d decay = rate sigmoid(decay) * the sum of `count` partial sums, in 64 bits: 16 columns to a workgroup, 64 parts of the sums, eight of them in flight.
 template <class T>
-__global__ __launch_bounds__(256) void hstu_scan_decay_kernel(const float* partial, int64_t count, int width, const void* decay, int f32, float rate, void* out) {
-    __shared__ double meet[16][17];
+__global__ __launch_bounds__(1024) void hstu_scan_decay_kernel(const float* partial, int64_t count, int width, const void* decay, int f32, float rate, void* out) {
+    __shared__ double meet[64][17];
     const int c = threadIdx.x & 15, part = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
     double sum = 0;
     if (col < width) {
         int64_t k = part;
-        for (; k + 48 < count; k += 64) {
-            float v[4];
+        for (; k + 448 < count; k += 512) {
+            float v[8];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = partial[(k + 16 * q) * width + col];
+            for (int q = 0; q < 8; ++q) v[q] = partial[(k + 64 * q) * width + col];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) sum += v[q];
+            for (int q = 0; q < 8; ++q) sum += v[q];
         }
-        for (; k < count; k += 16) sum += partial[k * width + col];
+        for (; k < count; k += 64) sum += partial[k * width + col];
     }
     meet[part][c] = sum;
     __syncthreads();
-    if (part || col >= width) return;
+    if (part >= 4) return;
+    sum = 0;
 #pragma unroll
-    for (int q = 1; q < 16; ++q) sum += meet[q][c];
+    for (int q = 0; q < 16; ++q) sum += meet[part + 4 * q][c];
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (part || col >= width) return;
     const double d = decay_at<T>(decay, f32, col), v = rate / (1. + exp(-d)) * sum;
     if (f32)
         ((float*)out)[col] = (float)v;

@@ -76,21 +76,7 @@ hstu::ScanParams scan_params(const HstuRecurrenceArgs* a) {
     return p;
 }
 
-// Whether rows are read two columns at a time (in 16 bits).
-bool scan_in_pairs(const HstuRecurrenceArgs* a, const HstuRecurrenceGrads* g) {
-    if (a->dtype == HSTU_FP32 || a->width % 2 != 0) return false;
-    int64_t odd = a->x_row_stride | a->decay_gate_row_stride | a->input_gate_row_stride;
-    bool pairs = true;
-    for (const void* ptr : {a->x, a->decay_gate, a->input_gate, (const void*)(g ? nullptr : a->out)}) pairs = pairs && aligned_to(ptr, 4);
-    if (g) {
-        odd |= g->d_out ? g->d_out_row_stride : 0;
-        for (const void* ptr : {g->d_out, (const void*)g->d_x, (const void*)g->d_decay_gate, (const void*)g->d_input_gate}) pairs = pairs && aligned_to(ptr, 4);
-    }
-    return pairs && odd % 2 == 0;
-}
-
-constexpr int kRows = 16, kWaves = 4;           // of a tile, in the forward
-constexpr int kBackRows = 8, kBackWaves = 8;    // ... and in the backward
+constexpr int kRows = 16, kWaves = 4;           // of a tile, forward and backward
 constexpr int kShortRows = 2, kShortWaves = 8;  // at a time, where sequences are short
 
 // Few rows to a sequence, and no state to save: a workgroup for each sequence.
@@ -98,8 +84,8 @@ bool scan_is_short(const HstuRecurrenceArgs* a) { return !a->saved && a->rows <=
 
 // How the tiles of a call are counted, and what they share, behind one another in the scratch memory.
 struct ScanPlan {
-    int64_t per_segment, segments, slots, words;
-    size_t tiles_at, strength_at, partial_at, bytes;
+    int64_t per_segment, segments, slots;
+    size_t groups_at, states_at, tickets_at, tiles_at, strength_at, partial_at, bytes;  // (what is in front of tiles_at is cleared)
 };
 
 // A segment is a sequence, or as many as have 512 rows on the average: half a tile is lost at its end.
@@ -110,23 +96,26 @@ ScanPlan scan_plan(const HstuRecurrenceArgs* a, bool backward) {
     if (s.per_segment < 1) s.per_segment = 1;
     s.segments = (a->batch + s.per_segment - 1) / s.per_segment;
     s.slots = a->rows / hstu::kTile + s.segments + 2;
-    s.words = (2 * s.slots + s.slots / hstu::kGroup + 1) * a->width + (int64_t)(a->width + 63) / 64 * (hstu::kTicketPitch / 2);
-    s.words += s.words & 1;
-    s.tiles_at = (size_t)s.words * 8;
-    s.strength_at = s.tiles_at + (size_t)s.slots * sizeof(hstu::Tile) + 8;
+    auto up = [](size_t bytes) { return (bytes + 15) / 16 * 16; };
+    s.groups_at = (size_t)s.slots * a->width * 8;
+    s.states_at = s.groups_at + (size_t)(s.slots / hstu::kGroup + 1) * a->width * 8;
+    s.tickets_at = s.states_at + (size_t)s.slots * a->width * 4;
+    s.tiles_at = up(s.tickets_at + (size_t)(a->width + 63) / 64 * hstu::kTicketPitch * 4);
+    s.strength_at = s.tiles_at + (size_t)s.slots * sizeof(hstu::Tile);
     s.partial_at = s.strength_at + (size_t)a->width * 4;
     s.bytes = s.partial_at + (backward ? (size_t)s.slots * a->width * 4 : 0);
     return s;
 }
 
 // Sets `p` for a call: 0, or the status.
-int set_plan(hstu::ScanParams& p, const ScanPlan& s, int cols, bool backward, void* scratch) {
-    p.col_blocks = (p.width + cols - 1) / cols;
+int set_plan(hstu::ScanParams& p, const ScanPlan& s, bool backward, void* scratch) {
+    p.col_blocks = (p.width + 63) / 64;
     if (s.slots > kMaxBlocks / p.col_blocks) return HSTU_ERR_UNSUPPORTED;
     p.segments = (int)s.segments, p.per_segment = (int)s.per_segment, p.slots = (int)s.slots, p.backward = backward;
-    p.sums = (unsigned long long*)scratch, p.states = p.sums + s.slots * p.width, p.groups = p.states + s.slots * p.width;
-    p.tickets = (unsigned*)(p.groups + (s.slots / hstu::kGroup + 1) * p.width), p.clear = s.words;
-    p.tiles = (hstu::Tile*)((char*)scratch + s.tiles_at), p.strength = (float*)((char*)scratch + s.strength_at);
+    char* at = (char*)scratch;
+    p.sums = (unsigned long long*)at, p.groups = (unsigned long long*)(at + s.groups_at), p.states = (unsigned*)(at + s.states_at);
+    p.tickets = (unsigned*)(at + s.tickets_at), p.tiles = (hstu::Tile*)(at + s.tiles_at), p.strength = (float*)(at + s.strength_at);
+    p.clear = (int64_t)(s.tiles_at / 16);
     return 0;
 }
 
@@ -174,22 +163,15 @@ int hstu_recurrent_scan(const HstuRecurrenceArgs* a, void* stream) {
     if (!a->workspace) return HSTU_ERR_NULL_POINTER;
     if (!aligned_to(a->workspace, 16)) return HSTU_ERR_MISALIGNED;
     if (a->workspace_bytes < (int64_t)need) return HSTU_ERR_BAD_SHAPE;
-    const bool pairs = scan_in_pairs(a, nullptr);
-    const int status = set_plan(p, scan_plan(a, false), pairs ? 128 : 64, false, a->workspace);
+    const int status = set_plan(p, scan_plan(a, false), false, a->workspace);
     if (status) return status;
     if (!device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
     const int cleared = launch_begin(a->dtype, p, (hipStream_t)stream);
     if (cleared || a->rows == 0) return cleared;
     return with_type(a->dtype, [&](auto* t) {
-        typedef std::remove_pointer_t<decltype(t)> T;
-        auto launch = [&](auto v) {
-            hipLaunchKernelGGL((hstu::hstu_scan_kernel<T, decltype(v)::value, kRows, kWaves>), dim3((unsigned)(p.slots * p.col_blocks)), dim3(64 * kWaves), 0,
-                               (hipStream_t)stream, p);
-            return launch_status("recurrence kernel launch");
-        };
-        if constexpr (sizeof(T) == 2)
-            if (pairs) return launch(std::integral_constant<int, 2>{});
-        return launch(std::integral_constant<int, 1>{});
+        hipLaunchKernelGGL((hstu::hstu_scan_kernel<std::remove_pointer_t<decltype(t)>, kRows, kWaves>), dim3((unsigned)(p.slots * p.col_blocks)), dim3(64 * kWaves), 0,
+                           (hipStream_t)stream, p);
+        return launch_status("recurrence kernel launch");
     });
 }
 
@@ -214,9 +196,8 @@ int hstu_recurrent_scan_bwd(const HstuRecurrenceArgs* a, const HstuRecurrenceGra
     p.saved = a->saved;
     p.dout = (const char*)g->d_out, p.dout_rs = g->d_out_row_stride, p.dfinal = g->d_final_state;
     p.dx = (char*)g->d_x, p.dr = (char*)g->d_decay_gate, p.di = (char*)g->d_input_gate, p.dinitial = g->d_initial_state;
-    const bool pairs = scan_in_pairs(a, g);
     const ScanPlan plan = scan_plan(a, true);
-    const int status = set_plan(p, plan, pairs ? 128 : 64, true, g->workspace);
+    const int status = set_plan(p, plan, true, g->workspace);
     if (status) return status;
     if (g->d_decay) p.partial = (float*)((char*)g->workspace + plan.partial_at);
     if (!device_is_gfx950()) return HSTU_ERR_BAD_DEVICE;
@@ -226,21 +207,13 @@ int hstu_recurrent_scan_bwd(const HstuRecurrenceArgs* a, const HstuRecurrenceGra
     if (cleared) return cleared;
     return with_type(a->dtype, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
-        auto launch = [&](auto v) {
-            hipLaunchKernelGGL((hstu::hstu_scan_bwd_kernel<T, decltype(v)::value, kBackRows, kBackWaves>), dim3((unsigned)(p.slots * p.col_blocks)),
-                               dim3(64 * kBackWaves), 0, (hipStream_t)stream, p);
-            return launch_status("recurrence backward kernel launch");
-        };
-        int rows = 0;
         if (a->rows > 0) {
-            rows = [&] {
-                if constexpr (sizeof(T) == 2)
-                    if (pairs) return launch(std::integral_constant<int, 2>{});
-                return launch(std::integral_constant<int, 1>{});
-            }();
+            hipLaunchKernelGGL((hstu::hstu_scan_bwd_kernel<T, kRows, kWaves>), dim3((unsigned)(p.slots * p.col_blocks)), dim3(64 * kWaves), 0, (hipStream_t)stream, p);
+            const int rows = launch_status("recurrence backward kernel launch");
+            if (rows) return rows;
         }
-        if (rows || !g->d_decay) return rows;
-        hipLaunchKernelGGL((hstu::hstu_scan_decay_kernel<T>), dim3((a->width + 15) / 16), dim3(256), 0, (hipStream_t)stream, p.partial, plan.slots, a->width, a->decay,
+        if (!g->d_decay) return 0;
+        hipLaunchKernelGGL((hstu::hstu_scan_decay_kernel<T>), dim3((a->width + 15) / 16), dim3(1024), 0, (hipStream_t)stream, p.partial, plan.slots, a->width, a->decay,
                            a->decay_f32, a->rate, g->d_decay);
         return launch_status("recurrence decay gradient kernel launch");
     });
