@@ -365,10 +365,11 @@ int hstu_recurrent_residual_norm_bwd(const HstuResidualNormArgs* a, const HstuRe
     p.dx = (char*)g->d_x, p.dy = (char*)g->d_y, p.dgate = a->gate ? (char*)g->d_gate : nullptr;
     void* to[hstu::P_COUNT] = {g->d_post_weight, g->d_post_bias, g->d_scale, g->d_pre_weight, g->d_pre_bias};
     hstu::ParameterGrads grads{};
+    int wanted = 0;
     for (int k = 0; k < hstu::P_COUNT; ++k)
         if (to[k] && p.param[k]) {
             if (!aligned_to(to[k], es)) return HSTU_ERR_MISALIGNED;
-            p.wanted |= 1 << k, grads.out[k] = to[k];
+            p.wanted |= 1 << k, grads.out[wanted] = to[k], grads.which[wanted++] = k;
         }
     if (p.wanted) {
         if (!g->workspace) return HSTU_ERR_NULL_POINTER;
@@ -387,7 +388,7 @@ int hstu_recurrent_residual_norm_bwd(const HstuResidualNormArgs* a, const HstuRe
             return launch_status("residual norm backward kernel launch");
         });
         if (status || !p.wanted) return status;
-        hipLaunchKernelGGL((hstu::hstu_residual_norm_sum_kernel<T>), dim3((a->width + 15) / 16, hstu::P_COUNT), dim3(256), 0, (hipStream_t)stream, p.partial, blocks,
+        hipLaunchKernelGGL((hstu::hstu_residual_norm_sum_kernel<T>), dim3((a->width + 15) / 16, wanted), dim3(1024), 0, (hipStream_t)stream, p.partial, blocks,
                            a->width, grads);
         return launch_status("residual norm parameter gradient kernel launch");
     });

@@ -64,17 +64,32 @@ __device__ __forceinline__ void store8(const float (&x)[8], T* row, int col, int
     }
 }
 
+// The sum over a wave, the same in all lanes for the compiler to know: rows of 16 lanes, then pairs of rows and halves by the instruction's broadcasts.
+__device__ __forceinline__ float wave_total(float v) {
+    v = group_sum<16>(v);
+    v += __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x142, 0xa, 0xf, false));
+    v += __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x143, 0xc, 0xf, false));
+    return __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
+}
+
 // Sums over the lanes of a row, in each of them.  More than one wave to a row: `meet` has two halves, which calls take in turn, so that
 // one barrier between write and read is enough.
 template <int LPR>
 struct RowSums {
     float* meet;  // [2][waves of the workgroup][2]
     int turn, wave, first_wave;
-    __device__ __forceinline__ RowSums(float* meet_) : meet(meet_), turn(0), wave(threadIdx.x / 64), first_wave(threadIdx.x / (LPR < 64 ? 64 : LPR) * (LPR < 64 ? 1 : LPR / 64)) {}
+    __device__ __forceinline__ RowSums(float* meet_) : meet(meet_), turn(0), wave(__builtin_amdgcn_readfirstlane(threadIdx.x / 64)) {
+        first_wave = LPR > 64 ? wave / (LPR / 64) * (LPR / 64) : wave;
+    }
     template <int N>
     __device__ __forceinline__ void operator()(float (&v)[N]) {
+        if constexpr (LPR < 64) {
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = group_sum<(LPR < 64 ? LPR : 64)>(v[k]);
+            for (int k = 0; k < N; ++k) v[k] = group_sum<LPR>(v[k]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; ++k) v[k] = wave_total(v[k]);
+        }
         if constexpr (LPR > 64) {
             float* here = meet + turn * 32;
             turn ^= 1;
@@ -93,37 +108,58 @@ struct RowSums {
     }
 };
 
-// v to v^, and r.  `mine`: how many of the lane's columns there are (the others hold another's).
-template <class SUMS>
-__device__ __forceinline__ float normalise(float (&v)[8], int mine, const ResidualNormParams& p, SUMS& sums) {
-    if (p.layer_norm) {
-        float m[1] = {0.f};
+// What of a lane's eight columns there is: all or none where rows are ALIGNED, else the first `count`.  The others hold columns that are another's.
+template <bool ALIGNED>
+struct Mine {
+    int count;
+    template <class F>
+    __device__ __forceinline__ float sum(F&& term) const {
+        float v = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m[0] += i < mine ? v[i] : 0.f;
-        sums(m);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] -= m[0] * p.inv_width;
+        for (int i = 0; i < 8; ++i)
+            if constexpr (ALIGNED)
+                v += term(i);
+            else
+                v += i < count ? term(i) : 0.f;
+        return !ALIGNED || count ? v : 0.f;
     }
-    float q[1] = {0.f};
+};
+
+// v to v^, and r: the instruction's root, good to a unit in the last place, corrected once by its residual.
+template <bool ALIGNED, class SUMS>
+__device__ __forceinline__ float normalise(float (&v)[8], const Mine<ALIGNED>& mine, const ResidualNormParams& p, SUMS& sums) {
+    if (p.layer_norm) {
+        float m[1] = {mine.sum([&](int i) { return v[i]; })};
+        sums(m);
+        m[0] *= p.inv_width;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[0] += i < mine ? v[i] * v[i] : 0.f;
+        for (int i = 0; i < 8; ++i) v[i] -= m[0];
+    }
+    float q[1] = {mine.sum([&](int i) { return v[i] * v[i]; })};
     sums(q);
-    const float r = 1.f / sqrtf(q[0] * p.inv_width + p.eps);
+    const float x = q[0] * p.inv_width + p.eps, r0 = __builtin_amdgcn_rsqf(x), h = x * r0, low = __builtin_fmaf(x, r0, -h);
+    const float fixed = __builtin_fmaf(0.5f * r0, __builtin_fmaf(-low, r0, __builtin_fmaf(-h, r0, 1.f)), r0), r = x > 0x1p-100f && x < 0x1p100f ? fixed : r0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] *= r;
     return r;
 }
 
 // g to N(g, v).
-template <class SUMS>
-__device__ __forceinline__ void normalise_grad(float (&g)[8], const float (&unit)[8], float r, int mine, const ResidualNormParams& p, SUMS& sums) {
-    float d[2] = {0.f, 0.f};
+template <bool ALIGNED, class SUMS>
+__device__ __forceinline__ void normalise_grad(float (&g)[8], const float (&unit)[8], float r, const Mine<ALIGNED>& mine, const ResidualNormParams& p, SUMS& sums) {
+    if (p.layer_norm) {
+        float d[2] = {mine.sum([&](int i) { return g[i] * unit[i]; }), mine.sum([&](int i) { return g[i]; })};
+        sums(d);
+        const float along = d[0] * p.inv_width, mean = d[1] * p.inv_width;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) d[0] += i < mine ? g[i] * unit[i] : 0.f, d[1] += i < mine ? g[i] : 0.f;
-    sums(d);
-    const float along = d[0] * p.inv_width, mean = p.layer_norm ? d[1] * p.inv_width : 0.f;
+        for (int i = 0; i < 8; ++i) g[i] = r * (__builtin_fmaf(-unit[i], along, g[i]) - mean);
+    } else {
+        float d[1] = {mine.sum([&](int i) { return g[i] * unit[i]; })};
+        sums(d);
+        const float along = d[0] * p.inv_width;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] = r * (g[i] - unit[i] * along - mean);
+        for (int i = 0; i < 8; ++i) g[i] = r * __builtin_fmaf(-unit[i], along, g[i]);
+    }
 }
 
 // keep / (1 - p) of eight elements from number `at` on.
@@ -146,31 +182,70 @@ __device__ __forceinline__ void kept8(const DropoutParams& d, uint64_t at, float
     }
 }
 
-// act(gate) and its derivative.
-__device__ __forceinline__ void activate(int act, float g, float& value, float& slope) {
-    value = g, slope = 1.f;
+// act(gate), and its derivative.
+__device__ __forceinline__ void activate(int act, const float (&g)[8], float (&value)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) value[i] = g[i];
     if (act == ACT_NONE) return;
-    const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * g));
-    value = act == ACT_SIGMOID ? s : g * s;
-    slope = act == ACT_SIGMOID ? s * (1.f - s) : s * (1.f + g * (1.f - s));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) value[i] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * g[i]));
+    if (act == ACT_SILU)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) value[i] *= g[i];
+}
+__device__ __forceinline__ void activate(int act, const float (&g)[8], float (&value)[8], float (&slope)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) value[i] = g[i], slope[i] = 1.f;
+    if (act == ACT_NONE) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        value[i] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * g[i]));
+        slope[i] = value[i] - value[i] * value[i];
+    }
+    if (act == ACT_SILU)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) slope[i] = __builtin_fmaf(g[i], slope[i], value[i]), value[i] *= g[i];
 }
 
+// A row of parameters, as it lies in memory.
+template <class T, bool ALIGNED>
+__device__ __forceinline__ void load_parameters(Cols<T> (&param)[P_COUNT], const ResidualNormParams& p, int col) {
+#pragma unroll
+    for (int k = 0; k < P_COUNT; ++k)
+        if (p.param[k]) load8<T, ALIGNED>(param[k], (const T*)p.param[k], col, p.width);
+}
+// v times one of them, v plus one of them: where there is one.
+template <class T>
+__device__ __forceinline__ void times(float (&v)[8], const Cols<T>& c, const char* there) {
+    if (!there) return;
+    float w[8];
+    c.get(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= w[i];
+}
+template <class T>
+__device__ __forceinline__ void plus(float (&v)[8], const Cols<T>& c, const char* there) {
+    if (!there) return;
+    float w[8];
+    c.get(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += w[i];
+}
+
+// 151302 rows of 1024 columns, layer norms with a gate: FWD_US us (1.55 GB).
 template <class T, int LPR, bool ALIGNED>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_residual_norm_kernel(const ResidualNormParams p) {
     constexpr int THREADS = LPR > 256 ? LPR : 256, GROUPS = THREADS / LPR;
     __shared__ float meet[64];
     RowSums<LPR> sums(meet);
     const int l = threadIdx.x % LPR;
-    const bool cols = 8 * l < p.width;
-    const int col = cols ? 8 * l : 0;
-    const int mine = min(max(p.width - 8 * l, 0), 8);
+    const Mine<ALIGNED> mine{min(max(p.width - 8 * l, 0), 8)};
+    const int col = mine.count ? 8 * l : 0;
     Cols<T> param[P_COUNT];
-#pragma unroll
-    for (int k = 0; k < P_COUNT; ++k)
-        if (p.param[k]) load8<T, ALIGNED>(param[k], (const T*)p.param[k], col, p.width);
+    load_parameters<T, ALIGNED>(param, p, col);
     for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < p.rows; base += (int64_t)gridDim.x * GROUPS) {
         const int64_t at = base + threadIdx.x / LPR, row = at < p.rows ? at : p.rows - 1;
-        const bool store = cols && at < p.rows;
+        const bool store = mine.count && at < p.rows;
         Cols<T> cx, cy, cg;
         load8<T, ALIGNED>(cy, (const T*)p.y + row * p.y_rs, col, p.width);
         if (p.gate) load8<T, ALIGNED>(cg, (const T*)p.gate + row * p.gate_rs, col, p.width);
@@ -179,53 +254,36 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_residual_norm_kern
         cy.get(v);
         if (p.param[P_POST_WEIGHT]) {
             normalise(v, mine, p, sums);
-            param[P_POST_WEIGHT].get(w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] *= w[i];
-            if (p.param[P_POST_BIAS]) {
-                param[P_POST_BIAS].get(w);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] += w[i];
-            }
+            times(v, param[P_POST_WEIGHT], p.param[P_POST_WEIGHT]);
+            plus(v, param[P_POST_BIAS], p.param[P_POST_BIAS]);
         }
         if (p.gate) {
+            float value[8];
             cg.get(w);
+            activate(p.act, w, value);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float value, slope;
-                activate(p.act, w[i], value, slope);
-                v[i] *= value;
-            }
+            for (int i = 0; i < 8; ++i) v[i] *= value[i];
         }
         if (p.drop.thresh) {
             kept8<ALIGNED>(p.drop, (uint64_t)row * p.width + col, w);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = w[i] != 0.f ? v[i] * w[i] : 0.f;
+            for (int i = 0; i < 8; ++i) v[i] = w[i] != 0.f ? v[i] * w[i] : 0.f;  // (what is dropped may be an infinity)
         }
-        if (p.param[P_SCALE]) {
-            param[P_SCALE].get(w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] *= w[i];
-        }
+        times(v, param[P_SCALE], p.param[P_SCALE]);
         cx.get(w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] += w[i];
         if (store) store8<T, ALIGNED>(v, (T*)p.out + row * p.width, col, p.width);
-        if (p.param[P_PRE_WEIGHT]) {
-            normalise(v, mine, p, sums);
-            param[P_PRE_WEIGHT].get(w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] *= w[i];
-            if (p.param[P_PRE_BIAS]) {
-                param[P_PRE_BIAS].get(w);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] += w[i];
-            }
-            if (store) store8<T, ALIGNED>(v, (T*)p.normed + row * p.width, col, p.width);
-        }
+        if (!p.param[P_PRE_WEIGHT]) continue;
+        normalise(v, mine, p, sums);
+        times(v, param[P_PRE_WEIGHT], p.param[P_PRE_WEIGHT]);
+        plus(v, param[P_PRE_BIAS], p.param[P_PRE_BIAS]);
+        if (store) store8<T, ALIGNED>(v, (T*)p.normed + row * p.width, col, p.width);
     }
 }
 
+// Results of the forward are worked out again; a group of lanes adds up the parameters' gradients over its rows, in a workgroup the groups meet in LDS, and
+// the kernel below adds the workgroups'.
 template <class T, int LPR, bool ALIGNED>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_residual_norm_bwd_kernel(const ResidualNormParams p) {
     constexpr int THREADS = LPR > 256 ? LPR : 256, GROUPS = THREADS / LPR;
@@ -233,101 +291,93 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_residual_norm_bwd_
     __shared__ float groups[THREADS * 8];
     RowSums<LPR> sums(meet);
     const int l = threadIdx.x % LPR;
-    const bool cols = 8 * l < p.width;
-    const int col = cols ? 8 * l : 0;
-    const int mine = min(max(p.width - 8 * l, 0), 8);
+    const Mine<ALIGNED> mine{min(max(p.width - 8 * l, 0), 8)};
+    const int col = mine.count ? 8 * l : 0;
     float total[P_COUNT][8];
 #pragma unroll
     for (int k = 0; k < P_COUNT; ++k)
 #pragma unroll
         for (int i = 0; i < 8; ++i) total[k][i] = 0.f;
     Cols<T> param[P_COUNT];
-#pragma unroll
-    for (int k = 0; k < P_COUNT; ++k)
-        if (p.param[k]) load8<T, ALIGNED>(param[k], (const T*)p.param[k], col, p.width);
+    load_parameters<T, ALIGNED>(param, p, col);
+    const bool post = p.param[P_POST_WEIGHT];
     for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < p.rows; base += (int64_t)gridDim.x * GROUPS) {
         const int64_t at = base + threadIdx.x / LPR, row = at < p.rows ? at : p.rows - 1;
-        const bool store = cols && at < p.rows;
-        const float counts = at < p.rows ? 1.f : 0.f;
+        const bool there = at < p.rows, store = mine.count && there;
         Cols<T> cx, cy, cg, cd, cn;
         load8<T, ALIGNED>(cy, (const T*)p.y + row * p.y_rs, col, p.width);
         if (p.gate) load8<T, ALIGNED>(cg, (const T*)p.gate + row * p.gate_rs, col, p.width);
         load8<T, ALIGNED>(cx, (const T*)p.x + row * p.x_rs, col, p.width);
         if (p.dout) load8<T, ALIGNED>(cd, (const T*)p.dout + row * p.dout_rs, col, p.width);
         if (p.dnormed) load8<T, ALIGNED>(cn, (const T*)p.dnormed + row * p.dnormed_rs, col, p.width);
-        // forward again: unit = y^, n, act(gate), its slope, keep, s
-        float unit[8], n[8], value[8], slope[8], keep[8], s[8], w[8];
+        // a group behind the last row goes along with it, without its gradients
+#pragma unroll
+        for (int i = 0; i < Cols<T>::WORDS; ++i) cd.w[i] = there && p.dout ? cd.w[i] : 0, cn.w[i] = there ? cn.w[i] : 0;
+        // forward again: unit = y^, branch = act(gate) n as dropped
+        float unit[8], n[8], value[8], slope[8], keep[8], branch[8], w[8], d[8];
         float r = 1.f;
         cy.get(unit);
-        if (p.param[P_POST_WEIGHT]) r = normalise(unit, mine, p, sums);
+        if (post) r = normalise(unit, mine, p, sums);
 #pragma unroll
         for (int i = 0; i < 8; ++i) n[i] = unit[i];
-        if (p.param[P_POST_WEIGHT]) {
-            param[P_POST_WEIGHT].get(w);
+        times(n, param[P_POST_WEIGHT], p.param[P_POST_WEIGHT]);
+        plus(n, param[P_POST_BIAS], p.param[P_POST_BIAS]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) n[i] *= w[i];
-        }
-        if (p.param[P_POST_BIAS]) {
-            param[P_POST_BIAS].get(w);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) n[i] += w[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) value[i] = 1.f, slope[i] = 0.f, keep[i] = 1.f;
+        for (int i = 0; i < 8; ++i) branch[i] = n[i];
         if (p.gate) {
             cg.get(w);
+            activate(p.act, w, value, slope);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) activate(p.act, w[i], value[i], slope[i]);
+            for (int i = 0; i < 8; ++i) branch[i] *= value[i];
         }
-        if (p.drop.thresh) kept8<ALIGNED>(p.drop, (uint64_t)row * p.width + col, keep);
-        float scale[8];
+        if (p.drop.thresh) {
+            kept8<ALIGNED>(p.drop, (uint64_t)row * p.width + col, keep);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) scale[i] = 1.f;
-        if (p.param[P_SCALE]) param[P_SCALE].get(scale);
-        float d[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = 0.f;
-        if (p.dout) cd.get(d);
+            for (int i = 0; i < 8; ++i) branch[i] = keep[i] != 0.f ? branch[i] * keep[i] : 0.f;
+        }
+        cd.get(d);
         if (p.dnormed) {
-            cx.get(s);
+            float s[8], g[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] += keep[i] != 0.f ? n[i] * value[i] * keep[i] * scale[i] : 0.f;
+            for (int i = 0; i < 8; ++i) s[i] = branch[i];
+            times(s, param[P_SCALE], p.param[P_SCALE]);
+            cx.get(w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] += w[i];
             const float rs = normalise(s, mine, p, sums);
-            float g[8];
             cn.get(g);
-            param[P_PRE_WEIGHT].get(w);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                total[P_PRE_WEIGHT][i] += counts != 0.f ? g[i] * s[i] : 0.f;
-                total[P_PRE_BIAS][i] += counts != 0.f ? g[i] : 0.f;
-                g[i] *= w[i];
-            }
+            for (int i = 0; i < 8; ++i) total[P_PRE_WEIGHT][i] = __builtin_fmaf(g[i], s[i], total[P_PRE_WEIGHT][i]);
+            if (p.param[P_PRE_BIAS])
+#pragma unroll
+                for (int i = 0; i < 8; ++i) total[P_PRE_BIAS][i] += g[i];
+            times(g, param[P_PRE_WEIGHT], p.param[P_PRE_WEIGHT]);
             normalise_grad(g, s, rs, mine, p, sums);
 #pragma unroll
             for (int i = 0; i < 8; ++i) d[i] += g[i];
         }
         if (p.dx && store) store8<T, ALIGNED>(d, (T*)p.dx + row * p.width, col, p.width);
+        if (p.param[P_SCALE]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            total[P_SCALE][i] += counts != 0.f && keep[i] != 0.f ? d[i] * n[i] * value[i] * keep[i] : 0.f;
-            d[i] = keep[i] != 0.f ? d[i] * scale[i] * keep[i] : 0.f;
+            for (int i = 0; i < 8; ++i) total[P_SCALE][i] = __builtin_fmaf(d[i], branch[i], total[P_SCALE][i]);
+            times(d, param[P_SCALE], p.param[P_SCALE]);
         }
-        if (p.dgate && store) {
+        if (p.drop.thresh)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[i] = keep[i] != 0.f ? d[i] * keep[i] : 0.f;
+        if (p.gate) {
             float g[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) g[i] = d[i] * n[i] * slope[i];
-            store8<T, ALIGNED>(g, (T*)p.dgate + row * p.width, col, p.width);
+            for (int i = 0; i < 8; ++i) g[i] = d[i] * n[i] * slope[i], d[i] *= value[i];
+            if (p.dgate && store) store8<T, ALIGNED>(g, (T*)p.dgate + row * p.width, col, p.width);
         }
+        if (post) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] *= value[i];
-        if (p.param[P_POST_WEIGHT]) {
-            param[P_POST_WEIGHT].get(w);
+            for (int i = 0; i < 8; ++i) total[P_POST_WEIGHT][i] = __builtin_fmaf(d[i], unit[i], total[P_POST_WEIGHT][i]);
+            if (p.param[P_POST_BIAS])
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                total[P_POST_WEIGHT][i] += counts != 0.f ? d[i] * unit[i] : 0.f;
-                total[P_POST_BIAS][i] += counts != 0.f ? d[i] : 0.f;
-                d[i] *= w[i];
-            }
+                for (int i = 0; i < 8; ++i) total[P_POST_BIAS][i] += d[i];
+            times(d, param[P_POST_WEIGHT], p.param[P_POST_WEIGHT]);
             normalise_grad(d, unit, r, mine, p, sums);
         }
         if (p.dy && store) store8<T, ALIGNED>(d, (T*)p.dy + row * p.width, col, p.width);
@@ -342,29 +392,43 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_residual_norm_bwd_
         for (int c = threadIdx.x; c < p.width; c += THREADS) {
             double v = 0;
             for (int g = 0; g < GROUPS; ++g) v += groups[g * LPR * 8 + c];
-            p.partial[((int64_t)blockIdx.x * P_COUNT + k) * p.width + c] = (float)v;
+            p.partial[((int64_t)k * gridDim.x + blockIdx.x) * p.width + c] = (float)v;
         }
     }
 }
 
-// Parameter k's gradient: the sum over `workgroups` of partial[workgroup][k][column], in 64 bits.  grid (columns / 16, P_COUNT): 16 parts of 16 columns.
+// A parameter's gradient: the sum over `workgroups` of partial[parameter][workgroup][column], in 64 bits.  grid (columns / 16, parameters that are wanted): 16
+// columns to a workgroup, 64 parts of the sums, eight of them in flight.
 struct ParameterGrads {
     void* out[P_COUNT];
+    int which[P_COUNT];
 };
 template <class T>
-__global__ __launch_bounds__(256) void hstu_residual_norm_sum_kernel(const float* partial, int64_t workgroups, int width, const ParameterGrads to) {
-    __shared__ double meet[16][17];
-    const int k = blockIdx.y, c = threadIdx.x & 15, part = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
-    if (!to.out[k]) return;
+__global__ __launch_bounds__(1024) void hstu_residual_norm_sum_kernel(const float* partial, int64_t workgroups, int width, const ParameterGrads to) {
+    __shared__ double meet[64][17];
+    const int c = threadIdx.x & 15, part = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
+    const float* from = partial + to.which[blockIdx.y] * workgroups * width + col;
     double v = 0;
-    if (col < width)
-        for (int64_t w = part; w < workgroups; w += 16) v += partial[(w * P_COUNT + k) * width + col];
+    if (col < width) {
+        int64_t k = part;
+        for (; k + 448 < workgroups; k += 512) {
+            float x[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) x[q] = from[(k + 64 * q) * width];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v += x[q];
+        }
+        for (; k < workgroups; k += 64) v += from[k * width];
+    }
     meet[part][c] = v;
     __syncthreads();
-    if (part || col >= width) return;
+    if (part >= 4) return;
+    v = 0;
 #pragma unroll
-    for (int i = 1; i < 16; ++i) v += meet[i][c];
-    ((T*)to.out[k])[col] = (T)(float)v;
+    for (int q = 0; q < 16; ++q) v += meet[part + 4 * q][c];
+    v += __shfl_xor(v, 16, 64);
+    v += __shfl_xor(v, 32, 64);
+    if (part == 0 && col < width) ((T*)to.out[blockIdx.y])[col] = (T)(float)v;
 }
 
 }  // namespace hstu
