@@ -202,13 +202,14 @@ def gated_residual_norm(
     Gradients for all tensors; nothing but the inputs is saved.  Tensors with forward-mode tangents are refused.
     """
     params = (post_weight, post_bias, scale, pre_weight, pre_bias)
-    state, drops = None, training and dropout_ratio != 0.0
+    drops = training and dropout_ratio != 0.0
+    ratio = word_seed = word_offset = 0
     if drops:
         _check_residual(x, y, gate, params, gate_activation, dropout_ratio)  # before the generator moves on
-        state = _dropout_state(dropout_ratio, training, x.numel(), x.device, seed)
-    ratio, word_seed, word_offset = state or (0.0, 0, 0)
-    call = (eps, layer_norm, MUL_U_ACTIVATIONS.get(gate_activation, -1), ratio, word_seed & _WORD64, word_offset & _WORD64)
-    out = native.front.gated_residual_norm(x, y, gate, *params, *call)
+        ratio, word_seed, word_offset = _dropout_state(dropout_ratio, training, x.numel(), x.device, seed)
+        word_seed, word_offset = word_seed & _WORD64, word_offset & _WORD64
+    act = MUL_U_ACTIVATIONS.get(gate_activation, -1)
+    out = native.front.gated_residual_norm(x, y, gate, post_weight, post_bias, scale, pre_weight, pre_bias, eps, layer_norm, act, ratio, word_seed, word_offset)
     if out is not None:
         return out
     if not drops:
@@ -222,7 +223,8 @@ def gated_residual_norm(
             out = out * p.view((1,) + tuple(x.shape[1:]))
         return out, None if pre_weight is None else out * 1
     params = tuple(None if p is None else p.contiguous() for p in params)
-    return _served(native.front.gated_residual_norm(_flat(x), _flat(y), None if gate is None else _flat(gate), *params, *call), "gated_residual_norm")
+    return _served(native.front.gated_residual_norm(_flat(x), _flat(y), None if gate is None else _flat(gate), *params, eps, layer_norm, act, ratio, word_seed,
+                                                    word_offset), "gated_residual_norm")
 
 
 def _check_residual(x, y, gate, params, gate_activation: str, dropout_ratio: float) -> None:
