@@ -99,18 +99,34 @@ struct ScanParams {
     float* partial;  // [slots][width], or null
 };
 
-// ROWS rows of a column of a tensor from row w0 on, the last one in front of `behind` again where there are no more.  Row addresses are the wave's, not
-// the lane's (`off`: bytes).
-template <class T, int ROWS>
-__device__ __forceinline__ void load_rows(T (&to)[ROWS], const char* base, int64_t rs, int64_t w0, int64_t behind, unsigned off) {
-    const char* row = base + min(w0, behind - 1) * rs * (int64_t)sizeof(T);
-    const int left = (int)min(behind - w0, (int64_t)ROWS);
-#pragma unroll
-    for (int j = 0; j < ROWS; ++j) {
-        to[j] = *(const T*)(row + off);
-        row += j + 1 < left ? rs * (int64_t)sizeof(T) : 0;
+// The rows of a tensor from one on, through a buffer descriptor: a row's offset is the wave's, a column's the lane's, and the device checks their sum, so that
+// what lies behind the last row (and what is meant for no column) is read as zero and not written at all.  A wave's sixteen rows at most.
+struct RowsFrom {
+    __amdgpu_buffer_rsrc_t at;
+    unsigned pitch;  // bytes from row to row: at most 2^26, so that sixteen rows end below 2^31
+    __device__ __forceinline__ RowsFrom(const char* base, int64_t pitch_, int64_t row, int64_t behind, unsigned bytes) : pitch((unsigned)pitch_) {
+        const int64_t rows = behind - row < 16 ? behind - row : 16;
+        const uint64_t first = (uint64_t)base + row * pitch_;
+        const unsigned size = base && rows > 0 ? (unsigned)(rows - 1) * pitch + bytes : 0;
+        at = __builtin_amdgcn_make_buffer_rsrc((void*)first, (short)0, (int)size, 0x00020000);
     }
-}
+    template <class T>
+    __device__ __forceinline__ T load(int j, unsigned off) const {
+        if constexpr (sizeof(T) == 4)
+            return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(at, (int)off, (int)(j * pitch), 0));
+        else
+            return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(at, (int)off, (int)(j * pitch), 0));
+    }
+    template <class T>
+    __device__ __forceinline__ void store(int j, unsigned off, float x) const {
+        const T v = (T)x;
+        if constexpr (sizeof(T) == 4)
+            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), at, (int)off, (int)(j * pitch), 0);
+        else
+            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, v), at, (int)off, (int)(j * pitch), 0);
+    }
+};
+constexpr unsigned kNowhere = 0x80000000u;  // the offset of a column that there is not, for stores: sizes and rows' offsets are below it
 
 // Rows behind the last sequence, or 0.
 __device__ __forceinline__ int64_t rows_end(const ScanParams& p) {
@@ -427,20 +443,21 @@ __global__ __launch_bounds__(64 * WAVES, 6) void hstu_scan_kernel(const ScanPara
     __syncthreads();
     const int at = __builtin_amdgcn_readfirstlane(taken.at), slot = __builtin_amdgcn_readfirstlane(taken.slot);
     if (at < 0) return;
-    const int64_t t0 = uniform(taken.first), behind = uniform(taken.behind), w0 = t0 + wave * ROWS, pitch = p.width * (int64_t)sizeof(T);
+    const int64_t behind = uniform(taken.behind), w0 = uniform(taken.first) + wave * ROWS;
     const int col = min(block * 64 + lane, p.width - 1);  // (a lane without a column goes along with the last)
     const bool mine = block * 64 + lane < p.width;
-    const unsigned off = col * (unsigned)sizeof(T);
-    char* out = p.out + w0 * pitch;
+    const unsigned bytes = p.width * (unsigned)sizeof(T), off = col * (unsigned)sizeof(T), off_out = mine ? off : kNowhere;
+    const RowsFrom out(p.out, bytes, w0, behind, bytes);
     if (__builtin_amdgcn_readfirstlane(taken.segment) == p.segments) {  // rows behind the last sequence
-        for (int j = 0; j < ROWS && w0 + j < behind; ++j, out += pitch)
-            if (mine) *(T*)(out + off) = (T)0.f;
+#pragma unroll
+        for (int j = 0; j < ROWS; ++j) out.store<T>(j, off_out, 0.f);
         return;
     }
     T x[ROWS], r[ROWS], i[ROWS];
-    load_rows(r, p.r, p.r_rs, w0, behind, off);
-    load_rows(i, p.i, p.i_rs, w0, behind, off);
-    load_rows(x, p.x, p.x_rs, w0, behind, off);
+    const RowsFrom x_rows(p.x, p.x_rs * sizeof(T), w0, behind, bytes), r_rows(p.r, p.r_rs * sizeof(T), w0, behind, bytes),
+        i_rows(p.i, p.i_rs * sizeof(T), w0, behind, bytes);
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) r[j] = r_rows.load<T>(j, off), i[j] = i_rows.load<T>(j, off), x[j] = x_rows.load<T>(j, off);
     const float strength = p.strength[col];
     map.template find<64 * WAVES>(p, taken);
     float a[ROWS], b[ROWS];
@@ -488,20 +505,13 @@ __global__ __launch_bounds__(64 * WAVES, 6) void hstu_scan_kernel(const ScanPara
     const float front = join_tile<WAVES>(p, slot, at, col, mine, wave == WAVES - 1, at == 0 || bits, needs, A * fA, begins ? H : __builtin_fmaf(A, fH, H), back, wave);
     if (p.saved && wave == 0 && mine) p.saved[(int64_t)(slot + at) * p.width + col] = front;
     H = needs && !cut ? __builtin_fmaf(fA, front, fH) : fH;
-    if (!begins && !(ends && p.final_state) && w0 + ROWS <= behind) {
-        if (mine)
-            rows(std::false_type{}, [&](int) {
-                *(T*)(out + off) = (T)H;
-                out += pitch;
-            });
+    if (!begins && !(ends && p.final_state)) {
+        rows(std::false_type{}, [&](int j) { out.store<T>(j, off_out, H); });
         return;
     }
     rows(std::true_type{}, [&](int j) {
-        if (w0 + j < behind && mine) {
-            *(T*)(out + off) = (T)H;
-            if (p.final_state && ends >> j & 1) p.final_state[(int64_t)map.ends[wave * ROWS + j] * p.width + col] = H;
-        }
-        out += pitch;
+        out.store<T>(j, off_out, H);
+        if (p.final_state && mine && ends >> j & 1) p.final_state[(int64_t)map.ends[wave * ROWS + j] * p.width + col] = H;
     });
 }
 
@@ -522,31 +532,22 @@ __global__ __launch_bounds__(64 * WAVES, 3) void hstu_scan_bwd_kernel(const Scan
     __syncthreads();
     const int turned = __builtin_amdgcn_readfirstlane(taken.at), slot = __builtin_amdgcn_readfirstlane(taken.slot);
     if (turned < 0) return;
-    const int64_t t0 = uniform(taken.first), behind = uniform(taken.behind), w0 = t0 + wave * ROWS, pitch = p.width * (int64_t)sizeof(T);
+    const int64_t behind = uniform(taken.behind), w0 = uniform(taken.first) + wave * ROWS;
     const int64_t same = slot + __builtin_amdgcn_readfirstlane(taken.in_front);  // the slot that the forward had for this tile
     const int col = min(block * 64 + lane, p.width - 1);
     const bool mine = block * 64 + lane < p.width;
-    const unsigned off = col * (unsigned)sizeof(T);
-    int64_t at = w0 * pitch;  // of a row of the results
-    auto put = [&](char* to, float d) { *(T*)(to + at + off) = (T)d; };
+    const unsigned bytes = p.width * (unsigned)sizeof(T), off = col * (unsigned)sizeof(T), off_out = mine ? off : kNowhere;
+    const RowsFrom dx(p.dx, bytes, w0, behind, bytes), dr(p.dr, bytes, w0, behind, bytes), di(p.di, bytes, w0, behind, bytes);  // (none: nothing is written)
     if (__builtin_amdgcn_readfirstlane(taken.segment) == p.segments) {  // rows behind the last sequence
-        for (int j = 0; j < ROWS && w0 + j < behind; ++j, at += pitch)
-            if (mine) {
-                if (p.dx) put(p.dx, 0.f);
-                if (p.dr) put(p.dr, 0.f);
-                if (p.di) put(p.di, 0.f);
-            }
+#pragma unroll
+        for (int j = 0; j < ROWS; ++j) dx.store<T>(j, off_out, 0.f), dr.store<T>(j, off_out, 0.f), di.store<T>(j, off_out, 0.f);
         return;
     }
     T x[ROWS], r[ROWS], i[ROWS], d[ROWS];
-    load_rows(r, p.r, p.r_rs, w0, behind, off);
-    load_rows(i, p.i, p.i_rs, w0, behind, off);
-    load_rows(x, p.x, p.x_rs, w0, behind, off);
-    if (p.dout)
-        load_rows(d, p.dout, p.dout_rs, w0, behind, off);
-    else
+    const RowsFrom x_rows(p.x, p.x_rs * sizeof(T), w0, behind, bytes), r_rows(p.r, p.r_rs * sizeof(T), w0, behind, bytes),
+        i_rows(p.i, p.i_rs * sizeof(T), w0, behind, bytes), d_rows(p.dout, p.dout_rs * sizeof(T), w0, behind, bytes);  // (no dout: zeros)
 #pragma unroll
-        for (int j = 0; j < ROWS; ++j) d[j] = (T)0.f;
+    for (int j = 0; j < ROWS; ++j) r[j] = r_rows.load<T>(j, off), i[j] = i_rows.load<T>(j, off), x[j] = x_rows.load<T>(j, off), d[j] = d_rows.load<T>(j, off);
     const float strength = p.strength[col], natural = strength * (1 / kLog2e);
     float h = p.saved[same * p.width + col];
     map.template find<64 * WAVES>(p, taken);
@@ -557,7 +558,7 @@ __global__ __launch_bounds__(64 * WAVES, 3) void hstu_scan_bwd_kernel(const Scan
     const uint64_t bits = marks(map.begins), end_bits = marks(map.ends);
     const unsigned begins = marks_of<ROWS>(bits, wave), ends = marks_of<ROWS>(end_bits, wave);
     // Waves whose rows all lie within one sequence have nothing to ask at each.
-    const bool plain = !begins && !ends && w0 + ROWS <= behind && p.dx && p.dr && p.di;
+    const bool plain = !begins && !ends;
     auto either = [&](auto&& pass) {
         if (plain)
             pass(std::true_type{});
@@ -571,7 +572,7 @@ __global__ __launch_bounds__(64 * WAVES, 3) void hstu_scan_bwd_kernel(const Scan
     auto from_behind = [&](auto all, int j, float now) { return decltype(all)::value || !(ends >> j & 1) ? now : 0.f; };  // c
     float A = 1.f, H = 0.f, C = 0.f, G[ROWS];  // G: dh as yet
 #pragma unroll
-    for (int j = 0; j < ROWS; ++j) G[j] = w0 + j < behind ? (float)d[j] : 0.f;
+    for (int j = 0; j < ROWS; ++j) G[j] = (float)d[j];
     if (p.dfinal && ends)
 #pragma unroll
         for (int j = 0; j < ROWS; ++j)
@@ -621,19 +622,15 @@ __global__ __launch_bounds__(64 * WAVES, 3) void hstu_scan_bwd_kernel(const Scan
         }
 #pragma unroll
         for (int j = 0; j < ROWS; ++j) {
-            const bool there = ALL || w0 + j < behind;
             const Gates<T>& q = g[j];
             const float u = q.si * (float)x[j], old = before(all, j, h);
             const float share = q.m > 0.f ? q.s * __builtin_amdgcn_rcpf(q.m) : 0.f;
-            const float dq = G[j] * q.a * (u * q.a * share - q.s * old), dx = G[j] * (q.m * q.si);
-            sum += there ? dq : 0.f;
+            const float dq = G[j] * q.a * (u * q.a * share - q.s * old), dxj = G[j] * (q.m * q.si);
+            sum += dq;  // (G is 0 in rows that there are not)
             h = __builtin_fmaf(q.a, old, q.m * u);
-            if (mine && there) {
-                if (ALL || p.dx) put(p.dx, dx);
-                if (ALL || p.dr) put(p.dr, natural * (1.f - q.s) * dq);
-                if (ALL || p.di) put(p.di, dx * (float)x[j] * (1.f - q.si));
-            }
-            at += pitch;
+            dx.store<T>(j, off_out, dxj);
+            dr.store<T>(j, off_out, natural * (1.f - q.s) * dq);
+            di.store<T>(j, off_out, dxj * (float)x[j] * (1.f - q.si));
         }
     });
     if (!p.partial) return;

@@ -46,6 +46,7 @@ bool known_type(int dtype) { return dtype == HSTU_BF16 || dtype == HSTU_FP16 || 
 int bytes_of(int dtype) { return dtype == HSTU_FP32 ? 4 : 2; }
 bool aligned_to(const void* ptr, int bytes) { return (reinterpret_cast<uintptr_t>(ptr) & (bytes - 1)) == 0; }
 
+constexpr int64_t kMaxPitch = 1 << 24;  // elements from row to row in the recurrence: a wave's sixteen rows are addressed in 31 bits
 constexpr int64_t kMaxBlocks = (1 << 22) - 1;  // a launch has fewer than 2^32 threads in a dimension, and a workgroup at most 1024
 
 // ---- the recurrence ----
@@ -55,7 +56,10 @@ int check_scan(const HstuRecurrenceArgs* a) {
     if (!a) return HSTU_ERR_NULL_POINTER;
     if (!known_type(a->dtype)) return HSTU_ERR_BAD_DTYPE;
     if (a->rows < 0 || a->width <= 0 || a->width > 65535 * 64 || a->batch <= 0 || a->batch > (1 << 30) || !(a->rate > 0.f)) return HSTU_ERR_BAD_SHAPE;
-    if (a->x_row_stride < 0 || a->decay_gate_row_stride < 0 || a->input_gate_row_stride < 0) return HSTU_ERR_BAD_SHAPE;
+    for (int64_t rs : {a->x_row_stride, a->decay_gate_row_stride, a->input_gate_row_stride}) {
+        if (rs < 0) return HSTU_ERR_BAD_SHAPE;
+        if (rs > kMaxPitch) return HSTU_ERR_UNSUPPORTED;
+    }
     if (!a->seq_offsets || !a->decay) return HSTU_ERR_NULL_POINTER;
     if (a->rows > 0 && (!a->x || !a->decay_gate || !a->input_gate)) return HSTU_ERR_NULL_POINTER;
     const int es = bytes_of(a->dtype);
@@ -185,6 +189,7 @@ int hstu_recurrent_scan_bwd(const HstuRecurrenceArgs* a, const HstuRecurrenceGra
     if (rc) return rc;
     if (!g) return HSTU_ERR_NULL_POINTER;
     if (g->d_out_row_stride < 0) return HSTU_ERR_BAD_SHAPE;
+    if (g->d_out_row_stride > kMaxPitch) return HSTU_ERR_UNSUPPORTED;
     if (!g->workspace || (a->rows > 0 && !a->saved)) return HSTU_ERR_NULL_POINTER;
     const int es = bytes_of(a->dtype);
     for (const void* ptr : {g->d_out, (const void*)g->d_x, (const void*)g->d_decay_gate, (const void*)g->d_input_gate})
