@@ -972,13 +972,13 @@ void check_recurrent(int rc) {
 
 bool float_type(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kFloat; }
 
-// [rows, width] or [rows, heads, dim] with the columns of a row side by side, at any distance between rows.
+// [rows, width] or [rows, heads, dim] with the columns of a row side by side, at a distance between rows that the kernels take.
 bool flat_rows(const Tensor& t) {
     if (!t.is_cuda() || t.numel() == 0 || (t.dim() != 2 && t.dim() != 3)) return false;
     const int64_t last = t.dim() - 1;
     if (t.size(last) > 1 && t.stride(last) != 1) return false;
     if (last == 2 && t.size(1) > 1 && t.stride(1) != t.size(2)) return false;
-    return t.size(0) == 1 || t.stride(0) >= 0;
+    return t.size(0) == 1 || (t.stride(0) >= 0 && t.stride(0) <= (1 << 24));
 }
 int64_t flat_pitch(const Tensor& t) { return t.size(0) == 1 ? 0 : t.stride(0); }
 int64_t flat_width(const Tensor& t) { return t.dim() == 3 ? t.size(1) * t.size(2) : t.size(1); }

@@ -47,7 +47,7 @@ int bytes_of(int dtype) { return dtype == HSTU_FP32 ? 4 : 2; }
 bool aligned_to(const void* ptr, int bytes) { return (reinterpret_cast<uintptr_t>(ptr) & (bytes - 1)) == 0; }
 
 constexpr int64_t kMaxPitch = 1 << 24;  // elements from row to row in the recurrence: a wave's sixteen rows are addressed in 31 bits
-constexpr int64_t kMaxBlocks = (1 << 22) - 1;  // a launch has fewer than 2^32 threads in a dimension, and a workgroup at most 1024
+constexpr int64_t kMaxBlocks = (1 << 24) - 1;  // a launch has fewer than 2^32 threads in a dimension, and these workgroups 256
 
 // ---- the recurrence ----
 

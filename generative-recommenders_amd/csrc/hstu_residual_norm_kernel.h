@@ -245,6 +245,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_residual_norm_kern
     load_parameters<T, ALIGNED>(param, p, col);
     for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < p.rows; base += (int64_t)gridDim.x * GROUPS) {
         const int64_t at = base + threadIdx.x / LPR, row = at < p.rows ? at : p.rows - 1;
+        if (LPR <= 64 && at >= p.rows) break;  // (where rows meet at barriers all go along, with the last one)
         const bool store = mine.count && at < p.rows;
         Cols<T> cx, cy, cg;
         load8<T, ALIGNED>(cy, (const T*)p.y + row * p.y_rs, col, p.width);
@@ -303,16 +304,20 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_residual_norm_bwd_
     const bool post = p.param[P_POST_WEIGHT];
     for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < p.rows; base += (int64_t)gridDim.x * GROUPS) {
         const int64_t at = base + threadIdx.x / LPR, row = at < p.rows ? at : p.rows - 1;
-        const bool there = at < p.rows, store = mine.count && there;
+        if (LPR <= 64 && at >= p.rows) break;
+        const bool there = LPR <= 64 || at < p.rows, store = mine.count && there;
         Cols<T> cx, cy, cg, cd, cn;
         load8<T, ALIGNED>(cy, (const T*)p.y + row * p.y_rs, col, p.width);
         if (p.gate) load8<T, ALIGNED>(cg, (const T*)p.gate + row * p.gate_rs, col, p.width);
         load8<T, ALIGNED>(cx, (const T*)p.x + row * p.x_rs, col, p.width);
         if (p.dout) load8<T, ALIGNED>(cd, (const T*)p.dout + row * p.dout_rs, col, p.width);
         if (p.dnormed) load8<T, ALIGNED>(cn, (const T*)p.dnormed + row * p.dnormed_rs, col, p.width);
-        // a group behind the last row goes along with it, without its gradients
+        // a group behind the last row goes along as a row of zeros
 #pragma unroll
-        for (int i = 0; i < Cols<T>::WORDS; ++i) cd.w[i] = there && p.dout ? cd.w[i] : 0, cn.w[i] = there ? cn.w[i] : 0;
+        for (int i = 0; i < Cols<T>::WORDS; ++i) {
+            cd.w[i] = there && p.dout ? cd.w[i] : 0;
+            if (LPR > 64 && !there) cx.w[i] = cy.w[i] = cg.w[i] = cn.w[i] = 0;
+        }
         // forward again: unit = y^, branch = act(gate) n as dropped
         float unit[8], n[8], value[8], slope[8], keep[8], branch[8], w[8], d[8];
         float r = 1.f;

@@ -47,7 +47,7 @@ def _check_rows(x: torch.Tensor, what: str) -> int:
 def _flat(x: torch.Tensor) -> torch.Tensor:
     """``x`` with the columns of a row side by side; a copy that gradients flow through where it needs one."""
     dense = (x.shape[-1] == 1 or x.stride(-1) == 1) and (x.dim() == 2 or x.shape[1] == 1 or x.stride(1) == x.shape[2])
-    return x if dense and (x.shape[0] == 1 or x.stride(0) >= 0) else x.clone(memory_format=torch.contiguous_format)
+    return x if dense and (x.shape[0] == 1 or 0 <= x.stride(0) <= 1 << 24) else x.clone(memory_format=torch.contiguous_format)
 
 
 def _check_recurrence(x, decay_gate, input_gate, decay, rate: float, what: str) -> int:

@@ -5,7 +5,7 @@
  *
  * Plain pointers and sizes; device pointers on the current HIP device; asynchronous on the stream given.  Nothing is
  * allocated and nothing read back to the host.  Index arrays hold int32 or int64 as the flag beside each says.  Row strides are in
- * elements, any that are not negative; the columns of a row lie side by side.  Pointers are aligned to their elements (tensors are read in
+ * elements, any that are not negative (in the recurrence up to 2^24); the columns of a row lie side by side.  Pointers are aligned to their elements (tensors are read in
  * wider pieces where their addresses and strides allow it).
  *
  * Status codes: 0 ok; negative values as in hstu_hip.h (-1 NULL pointer, -2 dtype, -4 alignment, -5 shape, -6 unsupported,
