@@ -117,13 +117,15 @@ struct RowsFrom {
         else
             return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(at, (int)off, (int)(j * pitch), 0));
     }
-    template <class T>
+    // STREAM: past the caches.  The backward's three results push each other out of them: a training step of 48 histories 197 us without, 192 so, 255 and 251 with what
+    // reads them next; the forward's one is better left for its reader (prefill of 96 histories and a reader 75 us, 78 so).
+    template <class T, bool STREAM = false>
     __device__ __forceinline__ void store(int j, unsigned off, float x) const {
         const T v = (T)x;
         if constexpr (sizeof(T) == 4)
-            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), at, (int)off, (int)(j * pitch), 0);
+            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), at, (int)off, (int)(j * pitch), STREAM ? 2 : 0);
         else
-            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, v), at, (int)off, (int)(j * pitch), 0);
+            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, v), at, (int)off, (int)(j * pitch), STREAM ? 2 : 0);
     }
 };
 constexpr unsigned kNowhere = 0x80000000u;  // the offset of a column that there is not, for stores: sizes and rows' offsets are below it
@@ -628,9 +630,9 @@ __global__ __launch_bounds__(64 * WAVES, 3) void hstu_scan_bwd_kernel(const Scan
             const float dq = G[j] * q.a * (u * q.a * share - q.s * old), dxj = G[j] * (q.m * q.si);
             sum += dq;  // (G is 0 in rows that there are not)
             h = __builtin_fmaf(q.a, old, q.m * u);
-            dx.store<T>(j, off_out, dxj);
-            dr.store<T>(j, off_out, natural * (1.f - q.s) * dq);
-            di.store<T>(j, off_out, dxj * (float)x[j] * (1.f - q.si));
+            dx.store<T, true>(j, off_out, dxj);
+            dr.store<T, true>(j, off_out, natural * (1.f - q.s) * dq);
+            di.store<T, true>(j, off_out, dxj * (float)x[j] * (1.f - q.si));
         }
     });
     if (!p.partial) return;
