@@ -200,8 +200,9 @@ __device__ __forceinline__ unsigned marks_of(uint64_t bits, int wave) {
 //
 // What was measured.  Tiles of rows regardless of sequences, each taking up all sums of its sequence in front of it: a third of the time went into waits
 // (five histories of up to 16000 rows, 1024 columns, 137 us; 98 without them).  A pass for the sums and another for the rows reads everything twice.  Two
-// columns to a lane: 231 us where one takes 206 (a training step of 48 histories, 512 columns), since half as many waves fit; eight rows to a lane 222.
-// All workgroups at one ticket counter were 18 ns each, so a block of columns has one of its own.
+// columns to a lane forward: 239 us where one takes 221 (a training step of 48 histories, 512 columns) and 151 where it takes 136 (the five histories).  Eight
+// rows to a lane forward: 216 us where sixteen take 206, and 167 where they take 135; thirty-two: 213 and 146.  Backward eight: 219 where sixteen take 206.
+// With all workgroups at one ticket counter, 3400 more of them of half the rows took 61 us more (18 ns each) and without tickets nothing more, so a block of columns has a counter of its own.
 constexpr int kGroup = 16, kGroupsBack = 8, kTicketPitch = 64;
 constexpr unsigned kCut = 0x7f800000u;  // A's bits where there is none
 
@@ -347,7 +348,7 @@ __device__ __forceinline__ float join_tile(const ScanParams& p, int slot, int at
 }
 
 // Which block of columns a workgroup takes: each as often as there are tiles, and each of the eight dies, which workgroups go to in turn, all of them
-// in turn (1024 columns, one die always at the same part of a row: 1261 us where others take 1105).
+// in turn (1024 columns, one die always at the same part of a row: 1261 us where so 1099).
 __device__ __forceinline__ int column_block(const ScanParams& p) { return (int)((blockIdx.x + blockIdx.x / p.col_blocks) % p.col_blocks); }
 
 // The tile that a workgroup takes up, to LDS: one thread's work, with a barrier behind it.
@@ -519,7 +520,7 @@ __global__ __launch_bounds__(64 * WAVES, 6) void hstu_scan_kernel(const ScanPara
 
 // The same from the last row to the first: G is to dh what h is to b, with a row's a on the way to the row in front of it.  h in front of each row is
 // worked out again from the state that the forward saved for the tile.  c = a G is what a row passes on.  Three waves of a SIMD, whose registers hold a row's gates
-// from the first pass to the last: with four they did not (232 us where this takes 216, a training step of 48 histories).
+// from the first pass to the last: with four 14 did not (207 us where this takes 190, a training step of 48 histories).
 template <class T, int ROWS, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 3) void hstu_scan_bwd_kernel(const ScanParams p) {
     static_assert(ROWS * WAVES == kTile && ROWS <= 16, "a row for each");

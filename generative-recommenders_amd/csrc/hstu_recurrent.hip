@@ -317,7 +317,7 @@ int with_row(int lanes, bool wide, F&& f) {
     }
 }
 
-// At most so many, which go on to further rows.  Forward: nearly none do (norm of 49781 rows of 512 columns 47 us, with 4096 workgroups 49); backward: two to a
+// At most so many, which go on to further rows.  Forward: nearly none do (norm of 49028 rows of 512 columns 47 us, with 4096 workgroups 49); backward: two to a
 // CU, as many as there is room for, and half as many sums to add up as with 1024 (a training step of 56328 rows 150 us, 157).
 constexpr int64_t kForwardWorkgroups = 16384, kBackwardWorkgroups = 512;
 

@@ -232,7 +232,7 @@ __device__ __forceinline__ void plus(float (&v)[8], const Cols<T>& c, const char
     for (int i = 0; i < 8; ++i) v[i] += w[i];
 }
 
-// 151302 rows of 1024 columns, layer norms with a gate: 320 us (1.55 GB).
+// 151302 rows of 1024 columns, layer norms with a gate: 307 us (1.55 GB, 5.0 TB/s); 56328 of 512 with dropout 52.
 template <class T, int LPR, bool ALIGNED>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_residual_norm_kernel(const ResidualNormParams p) {
     constexpr int THREADS = LPR > 256 ? LPR : 256, GROUPS = THREADS / LPR;
