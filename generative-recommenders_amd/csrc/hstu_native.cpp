@@ -16,6 +16,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <array>
+#include <cmath>
 #include <cstdlib>
 #include <optional>
 #include <tuple>
@@ -993,6 +994,8 @@ bool decay_of(const Tensor& decay, const Tensor& x) {
            (decay.scalar_type() == at::kFloat || decay.scalar_type() == x.scalar_type());
 }
 
+bool scan_rate(double rate) { return (float)rate > 0.f && std::isfinite((float)rate); }
+
 // [count, width] of fp32, dense
 bool state_rows(const Tensor& t, int64_t count, const Tensor& x) {
     return t.is_cuda() && t.dim() == 2 && t.size(0) == count && t.size(1) == flat_width(x) && t.scalar_type() == at::kFloat && t.is_contiguous() &&
@@ -1083,7 +1086,7 @@ struct ScanFunction : torch::autograd::Function<ScanFunction> {
 
 std::optional<std::tuple<Tensor, OptTensor>> gated_recurrence(const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& decay, const Tensor& offsets,
                                                               const OptTensor& initial, double rate, bool want_state, bool checked) {
-    if (!flat_rows(x) || !float_type(x) || !alike(r, x) || !alike(i, x) || !decay_of(decay, x) || !(rate > 0) || !((float)rate > 0.f)) return {};
+    if (!flat_rows(x) || !float_type(x) || !alike(r, x) || !alike(i, x) || !decay_of(decay, x) || !scan_rate(rate)) return {};
     if (!offsets.is_cuda() || offsets.dim() != 1 || offsets.numel() < 2 || !index_vector(offsets, offsets.numel(), x.device())) return {};
     if (initial && !state_rows(*initial, offsets.numel() - 1, x)) return {};
     if ((!checked && contract_checks()) || has_tangent({&x, &r, &i, &decay}, {&initial})) return {};
@@ -1099,7 +1102,7 @@ std::optional<std::tuple<Tensor, OptTensor>> gated_recurrence(const Tensor& x, c
 
 OptTensor gated_recurrence_step(const Tensor& states, const Tensor& x, const Tensor& r, const Tensor& i, const Tensor& decay, const OptTensor& slots,
                                 const OptTensor& new_slots, double rate, bool checked) {
-    if (!flat_rows(x) || !float_type(x) || !alike(r, x) || !alike(i, x) || !decay_of(decay, x) || !(rate > 0) || !((float)rate > 0.f)) return {};
+    if (!flat_rows(x) || !float_type(x) || !alike(r, x) || !alike(i, x) || !decay_of(decay, x) || !scan_rate(rate)) return {};
     if (!states.is_cuda() || states.dim() != 2 || states.size(1) != flat_width(x) || states.scalar_type() != at::kFloat || states.device() != x.device()) return {};
     if ((states.size(1) > 1 && states.stride(1) != 1) || (states.size(0) > 1 && states.stride(0) < states.size(1))) return {};
     if ((!slots && states.size(0) != x.size(0)) || (slots && !index_vector(*slots, x.size(0), x.device()))) return {};

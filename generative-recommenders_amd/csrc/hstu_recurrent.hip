@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <atomic>
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <type_traits>
@@ -55,7 +56,7 @@ constexpr int64_t kMaxBlocks = (1 << 24) - 1;  // a launch has fewer than 2^32 t
 int check_scan(const HstuRecurrenceArgs* a) {
     if (!a) return HSTU_ERR_NULL_POINTER;
     if (!known_type(a->dtype)) return HSTU_ERR_BAD_DTYPE;
-    if (a->rows < 0 || a->width <= 0 || a->width > 65535 * 64 || a->batch <= 0 || a->batch > (1 << 30) || !(a->rate > 0.f)) return HSTU_ERR_BAD_SHAPE;
+    if (a->rows < 0 || a->width <= 0 || a->width > 65535 * 64 || a->batch <= 0 || a->batch > (1 << 30) || !(a->rate > 0.f && std::isfinite(a->rate))) return HSTU_ERR_BAD_SHAPE;
     for (int64_t rs : {a->x_row_stride, a->decay_gate_row_stride, a->input_gate_row_stride}) {
         if (rs < 0) return HSTU_ERR_BAD_SHAPE;
         if (rs > kMaxPitch) return HSTU_ERR_UNSUPPORTED;
@@ -227,7 +228,7 @@ int hstu_recurrent_scan_bwd(const HstuRecurrenceArgs* a, const HstuRecurrenceGra
 int hstu_recurrent_step(const HstuRecurrenceStepArgs* a, void* stream) {
     if (!a) return HSTU_ERR_NULL_POINTER;
     if (!known_type(a->dtype)) return HSTU_ERR_BAD_DTYPE;
-    if (a->rows < 0 || a->width <= 0 || a->width > 65535 * 64 || a->state_rows < 0 || a->state_row_stride < 0 || !(a->rate > 0.f)) return HSTU_ERR_BAD_SHAPE;
+    if (a->rows < 0 || a->width <= 0 || a->width > 65535 * 64 || a->state_rows < 0 || a->state_row_stride < 0 || !(a->rate > 0.f && std::isfinite(a->rate))) return HSTU_ERR_BAD_SHAPE;
     if (a->x_row_stride < 0 || a->decay_gate_row_stride < 0 || a->input_gate_row_stride < 0) return HSTU_ERR_BAD_SHAPE;
     if (a->rows == 0) return 0;
     if (!a->x || !a->decay_gate || !a->input_gate || !a->out || !a->decay || (a->state_rows > 0 && !a->states)) return HSTU_ERR_NULL_POINTER;

@@ -57,7 +57,7 @@ def _check_recurrence(x, decay_gate, input_gate, decay, rate: float, what: str) 
     _require_device(decay, "decay")
     torch._assert(decay.dim() == 1 and decay.shape[0] == width, "decay must hold one value per column")
     torch._assert(decay.dtype in (x.dtype, torch.float32) and decay.device == x.device, "decay must be float32 or of x's type, on x's device")
-    torch._assert(0.0 < rate < float("inf") and torch.tensor(rate, dtype=torch.float32).item() > 0.0, "rate must be larger than 0")
+    torch._assert(0.0 < torch.tensor(rate, dtype=torch.float32).item() < float("inf"), "rate must be finite and larger than 0")
     return width
 
 

@@ -42,10 +42,10 @@ typedef struct HstuRecurrenceArgs {
     const void* decay_gate;     /* [rows, width] */
     const void* input_gate;     /* [rows, width] */
     int64_t x_row_stride, decay_gate_row_stride, input_gate_row_stride;
-    void* out;                  /* [rows, width] dense; unused by the backward */
+    void* out;                  /* [rows, width] dense, none of the inputs' memory; unused by the backward */
     const void* decay;          /* [width], fp32 or the type of x */
     int32_t decay_f32;
-    float rate;                 /* > 0 */
+    float rate;                 /* finite, > 0 */
     const void* seq_offsets;    /* [batch + 1] */
     int32_t seq_offsets_i64;
     int32_t batch;              /* at least 1 */
