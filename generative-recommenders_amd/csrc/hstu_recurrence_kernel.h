@@ -100,7 +100,8 @@ struct ScanParams {
 };
 
 // The rows of a tensor from one on, through a buffer descriptor: a row's offset is the wave's, a column's the lane's, and the device checks their sum, so that
-// what lies behind the last row (and what is meant for no column) is read as zero and not written at all.  A wave's sixteen rows at most.
+// what lies behind the last row's end (and what is meant for no column) is read as zero and not written at all.  Rows that there are not are read as whatever
+// lies in front of that end where rows are less than a row apart; results, whose rows are not, are written for none.  A wave's sixteen rows at most.
 struct RowsFrom {
     __amdgpu_buffer_rsrc_t at;
     unsigned pitch;  // bytes from row to row: at most 2^26, so that sixteen rows end below 2^31
@@ -629,7 +630,9 @@ __global__ __launch_bounds__(64 * WAVES, 3) void hstu_scan_bwd_kernel(const Scan
             const float u = q.si * (float)x[j], old = before(all, j, h);
             const float share = q.m > 0.f ? q.s * __builtin_amdgcn_rcpf(q.m) : 0.f;
             const float dq = G[j] * q.a * (u * q.a * share - q.s * old), dxj = G[j] * (q.m * q.si);
-            sum += dq;  // (G is 0 in rows that there are not)
+            // Rows that there are not may have come from rows that there are, where those lie less than a row apart (one row, rows that were broadcast).  Only a
+            // wave with a sequence's last row has any.
+            sum += ALL || w0 + j < behind ? dq : 0.f;
             h = __builtin_fmaf(q.a, old, q.m * u);
             dx.store<T, true>(j, off_out, dxj);
             dr.store<T, true>(j, off_out, natural * (1.f - q.s) * dq);
