@@ -994,6 +994,11 @@ bool decay_of(const Tensor& decay, const Tensor& x) {
            (decay.scalar_type() == at::kFloat || decay.scalar_type() == x.scalar_type());
 }
 
+// Columns and sequences are counted in 32 bits behind the C ABI, which refuses more of them than this where it sees them all.
+void check_scan_sizes(const Tensor& x, int64_t batch) {
+    if (flat_width(x) > 65535 * 64 || batch > (1 << 30)) check_recurrent(HSTU_ERR_UNSUPPORTED);
+}
+
 bool scan_rate(double rate) { return (float)rate > 0.f && std::isfinite((float)rate); }
 
 // [count, width] of fp32, dense
@@ -1090,6 +1095,7 @@ std::optional<std::tuple<Tensor, OptTensor>> gated_recurrence(const Tensor& x, c
     if (!offsets.is_cuda() || offsets.dim() != 1 || offsets.numel() < 2 || !index_vector(offsets, offsets.numel(), x.device())) return {};
     if (initial && !state_rows(*initial, offsets.numel() - 1, x)) return {};
     if ((!checked && contract_checks()) || has_tangent({&x, &r, &i, &decay}, {&initial})) return {};
+    check_scan_sizes(x, offsets.numel() - 1);
     RECORD_USER_SCOPE("gated_recurrence");
     const bool grad = wants_grad({&x, &r, &i, &decay}) || (initial && wants_grad({&*initial}));
     if (!grad) {
@@ -1108,6 +1114,7 @@ OptTensor gated_recurrence_step(const Tensor& states, const Tensor& x, const Ten
     if ((!slots && states.size(0) != x.size(0)) || (slots && !index_vector(*slots, x.size(0), x.device()))) return {};
     if (new_slots && !index_vector(*new_slots, x.size(0), x.device())) return {};
     if ((!checked && contract_checks()) || wants_grad({&states, &x, &r, &i, &decay}) || has_tangent({&states, &x, &r, &i, &decay})) return {};
+    check_scan_sizes(x, 1);
     HstuRecurrenceStepArgs a{};
     a.x = x.const_data_ptr(), a.decay_gate = r.const_data_ptr(), a.input_gate = i.const_data_ptr();
     a.x_row_stride = flat_pitch(x), a.decay_gate_row_stride = flat_pitch(r), a.input_gate_row_stride = flat_pitch(i);

@@ -79,7 +79,7 @@ def gated_recurrence(
     """``h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(input_gate_t) x_t`` with ``a_t = exp(-rate softplus(decay) sigmoid(decay_gate_t))``
     along each sequence, for every column by itself; returns ``h`` in the shape and type of ``x``, and the last ``h`` of every sequence.
 
-    ``x``, ``decay_gate``, ``input_gate``: ``[L, width]`` or ``[L, H, D]``, bf16, fp16 or fp32, any distance between rows (the column
+    ``x``, ``decay_gate``, ``input_gate``: ``[L, width]`` or ``[L, H, D]``, bf16, fp16 or fp32, at most 4194240 columns, any distance between rows (the column
     slices of ``hstu_compute_uqvk`` are read in place); ``decay``: ``[width]``, float32 or of x's type.  Rows ``seq_offsets[b]`` up to
     ``seq_offsets[b + 1]`` are sequence ``b``; it begins with ``initial_state[b]`` (``[B, width]``, float32) or with zeros.  ``return_state``: the second
     result is ``[B, width]``, float32, what ``initial_state`` or ``gated_recurrence_step`` goes on from (a sequence without rows keeps its

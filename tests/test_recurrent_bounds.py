@@ -136,3 +136,26 @@ def test_rows_that_are_one_row(pkg, dev, dtype, lengths):
     want = torch.autograd.grad(total, leaf)[0]
     # rounding aside (a few hundred half steps of fp32 of what is summed up), not a multiple of a row's share too much
     assert (a[5].cpu().double() - want).abs().max() <= 2e-3 * want.abs().max(), "d decay"
+
+
+@pytest.mark.gpu
+def test_widths_past_32_bits(pkg, dev):
+    """A row of 2^32 + 64 columns is refused, not taken for one of 64."""
+    width = (1 << 32) + 64
+    x = torch.empty((1, width), dtype=BF, device=dev)
+    offsets = torch.tensor([0, 1], device=dev)
+    with pytest.raises(NotImplementedError):
+        pkg.gated_recurrence(x, x, x, x[0], offsets)
+    states = torch.empty((1, 1), device=dev).expand(1, width)
+    with pytest.raises((NotImplementedError, AssertionError)):
+        pkg.gated_recurrence_step(states, x, x, x, x[0])
+
+
+@pytest.mark.gpu
+def test_a_step_in_inference_mode(pkg, dev):
+    x, w = torch.randn((3, 32), device=dev), torch.zeros(32, device=dev)
+    want = torch.zeros((3, 32), device=dev)
+    out = pkg.gated_recurrence_step(want, x, x, x, w)
+    with torch.inference_mode():
+        states = torch.zeros((3, 32), device=dev)
+        assert torch.equal(pkg.gated_recurrence_step(states, x, x, x, w), out) and torch.equal(states, want)
