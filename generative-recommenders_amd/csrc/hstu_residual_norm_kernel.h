@@ -305,19 +305,17 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_residual_norm_bwd_
     for (int64_t base = (int64_t)blockIdx.x * GROUPS; base < p.rows; base += (int64_t)gridDim.x * GROUPS) {
         const int64_t at = base + threadIdx.x / LPR, row = at < p.rows ? at : p.rows - 1;
         if (LPR <= 64 && at >= p.rows) break;
-        const bool there = LPR <= 64 || at < p.rows, store = mine.count && there;
+        // A group behind the last row goes along with it where rows meet at barriers, and adds nothing to the parameters' gradients; the same for a wave, which
+        // has one group there.
+        const bool there = LPR <= 64 || __builtin_amdgcn_readfirstlane(at < p.rows), store = mine.count && there;
         Cols<T> cx, cy, cg, cd, cn;
         load8<T, ALIGNED>(cy, (const T*)p.y + row * p.y_rs, col, p.width);
         if (p.gate) load8<T, ALIGNED>(cg, (const T*)p.gate + row * p.gate_rs, col, p.width);
         load8<T, ALIGNED>(cx, (const T*)p.x + row * p.x_rs, col, p.width);
         if (p.dout) load8<T, ALIGNED>(cd, (const T*)p.dout + row * p.dout_rs, col, p.width);
         if (p.dnormed) load8<T, ALIGNED>(cn, (const T*)p.dnormed + row * p.dnormed_rs, col, p.width);
-        // a group behind the last row goes along as a row of zeros
 #pragma unroll
-        for (int i = 0; i < Cols<T>::WORDS; ++i) {
-            cd.w[i] = there && p.dout ? cd.w[i] : 0;
-            if (LPR > 64 && !there) cx.w[i] = cy.w[i] = cg.w[i] = cn.w[i] = 0;
-        }
+        for (int i = 0; i < Cols<T>::WORDS; ++i) cd.w[i] = p.dout ? cd.w[i] : 0;
         // forward again: unit = y^, branch = act(gate) n as dropped
         float unit[8], n[8], value[8], slope[8], keep[8], branch[8], w[8], d[8];
         float r = 1.f;
@@ -351,9 +349,10 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_residual_norm_bwd_
             for (int i = 0; i < 8; ++i) s[i] += w[i];
             const float rs = normalise(s, mine, p, sums);
             cn.get(g);
+            if (there)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) total[P_PRE_WEIGHT][i] = __builtin_fmaf(g[i], s[i], total[P_PRE_WEIGHT][i]);
-            if (p.param[P_PRE_BIAS])
+                for (int i = 0; i < 8; ++i) total[P_PRE_WEIGHT][i] = __builtin_fmaf(g[i], s[i], total[P_PRE_WEIGHT][i]);
+            if (there && p.param[P_PRE_BIAS])
 #pragma unroll
                 for (int i = 0; i < 8; ++i) total[P_PRE_BIAS][i] += g[i];
             times(g, param[P_PRE_WEIGHT], p.param[P_PRE_WEIGHT]);
@@ -363,8 +362,9 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_residual_norm_bwd_
         }
         if (p.dx && store) store8<T, ALIGNED>(d, (T*)p.dx + row * p.width, col, p.width);
         if (p.param[P_SCALE]) {
+            if (there)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) total[P_SCALE][i] = __builtin_fmaf(d[i], branch[i], total[P_SCALE][i]);
+                for (int i = 0; i < 8; ++i) total[P_SCALE][i] = __builtin_fmaf(d[i], branch[i], total[P_SCALE][i]);
             times(d, param[P_SCALE], p.param[P_SCALE]);
         }
         if (p.drop.thresh)
@@ -377,9 +377,10 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void hstu_residual_norm_bwd_
             if (p.dgate && store) store8<T, ALIGNED>(g, (T*)p.dgate + row * p.width, col, p.width);
         }
         if (post) {
+            if (there)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) total[P_POST_WEIGHT][i] = __builtin_fmaf(d[i], unit[i], total[P_POST_WEIGHT][i]);
-            if (p.param[P_POST_BIAS])
+                for (int i = 0; i < 8; ++i) total[P_POST_WEIGHT][i] = __builtin_fmaf(d[i], unit[i], total[P_POST_WEIGHT][i]);
+            if (there && p.param[P_POST_BIAS])
 #pragma unroll
                 for (int i = 0; i < 8; ++i) total[P_POST_BIAS][i] += d[i];
             times(d, param[P_POST_WEIGHT], p.param[P_POST_WEIGHT]);
