@@ -1232,6 +1232,7 @@ std::optional<OutAndNormed> gated_residual_norm(const Tensor& x, const Tensor& y
         grad = grad || wants_grad({&*t});
     }
     if ((post_bias && !post_weight) || (pre_bias && !pre_weight) || !(dropout >= 0 && dropout < 1) || width > 8192) return {};
+    if (!((float)eps >= 0.f && std::isfinite((float)eps))) return {};
     if (has_tangent({&x, &y}, {&gate, &post_weight, &post_bias, &scale, &pre_weight, &pre_bias})) return {};
     const ResidualNormCall c{eps, layer_norm, activation, dropout, seed, offset};
     RECORD_USER_SCOPE("gated_residual_norm");

@@ -277,6 +277,7 @@ int fill_residual(const HstuResidualNormArgs* a, hstu::ResidualNormParams& p, bo
     if (!a) return HSTU_ERR_NULL_POINTER;
     if (!known_type(a->dtype)) return HSTU_ERR_BAD_DTYPE;
     if (a->rows < 0 || a->width <= 0 || a->x_row_stride < 0 || a->y_row_stride < 0 || a->gate_row_stride < 0) return HSTU_ERR_BAD_SHAPE;
+    if (!(a->eps >= 0.f && std::isfinite(a->eps))) return HSTU_ERR_BAD_SHAPE;
     if (a->gate_activation < 0 || a->gate_activation > 2 || !(a->dropout_ratio >= 0. && a->dropout_ratio < 1.)) return HSTU_ERR_BAD_SHAPE;
     if ((a->post_bias && !a->post_weight) || (a->pre_bias && !a->pre_weight)) return HSTU_ERR_NULL_POINTER;
     if (a->width > 8192) return HSTU_ERR_UNSUPPORTED;

@@ -194,8 +194,8 @@ def gated_residual_norm(
 
     ``x`` (the residual stream), ``y`` (a block's output), ``gate``: ``[L, width]`` or ``[L, H, D]``, bf16, fp16 or fp32, any distance between rows;
     parameters ``[width]`` of the same type, shared by the rows.  ``norm(v)`` is ``v / sqrt(mean(v^2) + eps) * weight + bias`` over a whole row, with
-    ``layer_norm`` of ``v`` less its mean; ``post_*`` are those of the norm behind the block (left out without ``post_weight``), ``pre_*`` those of the one in
-    front of the next (without ``pre_weight`` the second result is None).  ``act`` is ``gate_activation``: ``"none"``, ``"sigmoid"`` or ``"silu"``;
+    ``layer_norm`` of ``v`` less its mean; ``eps`` may be 0 (a row whose mean square is 0 is NaN then).  ``post_*`` are those of the norm behind the block
+    (left out without ``post_weight``), ``pre_*`` those of the one in front of the next (without ``pre_weight`` the second result is None).  ``act`` is ``gate_activation``: ``"none"``, ``"sigmoid"`` or ``"silu"``;
     without ``gate`` and ``scale`` both are 1.  Everything in fp32, each result rounded once: the second norm takes the sum as it is, not rounded.
     Dropout runs when ``training`` and ``dropout_ratio > 0``, from the Philox stream of ``seed = (seed, offset)`` or of the device's default generator, as in
     ``norm_mul_dropout``; its mask is not stored but computed again for the backward.  (A captured call drops the same elements at every replay.)
@@ -205,7 +205,7 @@ def gated_residual_norm(
     drops = training and dropout_ratio != 0.0
     ratio = word_seed = word_offset = 0
     if drops:
-        _check_residual(x, y, gate, params, gate_activation, dropout_ratio)  # before the generator moves on
+        _check_residual(x, y, gate, params, eps, gate_activation, dropout_ratio)  # before the generator moves on
         ratio, word_seed, word_offset = _dropout_state(dropout_ratio, training, x.numel(), x.device, seed)
         word_seed, word_offset = word_seed & _WORD64, word_offset & _WORD64
     act = MUL_U_ACTIVATIONS.get(gate_activation, -1)
@@ -213,7 +213,7 @@ def gated_residual_norm(
     if out is not None:
         return out
     if not drops:
-        _check_residual(x, y, gate, params, gate_activation, dropout_ratio)
+        _check_residual(x, y, gate, params, eps, gate_activation, dropout_ratio)
     _check_no_tangents(x, y, gate, *params)
     if (x.shape[1] if x.dim() == 2 else x.shape[1] * x.shape[2]) > 8192:
         raise NotImplementedError("rows are at most 8192 columns wide")
@@ -227,12 +227,13 @@ def gated_residual_norm(
                                                     word_offset), "gated_residual_norm")
 
 
-def _check_residual(x, y, gate, params, gate_activation: str, dropout_ratio: float) -> None:
+def _check_residual(x, y, gate, params, eps: float, gate_activation: str, dropout_ratio: float) -> None:
     width = _check_rows(x, "gated_residual_norm")
     _rows_like("y", y, x)
     if gate is not None:
         _rows_like("gate", gate, x)
     torch._assert(gate_activation in MUL_U_ACTIVATIONS, "gate_activation must be none, sigmoid or silu")
+    torch._assert(0.0 <= torch.tensor(eps, dtype=torch.float32).item() < float("inf"), "eps must be finite and not negative")
     torch._assert(0.0 <= dropout_ratio < 1.0, "dropout_ratio must be below 1")
     for p, name in zip(params, ("post_weight", "post_bias", "scale", "pre_weight", "pre_bias")):
         if p is not None:
