@@ -105,11 +105,14 @@ def gated_recurrence(
     if hip_backend.contract_checks_enabled():
         _check_offsets(seq_offsets, x.shape[0])
     if x.numel() == 0:
-        # no rows, or none with columns; the graph, if there is one, goes on
-        state = None
-        if return_state:
-            state = x.new_zeros((batch, width), dtype=torch.float32) if initial_state is None else initial_state.clone()
-        return x * decay_gate * input_gate * decay.to(x.dtype).view((1,) + tuple(x.shape[1:])), state
+        # No rows, or none with columns; the graph, if there is one, goes on, from every input to both results: gradients of zero, and the states' own.
+        out = x * decay_gate * input_gate * decay.to(x.dtype).view((1,) + tuple(x.shape[1:]))
+        if initial_state is not None:
+            out = torch.cat([out, initial_state[:0].to(x.dtype).view((0,) + tuple(x.shape[1:]))])
+        if not return_state:
+            return out, None
+        state = x.new_zeros((batch, width), dtype=torch.float32) if initial_state is None else initial_state
+        return out, torch.cat([state, out.flatten(1)[:0].float()])
     initial_state = None if initial_state is None else initial_state.contiguous()
     return _served(native.front.gated_recurrence(_flat(x), _flat(decay_gate), _flat(input_gate), decay.contiguous(), seq_offsets, initial_state, rate, return_state,
                                                  True), "gated_recurrence")

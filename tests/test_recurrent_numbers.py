@@ -40,3 +40,32 @@ def test_an_eps_that_is_none(pkg, dev, eps):
             with pytest.raises(AssertionError):
                 pkg.gated_residual_norm(x, x, post_weight=w, eps=eps, **more)
             assert torch.cuda.default_generators[0].get_offset() == before
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(0, 16), (0, 2, 8), (3, 0)], ids=str)
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_graphs_of_no_rows(pkg, dev, dtype, shape):
+    """Every input of a call with nothing in it is in the graph of both results, as with rows: gradients of zeros, and the states' own."""
+    width = 16 if shape[0] == 0 else 0
+    offsets = torch.zeros(4, dtype=torch.int64, device=dev)
+    for given in (True, False):
+        leaves = [torch.zeros(shape, dtype=dtype, device=dev).requires_grad_() for _ in range(3)] + [torch.ones(width, device=dev).requires_grad_()]
+        if given:
+            leaves.append(torch.randn((3, width), device=dev).requires_grad_())
+        initial = leaves[4] if given else None
+        out, none = pkg.gated_recurrence(*leaves[:4], offsets, initial)
+        assert none is None and out.shape == shape and out.dtype == dtype
+        for got, leaf in zip(torch.autograd.grad(out, leaves, torch.zeros_like(out)), leaves):
+            assert torch.equal(got, torch.zeros_like(leaf))
+        out, state = pkg.gated_recurrence(*leaves[:4], offsets, initial, return_state=True)
+        assert torch.equal(state, initial if given else torch.zeros((3, width), device=dev)) and state.dtype == F32
+        d = torch.randn((3, width), device=dev)
+        for only_state in (True, False):
+            results, grads = ((state,), (d,)) if only_state else ((out, state), (torch.zeros_like(out), d))
+            got = torch.autograd.grad(results, leaves, grads, retain_graph=True)
+            assert all(torch.equal(g, torch.zeros_like(leaf)) for g, leaf in zip(got[:4], leaves))
+            assert not given or torch.equal(got[4], d)
+    with torch.no_grad():
+        out, state = pkg.gated_recurrence(*leaves[:4], offsets, return_state=True)
+    assert not out.requires_grad and not state.requires_grad
