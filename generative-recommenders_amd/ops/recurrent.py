@@ -217,9 +217,6 @@ def gated_residual_norm(
         return out
     if not drops:
         _check_residual(x, y, gate, params, eps, gate_activation, dropout_ratio)
-    _check_no_tangents(x, y, gate, *params)
-    if (x.shape[1] if x.dim() == 2 else x.shape[1] * x.shape[2]) > 8192:
-        raise NotImplementedError("rows are at most 8192 columns wide")
     if x.numel() == 0:
         out = x + (y if gate is None else y * gate)  # nothing in them; the graph, if there is one, goes on, to gradients of zero for the parameters too
         for p in (p for p in params if p is not None):
@@ -245,3 +242,6 @@ def _check_residual(x, y, gate, params, eps: float, gate_activation: str, dropou
             torch._assert(p.dtype == x.dtype and p.device == x.device, f"{name} must have the type and device of x")
     torch._assert(params[0] is not None or params[1] is None, "post_bias without post_weight")
     torch._assert(params[3] is not None or params[4] is None, "pre_bias without pre_weight")
+    _check_no_tangents(x, y, gate, *params)
+    if width > 8192:
+        raise NotImplementedError("rows are at most 8192 columns wide")

@@ -69,3 +69,17 @@ def test_graphs_of_no_rows(pkg, dev, dtype, shape):
     with torch.no_grad():
         out, state = pkg.gated_recurrence(*leaves[:4], offsets, return_state=True)
     assert not out.requires_grad and not state.requires_grad
+
+
+@pytest.mark.gpu
+def test_a_refused_call_leaves_the_generator(pkg, dev):
+    x, wide = torch.zeros((2, 64), device=dev), torch.zeros((2, 8200), device=dev)
+    before = torch.cuda.default_generators[0].get_offset()
+    with pytest.raises(NotImplementedError):
+        pkg.gated_residual_norm(wide, wide, dropout_ratio=0.5, training=True)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(NotImplementedError):
+            pkg.gated_residual_norm(x, torch.autograd.forward_ad.make_dual(x, x), dropout_ratio=0.5, training=True)
+    assert torch.cuda.default_generators[0].get_offset() == before
+    pkg.gated_residual_norm(x, x, dropout_ratio=0.5, training=True)
+    assert torch.cuda.default_generators[0].get_offset() > before
