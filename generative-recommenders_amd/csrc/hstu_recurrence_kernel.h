@@ -630,8 +630,8 @@ __global__ __launch_bounds__(64 * WAVES, 3) void hstu_scan_bwd_kernel(const Scan
             const float u = q.si * (float)x[j], old = before(all, j, h);
             const float share = q.m > 0.f ? q.s * __builtin_amdgcn_rcpf(q.m) : 0.f;
             const float dq = G[j] * q.a * (u * q.a * share - q.s * old), dxj = G[j] * (q.m * q.si);
-            // Rows that there are not may have come from rows that there are, where those lie less than a row apart (one row, rows that were broadcast).  Only a
-            // wave with a sequence's last row has any.
+            // Rows that there are not may have come from rows that there are, where those lie less than a row apart (one row, rows that were broadcast).  A wave has
+            // some beside its segment's last row, or has none that there is and is left out below.
             sum += ALL || w0 + j < behind ? dq : 0.f;
             h = __builtin_fmaf(q.a, old, q.m * u);
             dx.store<T, true>(j, off_out, dxj);
@@ -641,7 +641,7 @@ __global__ __launch_bounds__(64 * WAVES, 3) void hstu_scan_bwd_kernel(const Scan
     });
     if (!p.partial) return;
     __syncthreads();
-    passed[wave][lane] = sum;
+    passed[wave][lane] = w0 < behind ? sum : 0.f;  // (h behind the last row may be no number)
     __syncthreads();
     if (wave || !mine) return;
     float total = 0.f;

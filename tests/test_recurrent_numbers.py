@@ -6,7 +6,8 @@ import ctypes
 import pytest
 import torch
 
-from test_recurrent import BF, F32, FP, NORMS, abi, check_norm, norm_case
+from oracle import recurrent_oracle as oracle
+from test_recurrent import BF, F32, FP, NORMS, abi, check_norm, norm_case, offsets_of, within
 
 
 @pytest.mark.gpu
@@ -83,3 +84,26 @@ def test_a_refused_call_leaves_the_generator(pkg, dev):
     assert torch.cuda.default_generators[0].get_offset() == before
     pkg.gated_residual_norm(x, x, dropout_ratio=0.5, training=True)
     assert torch.cuda.default_generators[0].get_offset() > before
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("length", [1, 2, 16, 20, 40, 63, 70])
+def test_a_state_that_is_too_large(pkg, dev, length):
+    """A last state past fp32 is an infinity; the decays' gradient, to which rows behind it have nothing to add, is finite."""
+    width = 8
+    x = torch.zeros((length, width))
+    x[-1] = 3.2e38
+    r, i = torch.full_like(x, -1e30), torch.full_like(x, 20.0)
+    r[-1] = 0.0  # the rows in front of the last leave the state as it is
+    decay = torch.full((width,), -3.0)
+    initial = torch.full((1, width), 3.2e38)
+    case = dict(x=x, decay_gate=r, input_gate=i, decay=decay, offsets=offsets_of([length]), initial=initial)
+    dout = torch.zeros_like(x)
+    dout[-1] = 1e-30
+    h, _, *_ = oracle.scan(**case)
+    leaves = [case[k].to(dev).requires_grad_() for k in ("x", "decay_gate", "input_gate", "decay", "initial")]
+    out, _ = pkg.gated_recurrence(*leaves[:4], case["offsets"].to(dev), leaves[4])
+    assert bool(torch.isinf(out[-1]).all()) and bool((h[-1] > torch.finfo(F32).max).all())
+    got = torch.autograd.grad(out, leaves, dout.to(dev))
+    want = oracle.scan_grad(**case, dout=dout)
+    within(got[3], *want["decay"], "d decay")
