@@ -199,8 +199,10 @@ __device__ __forceinline__ void activate(int act, const float (&g)[8], float (&v
     if (act == ACT_NONE) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        value[i] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896340736f * g[i]));
-        slope[i] = value[i] - value[i] * value[i];
+        // With s = 1 / (1 + e), 1 - s is e s to its own last places (as a difference it is 1 % off at 12 and 0 from 17.4 on), and 0 s where e is an infinity.
+        const float e = __builtin_amdgcn_exp2f(-1.44269504088896340736f * g[i]);
+        value[i] = __builtin_amdgcn_rcpf(1.f + e);
+        slope[i] = value[i] * (fminf(e, 0x1p126f) * value[i]);
     }
     if (act == ACT_SILU)
 #pragma unroll

@@ -107,3 +107,39 @@ def test_a_state_that_is_too_large(pkg, dev, length):
     got = torch.autograd.grad(out, leaves, dout.to(dev))
     want = oracle.scan_grad(**case, dout=dout)
     within(got[3], *want["decay"], "d decay")
+
+
+# Halves of a unit in fp32's last place that a sigmoid and what it leaves of 1 may be off by, each of itself: -x log2(e) is rounded, and so is its log2(e) (to a
+# quarter of a half), which an exponential makes |x| times as much of; exponential and reciprocal two each, sum and product one each, 1 - s (where s is the smaller) one and s's own.
+def sigmoid_steps(x):
+    return 1.25 * x.abs() + 10
+
+
+OPEN = [0.0, 0.3, 1.0, 2.5, 5.0, 8.0, 9.5, 11.0, 12.0, 13.5, 15.0, 16.0, 17.0, 17.5, 20.0, 30.0, 50.0, 80.0]
+
+
+def ends(dtype, width, seed):
+    """Gates from -80 to 80, a value to a row."""
+    values = torch.tensor(OPEN + [-v for v in OPEN[1:]], dtype=torch.float64)
+    g = torch.Generator().manual_seed(seed)
+    return (values.view(-1, 1) + 0.25 * torch.rand((len(values), width), generator=g, dtype=torch.float64)).to(dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["sigmoid", "silu"])
+@pytest.mark.parametrize("width", [64, 100, 1024])
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_norm_gates_that_are_open(pkg, dev, dtype, width, act):
+    """The gate's gradient is dout y act'(gate), good to its own last places where act' is far below 1."""
+    gate = ends(dtype, width, 3)
+    g = torch.Generator().manual_seed(4)
+    y, dout = ((torch.randn(gate.shape, generator=g)).to(dtype) for _ in range(2))
+    leaf = gate.to(dev).requires_grad_()
+    out, _ = pkg.gated_residual_norm(torch.zeros_like(leaf.detach()), y.to(dev), leaf, gate_activation=act)
+    got = torch.autograd.grad(out, leaf, dout.to(dev))[0]
+    z = gate.double()
+    s, rest = torch.sigmoid(z), torch.sigmoid(-z)
+    slope, size = (s * rest, s * rest) if act == "sigmoid" else (s * (1 + z * rest), s * (1 + z.abs() * rest))
+    by = dout.double() * y.double()
+    # both factors' steps, the products of the slope (SiLU: one more sum) and the two with dout and y: six roundings
+    within(got, by * slope, oracle.F32 * (2 * sigmoid_steps(z) + 6) * (by.abs() * size) + 2.0**-122, "dgate", dtype)
