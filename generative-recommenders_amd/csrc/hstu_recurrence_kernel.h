@@ -22,30 +22,52 @@ __device__ __forceinline__ float sigmoid_of(float x) { return __builtin_amdgcn_r
 // rate softplus(d) log2(e)
 __device__ __forceinline__ float strength_of(float d, float rate) { return rate * (fmaxf(d, 0.f) + log1pf(expf(-fabsf(d)))) * kLog2e; }
 
-// What a row's gates make of it.  1 - a and 1 - a^2 are wanted to their own last places: a is close to one in layers that remember, and what it
+// 1 - a = 1 - 2^-z, and a.  1 - a and 1 - a^2 are wanted to their own last places: a is close to one in layers that remember, and what it
 // is off by counts once for each of the 1 / (1 - a) rows that h goes back over.  So for small z both come from the series of
 // 1 - exp(-z) = z (1 - z/2 + z^2/6 - ...), to z^6 below 1/4 for fp32 tensors and to z^4 below 1/16 for others (off by 1.4e-7 of it at most), and from the
-// instruction's exp(-z), good to a unit in the last place, above.
+// instruction's exp(-z), good to a unit in the last place, above.  z has the log2(e) in it; the series' terms have powers of log(2) for it.
+template <class T>
+__device__ __forceinline__ float lost_of(float z, float& a) {
+    constexpr float k1 = 0.69314718056f, k2 = -k1 * k1 / 2, k3 = k1 * k1 * k1 / 6, k4 = k2 * k2 / -6, k5 = k3 * k1 * k1 / 20, k6 = k3 * k3 / -20;
+    const float far = __builtin_amdgcn_exp2f(-z);
+    float series;
+    if constexpr (sizeof(T) == 4)
+        series = __builtin_fmaf(z, __builtin_fmaf(z, k6, k5), k4);
+    else
+        series = k4;
+    series = z * __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, series, k3), k2), k1);
+    const bool near = z < (sizeof(T) == 4 ? .25f : .0625f) * kLog2e;
+    a = near ? 1.f - series : far;
+    return near ? series : 1.f - far;
+}
+
+// What a row's gates make of it; `strength` has the log2(e) in it.
 template <class T>
 struct Gates {
-    float s, a, m, si;
-    __device__ __forceinline__ Gates() {}
-    // `strength` has the log2(e) in it, so that a = 2^-z; the series' terms have powers of log(2) for it.
+    float a, m, si;
     __device__ __forceinline__ Gates(float r, float i, float strength) {
-        constexpr float k1 = 0.69314718056f, k2 = -k1 * k1 / 2, k3 = k1 * k1 * k1 / 6, k4 = k2 * k2 / -6, k5 = k3 * k1 * k1 / 20, k6 = k3 * k3 / -20;
-        s = sigmoid_of(r), si = sigmoid_of(i);
-        const float z = strength * s, far = __builtin_amdgcn_exp2f(-z);
-        float series;
-        if constexpr (sizeof(T) == 4)
-            series = __builtin_fmaf(z, __builtin_fmaf(z, k6, k5), k4);
-        else
-            series = k4;
-        series = z * __builtin_fmaf(z, __builtin_fmaf(z, __builtin_fmaf(z, series, k3), k2), k1);
-        const bool near = z < (sizeof(T) == 4 ? .25f : .0625f) * kLog2e;
-        const float e = near ? series : 1.f - far;
-        a = near ? 1.f - series : far;
-        m = __builtin_amdgcn_sqrtf(e * (2.f - e));
+        si = sigmoid_of(i);
+        const float lost = lost_of<T>(strength * sigmoid_of(r), a);
+        m = __builtin_amdgcn_sqrtf(lost * (2.f - lost));
     }
+};
+
+// The same for the backward, which wants 1 - s and 1 - sigmoid(i) besides, to their own last places too (as differences they are 1 % off at gates of 12 and 0
+// from 17.4 on).  With s = 1 / (1 + e), 1 - s is e s; where e is an infinity that is 0 here, as is all that it is a factor of, by s.  In one register with s, the
+// smaller of the two with a sign, it takes two more selections (32 long histories 857 us where this takes 852).
+template <class T>
+struct BackGates {
+    float a, in, per, e, shut;  // in: m sigmoid(i); per: s / m^2; e: s = 1 / (1 + e); shut: 1 - sigmoid(i)
+    __device__ __forceinline__ BackGates() {}
+    __device__ __forceinline__ BackGates(float r, float i, float strength) {
+        e = __builtin_amdgcn_exp2f(-kLog2e * r);
+        const float ei = __builtin_amdgcn_exp2f(-kLog2e * i), s = __builtin_amdgcn_rcpf(1.f + e), si = __builtin_amdgcn_rcpf(1.f + ei), lost = lost_of<T>(strength * s, a),
+                    m2 = lost * (2.f - lost);
+        in = __builtin_amdgcn_sqrtf(m2) * si, per = m2 >= 0x1p-126f ? s * __builtin_amdgcn_rcpf(m2) : 0.f;  // (less has no reciprocal)
+        shut = fminf(ei, 0x1p126f) * si;
+    }
+    // s and 1 - s
+    __device__ __forceinline__ void halves(float& s, float& rest) const { s = __builtin_amdgcn_rcpf(1.f + e), rest = fminf(e, 0x1p126f) * s; }
 };
 
 template <class T>
@@ -555,9 +577,14 @@ __global__ __launch_bounds__(64 * WAVES, 3) void hstu_scan_bwd_kernel(const Scan
     const float strength = p.strength[col], natural = strength * (1 / kLog2e);
     float h = p.saved[same * p.width + col];
     map.template find<64 * WAVES>(p, taken);
-    Gates<T> g[ROWS];
+    BackGates<T> g[ROWS];
+    float b[ROWS];  // what a row adds to h
 #pragma unroll
-    for (int j = 0; j < ROWS; ++j) g[j] = Gates<T>((float)r[j], (float)i[j], strength);
+    for (int j = 0; j < ROWS; ++j) {  // (the compiler kept from working these out side by side or twice, which takes registers that there are not)
+        g[j] = BackGates<T>((float)r[j], (float)i[j], strength);
+        b[j] = g[j].in * (float)x[j];
+        asm("" : "+v"(g[j].in), "+v"(g[j].e), "+v"(g[j].per), "+v"(g[j].shut), "+v"(g[j].a), "+v"(b[j]));
+    }
     __syncthreads();
     const uint64_t bits = marks(map.begins), end_bits = marks(map.ends);
     const unsigned begins = marks_of<ROWS>(bits, wave), ends = marks_of<ROWS>(end_bits, wave);
@@ -584,7 +611,7 @@ __global__ __launch_bounds__(64 * WAVES, 3) void hstu_scan_bwd_kernel(const Scan
     either([&](auto all) {
 #pragma unroll
         for (int j = 0; j < ROWS; ++j) {
-            H = __builtin_fmaf(g[j].a, before(all, j, H), g[j].m * g[j].si * (float)x[j]);
+            H = __builtin_fmaf(g[j].a, before(all, j, H), b[j]);
             A *= g[j].a;
         }
 #pragma unroll
@@ -613,9 +640,6 @@ __global__ __launch_bounds__(64 * WAVES, 3) void hstu_scan_bwd_kernel(const Scan
     if (needs && !cut) fC = __builtin_fmaf(fA, front, fC);
     // G of every row from the last to the first, then the results along with h from the first to the last
     float sum = 0.f;
-    // Products of gates and x are worked out again below: kept from above they would take registers that there are not.
-#pragma unroll
-    for (int j = 0; j < ROWS; ++j) asm("" : "+v"(g[j].si));
     either([&](auto all) {
         constexpr bool ALL = decltype(all)::value;
 #pragma unroll
@@ -626,17 +650,17 @@ __global__ __launch_bounds__(64 * WAVES, 3) void hstu_scan_bwd_kernel(const Scan
         }
 #pragma unroll
         for (int j = 0; j < ROWS; ++j) {
-            const Gates<T>& q = g[j];
-            const float u = q.si * (float)x[j], old = before(all, j, h);
-            const float share = q.m > 0.f ? q.s * __builtin_amdgcn_rcpf(q.m) : 0.f;
-            const float dq = G[j] * q.a * (u * q.a * share - q.s * old), dxj = G[j] * (q.m * q.si);
+            const BackGates<T>& q = g[j];
+            float open, rest;
+            q.halves(open, rest);
+            const float old = before(all, j, h), dxj = G[j] * q.in, dq = G[j] * q.a * (b[j] * q.a * q.per - open * old);
             // Rows that there are not may have come from rows that there are, where those lie less than a row apart (one row, rows that were broadcast).  A wave has
             // some beside its segment's last row, or has none that there is and is left out below.
             sum += ALL || w0 + j < behind ? dq : 0.f;
-            h = __builtin_fmaf(q.a, old, q.m * u);
+            h = __builtin_fmaf(q.a, old, b[j]);
             dx.store<T, true>(j, off_out, dxj);
-            dr.store<T, true>(j, off_out, natural * (1.f - q.s) * dq);
-            di.store<T, true>(j, off_out, dxj * (float)x[j] * (1.f - q.si));
+            dr.store<T, true>(j, off_out, natural * rest * dq);
+            di.store<T, true>(j, off_out, G[j] * b[j] * q.shut);
         }
     });
     if (!p.partial) return;

@@ -143,3 +143,50 @@ def test_norm_gates_that_are_open(pkg, dev, dtype, width, act):
     by = dout.double() * y.double()
     # both factors' steps, the products of the slope (SiLU: one more sum) and the two with dout and y: six roundings
     within(got, by * slope, oracle.F32 * (2 * sigmoid_steps(z) + 6) * (by.abs() * size) + 2.0**-122, "dgate", dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [64, 72])
+@pytest.mark.parametrize("dtype", [BF, FP, F32])
+def test_recurrence_gates_that_are_open(pkg, dev, dtype, width):
+    """Both gates' gradients have a factor 1 - s, good to its own last places where s is close to 1.  Sequences of one row that begin with nothing: no sums."""
+    gate = ends(dtype, width, 5)
+    other = gate.roll(7, 0)
+    rows = gate.shape[0]
+    g = torch.Generator().manual_seed(6)
+    x, dout = ((torch.randn(gate.shape, generator=g)).to(dtype) for _ in range(2))
+    decay = torch.log(torch.expm1(-torch.log(0.5 + 0.45 * torch.rand(width, generator=g, dtype=torch.float64)) / 8.0)).float()
+    case = dict(x=x, decay_gate=gate, input_gate=other, decay=decay, offsets=offsets_of([1] * rows))
+    leaves = [case[k].to(dev).requires_grad_() for k in ("x", "decay_gate", "input_gate", "decay")]
+    out, _ = pkg.gated_recurrence(*leaves, case["offsets"].to(dev))
+    got = torch.autograd.grad(out, leaves, dout.to(dev))
+    strength, s, z, a, m, i, u = oracle.gates(x, gate, other, decay, 8.0)
+    r_rest, i_rest, d = torch.sigmoid(-gate.double()), torch.sigmoid(-other.double()), dout.double()
+    want_r, want_i = strength * r_rest * d * u * a * a * s / m, d * m * u * i_rest
+    # as the oracle counts them: a^2 and m by Z z and B of themselves, a product each; then the two gates' own
+    steps = 3 * oracle.Z * z + 2 * oracle.B + 2 * sigmoid_steps(gate.double()) + 2 * sigmoid_steps(other.double())
+    within(got[1], want_r, oracle.F32 * steps * want_r.abs() + 2.0**-122, "d decay_gate", dtype)
+    within(got[2], want_i, oracle.F32 * steps * want_i.abs() + 2.0**-122, "d input_gate", dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_columns_that_hardly_forget(pkg, dev, dtype):
+    """1 - a^2 down to nothing at all: results and gradients are numbers, and what a row lets in is lost only where its square is below fp32's normal numbers."""
+    gate = ends(dtype, 72, 7)
+    rows = gate.shape[0]
+    g = torch.Generator().manual_seed(8)
+    x, dout = ((torch.randn(gate.shape, generator=g)).to(dtype) for _ in range(2))
+    initial = torch.randn((3, 72), generator=g)
+    case = dict(x=x, decay_gate=gate, input_gate=gate.roll(5, 0), decay=torch.linspace(-110, -10, 72), offsets=offsets_of([9, 1, rows - 10]), initial=initial)
+    leaves = [case[k].to(dev).requires_grad_() for k in ("x", "decay_gate", "input_gate", "decay", "initial")]
+    out, _ = pkg.gated_recurrence(*leaves[:4], case["offsets"].to(dev), leaves[4])
+    got = dict(zip(("x", "decay_gate", "input_gate", "decay", "initial"), torch.autograd.grad(out, leaves, dout.to(dev))))
+    h, _, err, *_ = oracle.scan(**case)
+    want = oracle.scan_grad(**case, dout=dout)
+    # a row's m is below 2^-63 where its square is lost: of h each row's m u, of the gradients m, m u and, s / m being m / (2 strength) there, half of that
+    most = float(x.double().abs().max())
+    total = float(dout.double().abs().sum(0).max())
+    within(out, h, err + rows * most * 2.0**-63, "out", dtype)
+    for k, (value, bound) in want.items():
+        within(got[k], value, bound + (rows if k == "decay" else 1) * total * (most + rows * most) * 2.0**-63 + 2.0**-122, "d " + k, F32 if k in ("decay", "initial") else dtype)
