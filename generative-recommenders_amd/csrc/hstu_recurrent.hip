@@ -84,8 +84,15 @@ hstu::ScanParams scan_params(const HstuRecurrenceArgs* a) {
 constexpr int kRows = 16, kWaves = 4;           // of a tile, forward and backward
 constexpr int kShortRows = 2, kShortWaves = 8;  // at a time, where sequences are short
 
-// Few rows to a sequence, and no state to save: a workgroup for each sequence.
-bool scan_is_short(const HstuRecurrenceArgs* a) { return !a->saved && a->rows <= 16 * (int64_t)a->batch + 48 && a->rows <= 4096 && a->batch < 65535; }
+// Few rows to a sequence, and no state to save: a workgroup for each sequence and 64 columns, in one launch.  It walks its sequence, 16 rows in 0.6 us, where tiles take two
+// launches, 10 us at least, and any length side by side.  Measured so and by tiles (us, 512 columns, bf16, from states to states): 8 sequences of 16 rows 4.9 and
+// 10.7, 256 of 16 rows 8.4 and 14.4; one of 64 rows 5.1 and 10.3, of 256 13.2 and 11.4, of 1024 46 and 14.  A workgroup costs 3 ns: 512 single rows, 4096 of
+// them, 13.3 and 15.4, 768 single rows 18.9 and 17.3, 2000 45 and 21; 1024 and 4096 columns cross over at 4096 workgroups, too.  What a call does not say is which
+// sequence is long, and 16 rows on the average and 4096 in all bound what one among single rows can cost (300 of them, one of 3797 rows: 165 and 24), not what
+// sequences of one length gain (256 of 64 rows 18.7 and 26.4).
+bool scan_is_short(const HstuRecurrenceArgs* a) {
+    return !a->saved && a->rows <= 16 * (int64_t)a->batch + 48 && a->rows <= 4096 && (int64_t)a->batch * ((a->width + 63) / 64) <= 4096;
+}
 
 // How the tiles of a call are counted, and what they share, behind one another in the scratch memory.
 struct ScanPlan {
@@ -93,7 +100,8 @@ struct ScanPlan {
     size_t groups_at, states_at, tickets_at, tiles_at, strength_at, partial_at, bytes;  // (what is in front of tiles_at is cleared)
 };
 
-// A segment is a sequence, or as many as have 512 rows on the average: half a tile is lost at its end.
+// A segment is a sequence, or as many as have 512 rows on the average: half a tile is lost at its end, and more tiles wait for each other where segments are longer
+// (128, 256, 512, 1024 rows: a training step of 400 sequences of 20 .. 150 rows 128, 117, 113, 113 us; prefill of 96 of 20 .. 1023 rows 57.6, 57.6, 57.6, 59.2).
 ScanPlan scan_plan(const HstuRecurrenceArgs* a, bool backward) {
     ScanPlan s{};
     s.per_segment = a->rows > 0 ? (512 * (int64_t)a->batch + a->rows - 1) / a->rows : a->batch;

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import recurrent_oracle as oracle
-from test_recurrent import BF, F32, FP, NORMS, abi, check_norm, norm_case, offsets_of, within
+from test_recurrent import BF, F32, FP, NORMS, abi, check_norm, check_scan, norm_case, offsets_of, scan_case, within
 
 
 @pytest.mark.gpu
@@ -190,3 +190,13 @@ def test_columns_that_hardly_forget(pkg, dev, dtype):
     within(out, h, err + rows * most * 2.0**-63, "out", dtype)
     for k, (value, bound) in want.items():
         within(got[k], value, bound + (rows if k == "decay" else 1) * total * (most + rows * most) * 2.0**-63 + 2.0**-122, "d " + k, F32 if k in ("decay", "initial") else dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch, width", [(64, 4096), (64, 4100), (65, 4096), (512, 512), (513, 512), (4096, 64), (4097, 64), (1100, 200)])
+def test_where_many_short_sequences_end(pkg, dev, batch, width):
+    """On both sides of the rule for a workgroup per sequence and 64 columns: 4096 of them."""
+    lengths = [(k * 7) % 3 for k in range(batch)]
+    lengths[-1] = 5
+    case, *_ = scan_case(lengths, width, BF, seed=batch, behind=2)
+    check_scan(pkg, dev, case, None, None, grads=False)
