@@ -140,8 +140,8 @@ struct RowsFrom {
         else
             return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(at, (int)off, (int)(j * pitch), 0));
     }
-    // STREAM: past the caches.  The backward's three results push each other out of them: a training step of 48 histories 197 us without, 192 so, 255 and 251 with what
-    // reads them next; the forward's one is better left for its reader (prefill of 96 histories and a reader 75 us, 78 so).
+    // STREAM: past the caches.  The backward's three results push each other out of them: without it a training step of 48 histories took 3 % more, and 2 % with what
+    // reads them next; the forward's one is better left for its reader (prefill of 96 histories and a reader 4 % more so).
     template <class T, bool STREAM = false>
     __device__ __forceinline__ void store(int j, unsigned off, float x) const {
         const T v = (T)x;
@@ -221,11 +221,11 @@ __device__ __forceinline__ unsigned marks_of(uint64_t bits, int wave) {
 // once, and for those every kGroup-th joins the sums of its kGroup into one, and its state is defined by that: A_group (state in front of the
 // group) + H_group.  So every state has one definition, and results do not depend on which tile was first.
 //
-// What was measured.  Tiles of rows regardless of sequences, each taking up all sums of its sequence in front of it: a third of the time went into waits
-// (five histories of up to 16000 rows, 1024 columns, 137 us; 98 without them).  A pass for the sums and another for the rows reads everything twice.  Two
-// columns to a lane forward: 239 us where one takes 221 (a training step of 48 histories, 512 columns) and 151 where it takes 136 (the five histories).  Eight
-// rows to a lane forward: 216 us where sixteen take 206, and 167 where they take 135; thirty-two: 213 and 146.  Backward eight: 219 where sixteen take 206.
-// With all workgroups at one ticket counter, 3400 more of them of half the rows took 61 us more (18 ns each) and without tickets nothing more, so a block of columns has a counter of its own.
+// What was measured, each against the rest of the kernel as it was then: what the whole call took more.  Tiles of rows regardless of sequences, each taking up all
+// sums of its sequence in front of it: a third of the time went into waits (five histories of up to 16000 rows, 1024 columns).  A pass for the sums and another
+// for the rows reads everything twice.  Two columns to a lane forward: 8 % (a training step of 48 histories, 512 columns) and 11 % (the five histories).  Eight
+// rows to a lane forward: 5 and 24 % more than sixteen, thirty-two 3 and 8 %; backward eight 6 % (the training step).  With all workgroups at one ticket counter,
+// 3400 more of them of half the rows took 61 us more (18 ns each) and without tickets nothing more, so a block of columns has a counter of its own.
 constexpr int kGroup = 16, kGroupsBack = 8, kTicketPitch = 64;
 constexpr unsigned kCut = 0x7f800000u;  // A's bits where there is none
 
@@ -371,7 +371,7 @@ __device__ __forceinline__ float join_tile(const ScanParams& p, int slot, int at
 }
 
 // Which block of columns a workgroup takes: each as often as there are tiles, and each of the eight dies, which workgroups go to in turn, all of them
-// in turn (1024 columns, one die always at the same part of a row: 1261 us where so 1099).
+// in turn (a training step of 32 long histories, 1024 columns, took 15 % more with one die always at the same part of a row).
 __device__ __forceinline__ int column_block(const ScanParams& p) { return (int)((blockIdx.x + blockIdx.x / p.col_blocks) % p.col_blocks); }
 
 // The tile that a workgroup takes up, to LDS: one thread's work, with a barrier behind it.
@@ -543,7 +543,7 @@ __global__ __launch_bounds__(64 * WAVES, 6) void hstu_scan_kernel(const ScanPara
 
 // The same from the last row to the first: G is to dh what h is to b, with a row's a on the way to the row in front of it.  h in front of each row is
 // worked out again from the state that the forward saved for the tile.  c = a G is what a row passes on.  Three waves of a SIMD, whose registers hold a row's gates
-// from the first pass to the last: with four 14 did not (207 us where this takes 190, a training step of 48 histories).
+// from the first pass to the last: with four 14 registers were kept in memory (a training step of 48 histories took 9 % more).
 template <class T, int ROWS, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 3) void hstu_scan_bwd_kernel(const ScanParams p) {
     static_assert(ROWS * WAVES == kTile && ROWS <= 16, "a row for each");

@@ -83,7 +83,7 @@ def gated_recurrence(
     slices of ``hstu_compute_uqvk`` are read in place); ``decay``: ``[width]``, float32 or of x's type.  Rows ``seq_offsets[b]`` up to
     ``seq_offsets[b + 1]`` are sequence ``b``; it begins with ``initial_state[b]`` (``[B, width]``, float32) or with zeros.  ``return_state``: the second
     result is ``[B, width]``, float32, what ``initial_state`` or ``gated_recurrence_step`` goes on from (a sequence without rows keeps its
-    own); else None.  h is fp32 throughout and rounded once for each row.  A row whose ``decay_gate`` is as low as its type goes leaves the state as it is.
+    own); else None.  h is fp32 throughout and rounded once for each row.  A row whose ``decay_gate`` is as low as its type goes leaves the state as it is (if its ``x`` is a number: 0 times an infinity is none).
     Rows behind the last sequence are zero.  Gradients for ``x``, both gates, ``decay`` and ``initial_state``; the backward computes h again, from a state
     for every 64 rows that the forward keeps.
 
@@ -135,8 +135,8 @@ def gated_recurrence_step(
     back to where it was read.  Returns the rows, as ``gated_recurrence`` gives them.  A row whose slot is neither -1 nor one of the states comes back NaN
     and is not kept; a state whose new slot is not one of the states is not kept either.  No gradients.
 
-    Caller contract: no state is put twice in a call, and none that another row reads (``HSTU_HIP_CHECK_CONTRACT=1`` raises, and where a slot
-    is none of the above).
+    Caller contract: the states' memory is none of the other tensors'; no state is put twice in a call, and none that another row reads (``HSTU_HIP_CHECK_CONTRACT=1`` raises for
+    slots, and where one is none of the above).
     """
     out = native.front.gated_recurrence_step(states, x, decay_gate, input_gate, decay, slots, new_slots, rate, False)
     if out is not None:
