@@ -32,7 +32,7 @@ const char* hstu_recurrent_last_error(void);
  *     z = rate * log(1 + exp(decay_c)) * sigmoid(decay_gate_t),  a = exp(-z)
  *     h_t = a * h_{t-1} + sqrt(1 - a^2) * sigmoid(input_gate_t) * x_t
  * h in front of a sequence's first row is initial_state[b], or 0.  out_t is h_t rounded to its type, final_state[b] the last h of the
- * sequence (its initial state where it has no rows), not rounded.  Where decay_gate is so low that its sigmoid is 0, a row leaves the state as it is.
+ * sequence (its initial state where it has no rows), not rounded.  Where decay_gate is so low that its sigmoid is 0, a row of finite x leaves the state as it is.
  * A column with an infinity or a NaN is not finite from that row to the end of its sequence; other columns and sequences are not touched by it.
  * Rows behind the last sequence become zero.  seq_offsets begin at 0 and do not decrease; nothing is read or written out of
  * bounds where they do, but the results are no one's.
@@ -59,6 +59,7 @@ typedef struct HstuRecurrenceArgs {
     int64_t workspace_bytes;
 } HstuRecurrenceArgs;
 
+/* What calls with these arguments need.  The forward's workspace goes by whether `saved` is NULL, so that is set first. */
 size_t hstu_recurrent_scan_workspace_bytes(const HstuRecurrenceArgs* args);
 size_t hstu_recurrent_scan_saved_bytes(const HstuRecurrenceArgs* args);
 int hstu_recurrent_scan(const HstuRecurrenceArgs* args, void* stream);
@@ -86,7 +87,7 @@ int hstu_recurrent_scan_bwd(const HstuRecurrenceArgs* args, const HstuRecurrence
  * One row for each of `rows` sequences: row r goes on from state slots[r] (-1: from nothing, zeros), and its new state is put into
  * new_slots[r] (-1: into none).  Without slots row r has state r; without new_slots they are slots.  A row whose slot is neither -1 nor one of the
  * states comes out NaN and is not put anywhere; nor is one whose new slot is not one.  No state may be put twice in a call, and none that
- * another row of the call reads.
+ * another row of the call reads; the states' memory is none of the other arguments'.
  */
 typedef struct HstuRecurrenceStepArgs {
     const void* x;              /* [rows, width] */
