@@ -83,8 +83,8 @@ def gated_recurrence(
     slices of ``hstu_compute_uqvk`` are read in place); ``decay``: ``[width]``, float32 or of x's type.  Rows ``seq_offsets[b]`` up to
     ``seq_offsets[b + 1]`` are sequence ``b``; it begins with ``initial_state[b]`` (``[B, width]``, float32) or with zeros.  ``return_state``: the second
     result is ``[B, width]``, float32, what ``initial_state`` or ``gated_recurrence_step`` goes on from (a sequence without rows keeps its
-    own); else None.  h is fp32 throughout and rounded once for each row.  A row whose ``decay_gate`` is as low as its type goes leaves the state as it is (if its ``x`` is a number: 0 times an infinity is none).
-    Rows behind the last sequence are zero.  Gradients for ``x``, both gates, ``decay`` and ``initial_state``; the backward computes h again, from a state
+    own); else None.  h is fp32 throughout and rounded once for each row.  A row of finite ``x`` whose ``decay_gate`` is as low as its type goes leaves
+    the state as it is.  Rows behind the last sequence are zero.  Gradients for ``x``, both gates, ``decay`` and ``initial_state``; the backward computes h again, from a state
     for every 64 rows that the forward keeps.
 
     Caller contract: ``seq_offsets`` begin at 0, do not decrease and do not end behind the rows (``HSTU_HIP_CHECK_CONTRACT=1`` raises where they
@@ -135,8 +135,8 @@ def gated_recurrence_step(
     back to where it was read.  Returns the rows, as ``gated_recurrence`` gives them.  A row whose slot is neither -1 nor one of the states comes back NaN
     and is not kept; a state whose new slot is not one of the states is not kept either.  No gradients.
 
-    Caller contract: the states' memory is none of the other tensors'; no state is put twice in a call, and none that another row reads (``HSTU_HIP_CHECK_CONTRACT=1`` raises for
-    slots, and where one is none of the above).
+    Caller contract: no state is put twice in a call, and none that another row reads (``HSTU_HIP_CHECK_CONTRACT=1`` raises, and where a slot
+    is none of the above); the states' memory is none of the other tensors'.
     """
     out = native.front.gated_recurrence_step(states, x, decay_gate, input_gate, decay, slots, new_slots, rate, False)
     if out is not None:
@@ -197,7 +197,7 @@ def gated_residual_norm(
 
     ``x`` (the residual stream), ``y`` (a block's output), ``gate``: ``[L, width]`` or ``[L, H, D]``, bf16, fp16 or fp32, any distance between rows;
     parameters ``[width]`` of the same type, shared by the rows.  ``norm(v)`` is ``v / sqrt(mean(v^2) + eps) * weight + bias`` over a whole row, with
-    ``layer_norm`` of ``v`` less its mean; ``eps`` may be 0 (a row whose mean square is 0 is NaN then).  ``post_*`` are those of the norm behind the block
+    ``layer_norm`` of ``v`` less its mean; ``eps`` may be 0 (a row whose mean square is 0 in fp32 is NaN then).  ``post_*`` are those of the norm behind the block
     (left out without ``post_weight``), ``pre_*`` those of the one in front of the next (without ``pre_weight`` the second result is None).  ``act`` is ``gate_activation``: ``"none"``, ``"sigmoid"`` or ``"silu"``;
     without ``gate`` and ``scale`` both are 1.  Everything in fp32, each result rounded once: the second norm takes the sum as it is, not rounded.
     Dropout runs when ``training`` and ``dropout_ratio > 0``, from the Philox stream of ``seed = (seed, offset)`` or of the device's default generator, as in

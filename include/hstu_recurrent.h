@@ -134,7 +134,7 @@ typedef struct HstuResidualNormArgs {
     const void* pre_bias;
     void* out;                  /* [rows, width] dense; unused by the backward, as normed */
     void* normed;
-    float eps;                  /* finite, not negative; 0: a row whose v^2 has a mean of 0 is NaN */
+    float eps;                  /* finite, not negative; below 2^-126 as 0: a row whose v^2 has a mean of 0 in fp32 is NaN */
     int32_t layer_norm;
     int32_t gate_activation;
     int32_t dtype;              /* HstuDtype: bf16, fp16 or fp32 */

@@ -83,7 +83,7 @@ def scan_grad(x, decay_gate, input_gate, decay, offsets, dout=None, dfinal=None,
     q_err = total_err * (let_in.abs() + kept.abs()) + total.abs() * a * s * before_err + F32 * (3 * Z * z + 2 * B) * sizes
     out = {
         "x": (total * m * i, total_err * m * i + 2 * B * F32 * total_size * m * i),
-        "decay_gate": (strength * (1 - s) * q, strength * ((1 - s) * q_err + 2 * Z * F32 * sizes)),  # (1 - s has s's error, not its own)
+        "decay_gate": (strength * (1 - s) * q, strength * ((1 - s) * q_err + 2 * Z * F32 * sizes)),  # (s's error for 1 - s: more than its own)
         "input_gate": (total * m * u * (1 - i), m * u.abs() * (total_err + 2 * B * F32 * total_size)),
         "initial": (d0, d0_err),
     }
